@@ -43,6 +43,11 @@ extern "C" {
 /* RopeType, include/mini_llama/model.h:11-14. */
 #define MLB_ROPE_NORMAL 0
 #define MLB_ROPE_NEOX 1
+#define MLB_ROPE_NONE (-1) /* mlb_paged_kv_append: rows stored as they are */
+
+/* Element type of activations where an entry point takes more than fp32. */
+#define MLB_ACT_F32 0
+#define MLB_ACT_BF16 1
 
 /* Weight kinds in the upload order of UploadModelWeightsToCuda,
  * src/model.cc:353-369. */
@@ -154,6 +159,20 @@ int mlb_rope(float* q_dev, float* k_dev, int n_heads, int n_kv_heads,
 /* Index of the largest logit, lowest index on ties (ArgMax, src/ops.cc:220). */
 int mlb_argmax(const float* x_dev, int n, int* index_host, int device_id, void* stream);
 
+/* Of every row of logits [rows, vocab] (a row stride in elements apart; any
+ * alignment; logits_type MLB_ACT_*): the log probability of tokens[row], the
+ * entropy in nats, and the top_k (0..32) most likely tokens, lower index first
+ * among equals, with their log probabilities (top_ids and top_logprob are
+ * [rows, top_k]). Logits of -inf have probability 0. A token outside [0, vocab)
+ * (a padded row) gets NaN; rows that hold NaN or +inf get NaN sums, and -1 with
+ * NaN where fewer than top_k logits are numbers. Asynchronous on `stream`, no
+ * workspace. No reference counterpart (MiniSampler, src/sampler.cc:107-183,
+ * keeps its probabilities to itself). */
+int mlb_logprobs(int logits_type, const void* logits_dev, long long row_stride, int rows,
+                 int vocab, const int* tokens_dev, int top_k, float* logprob_dev,
+                 float* entropy_dev, int* top_ids_dev, float* top_logprob_dev, int device_id,
+                 void* stream);
+
 /* ------------------------------------------------------ KV cache + attention
  * The cache is two fp32 arrays [n_layers][max_seq_len][n_kv_heads][head_dim]
  * (keys, values), the layout of CudaKvCache (src/cuda_kv_cache.cc:328-333). */
@@ -194,6 +213,67 @@ int mlb_attention_decode_noalloc(const float* q_dev, const float* keys_dev,
                                  int max_seq_len, int layer, int pos, int n_heads,
                                  int n_kv_heads, int head_dim, int mode,
                                  float* out_dev, int device_id, void* stream);
+
+/* ------------------------------------------------- paged 4-bit KV cache
+ * A pool of pages of page_size tokens (a multiple of 16), each holding every
+ * KV head's keys and values as Q4_0 blocks of 32 elements (4.5 bits per
+ * element; QuantizeToQ40, src/quant.cc:201-276, bit for bit). The pool is one
+ * device buffer of n_layers * n_pages pages, 16-byte aligned, which the caller
+ * owns; its layout is the library's own. head_dim: a multiple of 8 up to 128.
+ * No reference counterpart (CudaKvCache, src/cuda_kv_cache.cc:60-92, is one
+ * contiguous fp32 slab per sequence).
+ *
+ * The calls take ragged sequences on the device, all int32: row_offsets
+ * [n_seqs + 1] (non-decreasing; rows row_offsets[s] .. row_offsets[s + 1] - 1
+ * of the call belong to sequence s), seq_lens [n_seqs] (the sequence's length
+ * with these rows, which are its last) and page_table [n_seqs, max_pages]
+ * (entry j holds positions j * page_size ..). Nothing is read back to the host:
+ * calls are asynchronous on `stream` and can be captured in a CUDA graph that
+ * is replayed with new lengths and tables. What the device arrays hold is
+ * checked where it is used, and never followed out of bounds: rows at or past
+ * row_offsets[n_seqs] and rows at a negative position are left as they were, a
+ * position past the table or on a page outside [0, n_pages) is not stored, and
+ * attention does not see it. Rows of activations are contiguous [heads,
+ * head_dim], 16-byte aligned, a row stride (in elements) apart; act_type is
+ * MLB_ACT_F32 or MLB_ACT_BF16. Non-finite inputs make their own block of 32
+ * unspecified. Two rows of one call must not store to the same position of
+ * the same page. */
+int mlb_paged_kv_page_bytes(int page_size, int n_kv_heads, int head_dim, size_t* bytes);
+/* Stores the rows of k and v [n_rows, n_kv_heads, head_dim] at their positions,
+ * k rotated first (rope_type MLB_ROPE_*), and writes q [n_rows, n_heads,
+ * head_dim] rotated to q_out (may be q itself; n_heads = 0: no queries). Angles
+ * and rotation are computed in 64 bits and rounded once; mlb_rope's fp32
+ * angles differ from that by up to pos * 2^-24. */
+int mlb_paged_kv_append(void* pages_dev, int n_layers, int n_pages, int page_size, int n_kv_heads,
+                        int head_dim, int layer, int act_type, const void* k_dev,
+                        long long k_stride, const void* v_dev, long long v_stride,
+                        const void* q_dev, long long q_stride, int n_heads, void* q_out_dev,
+                        long long q_out_stride, int n_rows, int n_seqs, const int* row_offsets_dev,
+                        const int* seq_lens_dev, const int* page_table_dev, int max_pages,
+                        float theta, int rope_type, int device_id, void* stream);
+/* The values that the same rows' codes stand for, fp32 [n_rows, n_kv_heads,
+ * head_dim] each; zeros for rows that are not stored. */
+int mlb_paged_kv_read(const void* pages_dev, int n_layers, int n_pages, int page_size,
+                      int n_kv_heads, int head_dim, int layer, int n_rows, int n_seqs,
+                      const int* row_offsets_dev, const int* seq_lens_dev,
+                      const int* page_table_dev, int max_pages, float* k_out_dev,
+                      float* v_out_dev, int device_id, void* stream);
+/* out = softmax(scale q K^T) V of every row over the positions up to its own
+ * (CudaAttentionDecodeDeviceInput, include/mini_llama/cuda_attention.h:13, for
+ * ragged sequences; GQA head map h / (n_heads / n_kv_heads)): one row per
+ * sequence while decoding, a few to check drafted tokens, many for a prompt. A
+ * row that sees nothing gets zeros. q and out may not overlap. The workspace
+ * (16-byte aligned, mlb_paged_attention_workspace bytes, contents irrelevant)
+ * belongs to the call until it has finished on the device. */
+int mlb_paged_attention_workspace(int act_type, int n_rows, int n_seqs, int n_heads,
+                                  int n_kv_heads, int head_dim, int device_id, size_t* bytes);
+int mlb_paged_attention(const void* pages_dev, int n_layers, int n_pages, int page_size,
+                        int n_kv_heads, int head_dim, int layer, int act_type, const void* q_dev,
+                        long long q_stride, int n_heads, int n_rows, int n_seqs,
+                        const int* row_offsets_dev, const int* seq_lens_dev,
+                        const int* page_table_dev, int max_pages, float scale, void* out_dev,
+                        long long out_stride, void* workspace_dev, size_t workspace_bytes,
+                        int device_id, void* stream);
 
 /* --------------------------------------------------------- prepared weights
  * A weight repacked once into the B200 GEMV layout (what the decode path

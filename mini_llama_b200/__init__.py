@@ -11,6 +11,7 @@ kernels. Errors raise ``MlbError`` (the reference's std::runtime_error) or
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -22,26 +23,34 @@ from .configs import (F32, Q4_0, Q4_1, Q8_0, W_BK, W_BQ, W_BV, W_DOWN, W_FFN_NOR
                       W_WQ, W_WV, W_ATTENTION_NORM)
 
 ROPE_NORMAL, ROPE_NEOX = 0, 1
+ROPE_NONE = -1  # MLB_ROPE_NONE: CudaPagedKvCache.AppendDevice stores rows as they are
 ATTN_CPU_COMPAT, ATTN_STANDARD = 0, 1
 KV_F32, KV_BF16 = 0, 1  # MLB_KV_F32, MLB_KV_BF16: KV cache element type of a Batch
 ERR_TIMEOUT = -5  # MLB_ERR_TIMEOUT: a bounded device wait gave up
 
 __all__ = [
-    "F32", "Q8_0", "Q4_0", "Q4_1", "ROPE_NORMAL", "ROPE_NEOX", "ATTN_CPU_COMPAT",
+    "F32", "Q8_0", "Q4_0", "Q4_1", "ROPE_NORMAL", "ROPE_NEOX", "ROPE_NONE", "ATTN_CPU_COMPAT",
     "ATTN_STANDARD", "Sampler", "MlbError", "MlbRangeError", "CudaQuantBuilt", "CudaDeviceCount",
     "CudaQ80LinearDeviceInput", "CudaQ40LinearDeviceInput", "CudaQ41LinearDeviceInput",
     "CudaLinearDeviceInput", "CudaQ80Linear", "CudaQ40Linear", "CudaQ41Linear", "CudaLinear",
     "CudaRmsNormDeviceWeight", "CudaSiluDeviceInput", "CudaElementwiseMulDeviceInput",
     "CudaElementwiseAddDeviceInput", "CudaSoftmax", "CudaEmbeddingLookupDeviceWeight",
-    "CudaRopeDeviceInput", "CudaArgMax", "CudaKvCache", "CudaAttentionDecodeDeviceInput",
+    "CudaRopeDeviceInput", "CudaArgMax", "CudaLogProbs", "CudaKvCache",
+    "CudaAttentionDecodeDeviceInput", "CudaPagedKvCache", "CudaPagedAttentionDeviceInput",
     "QMatrix", "CudaModel", "Context", "Batch", "ForwardToken", "configs", "tp_plan", "nccl_unique_id",
 ]
 
 
-def _torch():
-    import torch  # device memory and streams only
+_torch_module = None
 
-    return torch
+
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch  # device memory and streams only
+
+        _torch_module = torch
+    return _torch_module
 
 
 def _ptr(t):
@@ -228,6 +237,77 @@ def CudaArgMax(x, device_id=0, stream=None) -> int:
     return out.value
 
 
+def _on_stream(call, device, stream):
+    """Runs a call with `stream` (a cudaStream_t address) current on `device`, so
+    that memory it allocates and frees is reused in that stream's order only."""
+    torch = _torch()
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        return call()
+
+
+def _raw_stream(device):
+    return _torch().cuda.current_stream(device).cuda_stream
+
+
+def _act_type(who, t):
+    torch = _torch()
+    if t.dtype is torch.float32:
+        return 0  # MLB_ACT_F32
+    if t.dtype is torch.bfloat16:
+        return 1  # MLB_ACT_BF16
+    raise MlbError(-1, f"{who}: expected float32 or bfloat16, got {t.dtype}")
+
+
+def _on_device(who, name, t, index):
+    if t.get_device() != index:
+        raise MlbError(-1, f"{who}: {name} is on {t.device}, expected cuda:{index}")
+
+
+def _int_tensor(who, name, t, shape, index):
+    if t.dtype is not _torch().int32 or t.shape != shape or not t.is_contiguous():
+        raise MlbError(-1, f"{who}: expected contiguous int32 {name} of shape {list(shape)}, got "
+                           f"{t.dtype} {list(t.shape)}")
+    if t.get_device() != index:
+        raise MlbError(-1, f"{who}: {name} is on {t.device}, expected cuda:{index}")
+
+
+def CudaLogProbs(logits, tokens, top_k=0, stream=None):
+    """Log probability of tokens[row], entropy (nats) and the top_k (0..32) most
+    likely tokens of every row of logits [rows, vocab] (fp32 or bf16; any row
+    stride), lower index first among equals (mlb_logprobs). Returns (logprobs
+    [rows], entropy [rows], top_ids int32 [rows, top_k], top_logprobs [rows,
+    top_k]). A token outside [0, vocab) marks a padded row: its log probability
+    is NaN. Runs on logits' device."""
+    torch = _torch()
+    who = "LogProbs"
+    if logits.dim() == 1:
+        logits = logits[None]
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise MlbError(-1, f"{who}: expected logits [rows, vocab], got {list(logits.shape)}")
+    act = _act_type(who, logits)
+    rows, vocab = logits.shape
+    if not 0 <= top_k <= min(32, vocab):
+        raise MlbError(-1, f"{who}: top_k must be 0 to {min(32, vocab)}, got {top_k}")
+    if not logits.is_cuda:
+        raise MlbError(-1, f"{who}: logits must be on a CUDA device")
+    index = logits.get_device()
+    _int_tensor(who, "tokens", tokens, (rows,), index)
+    if stream is not None:
+        return _on_stream(lambda: CudaLogProbs(logits, tokens, top_k), logits.device, stream)
+    stride = logits.stride(0) if rows > 1 else vocab
+    if logits.stride(1) != 1 or stride < vocab:
+        logits, stride = logits.contiguous(), vocab
+    dev = logits.device
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    check(lib().mlb_logprobs(act, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), top_k,
+                             logprob.data_ptr(), entropy.data_ptr(), ids.data_ptr(),
+                             top.data_ptr(), index, _raw_stream(dev)))
+    return logprob, entropy, ids, top
+
+
 # -------------------------------------------------------- KV cache, attention
 
 class CudaKvCache:
@@ -307,6 +387,236 @@ def CudaAttentionDecodeDeviceInput(q, kv_cache: CudaKvCache, layer, pos, n_heads
     check(lib().mlb_attention_decode(_ptr(q.contiguous()), _ptr(kv_cache.keys),
                                      _ptr(kv_cache.values), L, S, layer, pos, n_heads, n_kv_heads,
                                      head_dim, mode, _ptr(out), device_id, _stream(stream)))
+    return out
+
+
+def _row_stride(t):
+    """Row stride of [rows, heads, head_dim] whose rows the kernels can read as
+    they are (contiguous, 16-byte aligned), or 0."""
+    rows, heads, dim = t.shape
+    row = heads * dim
+    if t.is_contiguous():
+        stride = row
+    else:
+        stride, head, one = t.stride()
+        if (one != 1 and dim > 1) or (head != dim and heads > 1):
+            return 0
+        if rows <= 1:
+            stride = row
+        elif stride < row:
+            return 0
+    return 0 if stride * t.element_size() % 16 or t.data_ptr() % 16 else stride
+
+
+def _aligned_rows(t):
+    stride = _row_stride(t)
+    if stride == 0:
+        t = t.clone(memory_format=_torch().contiguous_format)
+        stride = t.shape[1] * t.shape[2]
+    return t, stride
+
+
+@functools.lru_cache(maxsize=None)
+def _paged_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim, device_id):
+    n = ctypes.c_size_t()
+    check(lib().mlb_paged_attention_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim,
+                                              device_id, ctypes.byref(n)))
+    return n.value
+
+
+class CudaPagedKvCache:
+    """Keys and values of many sequences in a pool of n_pages pages of page_size
+    tokens per layer (a multiple of 16), held as Q4_0 blocks: 4.5 bits per
+    element (mlb_paged_kv_*). Which pages a sequence owns is the caller's, given
+    to every call as device int32 tensors: row_offsets [n_seqs + 1] (which rows
+    of the call belong to which sequence), seq_lens [n_seqs] (lengths with these
+    rows, which are a sequence's last) and page_table [n_seqs, max_pages]. Rows
+    behind the last sequence are left as they were; positions past the table or
+    on a page outside the pool are neither stored nor seen. Calls do not
+    synchronise and may be captured in a CUDA graph. head_dim: a multiple of 8
+    up to 128."""
+
+    def __init__(self, n_layers=0, n_pages=0, page_size=0, n_kv_heads=0, head_dim=0, device_id=0):
+        self.pages = None
+        self._shape = (0, 0, 0, 0, 0)
+        self.device_id = device_id
+        if n_layers:
+            self.Reset(n_layers, n_pages, page_size, n_kv_heads, head_dim, device_id)
+
+    def Reset(self, n_layers, n_pages, page_size, n_kv_heads, head_dim, device_id=0):
+        torch = _torch()
+        for name, v in (("n_layers", n_layers), ("n_pages", n_pages)):
+            if v <= 0:
+                raise MlbError(-1, f"CudaPagedKvCache: {name} must be positive")
+        n = ctypes.c_size_t()
+        check(lib().mlb_paged_kv_page_bytes(page_size, n_kv_heads, head_dim, ctypes.byref(n)))
+        self.device_id = device_id
+        self._shape = (n_layers, n_pages, page_size, n_kv_heads, head_dim)
+        self.pages = torch.zeros((n_layers, n_pages, n.value), dtype=torch.uint8,
+                                 device=torch.device("cuda", device_id))
+
+    def Clear(self):
+        if self.pages is not None:
+            self.pages.zero_()
+
+    def empty(self):
+        return self.pages is None
+
+    def n_layers(self):
+        return self._shape[0]
+
+    def n_pages(self):
+        return self._shape[1]
+
+    def page_size(self):
+        return self._shape[2]
+
+    def n_kv_heads(self):
+        return self._shape[3]
+
+    def head_dim(self):
+        return self._shape[4]
+
+    def bytes(self):
+        return 0 if self.pages is None else self.pages.numel()
+
+    def _layer(self, who, layer):
+        if self.pages is None:
+            raise MlbError(-1, f"{who}: paged KV cache is empty")
+        if not 0 <= layer < self._shape[0]:
+            raise MlbRangeError(f"{who}: layer out of range")
+
+    def _sequences(self, who, row_offsets, seq_lens, page_table):
+        """(n_seqs, max_pages) of a call's sequences."""
+        n = seq_lens.numel()
+        if page_table.dim() != 2 or page_table.shape[1] == 0:
+            raise MlbError(-1, f"{who}: expected page_table [n_seqs, max_pages]")
+        width = page_table.shape[1]
+        _int_tensor(who, "seq_lens", seq_lens, (n,), self.device_id)
+        _int_tensor(who, "row_offsets", row_offsets, (n + 1,), self.device_id)
+        _int_tensor(who, "page_table", page_table, (n, width), self.device_id)
+        return n, width
+
+    def AppendDevice(self, layer, k, v, row_offsets, seq_lens, page_table, theta=10000.0,
+                     rope_type=ROPE_NORMAL, q=None, q_out=None, stream=None):
+        """Stores k and v [rows, n_kv_heads, head_dim] (fp32 or bf16) at their
+        positions, k rotated on the way, and returns q [rows, n_heads, head_dim]
+        rotated to the same positions, in q_out if given (q itself: in place).
+        rope_type ROPE_NONE stores k and returns q as they are."""
+        who = "CudaPagedKvCache"
+        self._layer(who, layer)
+        n_layers, n_pages, page_size, kv, dim = self._shape
+        if k.dim() != 3 or k.shape[1:] != (kv, dim) or v.shape != k.shape:
+            raise MlbError(-1, f"{who}: expected k and v [rows, {kv}, {dim}], got "
+                               f"{list(k.shape)} and {list(v.shape)}")
+        act = _act_type(who, k)
+        if v.dtype is not k.dtype:
+            raise MlbError(-1, f"{who}: k and v differ in type")
+        rows = k.shape[0]
+        _on_device(who, "k", k, self.device_id)
+        _on_device(who, "v", v, self.device_id)
+        n_seqs, max_pages = self._sequences(who, row_offsets, seq_lens, page_table)
+        if stream is not None:
+            return _on_stream(lambda: self.AppendDevice(
+                layer, k, v, row_offsets, seq_lens, page_table, theta, rope_type, q, q_out),
+                self.pages.device, stream)
+        k, ks = _aligned_rows(k)
+        v, vs = _aligned_rows(v)
+        heads = qs = qos = 0
+        q_at = out_at = None
+        if q is not None:
+            if (q.dim() != 3 or q.shape[0] != rows or q.shape[2] != dim or q.shape[1] == 0
+                    or q.dtype is not k.dtype):
+                raise MlbError(-1, f"{who}: expected q [{rows}, n_heads, {dim}] of k's type, got "
+                                   f"{q.dtype} {list(q.shape)}")
+            _on_device(who, "q", q, self.device_id)
+            heads = q.shape[1]
+            if q_out is None:
+                q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+                qos = heads * dim
+            else:
+                _on_device(who, "q_out", q_out, self.device_id)
+                if q_out.shape == q.shape and q_out.dtype is q.dtype:
+                    qos = _row_stride(q_out)
+                if qos == 0:
+                    raise MlbError(-1, f"{who}: q_out must be shaped like q, with 16-byte aligned "
+                                       "rows")
+            q, qs = _aligned_rows(q)
+            q_at, out_at = q.data_ptr(), q_out.data_ptr()
+        elif q_out is not None:
+            raise MlbError(-1, f"{who}: q_out without q")
+        check(lib().mlb_paged_kv_append(
+            self.pages.data_ptr(), n_layers, n_pages, page_size, kv, dim, layer, act, k.data_ptr(),
+            ks, v.data_ptr(), vs, q_at, qs, heads, out_at, qos, rows, n_seqs,
+            row_offsets.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), max_pages, theta,
+            rope_type, self.device_id, _raw_stream(self.device_id)))
+        return q_out
+
+    def ReadDevice(self, layer, row_offsets, seq_lens, page_table, n_rows, stream=None):
+        """fp32 keys and values [n_rows, n_kv_heads, head_dim] that the codes of
+        the sequences' last rows stand for (row_offsets as in AppendDevice; whole
+        sequences: the running sum of seq_lens). Rows that are not stored are 0."""
+        torch = _torch()
+        who = "CudaPagedKvCache"
+        self._layer(who, layer)
+        if n_rows < 0:
+            raise MlbError(-1, f"{who}: negative row count")
+        n_seqs, max_pages = self._sequences(who, row_offsets, seq_lens, page_table)
+        if stream is not None:
+            return _on_stream(lambda: self.ReadDevice(layer, row_offsets, seq_lens, page_table,
+                                                      n_rows), self.pages.device, stream)
+        n_layers, n_pages, page_size, kv, dim = self._shape
+        k = torch.empty((n_rows, kv, dim), dtype=torch.float32, device=self.pages.device)
+        v = torch.empty((n_rows, kv, dim), dtype=torch.float32, device=self.pages.device)
+        check(lib().mlb_paged_kv_read(
+            self.pages.data_ptr(), n_layers, n_pages, page_size, kv, dim, layer, n_rows, n_seqs,
+            row_offsets.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), max_pages,
+            k.data_ptr(), v.data_ptr(), self.device_id, _raw_stream(self.device_id)))
+        return k, v
+
+
+def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offsets, seq_lens,
+                                  page_table, n_heads, n_kv_heads, head_dim, scale=None, out=None,
+                                  stream=None):
+    """Attention of q [rows, n_heads, head_dim] (fp32 or bf16), each row over the
+    positions of its sequence up to its own (mlb_paged_attention): one row per
+    sequence while decoding, a few to check drafted tokens, many for a prompt.
+    scale defaults to 1 / sqrt(head_dim). A row that sees nothing gets zeros."""
+    torch = _torch()
+    who = "CudaPagedAttention"
+    kv_cache._layer(who, layer)
+    n_layers, n_pages, page_size, kv, dim = kv_cache._shape
+    if kv != n_kv_heads or dim != head_dim:
+        raise MlbError(-1, f"{who}: KV cache shape does not match attention shape")
+    if n_heads <= 0 or n_heads % n_kv_heads != 0:
+        raise MlbError(-1, f"{who}: n_heads must be divisible by n_kv_heads")
+    if q.dim() != 3 or q.shape[1:] != (n_heads, head_dim):
+        raise MlbError(-1, f"{who}: expected q [rows, {n_heads}, {head_dim}], got {list(q.shape)}")
+    act = _act_type(who, q)
+    index = kv_cache.device_id
+    _on_device(who, "q", q, index)
+    n_seqs, max_pages = kv_cache._sequences(who, row_offsets, seq_lens, page_table)
+    if stream is not None:
+        return _on_stream(lambda: CudaPagedAttentionDeviceInput(
+            q, kv_cache, layer, row_offsets, seq_lens, page_table, n_heads, n_kv_heads, head_dim,
+            scale, out), q.device, stream)
+    rows = q.shape[0]
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out_stride = n_heads * head_dim
+    else:
+        _on_device(who, "out", out, index)
+        out_stride = _row_stride(out) if out.shape == q.shape and out.dtype is q.dtype else 0
+        if out_stride == 0:
+            raise MlbError(-1, f"{who}: out must be shaped like q, with 16-byte aligned rows")
+    q, q_stride = _aligned_rows(q)
+    size = _paged_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim, index)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    check(lib().mlb_paged_attention(
+        kv_cache.pages.data_ptr(), n_layers, n_pages, page_size, kv, dim, layer, act, q.data_ptr(),
+        q_stride, n_heads, rows, n_seqs, row_offsets.data_ptr(), seq_lens.data_ptr(),
+        page_table.data_ptr(), max_pages, head_dim ** -0.5 if scale is None else scale,
+        out.data_ptr(), out_stride, ws.data_ptr(), size, index, _raw_stream(index)))
     return out
 
 

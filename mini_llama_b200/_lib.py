@@ -13,6 +13,7 @@ from . import build as _build
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 _c_int, _c_size_t, _c_float, _c_u64 = ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_uint64
+_c_ll = ctypes.c_longlong
 _vp, _fp = ctypes.c_void_p, ctypes.POINTER(ctypes.c_float)
 _ip = ctypes.POINTER(ctypes.c_int)
 
@@ -60,6 +61,20 @@ SIGNATURES = [
                                       _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
     ("mlb_attention_decode_noalloc", _c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,
                                               _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
+    ("mlb_logprobs", _c_int, [_c_int, _vp, _c_ll, _c_int, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp,
+                              _c_int, _vp]),
+    ("mlb_paged_kv_page_bytes", _c_int, [_c_int, _c_int, _c_int, ctypes.POINTER(_c_size_t)]),
+    ("mlb_paged_kv_append", _c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                     _vp, _c_ll, _vp, _c_ll, _vp, _c_ll, _c_int, _vp, _c_ll,
+                                     _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_float, _c_int,
+                                     _c_int, _vp]),
+    ("mlb_paged_kv_read", _c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                   _c_int, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp]),
+    ("mlb_paged_attention_workspace", _c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                               _c_int, ctypes.POINTER(_c_size_t)]),
+    ("mlb_paged_attention", _c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                     _vp, _c_ll, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int,
+                                     _c_float, _vp, _c_ll, _vp, _c_size_t, _c_int, _vp]),
     ("mlb_qmatrix_create", _c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _c_int,
                                     ctypes.POINTER(_vp)]),
     ("mlb_qmatrix_synthesize", _c_int, [_c_int, _c_int, _c_int, _c_u64, _c_u64, _c_int, _c_int,

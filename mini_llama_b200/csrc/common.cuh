@@ -54,6 +54,27 @@ int guarded(F&& f) {
 // Selects `device_id` for the calling thread (CudaSetDevice, src/cuda_runtime.cc).
 void set_device(int device_id);
 
+// Selects `device_id` for a call and the caller's device again after it.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device_id) {
+    if (cudaGetDevice(&was_) != cudaSuccess) was_ = -1;
+    if (was_ == device_id) {
+      was_ = -1;
+      return;
+    }
+    set_device(device_id);
+  }
+  ~DeviceScope() {
+    if (was_ >= 0) cudaSetDevice(was_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+
+ private:
+  int was_ = -1;
+};
+
 // Zeroes `bytes` of device memory and waits until it is done. cudaMemset runs
 // on the legacy default stream, which the library's non-blocking streams are
 // not ordered against: without the wait a large clear (a KV cache) can still

@@ -1,0 +1,787 @@
+// paged_attn.cu — causal attention over the paged Q4_0 KV cache.
+//
+// Row i of a sequence's n rows sits at position p_i = len - n + i and sees
+// positions 0..p_i. With codes q (integers -8..7) and block scales d,
+//
+//   s_t = scale * sum_w dK[t,w] * (sum_{j in group w} Q_j qK[t,j])
+//   O_j = sum_t (p_t dV[t,w(j)]) qV[t,j] / sum_t p_t,   p_t = exp(s_t - max)
+//
+// The integers are exact in fp16 and bf16, so the tensor cores multiply codes
+// and the scales are applied outside in fp32: to the accumulators of each
+// 32-dimension group for K, to the probabilities for V. Nothing of the cache is
+// rounded a second time.
+//
+// Decode form: a warp takes 32 tokens at a time. S = Q K^T is mma.m16n8k16 with
+// tokens as columns; its accumulators are already the column operand of
+// O^T = V^T P^T, so nothing is transposed and O^T of 8 rows is 32 registers.
+// Both operands that are not codes are fp16: queries, each row first scaled by a
+// power of two so that its largest element is near 2^13, and P dV, with
+// p_t = 2^(s_t - max + F) and F such that 2^F max(dV) is below 2^14 (F follows
+// the largest scale met so far as max does the largest score, and drops out of
+// the quotient). fp32 calls keep both as hi + lo pairs, off by at most 2^-22 of
+// the value or 2^-38 of the largest; bf16 queries are exact in one fp16 (down to
+// 2^-27 of the row's largest), and P dV in one fp16 is off by at most 2^-11, an
+// eighth of the bf16 output's own half step.
+//
+// Work: the blocks of all (sequence, KV head, row tile) units are laid end to
+// end in chunks of 128 tokens and cut into equal runs, one per CTA, so uneven
+// lengths cost nothing; a unit cut between CTAs leaves partial (max, sum, O)
+// records that a second kernel joins in chunk order, so results do not depend on
+// timing.
+#include <algorithm>
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <utility>
+
+#include "paged.cuh"
+
+namespace mlb {
+
+namespace {
+
+constexpr int kDecWarps = 4;
+constexpr int kDecThreads = kDecWarps * 32;
+constexpr int kChunkTokens = 32 * kDecWarps;  // one warp iteration each
+constexpr int kStages = 4;                    // 32-token stages in flight per warp
+
+struct DecArgs {
+  PagedCache cache;
+  PagedSeqs seqs;
+  const void* q;
+  void* out;
+  long long q_stride, out_stride;
+  int n_heads, group;
+  float scale_log2;  // scale * log2(e)
+  int4* split;       // per CTA: {parts, first record, row-tile key...} (two int4)
+  float* partial;    // per CTA two records of R x (32 G) + 2 R floats
+};
+
+struct SeqWork {
+  int len, n, row0, tiles, chunks;
+  long long cost;
+};
+
+__device__ __forceinline__ SeqWork seq_work(const DecArgs& a, int s, int tile_rows) {
+  SeqWork w;
+  const int cap = a.seqs.max_pages * a.cache.page_size;
+  w.len = min(max(a.seqs.seq_lens[s], 0), cap);
+  w.row0 = max(a.seqs.row_offsets[s], 0);
+  w.n = max(min(a.seqs.row_offsets[s + 1], a.seqs.n_rows) - w.row0, 0);
+  w.tiles = (int)(((long long)w.n * a.group + tile_rows - 1) / tile_rows);
+  w.chunks = max(1, (w.len + kChunkTokens - 1) / kChunkTokens);
+  w.cost = (long long)w.tiles * a.cache.kv * w.chunks;
+  return w;
+}
+
+// Inclusive block-wide scan of one value per thread (kDecThreads threads).
+__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) v += warp_sums[w];
+  __syncthreads();
+  return v;
+}
+
+__device__ __forceinline__ long long run_begin(long long total, int i, int n) {
+  return total * i / n;
+}
+
+// G consecutive 32-bit words of shared memory.
+template <int G>
+__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[G]) {
+  if constexpr (G == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else if constexpr (G == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x, w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < G; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+}
+
+__device__ __forceinline__ uint32_t hsub2_u(uint32_t x, uint32_t y) {
+  return h2_as_u32(__hsub2(u32_as_h2(x), u32_as_h2(y)));
+}
+
+// Eight 4-bit codes of a word as fp16 pairs (nibble i, nibble i + 4), minus 8:
+// 1024 + q and 1024 + 16 q are exact fp16, the second form saves the shift.
+__device__ __forceinline__ void codes_f16(uint32_t x, uint32_t (&r)[4]) {
+  const uint32_t magic = 0x64006400u, bias = 0x64086408u;  // 1024, 1032
+  const __half2 sixteenth = u32_as_h2(0x2C002C00u), m72 = u32_as_h2(0xD480D480u);
+  const uint32_t y = x >> 8;
+  r[0] = hsub2_u(lop3_and_or(x, 0x000F000Fu, magic), bias);
+  r[1] = h2_as_u32(__hfma2(u32_as_h2(lop3_and_or(x, 0x00F000F0u, magic)), sixteenth, m72));
+  r[2] = hsub2_u(lop3_and_or(y, 0x000F000Fu, magic), bias);
+  r[3] = h2_as_u32(__hfma2(u32_as_h2(lop3_and_or(y, 0x00F000F0u, magic)), sixteenth, m72));
+}
+
+// F of the largest V scale met so far: 2^F d < 2^14.
+__device__ __forceinline__ float shift_of(uint32_t d_bits) {
+  return (float)(28 - max((int)(d_bits >> 10), 1));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Words of a query row: 8 dimensions from d0, zeros past head_dim.
+__device__ __forceinline__ void load_q8(const float* p, float (&e)[8]) {
+  const float4 a = load_act4(p), b = load_act4(p + 4);
+  e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
+  e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
+}
+__device__ __forceinline__ void load_q8(const __nv_bfloat16* p, float (&e)[8]) {
+  const float4 a = load_act4(p), b = load_act4(p + 4);
+  e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
+  e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  return h2_as_u32(__floats2half2_rn(lo, hi));
+}
+
+// One row's query elements of this lane, scaled by a power of two, as MMA A
+// words: word (w, i) = dims 32 w + 8 c + (i, i + 4). inv receives 2^-shift.
+template <int G, class T>
+__device__ __forceinline__ void load_query(const T* row, int head_dim, int c, bool split,
+                                           uint32_t (&hi)[G][4], uint32_t (&lo)[G][4],
+                                           float& inv) {
+  float e[G][8];
+  float amax = 0.0f;
+#pragma unroll
+  for (int w = 0; w < G; ++w) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[w][i] = 0.0f;
+    const int d0 = 32 * w + 8 * c;
+    if (row && d0 < head_dim) load_q8(row + d0, e[w]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(e[w][i]));
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const int ex = (int)(__float_as_uint(amax) >> 23);
+  // zero rows, subnormal rows and infinities stay as they are
+  const int sh = (ex == 0 || ex == 255) ? 0 : min(max(13 - (ex - 127), -126), 126);
+  const float sf = __uint_as_float((uint32_t)(127 + sh) << 23);
+  inv = __uint_as_float((uint32_t)(127 - sh) << 23);
+#pragma unroll
+  for (int w = 0; w < G; ++w)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = e[w][i] * sf, y = e[w][i + 4] * sf;
+      hi[w][i] = pack_f16(x, y);
+      if (split) {
+        const float2 h = __half22float2(u32_as_h2(hi[w][i]));
+        lo[w][i] = pack_f16(x - h.x, y - h.y);
+      }
+    }
+}
+
+// NT 8-row tiles per unit. SPLIT: queries and P dV as hi + lo pairs.
+template <int G, int NT, class T>
+__global__ void __launch_bounds__(kDecThreads, NT > 1 ? 2 : 3)
+    paged_attn_decode_kernel(DecArgs a) {
+  constexpr bool SPLIT = sizeof(T) == 4;
+  constexpr int R = 8 * NT;
+  constexpr int MT = SPLIT ? NT : (NT + 1) / 2;
+  constexpr int BLOCK = 576 * G;
+  constexpr int STAGE = 2 * BLOCK;
+  constexpr int D = 32 * G;
+  constexpr int REC = R * D + 2 * R;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ long long warp_sums[kDecWarps];
+  __shared__ long long found_base;
+  __shared__ int found_seq;
+  __shared__ int stage_ok[kDecWarps][kStages][2];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int cta = blockIdx.x;
+
+  // total work and this CTA's run
+  long long total = 0;
+  for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
+    const int s = s0 + threadIdx.x;
+    total += s < a.seqs.n_seqs ? seq_work(a, s, R).cost : 0;
+  }
+  {
+    const long long t = block_scan(total, warp_sums);
+    if (threadIdx.x == kDecThreads - 1) found_base = t;
+    __syncthreads();
+    total = found_base;
+    __syncthreads();
+  }
+  const int nrun = (int)min((long long)gridDim.x, total);
+  int4* split = a.split + 2 * cta;
+  if (cta >= nrun) {
+    if (threadIdx.x == 0) split[0] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  const long long begin = run_begin(total, cta, nrun), end = run_begin(total, cta + 1, nrun);
+  const long long prev = cta > 0 ? run_begin(total, cta - 1, nrun) : 0;
+
+  // the sequence that holds `begin`
+  {
+    long long base = 0;
+    for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
+      const int s = s0 + threadIdx.x;
+      const long long cost = s < a.seqs.n_seqs ? seq_work(a, s, R).cost : 0;
+      const long long incl = block_scan(cost, warp_sums) + base;
+      if (cost > 0 && begin >= incl - cost && begin < incl) {
+        found_seq = s;
+        found_base = incl - cost;
+      }
+      if (threadIdx.x == kDecThreads - 1) warp_sums[0] = incl;
+      __syncthreads();
+      base = warp_sums[0];
+      __syncthreads();
+      if (base > begin) break;
+    }
+  }
+  int seq = found_seq;
+  long long base = found_base;
+  SeqWork sw = seq_work(a, seq, R);
+  if (threadIdx.x == 0) split[0] = make_int4(0, 0, 0, 0);
+
+  uint8_t* ring = smem + warp * (kStages * STAGE);
+  const size_t page_bytes = paged_page_bytes(a.cache.page_size, a.cache.kv, a.cache.head_dim);
+  const int bpp = a.cache.page_size / kPagedBlock;
+
+  for (long long at = begin; at < end;) {
+    while (at >= base + sw.cost) {  // next sequence with rows
+      base += sw.cost;
+      ++seq;
+      sw = seq_work(a, seq, R);
+    }
+    const long long u = (at - base) / sw.chunks;  // unit within the sequence
+    const long long unit_begin = base + u * sw.chunks;
+    const int head = (int)(u / sw.tiles), tile = (int)(u - (long long)head * sw.tiles);
+    const int chunk0 = (int)(at - unit_begin);
+    const int chunk1 = (int)min((long long)sw.chunks, end - unit_begin);
+    if (threadIdx.x == 0 && at == begin && unit_begin < begin && prev <= unit_begin) {
+      // this CTA holds the second part of a unit that an earlier one began
+      const long long unit_end = unit_begin + sw.chunks;
+      int last = cta;
+      while (last + 1 < nrun && run_begin(total, last + 1, nrun) < unit_end) ++last;
+      split[0] = make_int4(last - cta + 2, prev == unit_begin ? 0 : 1, seq, head);
+      split[1] = make_int4(tile, 0, 0, 0);
+    }
+
+    // stage copies: this warp's blocks 8 chunk + 2 warp, + 1
+    const int nblk = (sw.len + kPagedBlock - 1) / kPagedBlock;
+    const int iters = chunk1 - chunk0;
+    const int* table = a.seqs.table + (size_t)seq * a.seqs.max_pages;
+    int ids = -1;  // pages of the blocks of 16 iterations: lane 2 i + b
+    auto load_ids = [&](int it0) {
+      const int b = (chunk0 + it0 + (lane >> 1)) * (2 * kDecWarps) + 2 * warp + (lane & 1);
+      ids = b < nblk ? table[b / bpp] : -1;
+    };
+    auto issue = [&](int it) {
+      if (it < iters) {
+        if ((it & 15) == 0) load_ids(it);
+        const int st = it % kStages;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int page = __shfl_sync(0xffffffffu, ids, 2 * (it & 15) + b);
+          const bool ok = page >= 0 && page < a.cache.n_pages;
+          const int blk = (chunk0 + it) * (2 * kDecWarps) + 2 * warp + b;
+          if (lane == 0) stage_ok[warp][st][b] = ok;
+          if (ok) {
+            const uint8_t* src = a.cache.layer + page * page_bytes +
+                                 ((size_t)head * bpp + blk % bpp) * BLOCK;
+            uint8_t* dst = ring + st * STAGE + b * BLOCK;
+            for (int i = lane; i < BLOCK / 16; i += 32) cp_async16(dst + i * 16, src + i * 16);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+    // queries: row r of the tile is flat row tile R + r = token * group + head
+    uint32_t qa[MT][G][2][4];
+    float rs[NT];   // score factor of this lane's row in each 8-row tile
+    int vis[NT];    // positions it sees
+    int vis_min = 0x7fffffff;  // least of the tile's rows (rows past the last: none)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const long long flat = (long long)tile * R + t * 8 + g;
+      const bool live = flat < (long long)sw.n * a.group;
+      const int i = live ? (int)(flat / a.group) : 0;
+      const int hq = head * a.group + (live ? (int)(flat - (long long)i * a.group) : 0);
+      vis[t] = live ? max(sw.len - sw.n + i + 1, 0) : 0;
+      if (live) vis_min = min(vis_min, vis[t]);
+      const T* row = live ? static_cast<const T*>(a.q) + (long long)(sw.row0 + i) * a.q_stride +
+                                (size_t)hq * a.cache.head_dim
+                          : nullptr;
+      uint32_t hi[G][4], lo[G][4];
+      float inv;
+      load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
+      rs[t] = inv * a.scale_log2;
+      const int mt = SPLIT ? t : t / 2;
+#pragma unroll
+      for (int w = 0; w < G; ++w)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (SPLIT) {
+            qa[mt][w][k][0] = hi[w][2 * k];
+            qa[mt][w][k][1] = lo[w][2 * k];
+            qa[mt][w][k][2] = hi[w][2 * k + 1];
+            qa[mt][w][k][3] = lo[w][2 * k + 1];
+          } else {
+            qa[mt][w][k][t & 1] = hi[w][2 * k];
+            qa[mt][w][k][2 + (t & 1)] = hi[w][2 * k + 1];
+            if (NT == 1) {
+              qa[mt][w][k][1] = 0u;
+              qa[mt][w][k][3] = 0u;
+            }
+          }
+        }
+    }
+    vis_min = __reduce_min_sync(0xffffffffu, vis_min);
+
+    float o[NT][2 * G][4];
+    float m[NT], l[NT];
+    uint32_t dtop = 0;              // largest V scale so far, fp16 bits
+    float shift = shift_of(dtop);  // F
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t] = -INFINITY;
+      l[t] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[t][i][j] = 0.0f;
+    }
+
+    for (int it = 0; it < iters; ++it) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();
+      const int st = it % kStages;
+      const uint8_t* stage = ring + st * STAGE;
+      const int tok0 = ((chunk0 + it) * (2 * kDecWarps) + 2 * warp) * kPagedBlock;
+      const bool ok0 = stage_ok[warp][st][0], ok1 = stage_ok[warp][st][1];
+      const bool whole = ok0 && ok1 && tok0 + 32 <= vis_min;
+
+      // scores of 32 tokens: s[t][n-tile][token parity]
+      float2 s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        const uint8_t* block = stage + (nt >> 1) * BLOCK;
+        uint32_t kw[G], ks[G];
+        lds_words<G>(block + ((nt & 1) * 8 + g) * 16 * G + c * 4 * G, kw);
+        lds_words<G>(block + 512 * G + ((nt & 1) * 4 + c) * 4 * G, ks);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][nt] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < G; ++w) {
+          uint32_t b[4];
+          codes_f16(kw[w], b);
+          const float2 d = __half22float2(u32_as_h2(ks[w]));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            float acc[4];
+            mma_16816_z(acc, qa[mt][w][0], b[0], b[1]);
+            mma_16816(acc, qa[mt][w][1], b[2], b[3]);
+            if (SPLIT) {
+              s[mt][nt].x = fmaf(d.x, acc[0] + acc[2], s[mt][nt].x);
+              s[mt][nt].y = fmaf(d.y, acc[1] + acc[3], s[mt][nt].y);
+            } else {
+              s[2 * mt][nt].x = fmaf(d.x, acc[0], s[2 * mt][nt].x);
+              s[2 * mt][nt].y = fmaf(d.y, acc[1], s[2 * mt][nt].y);
+              if (2 * mt + 1 < NT) {
+                float2& r = s[2 * mt + 1 < NT ? 2 * mt + 1 : 0][nt];
+                r.x = fmaf(d.x, acc[2], r.x);
+                r.y = fmaf(d.y, acc[3], r.y);
+              }
+            }
+          }
+        }
+      }
+
+      // hidden[t] bit 2 nt + parity: token not seen by the row
+      uint32_t hidden[NT], hidden_all = 0;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        hidden[t] = 0;
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          s[t][nt].x *= rs[t];
+          s[t][nt].y *= rs[t];
+        }
+      }
+      if (!whole) {
+        hidden_all = 0xffu;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt) {
+            const int tok = tok0 + nt * 8 + 2 * c;
+            const bool ok = nt < 2 ? ok0 : ok1;
+            if (!ok || tok >= vis[t]) {
+              s[t][nt].x = -INFINITY;
+              hidden[t] |= 1u << (2 * nt);
+            }
+            if (!ok || tok + 1 >= vis[t]) {
+              s[t][nt].y = -INFINITY;
+              hidden[t] |= 2u << (2 * nt);
+            }
+          }
+          hidden_all &= hidden[t];
+        }
+      }
+
+      // largest V scale of the tokens that some row sees
+      __half2 dmax = u32_as_h2(0u);
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        uint32_t vs[G];
+        lds_words<G>(stage + (nt >> 1) * BLOCK + 544 * G + ((nt & 1) * 4 + c) * 4 * G, vs);
+        const uint32_t keep = (hidden_all >> (2 * nt) & 1 ? 0u : 0xffffu) |
+                              (hidden_all >> (2 * nt) & 2 ? 0u : 0xffff0000u);
+#pragma unroll
+        for (int w = 0; w < G; ++w) dmax = __hmax2(dmax, u32_as_h2(vs[w] & keep));
+      }
+      const uint32_t db = h2_as_u32(dmax);
+      const uint32_t dnow = __reduce_max_sync(0xffffffffu, max(db & 0xffffu, db >> 16));
+      const float shift_was = shift;
+      if (dnow > dtop) {
+        dtop = dnow;
+        shift = shift_of(dtop);
+      }
+
+      // online softmax
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float mx = fmaxf(s[t][0].x, s[t][0].y);
+#pragma unroll
+        for (int nt = 1; nt < 4; ++nt) mx = fmaxf(mx, fmaxf(s[t][nt].x, s[t][nt].y));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (shift != shift_was || __any_sync(0xffffffffu, mx > m[t])) {
+          const float mn = fmaxf(m[t], mx);
+          const float al = m[t] == -INFINITY ? 0.0f : ex2((m[t] - mn) + (shift - shift_was));
+          m[t] = mn;
+          l[t] *= al;
+          const float a0 = __shfl_sync(0xffffffffu, al, 8 * c);      // row 2 c
+          const float a1 = __shfl_sync(0xffffffffu, al, 8 * c + 4);  // row 2 c + 1
+#pragma unroll
+          for (int i = 0; i < 2 * G; ++i) {
+            o[t][i][0] *= a0;
+            o[t][i][1] *= a1;
+            o[t][i][2] *= a0;
+            o[t][i][3] *= a1;
+          }
+        }
+        const float ref = m[t] == -INFINITY ? 0.0f : m[t] - shift;  // -inf: nothing seen yet
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          s[t][nt].x = ex2(s[t][nt].x - ref);
+          s[t][nt].y = ex2(s[t][nt].y - ref);
+          l[t] += s[t][nt].x + s[t][nt].y;
+        }
+      }
+
+      // O^T += V^T (P dV)^T, block by block
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint8_t* block = stage + b * BLOCK;
+        uint32_t v0[G], v1[G], d0[G], d1[G];
+        lds_words<G>(block + 256 * G + lane * 4 * G, v0);
+        lds_words<G>(block + 384 * G + lane * 4 * G, v1);
+        lds_words<G>(block + 544 * G + c * 4 * G, d0);
+        lds_words<G>(block + 544 * G + (4 + c) * 4 * G, d1);
+#pragma unroll
+        for (int w = 0; w < G; ++w) {
+          uint32_t x0[4], x1[4];
+          codes_f16(v0[w], x0);
+          codes_f16(v1[w], x1);
+          const float2 e0 = __half22float2(u32_as_h2(d0[w]));
+          const float2 e1 = __half22float2(u32_as_h2(d1[w]));
+          const uint32_t a0[4] = {x0[0], x0[1], x1[0], x1[1]};
+          const uint32_t a1[4] = {x0[2], x0[3], x1[2], x1[3]};
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float p0 = s[t][2 * b].x * e0.x, p1 = s[t][2 * b].y * e0.y;
+            float p2 = s[t][2 * b + 1].x * e1.x, p3 = s[t][2 * b + 1].y * e1.y;
+            if (!whole) {  // a hidden token's scale may be anything
+              const uint32_t h = hidden[t] >> (4 * b);
+              p0 = h & 1 ? 0.0f : p0;
+              p1 = h & 2 ? 0.0f : p1;
+              p2 = h & 4 ? 0.0f : p2;
+              p3 = h & 8 ? 0.0f : p3;
+            }
+            const uint32_t h0 = pack_f16(p0, p1), h1 = pack_f16(p2, p3);
+            mma_16816(o[t][2 * w], a0, h0, h1);
+            mma_16816(o[t][2 * w + 1], a1, h0, h1);
+            if (SPLIT) {
+              const float2 f0 = __half22float2(u32_as_h2(h0)), f1 = __half22float2(u32_as_h2(h1));
+              const uint32_t l0 = pack_f16(p0 - f0.x, p1 - f0.y);
+              const uint32_t l1 = pack_f16(p2 - f1.x, p3 - f1.y);
+              mma_16816(o[t][2 * w], a0, l0, l1);
+              mma_16816(o[t][2 * w + 1], a1, l0, l1);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      issue(it + kStages - 1);
+    }
+
+    // join the warps: each leaves (O, max, sum) of its tokens in its ring
+    cp_async_wait_all();
+    __syncwarp();
+    float* rec = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
+      l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
+      if (c == 0) {
+        rec[R * D + t * 8 + g] = m[t] == -INFINITY ? m[t] : m[t] - shift;
+        rec[R * D + R + t * 8 + g] = l[t];
+      }
+      // lane holds rows 2 c, 2 c + 1 and dims 32 w + 4 g + 0..3
+#pragma unroll
+      for (int w = 0; w < G; ++w)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float4*>(rec + (t * 8 + 2 * c + e) * D + 32 * w + 4 * g) =
+              make_float4(o[t][2 * w][e], o[t][2 * w][2 + e], o[t][2 * w + 1][e],
+                          o[t][2 * w + 1][2 + e]);
+    }
+    __syncthreads();
+    const bool complete = chunk0 == 0 && chunk1 == sw.chunks;
+    float* part = a.partial + ((size_t)cta * 2 + (at == begin ? 0 : 1)) * REC;
+    const float* all = reinterpret_cast<const float*>(smem);
+    constexpr int RING = kStages * STAGE / 4;
+    for (int i = threadIdx.x; i < R * (D / 4); i += kDecThreads) {
+      const int r = i / (D / 4), d0 = (i - r * (D / 4)) * 4;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, all[w * RING + R * D + r]);
+      float sum = 0.0f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        const float mw = all[w * RING + R * D + r];
+        const float f = mw == mx ? 1.0f : ex2(mw - mx);
+        const float4 y = *reinterpret_cast<const float4*>(all + w * RING + r * D + d0);
+        sum = fmaf(f, all[w * RING + R * D + R + r], sum);
+        x.x = fmaf(f, y.x, x.x);
+        x.y = fmaf(f, y.y, x.y);
+        x.z = fmaf(f, y.z, x.z);
+        x.w = fmaf(f, y.w, x.w);
+      }
+      if (complete) {
+        const long long flat = (long long)tile * R + r;
+        if (flat >= (long long)sw.n * a.group || d0 >= a.cache.head_dim) continue;
+        const int tk = (int)(flat / a.group);
+        const int hq = head * a.group + (int)(flat - (long long)tk * a.group);
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing: zeros
+        store_act4(static_cast<T*>(a.out) + (long long)(sw.row0 + tk) * a.out_stride +
+                       (size_t)hq * a.cache.head_dim + d0,
+                   make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+      } else {
+        *reinterpret_cast<float4*>(part + r * D + d0) = x;
+        if (d0 == 0) {
+          part[R * D + r] = mx;
+          part[R * D + R + r] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    at = unit_begin + chunk1;
+  }
+  pdl_launch_dependents();
+}
+
+// Joins the parts of units that were cut between CTAs: block (i, y) joins rows
+// 4 y .. 4 y + 3 of the unit whose second part CTA i holds, one warp per row.
+template <int G, int NT, class T>
+__global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(DecArgs a) {
+  constexpr int R = 8 * NT;
+  constexpr int D = 32 * G;
+  constexpr int REC = R * D + 2 * R;
+  pdl_wait();
+  const int4 s0 = a.split[2 * blockIdx.x];
+  const int parts = s0.x;
+  if (parts == 0) return;
+  const int tile = a.split[2 * blockIdx.x + 1].x;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const SeqWork sw = seq_work(a, s0.z, R);
+  const long long flat = (long long)tile * R + r;
+  if (flat >= (long long)sw.n * a.group) return;
+  const float* first = a.partial + ((size_t)(blockIdx.x - 1) * 2 + s0.y) * REC;
+  const float* rest = a.partial + (size_t)blockIdx.x * 2 * REC;  // part p >= 1: + 2 (p - 1) REC
+  auto rec = [&](int p) { return p == 0 ? first : rest + (size_t)(p - 1) * 2 * REC; };
+  float mx = -INFINITY;
+  for (int p = lane; p < parts; p += 32) mx = fmaxf(mx, rec(p)[R * D + r]);
+  mx = warp_max(mx);
+  float sum = 0.0f, x[G];
+#pragma unroll
+  for (int w = 0; w < G; ++w) x[w] = 0.0f;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float* q = rec(p);
+    const float mp = q[R * D + r];
+    const float f = mp == mx ? 1.0f : ex2(mp - mx);
+    sum = fmaf(f, q[R * D + R + r], sum);
+#pragma unroll
+    for (int w = 0; w < G; ++w) x[w] = fmaf(f, q[r * D + 32 * w + lane], x[w]);
+  }
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int tk = (int)(flat / a.group);
+  const int hq = s0.w * a.group + (int)(flat - (long long)tk * a.group);
+  T* out = static_cast<T*>(a.out) + (long long)(sw.row0 + tk) * a.out_stride +
+           (size_t)hq * a.cache.head_dim;
+#pragma unroll
+  for (int w = 0; w < G; ++w)
+    if (32 * w + lane < a.cache.head_dim) {
+      if constexpr (sizeof(T) == 4)
+        out[32 * w + lane] = x[w] * f;
+      else
+        out[32 * w + lane] = __float2bfloat16_rn(x[w] * f);
+    }
+}
+
+// 8-row tiles per unit: two where the call's rows per KV head and sequence are
+// more than 8 on average, so that each block's codes are widened once for 16.
+int dec_tiles(int n_rows, int n_seqs, int group) {
+  return (long long)n_rows * group > 8LL * n_seqs ? 2 : 1;
+}
+
+int dec_grid(int sms, int nt) { return sms * (nt > 1 ? 2 : 3); }
+
+size_t dec_workspace(int grid, int groups, int nt) {
+  const size_t rec = (size_t)8 * nt * 32 * groups + 16 * nt;
+  return (size_t)grid * (2 * sizeof(int4) + 2 * rec * sizeof(float));
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.
+template <class K>
+void allow_smem(K kernel, size_t bytes, int device_id) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, bool> seen;
+  std::lock_guard<std::mutex> lock(mu);
+  bool& s = seen[{reinterpret_cast<const void*>(kernel), device_id}];
+  if (s) return;
+  MLB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  s = true;
+}
+
+template <int G, int NT, class T>
+void launch_decode(const DecArgs& a, int grid, int device_id, cudaStream_t stream) {
+  constexpr size_t smem = (size_t)kDecWarps * kStages * 2 * 576 * G;
+  static_assert(smem / kDecWarps >= (size_t)(8 * NT * 32 * G + 16 * NT) * 4, "record fits the ring");
+  allow_smem(paged_attn_decode_kernel<G, NT, T>, smem, device_id);
+  paged_attn_decode_kernel<G, NT, T><<<grid, kDecThreads, smem, stream>>>(a);
+  MLB_CUDA(cudaGetLastError());
+  launch_pdl(paged_attn_join_kernel<G, NT, T>, dim3(grid, 2 * NT), dim3(kDecThreads), 0, stream,
+             true, a);
+}
+
+template <class T>
+void decode_dispatch(const DecArgs& a, int groups, int nt, int grid, int device_id,
+                     cudaStream_t s) {
+  switch (groups * 4 + nt) {
+    case 4 + 1: return launch_decode<1, 1, T>(a, grid, device_id, s);
+    case 4 + 2: return launch_decode<1, 2, T>(a, grid, device_id, s);
+    case 8 + 1: return launch_decode<2, 1, T>(a, grid, device_id, s);
+    case 8 + 2: return launch_decode<2, 2, T>(a, grid, device_id, s);
+    case 12 + 1: return launch_decode<3, 1, T>(a, grid, device_id, s);
+    case 12 + 2: return launch_decode<3, 2, T>(a, grid, device_id, s);
+    case 16 + 1: return launch_decode<4, 1, T>(a, grid, device_id, s);
+    default: return launch_decode<4, 2, T>(a, grid, device_id, s);
+  }
+}
+
+void check_heads(const char* who, int n_heads, int kv) {
+  if (n_heads <= 0) invalid(std::string(who) + ": n_heads must be positive");
+  if (n_heads % kv != 0) invalid(std::string(who) + ": n_heads must be divisible by n_kv_heads");
+}
+
+}  // namespace
+
+}  // namespace mlb
+
+using namespace mlb;
+
+extern "C" int mlb_paged_attention_workspace(int act_type, int n_rows, int n_seqs, int n_heads,
+                                             int n_kv_heads, int head_dim, int device_id,
+                                             size_t* bytes) {
+  return guarded([&] {
+    const char* who = "CudaPagedAttention";
+    if (!bytes) invalid("CudaPagedAttention: null output");
+    paged_check_act(who, act_type);
+    paged_check_shape(who, kPagedBlock, n_kv_heads, head_dim);
+    check_heads(who, n_heads, n_kv_heads);
+    if (n_rows < 0 || n_seqs < 0) invalid("CudaPagedAttention: negative row or sequence count");
+    DeviceScope scope(device_id);
+    const int nt = dec_tiles(n_rows, n_seqs, n_heads / n_kv_heads);
+    *bytes = dec_workspace(dec_grid(sm_count(device_id), nt), paged_groups(head_dim), nt);
+  });
+}
+
+extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages, int page_size,
+                                   int n_kv_heads, int head_dim, int layer, int act_type,
+                                   const void* q, long long q_stride, int n_heads, int n_rows,
+                                   int n_seqs, const int* row_offsets, const int* seq_lens,
+                                   const int* page_table, int max_pages, float scale, void* out,
+                                   long long out_stride, void* workspace, size_t workspace_bytes,
+                                   int device_id, void* stream) {
+  return guarded([&] {
+    const char* who = "CudaPagedAttention";
+    DecArgs a;
+    a.cache = paged_cache(who, const_cast<void*>(pages), n_layers, n_pages, page_size, n_kv_heads,
+                          head_dim, layer);
+    a.seqs = paged_seqs(who, n_rows, n_seqs, row_offsets, seq_lens, page_table, max_pages,
+                        page_size);
+    paged_check_act(who, act_type);
+    check_heads(who, n_heads, n_kv_heads);
+    if (!std::isfinite(scale)) invalid("CudaPagedAttention: scale must be finite");
+    if (n_rows > 0) {
+      paged_check_rows(who, "q", q, q_stride, n_heads, head_dim, act_type);
+      paged_check_rows(who, "out", out, out_stride, n_heads, head_dim, act_type);
+    }
+    DeviceScope scope(device_id);
+    if (n_rows == 0 || n_seqs == 0) return;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.n_heads = n_heads;
+    a.group = n_heads / n_kv_heads;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const int groups = paged_groups(head_dim);
+    const int nt = dec_tiles(n_rows, n_seqs, a.group);
+    const int most = dec_grid(sm_count(device_id), nt);
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+        workspace_bytes < dec_workspace(most, groups, nt))
+      invalid("CudaPagedAttention: workspace is null, unaligned or too small");
+    a.split = static_cast<int4*>(workspace);
+    a.partial = reinterpret_cast<float*>(a.split + 2 * (size_t)most);
+    // no more CTAs than chunks that the page table and the rows can make
+    const long long tiles =
+        ((long long)n_rows * a.group + 8 * nt - 1) / (8 * nt) + n_seqs;
+    const long long chunks =
+        ((long long)max_pages * page_size + kChunkTokens - 1) / kChunkTokens;
+    const int grid = (int)std::min<long long>(most, tiles * n_kv_heads * chunks);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (act_type == MLB_ACT_BF16)
+      decode_dispatch<__nv_bfloat16>(a, groups, nt, grid, device_id, s);
+    else
+      decode_dispatch<float>(a, groups, nt, grid, device_id, s);
+  });
+}
