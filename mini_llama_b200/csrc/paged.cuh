@@ -35,7 +35,7 @@ namespace mlb {
 constexpr int kPagedBlock = 16;  // tokens per block
 constexpr int kPagedMaxHeadDim = 128;
 
-// One layer of a cache and the sequences of a call.
+// One layer of a cache (fewer than 2^31 blocks) and the sequences of a call.
 struct PagedSeqs {
   const int* row_offsets;  // [n_seqs + 1]
   const int* seq_lens;     // [n_seqs], the call's rows included
@@ -73,6 +73,8 @@ inline PagedCache paged_cache(const char* who, void* pages, int n_layers, int n_
   if (layer < 0 || layer >= n_layers) out_of_range(w + ": layer out of range");
   if (reinterpret_cast<uintptr_t>(pages) % 16 != 0)
     invalid(w + ": pages must be 16-byte aligned");
+  if ((long long)n_pages * kv * (page_size / kPagedBlock) >= (1LL << 31))
+    invalid(w + ": a layer must have fewer than 2^31 blocks of 16 tokens");
   PagedCache c;
   c.layer = static_cast<uint8_t*>(pages) +
             (size_t)layer * n_pages * paged_page_bytes(page_size, kv, head_dim);
@@ -142,6 +144,13 @@ __device__ __forceinline__ void store_act4(float* p, const float4& v) {
 }
 __device__ __forceinline__ void store_act4(__nv_bfloat16* p, const float4& v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+__device__ __forceinline__ void store_act2(float* p, float x, float y) {
+  *reinterpret_cast<float2*>(p) = make_float2(x, y);
+}
+__device__ __forceinline__ void store_act2(__nv_bfloat16* p, float x, float y) {
+  *reinterpret_cast<uint32_t*>(p) = pack_bf16(x, y);
 }
 
 // The sequence that row r belongs to: the last s with row_offsets[s] <= r, found

@@ -11,20 +11,20 @@
 // 32-dimension group for K, to the probabilities for V. Nothing of the cache is
 // rounded a second time.
 //
-// Decode form: a warp takes 32 tokens at a time. S = Q K^T is mma.m16n8k16 with
+// Decode form: a warp takes 16 tokens at a time. S = Q K^T is mma.m16n8k16 with
 // tokens as columns; its accumulators are already the column operand of
 // O^T = V^T P^T, so nothing is transposed and O^T of 8 rows is 32 registers.
 // Both operands that are not codes are fp16: queries, each row first scaled by a
-// power of two so that its largest element is near 2^13, and P dV, with
-// p_t = 2^(s_t - max + F) and F such that 2^F max(dV) is below 2^14 (F follows
-// the largest scale met so far as max does the largest score, and drops out of
-// the quotient). fp32 calls keep both as hi + lo pairs, off by at most 2^-22 of
-// the value or 2^-38 of the largest; bf16 queries are exact in one fp16 (down to
-// 2^-27 of the row's largest), and P dV in one fp16 is off by at most 2^-11, an
-// eighth of the bf16 output's own half step.
+// power of two so that its largest element is near 2^13, and p 2^F dV with F such
+// that 2^F max(dV) is below 2^14 and 2^F at most 2^15 (F follows the largest
+// scale met so far, as max does the largest score, and comes off at the end).
+// fp32 calls keep both as hi + lo pairs, off by at most 2^-21 of the value, or
+// 2^-25 2^-F where that is larger; bf16 queries are exact in one fp16 (down to
+// 2^-27 of the row's largest), and p 2^F and its product with dV in one fp16
+// each are off by at most 2^-10, a quarter of the bf16 output's own half step.
 //
 // Work: the blocks of all (sequence, KV head, row tile) units are laid end to
-// end in chunks of 128 tokens and cut into equal runs, one per CTA, so uneven
+// end in chunks of 64 tokens and cut into equal runs, one per CTA, so uneven
 // lengths cost nothing; a unit cut between CTAs leaves partial (max, sum, O)
 // records that a second kernel joins in chunk order, so results do not depend on
 // timing.
@@ -32,6 +32,7 @@
 #include <cmath>
 #include <map>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 
 #include "paged.cuh"
@@ -42,8 +43,12 @@ namespace {
 
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = kDecWarps * 32;
-constexpr int kChunkTokens = 32 * kDecWarps;  // one warp iteration each
-constexpr int kStages = 4;                    // 32-token stages in flight per warp
+constexpr int kChunkTokens = kPagedBlock * kDecWarps;  // one block per warp
+constexpr int kStages = 5;                    // blocks on their way per warp, and in use
+constexpr int kMaxSegs = 32;                  // segments of a run listed at a time
+
+// CTAs per SM: 128 registers a thread for one 8-row tile, 168 for two.
+__host__ __device__ constexpr int dec_ctas(int nt) { return nt > 1 ? 3 : 4; }
 
 struct DecArgs {
   PagedCache cache;
@@ -55,6 +60,11 @@ struct DecArgs {
   float scale_log2;  // scale * log2(e)
   int4* split;       // per CTA: {parts, first record, row-tile key...} (two int4)
   float* partial;    // per CTA two records of R x (32 G) + 2 R floats
+};
+
+// Part of a CTA's run: chunks [chunk0, chunk1) of one (sequence, KV head, row tile).
+struct Seg {
+  int seq, head, tile, chunk0, chunk1, chunks, len, n, row0, record;
 };
 
 struct SeqWork {
@@ -112,8 +122,8 @@ __device__ __forceinline__ uint32_t hsub2_u(uint32_t x, uint32_t y) {
   return h2_as_u32(__hsub2(u32_as_h2(x), u32_as_h2(y)));
 }
 
-// Eight 4-bit codes of a word as fp16 pairs (nibble i, nibble i + 4), minus 8:
-// 1024 + q and 1024 + 16 q are exact fp16, the second form saves the shift.
+// Eight 4-bit codes of a word as fp16 pairs (nibble i, nibble i + 4), minus 8.
+// 1024 + q and 1024 + 16 q are exact fp16; the second form saves a shift.
 __device__ __forceinline__ void codes_f16(uint32_t x, uint32_t (&r)[4]) {
   const uint32_t magic = 0x64006400u, bias = 0x64086408u;  // 1024, 1032
   const __half2 sixteenth = u32_as_h2(0x2C002C00u), m72 = u32_as_h2(0xD480D480u);
@@ -124,10 +134,37 @@ __device__ __forceinline__ void codes_f16(uint32_t x, uint32_t (&r)[4]) {
   r[3] = h2_as_u32(__hfma2(u32_as_h2(lop3_and_or(y, 0x00F000F0u, magic)), sixteenth, m72));
 }
 
-// F of the largest V scale met so far: 2^F d < 2^14.
-__device__ __forceinline__ float shift_of(uint32_t d_bits) {
-  return (float)(28 - max((int)(d_bits >> 10), 1));
+// Two fp32 at a time.
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
 }
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// F of the largest V scale met so far: 2^F d < 2^14, and 2^F itself within fp16.
+__device__ __forceinline__ int shift_of(uint32_t d_bits) {
+  return min(28 - max((int)(d_bits >> 10), 1), 15);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -173,14 +210,15 @@ __device__ __forceinline__ void load_query(const T* row, int head_dim, int c, bo
   const int ex = (int)(__float_as_uint(amax) >> 23);
   // zero rows, subnormal rows and infinities stay as they are
   const int sh = (ex == 0 || ex == 255) ? 0 : min(max(13 - (ex - 127), -126), 126);
-  const float sf = __uint_as_float((uint32_t)(127 + sh) << 23);
-  inv = __uint_as_float((uint32_t)(127 - sh) << 23);
+  const float sf = pow2(sh);
+  inv = pow2(-sh);
 #pragma unroll
   for (int w = 0; w < G; ++w)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float x = e[w][i] * sf, y = e[w][i + 4] * sf;
       hi[w][i] = pack_f16(x, y);
+      lo[w][i] = 0u;
       if (split) {
         const float2 h = __half22float2(u32_as_h2(hi[w][i]));
         lo[w][i] = pack_f16(x - h.x, y - h.y);
@@ -190,20 +228,20 @@ __device__ __forceinline__ void load_query(const T* row, int head_dim, int c, bo
 
 // NT 8-row tiles per unit. SPLIT: queries and P dV as hi + lo pairs.
 template <int G, int NT, class T>
-__global__ void __launch_bounds__(kDecThreads, NT > 1 ? 2 : 3)
-    paged_attn_decode_kernel(DecArgs a) {
+__global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_kernel(DecArgs a) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int R = 8 * NT;
   constexpr int MT = SPLIT ? NT : (NT + 1) / 2;
   constexpr int BLOCK = 576 * G;
-  constexpr int STAGE = 2 * BLOCK;
   constexpr int D = 32 * G;
   constexpr int REC = R * D + 2 * R;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint4 queries[MT * G * 2 * 32];  // MMA A words of the tile, by (m-tile, w, k half, lane)
   __shared__ long long warp_sums[kDecWarps];
   __shared__ long long found_base;
   __shared__ int found_seq;
-  __shared__ int stage_ok[kDecWarps][kStages][2];
+  __shared__ int slot_ok[kDecWarps][kStages];
+  __shared__ Seg segs[kMaxSegs];
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -254,372 +292,442 @@ __global__ void __launch_bounds__(kDecThreads, NT > 1 ? 2 : 3)
   SeqWork sw = seq_work(a, seq, R);
   if (threadIdx.x == 0) split[0] = make_int4(0, 0, 0, 0);
 
-  uint8_t* ring = smem + warp * (kStages * STAGE);
-  const size_t page_bytes = paged_page_bytes(a.cache.page_size, a.cache.kv, a.cache.head_dim);
+  uint8_t* ring = smem + warp * (kStages * BLOCK);
   const int bpp = a.cache.page_size / kPagedBlock;
 
   for (long long at = begin; at < end;) {
-    while (at >= base + sw.cost) {  // next sequence with rows
-      base += sw.cost;
-      ++seq;
-      sw = seq_work(a, seq, R);
+    // the next segments of the run, every thread in step, thread 0 noting them
+    int n_segs = 0;
+    while (at < end && n_segs < kMaxSegs) {
+      while (at >= base + sw.cost) {  // next sequence with rows
+        base += sw.cost;
+        ++seq;
+        sw = seq_work(a, seq, R);
+      }
+      const long long u = (at - base) / sw.chunks;  // unit within the sequence
+      const long long unit_begin = base + u * sw.chunks;
+      Seg sg;
+      sg.seq = seq;
+      sg.head = (int)(u / sw.tiles);
+      sg.tile = (int)(u - (long long)sg.head * sw.tiles);
+      sg.chunk0 = (int)(at - unit_begin);
+      sg.chunk1 = (int)min((long long)sw.chunks, end - unit_begin);
+      sg.chunks = sw.chunks;
+      sg.len = sw.len;
+      sg.n = sw.n;
+      sg.row0 = sw.row0;
+      sg.record = at == begin ? 0 : 1;
+      if (threadIdx.x == 0) {
+        segs[n_segs] = sg;
+        if (at == begin && unit_begin < begin && prev <= unit_begin) {
+          // this CTA holds the second part of a unit that an earlier one began;
+          // the last part is with the last run that begins before the unit ends
+          const long long unit_end = unit_begin + sw.chunks;
+          const int last = (int)((unit_end * nrun + total - 1) / total) - 1;
+          split[0] = make_int4(last - cta + 2, prev == unit_begin ? 0 : 1, seq, sg.head);
+          split[1] = make_int4(sg.tile, 0, 0, 0);
+        }
+      }
+      ++n_segs;
+      at = unit_begin + sg.chunk1;
     }
-    const long long u = (at - base) / sw.chunks;  // unit within the sequence
-    const long long unit_begin = base + u * sw.chunks;
-    const int head = (int)(u / sw.tiles), tile = (int)(u - (long long)head * sw.tiles);
-    const int chunk0 = (int)(at - unit_begin);
-    const int chunk1 = (int)min((long long)sw.chunks, end - unit_begin);
-    if (threadIdx.x == 0 && at == begin && unit_begin < begin && prev <= unit_begin) {
-      // this CTA holds the second part of a unit that an earlier one began
-      const long long unit_end = unit_begin + sw.chunks;
-      int last = cta;
-      while (last + 1 < nrun && run_begin(total, last + 1, nrun) < unit_end) ++last;
-      split[0] = make_int4(last - cta + 2, prev == unit_begin ? 0 : 1, seq, head);
-      split[1] = make_int4(tile, 0, 0, 0);
-    }
+    __syncthreads();
 
-    // stage copies: this warp's blocks 8 chunk + 2 warp, + 1
-    const int nblk = (sw.len + kPagedBlock - 1) / kPagedBlock;
-    const int iters = chunk1 - chunk0;
-    const int* table = a.seqs.table + (size_t)seq * a.seqs.max_pages;
-    int ids = -1;  // pages of the blocks of 16 iterations: lane 2 i + b
-    auto load_ids = [&](int it0) {
-      const int b = (chunk0 + it0 + (lane >> 1)) * (2 * kDecWarps) + 2 * warp + (lane & 1);
-      ids = b < nblk ? table[b / bpp] : -1;
-    };
-    auto issue = [&](int it) {
-      if (it < iters) {
-        if ((it & 15) == 0) load_ids(it);
-        const int st = it % kStages;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int page = __shfl_sync(0xffffffffu, ids, 2 * (it & 15) + b);
-          const bool ok = page >= 0 && page < a.cache.n_pages;
-          const int blk = (chunk0 + it) * (2 * kDecWarps) + 2 * warp + b;
-          if (lane == 0) stage_ok[warp][st][b] = ok;
-          if (ok) {
-            const uint8_t* src = a.cache.layer + page * page_bytes +
-                                 ((size_t)head * bpp + blk % bpp) * BLOCK;
-            uint8_t* dst = ring + st * STAGE + b * BLOCK;
-            for (int i = lane; i < BLOCK / 16; i += 32) cp_async16(dst + i * 16, src + i * 16);
+    // copies, running ahead of the arithmetic across segments: block 4 chunk + warp
+    int is = 0, ic = segs[0].chunk0, iw = 0, slot_in = 0;
+    int at_block = -1;  // place in the layer of this lane's block of the next 32, -1: none
+    auto issue = [&]() {
+      if (is < n_segs) {
+        const Seg& sg = segs[is];
+        if (iw == 0) {
+          const int bl = (ic + lane) * kDecWarps + warp;
+          at_block = -1;
+          if (bl * kPagedBlock < sg.len) {
+            const int p = bl / bpp;
+            const int page = a.seqs.table[(size_t)sg.seq * a.seqs.max_pages + p];
+            if (page >= 0 && page < a.cache.n_pages)
+              at_block = (page * a.cache.kv + sg.head) * bpp + (bl - p * bpp);
           }
+        }
+        const int from = __shfl_sync(0xffffffffu, at_block, iw);
+        if (lane == 0) slot_ok[warp][slot_in] = from >= 0;
+        if (from >= 0) {
+          const uint8_t* src = a.cache.layer + (size_t)from * BLOCK + lane * 16;
+          uint8_t* dst = ring + slot_in * BLOCK + lane * 16;
+#pragma unroll
+          for (int i = 0; i < BLOCK / 512; ++i) cp_async16(dst + i * 512, src + i * 512);
+          if (BLOCK % 512 != 0 && lane < BLOCK % 512 / 16)
+            cp_async16(dst + BLOCK / 512 * 512, src + BLOCK / 512 * 512);
+        }
+        slot_in = slot_in + 1 == kStages ? 0 : slot_in + 1;
+        iw = (iw + 1) & 31;
+        if (++ic == sg.chunk1) {
+          ++is;
+          iw = 0;
+          if (is < n_segs) ic = segs[is].chunk0;
         }
       }
       cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    for (int i = 0; i < kStages - 1; ++i) issue();
+    int slot = 0;
 
-    // queries: row r of the tile is flat row tile R + r = token * group + head
-    uint32_t qa[MT][G][2][4];
-    float rs[NT];   // score factor of this lane's row in each 8-row tile
-    int vis[NT];    // positions it sees
-    int vis_min = 0x7fffffff;  // least of the tile's rows (rows past the last: none)
+    for (int si = 0; si < n_segs; ++si) {
+      const Seg& sg = segs[si];
+
+      // queries: row r of the tile is flat row tile R + r = token * group + head
+      float rs[NT];  // score factor of this lane's row in each 8-row tile
+      int vis[NT];   // positions it sees
+      int vis_min = 0x7fffffff, vis_max = 0;  // of the tile's rows (rows past the last: none)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const long long flat = (long long)tile * R + t * 8 + g;
-      const bool live = flat < (long long)sw.n * a.group;
-      const int i = live ? (int)(flat / a.group) : 0;
-      const int hq = head * a.group + (live ? (int)(flat - (long long)i * a.group) : 0);
-      vis[t] = live ? max(sw.len - sw.n + i + 1, 0) : 0;
-      if (live) vis_min = min(vis_min, vis[t]);
-      const T* row = live ? static_cast<const T*>(a.q) + (long long)(sw.row0 + i) * a.q_stride +
-                                (size_t)hq * a.cache.head_dim
-                          : nullptr;
-      uint32_t hi[G][4], lo[G][4];
-      float inv;
-      load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
-      rs[t] = inv * a.scale_log2;
-      const int mt = SPLIT ? t : t / 2;
+      for (int t = 0; t < NT; ++t) {
+        const long long flat = (long long)sg.tile * R + t * 8 + g;
+        const bool live = flat < (long long)sg.n * a.group;
+        const int i = live ? (int)(flat / a.group) : 0;
+        const int hq = sg.head * a.group + (live ? (int)(flat - (long long)i * a.group) : 0);
+        vis[t] = live ? max(sg.len - sg.n + i + 1, 0) : 0;
+        if (live) vis_min = min(vis_min, vis[t]);
+        vis_max = max(vis_max, vis[t]);
+        const T* row = live ? static_cast<const T*>(a.q) + (long long)(sg.row0 + i) * a.q_stride +
+                                  (size_t)hq * a.cache.head_dim
+                            : nullptr;
+        uint32_t hi[G][4], lo[G][4];
+        float inv;
+        load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
+        rs[t] = inv * a.scale_log2;
+        // the warps share the tile; each writes its part of the words
 #pragma unroll
-      for (int w = 0; w < G; ++w)
+        for (int w = 0; w < G; ++w) {
+          if (w % kDecWarps != warp) continue;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (SPLIT) {
-            qa[mt][w][k][0] = hi[w][2 * k];
-            qa[mt][w][k][1] = lo[w][2 * k];
-            qa[mt][w][k][2] = hi[w][2 * k + 1];
-            qa[mt][w][k][3] = lo[w][2 * k + 1];
-          } else {
-            qa[mt][w][k][t & 1] = hi[w][2 * k];
-            qa[mt][w][k][2 + (t & 1)] = hi[w][2 * k + 1];
-            if (NT == 1) {
-              qa[mt][w][k][1] = 0u;
-              qa[mt][w][k][3] = 0u;
+          for (int k = 0; k < 2; ++k) {
+            uint4& q = queries[(((SPLIT ? t : t / 2) * G + w) * 2 + k) * 32 + lane];
+            if (SPLIT) {
+              q = make_uint4(hi[w][2 * k], lo[w][2 * k], hi[w][2 * k + 1], lo[w][2 * k + 1]);
+            } else if (t & 1) {
+              q.y = hi[w][2 * k];
+              q.w = hi[w][2 * k + 1];
+            } else {
+              q = make_uint4(hi[w][2 * k], 0u, hi[w][2 * k + 1], 0u);
             }
           }
         }
-    }
-    vis_min = __reduce_min_sync(0xffffffffu, vis_min);
+      }
+      vis_min = __reduce_min_sync(0xffffffffu, vis_min);
+      vis_max = __reduce_max_sync(0xffffffffu, vis_max);
+      __syncthreads();
 
-    float o[NT][2 * G][4];
-    float m[NT], l[NT];
-    uint32_t dtop = 0;              // largest V scale so far, fp16 bits
-    float shift = shift_of(dtop);  // F
+      float o[NT][2 * G][4];
+      float m[NT];
+      float2 l[NT];
+      uint32_t dtop = 0;           // largest V scale so far, fp16 bits
+      int shift = shift_of(dtop);  // F: O is in units of 2^-F
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      m[t] = -INFINITY;
-      l[t] = 0.0f;
+      for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < 2 * G; ++i)
+        for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[t][i][j] = 0.0f;
-    }
+          for (int j = 0; j < 4; ++j) o[t][i][j] = 0.0f;
+      }
 
-    for (int it = 0; it < iters; ++it) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncwarp();
-      const int st = it % kStages;
-      const uint8_t* stage = ring + st * STAGE;
-      const int tok0 = ((chunk0 + it) * (2 * kDecWarps) + 2 * warp) * kPagedBlock;
-      const bool ok0 = stage_ok[warp][st][0], ok1 = stage_ok[warp][st][1];
-      const bool whole = ok0 && ok1 && tok0 + 32 <= vis_min;
+      // One block of 16 tokens. WHOLE: every row of the tile sees all of them.
+      auto step = [&](auto whole_c, const uint8_t* block, int tok0) {
+        constexpr bool WHOLE = decltype(whole_c)::value;
 
-      // scores of 32 tokens: s[t][n-tile][token parity]
-      float2 s[NT][4];
+        // scores: s[t][n-tile] = tokens 8 nt + 2 c, + 1
+        float2 s[NT][2];
+        {
+          uint32_t kw[2][G], ks[2][G];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        const uint8_t* block = stage + (nt >> 1) * BLOCK;
-        uint32_t kw[G], ks[G];
-        lds_words<G>(block + ((nt & 1) * 8 + g) * 16 * G + c * 4 * G, kw);
-        lds_words<G>(block + 512 * G + ((nt & 1) * 4 + c) * 4 * G, ks);
+          for (int nt = 0; nt < 2; ++nt) {
+            lds_words<G>(block + (nt * 8 + g) * 16 * G + c * 4 * G, kw[nt]);
+            lds_words<G>(block + 512 * G + (nt * 4 + c) * 4 * G, ks[nt]);
+          }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][nt] = make_float2(0.f, 0.f);
+          for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < G; ++w) {
-          uint32_t b[4];
-          codes_f16(kw[w], b);
-          const float2 d = __half22float2(u32_as_h2(ks[w]));
+          for (int w = 0; w < G; ++w) {
+            uint32_t b[2][4];
+            codes_f16(kw[0][w], b[0]);
+            codes_f16(kw[1][w], b[1]);
+            const float2 d0 = __half22float2(u32_as_h2(ks[0][w]));
+            const float2 d1 = __half22float2(u32_as_h2(ks[1][w]));
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            float acc[4];
-            mma_16816_z(acc, qa[mt][w][0], b[0], b[1]);
-            mma_16816(acc, qa[mt][w][1], b[2], b[3]);
-            if (SPLIT) {
-              s[mt][nt].x = fmaf(d.x, acc[0] + acc[2], s[mt][nt].x);
-              s[mt][nt].y = fmaf(d.y, acc[1] + acc[3], s[mt][nt].y);
-            } else {
-              s[2 * mt][nt].x = fmaf(d.x, acc[0], s[2 * mt][nt].x);
-              s[2 * mt][nt].y = fmaf(d.y, acc[1], s[2 * mt][nt].y);
-              if (2 * mt + 1 < NT) {
-                float2& r = s[2 * mt + 1 < NT ? 2 * mt + 1 : 0][nt];
-                r.x = fmaf(d.x, acc[2], r.x);
-                r.y = fmaf(d.y, acc[3], r.y);
+            for (int mt = 0; mt < MT; ++mt) {
+              const uint4 u0 = queries[((mt * G + w) * 2 + 0) * 32 + lane];
+              const uint4 u1 = queries[((mt * G + w) * 2 + 1) * 32 + lane];
+              const uint32_t q0[4] = {u0.x, u0.y, u0.z, u0.w}, q1[4] = {u1.x, u1.y, u1.z, u1.w};
+              float acc[2][4];
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt) {
+                mma_16816_z(acc[nt], q0, b[nt][0], b[nt][1]);
+                mma_16816(acc[nt], q1, b[nt][2], b[nt][3]);
+              }
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt) {
+                const float2 d = nt ? d1 : d0;
+                const float2 x = make_float2(acc[nt][0], acc[nt][1]);
+                const float2 y = make_float2(acc[nt][2], acc[nt][3]);
+                if (SPLIT) {
+                  s[mt][nt] = fma2(d, add2(x, y), s[mt][nt]);
+                } else {
+                  constexpr int LAST = NT - 1;
+                  const int t1 = 2 * mt + 1 < NT ? 2 * mt + 1 : LAST;
+                  s[2 * mt][nt] = fma2(d, x, s[2 * mt][nt]);
+                  if (2 * mt + 1 < NT) s[t1][nt] = fma2(d, y, s[t1][nt]);
+                }
               }
             }
           }
         }
-      }
 
-      // hidden[t] bit 2 nt + parity: token not seen by the row
-      uint32_t hidden[NT], hidden_all = 0;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        hidden[t] = 0;
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          s[t][nt].x *= rs[t];
-          s[t][nt].y *= rs[t];
-        }
-      }
-      if (!whole) {
-        hidden_all = 0xffu;
+        // online softmax; hidden[t] bit 2 nt + parity: token not seen by the row
+        uint32_t hidden[NT], hidden_all = 0xfu;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+          hidden[t] = 0;
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt) {
-            const int tok = tok0 + nt * 8 + 2 * c;
-            const bool ok = nt < 2 ? ok0 : ok1;
-            if (!ok || tok >= vis[t]) {
-              s[t][nt].x = -INFINITY;
-              hidden[t] |= 1u << (2 * nt);
-            }
-            if (!ok || tok + 1 >= vis[t]) {
-              s[t][nt].y = -INFINITY;
-              hidden[t] |= 2u << (2 * nt);
+          for (int nt = 0; nt < 2; ++nt) {
+            s[t][nt] = mul2(s[t][nt], make_float2(rs[t], rs[t]));
+            if (!WHOLE) {
+              const int tok = tok0 + nt * 8 + 2 * c;
+              if (tok >= vis[t]) {
+                s[t][nt].x = -INFINITY;
+                hidden[t] |= 1u << (2 * nt);
+              }
+              if (tok + 1 >= vis[t]) {
+                s[t][nt].y = -INFINITY;
+                hidden[t] |= 2u << (2 * nt);
+              }
             }
           }
           hidden_all &= hidden[t];
-        }
-      }
-
-      // largest V scale of the tokens that some row sees
-      __half2 dmax = u32_as_h2(0u);
+          float mx = fmaxf(fmaxf(s[t][0].x, s[t][0].y), fmaxf(s[t][1].x, s[t][1].y));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (__any_sync(0xffffffffu, mx > m[t])) {
+            const float mn = fmaxf(m[t], mx);
+            const float al = m[t] == -INFINITY ? 0.0f : ex2(m[t] - mn);
+            m[t] = mn;
+            l[t].x *= al;
+            l[t].y *= al;
+            const float a0 = __shfl_sync(0xffffffffu, al, 8 * c);      // row 2 c
+            const float a1 = __shfl_sync(0xffffffffu, al, 8 * c + 4);  // row 2 c + 1
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        uint32_t vs[G];
-        lds_words<G>(stage + (nt >> 1) * BLOCK + 544 * G + ((nt & 1) * 4 + c) * 4 * G, vs);
-        const uint32_t keep = (hidden_all >> (2 * nt) & 1 ? 0u : 0xffffu) |
-                              (hidden_all >> (2 * nt) & 2 ? 0u : 0xffff0000u);
+            for (int i = 0; i < 2 * G; ++i) {
+              o[t][i][0] *= a0;
+              o[t][i][1] *= a1;
+              o[t][i][2] *= a0;
+              o[t][i][3] *= a1;
+            }
+          }
+          const float ref = m[t] == -INFINITY ? 0.0f : -m[t];  // -inf: nothing seen yet
 #pragma unroll
-        for (int w = 0; w < G; ++w) dmax = __hmax2(dmax, u32_as_h2(vs[w] & keep));
-      }
-      const uint32_t db = h2_as_u32(dmax);
-      const uint32_t dnow = __reduce_max_sync(0xffffffffu, max(db & 0xffffu, db >> 16));
-      const float shift_was = shift;
-      if (dnow > dtop) {
-        dtop = dnow;
-        shift = shift_of(dtop);
-      }
-
-      // online softmax
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float mx = fmaxf(s[t][0].x, s[t][0].y);
-#pragma unroll
-        for (int nt = 1; nt < 4; ++nt) mx = fmaxf(mx, fmaxf(s[t][nt].x, s[t][nt].y));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        if (shift != shift_was || __any_sync(0xffffffffu, mx > m[t])) {
-          const float mn = fmaxf(m[t], mx);
-          const float al = m[t] == -INFINITY ? 0.0f : ex2((m[t] - mn) + (shift - shift_was));
-          m[t] = mn;
-          l[t] *= al;
-          const float a0 = __shfl_sync(0xffffffffu, al, 8 * c);      // row 2 c
-          const float a1 = __shfl_sync(0xffffffffu, al, 8 * c + 4);  // row 2 c + 1
-#pragma unroll
-          for (int i = 0; i < 2 * G; ++i) {
-            o[t][i][0] *= a0;
-            o[t][i][1] *= a1;
-            o[t][i][2] *= a0;
-            o[t][i][3] *= a1;
+          for (int nt = 0; nt < 2; ++nt) {
+            s[t][nt] = add2(s[t][nt], make_float2(ref, ref));
+            s[t][nt].x = ex2(s[t][nt].x);
+            s[t][nt].y = ex2(s[t][nt].y);
+            l[t] = add2(l[t], s[t][nt]);
           }
         }
-        const float ref = m[t] == -INFINITY ? 0.0f : m[t] - shift;  // -inf: nothing seen yet
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          s[t][nt].x = ex2(s[t][nt].x - ref);
-          s[t][nt].y = ex2(s[t][nt].y - ref);
-          l[t] += s[t][nt].x + s[t][nt].y;
-        }
-      }
 
-      // O^T += V^T (P dV)^T, block by block
+        // V scales; F follows the largest that some row sees
+        uint32_t vd[2][G];
+        __half2 dmax = u32_as_h2(0u);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const uint8_t* block = stage + b * BLOCK;
-        uint32_t v0[G], v1[G], d0[G], d1[G];
+        for (int nt = 0; nt < 2; ++nt) {
+          lds_words<G>(block + 544 * G + (nt * 4 + c) * 4 * G, vd[nt]);
+          const uint32_t keep = WHOLE ? 0xffffffffu
+                                      : (hidden_all >> (2 * nt) & 1 ? 0u : 0xffffu) |
+                                            (hidden_all >> (2 * nt) & 2 ? 0u : 0xffff0000u);
+#pragma unroll
+          for (int w = 0; w < G; ++w) dmax = __hmax2(dmax, u32_as_h2(vd[nt][w] & keep));
+        }
+        const uint32_t db = h2_as_u32(dmax);
+        const uint32_t dnow = __reduce_max_sync(0xffffffffu, max(db & 0xffffu, db >> 16));
+        if (dnow > dtop) {
+          dtop = dnow;
+          const int now = shift_of(dtop);
+          if (now != shift) {
+            const float f = pow2(now - shift);
+            shift = now;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[t][i][j] *= f;
+          }
+        }
+
+        // p 2^F as fp16 pairs (and what they leave)
+        const float up = pow2(shift);
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            const float2 x = mul2(s[t][nt], make_float2(up, up));
+            ph[t][nt] = pack_f16(x.x, x.y);
+            if (SPLIT) {
+              const float2 h = __half22float2(u32_as_h2(ph[t][nt]));
+              pl[t][nt] = pack_f16(x.x - h.x, x.y - h.y);
+            }
+          }
+
+        // O^T += V^T (P dV)^T
+        uint32_t v0[G], v1[G];
         lds_words<G>(block + 256 * G + lane * 4 * G, v0);
         lds_words<G>(block + 384 * G + lane * 4 * G, v1);
-        lds_words<G>(block + 544 * G + c * 4 * G, d0);
-        lds_words<G>(block + 544 * G + (4 + c) * 4 * G, d1);
 #pragma unroll
         for (int w = 0; w < G; ++w) {
           uint32_t x0[4], x1[4];
           codes_f16(v0[w], x0);
           codes_f16(v1[w], x1);
-          const float2 e0 = __half22float2(u32_as_h2(d0[w]));
-          const float2 e1 = __half22float2(u32_as_h2(d1[w]));
           const uint32_t a0[4] = {x0[0], x0[1], x1[0], x1[1]};
           const uint32_t a1[4] = {x0[2], x0[3], x1[2], x1[3]};
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            float p0 = s[t][2 * b].x * e0.x, p1 = s[t][2 * b].y * e0.y;
-            float p2 = s[t][2 * b + 1].x * e1.x, p3 = s[t][2 * b + 1].y * e1.y;
-            if (!whole) {  // a hidden token's scale may be anything
-              const uint32_t h = hidden[t] >> (4 * b);
-              p0 = h & 1 ? 0.0f : p0;
-              p1 = h & 2 ? 0.0f : p1;
-              p2 = h & 4 ? 0.0f : p2;
-              p3 = h & 8 ? 0.0f : p3;
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              // P dV = hi + lo: hi d rounded, its remainder exact, lo d on top
+              const __half2 d = u32_as_h2(vd[j][w]), h = u32_as_h2(ph[t][j]);
+              const __half2 x = __hmul2(h, d);
+              hi[j] = h2_as_u32(x);
+              if (SPLIT)
+                lo[j] = h2_as_u32(__hfma2(u32_as_h2(pl[t][j]), d, __hfma2(h, d, __hneg2(x))));
+              if (!WHOLE) {  // a hidden token's scale may be anything
+                const uint32_t hb = hidden[t] >> (2 * j);
+                const uint32_t keep = (hb & 1 ? 0u : 0xffffu) | (hb & 2 ? 0u : 0xffff0000u);
+                hi[j] &= keep;
+                if (SPLIT) lo[j] &= keep;
+              }
             }
-            const uint32_t h0 = pack_f16(p0, p1), h1 = pack_f16(p2, p3);
-            mma_16816(o[t][2 * w], a0, h0, h1);
-            mma_16816(o[t][2 * w + 1], a1, h0, h1);
+            mma_16816(o[t][2 * w], a0, hi[0], hi[1]);
+            mma_16816(o[t][2 * w + 1], a1, hi[0], hi[1]);
             if (SPLIT) {
-              const float2 f0 = __half22float2(u32_as_h2(h0)), f1 = __half22float2(u32_as_h2(h1));
-              const uint32_t l0 = pack_f16(p0 - f0.x, p1 - f0.y);
-              const uint32_t l1 = pack_f16(p2 - f1.x, p3 - f1.y);
-              mma_16816(o[t][2 * w], a0, l0, l1);
-              mma_16816(o[t][2 * w + 1], a1, l0, l1);
+              mma_16816(o[t][2 * w], a0, lo[0], lo[1]);
+              mma_16816(o[t][2 * w + 1], a1, lo[0], lo[1]);
             }
           }
         }
-      }
-      __syncwarp();
-      issue(it + kStages - 1);
-    }
+      };
 
-    // join the warps: each leaves (O, max, sum) of its tokens in its ring
-    cp_async_wait_all();
-    __syncwarp();
-    float* rec = reinterpret_cast<float*>(ring);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
-      l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
-      if (c == 0) {
-        rec[R * D + t * 8 + g] = m[t] == -INFINITY ? m[t] : m[t] - shift;
-        rec[R * D + R + t * 8 + g] = l[t];
+      // every chunk but the last leaves its slot to the copies at once; the last
+      // one's slot takes the warp's result first
+      const int chunk1 = sg.chunk1;
+      for (int chunk = sg.chunk0;;) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        const int tok0 = (chunk * kDecWarps + warp) * kPagedBlock;
+        if (slot_ok[warp][slot] && tok0 < vis_max) {
+          if (tok0 + kPagedBlock <= vis_min)
+            step(std::true_type{}, ring + slot * BLOCK, tok0);
+          else
+            step(std::false_type{}, ring + slot * BLOCK, tok0);
+        }
+        __syncwarp();
+        if (++chunk == chunk1) break;
+        issue();
+        slot = slot + 1 == kStages ? 0 : slot + 1;
       }
-      // lane holds rows 2 c, 2 c + 1 and dims 32 w + 4 g + 0..3
+
+      // join the warps, 8 rows by D / 2 dimensions at a time: each leaves (O, max,
+      // sum) of its tokens in the slot that it has just used
+      const float down = pow2(-shift);
+      const bool complete = sg.chunk0 == 0 && chunk1 == sg.chunks;
+      float* part = a.partial + ((size_t)cta * 2 + sg.record) * REC;
+      constexpr int H = D / 2;
+      auto record_of = [&](int w) {
+        return reinterpret_cast<float*>(smem + (w * kStages + slot) * BLOCK);
+      };
 #pragma unroll
-      for (int w = 0; w < G; ++w)
+      for (int t = 0; t < NT; ++t) {
+        float sum = l[t].x + l[t].y;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        float* rec = record_of(warp);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float4*>(rec + (t * 8 + 2 * c + e) * D + 32 * w + 4 * g) =
-              make_float4(o[t][2 * w][e], o[t][2 * w][2 + e], o[t][2 * w + 1][e],
-                          o[t][2 * w + 1][2 + e]);
-    }
-    __syncthreads();
-    const bool complete = chunk0 == 0 && chunk1 == sw.chunks;
-    float* part = a.partial + ((size_t)cta * 2 + (at == begin ? 0 : 1)) * REC;
-    const float* all = reinterpret_cast<const float*>(smem);
-    constexpr int RING = kStages * STAGE / 4;
-    for (int i = threadIdx.x; i < R * (D / 4); i += kDecThreads) {
-      const int r = i / (D / 4), d0 = (i - r * (D / 4)) * 4;
-      float mx = -INFINITY;
+        for (int h = 0; h < 2; ++h) {
+          if (c == 0) {
+            rec[8 * H + g] = m[t];
+            rec[8 * H + 8 + g] = sum;
+          }
+          // lane holds rows 2 c, 2 c + 1 of every m-tile: two dimensions each
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, all[w * RING + R * D + r]);
-      float sum = 0.0f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i = 0; i < G; ++i)
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) {
-        const float mw = all[w * RING + R * D + r];
-        const float f = mw == mx ? 1.0f : ex2(mw - mx);
-        const float4 y = *reinterpret_cast<const float4*>(all + w * RING + r * D + d0);
-        sum = fmaf(f, all[w * RING + R * D + R + r], sum);
-        x.x = fmaf(f, y.x, x.x);
-        x.y = fmaf(f, y.y, x.y);
-        x.z = fmaf(f, y.z, x.z);
-        x.w = fmaf(f, y.w, x.w);
-      }
-      if (complete) {
-        const long long flat = (long long)tile * R + r;
-        if (flat >= (long long)sw.n * a.group || d0 >= a.cache.head_dim) continue;
-        const int tk = (int)(flat / a.group);
-        const int hq = head * a.group + (int)(flat - (long long)tk * a.group);
-        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing: zeros
-        store_act4(static_cast<T*>(a.out) + (long long)(sw.row0 + tk) * a.out_stride +
-                       (size_t)hq * a.cache.head_dim + d0,
-                   make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
-      } else {
-        *reinterpret_cast<float4*>(part + r * D + d0) = x;
-        if (d0 == 0) {
-          part[R * D + r] = mx;
-          part[R * D + R + r] = sum;
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<float2*>(rec + (2 * c + e) * H + 16 * i + 2 * g) =
+                  make_float2(o[t][h * G + i][e] * down, o[t][h * G + i][2 + e] * down);
+          __syncthreads();
+          for (int i = threadIdx.x; i < 8 * (H / 2); i += kDecThreads) {
+            const int r = i / (H / 2), x0 = (i - r * (H / 2)) * 2;
+            // pair x0 of m-tile x0 / 16: dims 32 w + 4 g + 2 (m-tile & 1)
+            const int mt = h * G + x0 / 16, d0 = 32 * (mt >> 1) + 2 * (x0 % 16) + 2 * (mt & 1);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, record_of(w)[8 * H + r]);
+            float all = 0.0f;
+            float2 x = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kDecWarps; ++w) {
+              const float mw = record_of(w)[8 * H + r];
+              const float f = mw == mx ? 1.0f : ex2(mw - mx);
+              const float2 y = *reinterpret_cast<const float2*>(record_of(w) + r * H + x0);
+              all = fmaf(f, record_of(w)[8 * H + 8 + r], all);
+              x.x = fmaf(f, y.x, x.x);
+              x.y = fmaf(f, y.y, x.y);
+            }
+            if (complete) {
+              const long long flat = (long long)sg.tile * R + t * 8 + r;
+              if (flat < (long long)sg.n * a.group && d0 < a.cache.head_dim) {
+                const int tk = (int)(flat / a.group);
+                const int hq = sg.head * a.group + (int)(flat - (long long)tk * a.group);
+                const float f = all == 0.0f ? 0.0f : 1.0f / all;  // sees nothing: zeros
+                store_act2(static_cast<T*>(a.out) + (long long)(sg.row0 + tk) * a.out_stride +
+                               (size_t)hq * a.cache.head_dim + d0,
+                           x.x * f, x.y * f);
+              }
+            } else {
+              *reinterpret_cast<float2*>(part + (t * 8 + r) * D + d0) = x;
+              if (d0 == 0) {
+                part[R * D + t * 8 + r] = mx;
+                part[R * D + R + t * 8 + r] = all;
+              }
+            }
+          }
+          __syncthreads();
         }
       }
+      issue();
+      slot = slot + 1 == kStages ? 0 : slot + 1;
     }
-    __syncthreads();
-    at = unit_begin + chunk1;
+    cp_async_wait_all();
+    __syncthreads();  // segs and the slots are used again
   }
   pdl_launch_dependents();
 }
 
-// Joins the parts of units that were cut between CTAs: block (i, y) joins rows
-// 4 y .. 4 y + 3 of the unit whose second part CTA i holds, one warp per row.
+// Joins the parts of units that were cut between CTAs: block (i, y) joins row y
+// of the unit whose second part CTA i holds. The warps take every fourth part,
+// so that up to 32 of them are on their way at a time, and join in order.
 template <int G, int NT, class T>
 __global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(DecArgs a) {
   constexpr int R = 8 * NT;
   constexpr int D = 32 * G;
   constexpr int REC = R * D + 2 * R;
+  __shared__ float xs[kDecWarps][D], sums[kDecWarps];
   pdl_wait();
   const int4 s0 = a.split[2 * blockIdx.x];
   const int parts = s0.x;
   if (parts == 0) return;
   const int tile = a.split[2 * blockIdx.x + 1].x;
-  const int lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y;
   const SeqWork sw = seq_work(a, s0.z, R);
   const long long flat = (long long)tile * R + r;
   if (flat >= (long long)sw.n * a.group) return;
@@ -632,8 +740,8 @@ __global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(DecArgs a)
   float sum = 0.0f, x[G];
 #pragma unroll
   for (int w = 0; w < G; ++w) x[w] = 0.0f;
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
+#pragma unroll 8
+  for (int p = warp; p < parts; p += kDecWarps) {
     const float* q = rec(p);
     const float mp = q[R * D + r];
     const float f = mp == mx ? 1.0f : ex2(mp - mx);
@@ -641,19 +749,28 @@ __global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(DecArgs a)
 #pragma unroll
     for (int w = 0; w < G; ++w) x[w] = fmaf(f, q[r * D + 32 * w + lane], x[w]);
   }
-  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int w = 0; w < G; ++w) xs[warp][32 * w + lane] = x[w];
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= a.cache.head_dim) return;
+  sum = 0.0f;
+  float y = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kDecWarps; ++w) {
+    sum += sums[w];
+    y += xs[w][d];
+  }
+  y *= sum == 0.0f ? 0.0f : 1.0f / sum;
   const int tk = (int)(flat / a.group);
   const int hq = s0.w * a.group + (int)(flat - (long long)tk * a.group);
   T* out = static_cast<T*>(a.out) + (long long)(sw.row0 + tk) * a.out_stride +
            (size_t)hq * a.cache.head_dim;
-#pragma unroll
-  for (int w = 0; w < G; ++w)
-    if (32 * w + lane < a.cache.head_dim) {
-      if constexpr (sizeof(T) == 4)
-        out[32 * w + lane] = x[w] * f;
-      else
-        out[32 * w + lane] = __float2bfloat16_rn(x[w] * f);
-    }
+  if constexpr (sizeof(T) == 4)
+    out[d] = y;
+  else
+    out[d] = __float2bfloat16_rn(y);
 }
 
 // 8-row tiles per unit: two where the call's rows per KV head and sequence are
@@ -662,7 +779,7 @@ int dec_tiles(int n_rows, int n_seqs, int group) {
   return (long long)n_rows * group > 8LL * n_seqs ? 2 : 1;
 }
 
-int dec_grid(int sms, int nt) { return sms * (nt > 1 ? 2 : 3); }
+int dec_grid(int sms, int nt) { return sms * dec_ctas(nt); }
 
 size_t dec_workspace(int grid, int groups, int nt) {
   const size_t rec = (size_t)8 * nt * 32 * groups + 16 * nt;
@@ -683,12 +800,12 @@ void allow_smem(K kernel, size_t bytes, int device_id) {
 
 template <int G, int NT, class T>
 void launch_decode(const DecArgs& a, int grid, int device_id, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)kDecWarps * kStages * 2 * 576 * G;
-  static_assert(smem / kDecWarps >= (size_t)(8 * NT * 32 * G + 16 * NT) * 4, "record fits the ring");
+  constexpr size_t smem = (size_t)kDecWarps * kStages * 576 * G;
+  static_assert((8 * 16 * G + 16) * 4 <= 576 * G, "a record of 8 rows and half the dimensions fits a slot");
   allow_smem(paged_attn_decode_kernel<G, NT, T>, smem, device_id);
   paged_attn_decode_kernel<G, NT, T><<<grid, kDecThreads, smem, stream>>>(a);
   MLB_CUDA(cudaGetLastError());
-  launch_pdl(paged_attn_join_kernel<G, NT, T>, dim3(grid, 2 * NT), dim3(kDecThreads), 0, stream,
+  launch_pdl(paged_attn_join_kernel<G, NT, T>, dim3(grid, 8 * NT), dim3(kDecThreads), 0, stream,
              true, a);
 }
 

@@ -67,14 +67,15 @@ def attention(q, k, v, length, n, scale, absent=()):
 def attention_bound(out, vabs, top, length, dtype):
     """Largest error of the kernels. Scores: queries kept to 2^-22 and up to 16
     truncated adds of 2^-23 per product, so at most top * 2^-18 each, doubled by
-    numerator and denominator; p: exp 2^-21, P dV kept to 2^-22 (bf16 calls: one
-    fp16, 2^-11, and the same for the query's lost low bits), sums over the
-    length one truncated add per 16 tokens and warp. An fp16 below 2^-14 is off by
-    up to 2^-25 instead: P dV is scaled so that the largest dV is at least 2^13,
-    so that is 2^-38 of the largest dV for each token, times codes up to 8 whose
-    values reach 7 dV: 2^-35 / 7 of the largest |v| per token."""
+    numerator and denominator; p: exp 2^-21, P dV kept to 2^-21 (bf16 calls: two
+    fp16 roundings, 2^-10), sums over the length one truncated add per 16 tokens
+    and warp. An fp16 below 2^-14 is off by up to 2^-25 instead: P dV is scaled by
+    2^F, the smaller of 2^15 and what brings the largest dV to at least 2^13, so
+    that is the larger of 2^-40 and 2^-38 of the largest dV for each token, times
+    codes up to 8 (the largest |v| is at most 8 dV, and at least 6 of them): per
+    token 2^-37 or 2^-35 / 6 of the largest |v|."""
     top, vmax = top
-    floor = length * 2.0 ** -35 / 7 * vmax
+    floor = length * torch.clamp(vmax * 2.0 ** -35 / 6, min=2.0 ** -37)
     rel = top * 2.0 ** -17 + (16 + length / 32) * 2.0 ** -22
     if dtype == torch.bfloat16:
         return vabs * (rel + 2.0 ** -10) + floor + out.abs() * 2.0 ** -8
