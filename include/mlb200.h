@@ -235,8 +235,9 @@ int mlb_attention_decode_noalloc(const float* q_dev, const float* keys_dev,
  * position past the table or on a page outside [0, n_pages) is not stored, and
  * attention does not see it. Rows of activations are contiguous [heads,
  * head_dim], 16-byte aligned, a row stride (in elements) apart; act_type is
- * MLB_ACT_F32 or MLB_ACT_BF16. Non-finite inputs make their own block of 32
- * unspecified. Two rows of one call must not store to the same position of
+ * MLB_ACT_F32 or MLB_ACT_BF16. What is stored is finite: a block's scale ends
+ * at fp16's largest number, and non-finite inputs leave some finite values in
+ * their own block of 32. Two rows of one call must not store to the same position of
  * the same page. */
 int mlb_paged_kv_page_bytes(int page_size, int n_kv_heads, int head_dim, size_t* bytes);
 /* Stores the rows of k and v [n_rows, n_kv_heads, head_dim] at their positions,
@@ -274,6 +275,11 @@ int mlb_paged_attention(const void* pages_dev, int n_layers, int n_pages, int pa
                         const int* page_table_dev, int max_pages, float scale, void* out_dev,
                         long long out_stride, void* workspace_dev, size_t workspace_bytes,
                         int device_id, void* stream);
+
+/* Waits in the prompt form of mlb_paged_attention are bounded; one that gave up
+ * leaves its rows unwritten. Waits for the device, returns the last such
+ * (MLB_ERR_TIMEOUT, site) since the call before, or (0, 0), and clears it. */
+int mlb_paged_attention_status(int device_id, int* code, int* where);
 
 /* --------------------------------------------------------- prepared weights
  * A weight repacked once into the B200 GEMV layout (what the decode path

@@ -37,6 +37,7 @@ __all__ = [
     "CudaElementwiseAddDeviceInput", "CudaSoftmax", "CudaEmbeddingLookupDeviceWeight",
     "CudaRopeDeviceInput", "CudaArgMax", "CudaLogProbs", "CudaKvCache",
     "CudaAttentionDecodeDeviceInput", "CudaPagedKvCache", "CudaPagedAttentionDeviceInput",
+    "paged_attention_status",
     "QMatrix", "CudaModel", "Context", "Batch", "ForwardToken", "configs", "tp_plan", "nccl_unique_id",
 ]
 
@@ -573,6 +574,15 @@ class CudaPagedKvCache:
             row_offsets.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), max_pages,
             k.data_ptr(), v.data_ptr(), self.device_id, _raw_stream(self.device_id)))
         return k, v
+
+
+def paged_attention_status(device_id=0):
+    """(status code, site) of the last bounded wait that gave up in the prompt
+    form of CudaPagedAttentionDeviceInput since the last call, (0, 0) if none
+    did (mlb_paged_attention_status). Waits for the device."""
+    code, where = ctypes.c_int(0), ctypes.c_int(0)
+    check(lib().mlb_paged_attention_status(device_id, ctypes.byref(code), ctypes.byref(where)))
+    return code.value, where.value
 
 
 def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offsets, seq_lens,

@@ -51,7 +51,8 @@ __device__ __forceinline__ void store_q4(uint8_t* block, bool value, int g, int 
   float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const uint16_t d = synth::float_to_half_ref(__fdiv_rn(amax, 7.0f));
+  // a scale past fp16 stays its largest number: what is stored is always finite
+  const uint16_t d = min((int)synth::float_to_half_ref(__fdiv_rn(amax, 7.0f)), 0x7bff);
   const float sd = synth::half_to_float(d);
   const float inv = sd == 0.0f ? 0.0f : __fdiv_rn(1.0f, sd);
   const float e[4] = {x.x, x.y, x.z, x.w};

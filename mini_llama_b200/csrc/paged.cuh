@@ -122,6 +122,22 @@ inline void paged_check_act(const char* who, int act) {
     invalid(std::string(who) + ": unknown activation type " + std::to_string(act));
 }
 
+// Arguments of the attention kernels.
+struct PagedAttnArgs {
+  PagedCache cache;
+  PagedSeqs seqs;
+  const void* q;
+  void* out;
+  long long q_stride, out_stride;
+  int n_heads, group;
+  float scale_log2;  // scale * log2(e)
+  int4* split;       // decode form, per CTA: {parts, first record, sequence, head}, {tile}
+  float* partial;    // decode form, per CTA: two records of R x (32 G) + 2 R floats
+};
+
+// Prompt form (paged_prompt.cu): many rows per sequence.
+void paged_prompt_launch(const PagedAttnArgs& a, int act_type, int device_id, cudaStream_t stream);
+
 #if defined(__CUDACC__)
 
 // One activation row's four elements from dimension d0 as fp32 (fp32 rows: one
@@ -170,6 +186,162 @@ __device__ __forceinline__ int paged_find_seq(const PagedSeqs& q, int r) {
   }
 }
 
+__device__ __forceinline__ uint32_t hsub2_u(uint32_t x, uint32_t y) {
+  return h2_as_u32(__hsub2(u32_as_h2(x), u32_as_h2(y)));
+}
+
+// Eight 4-bit codes of a word as fp16 pairs (nibble i, nibble i + 4), minus 8.
+// 1024 + q and 1024 + 16 q are exact fp16; the second form saves a shift.
+__device__ __forceinline__ void codes_f16(uint32_t x, uint32_t (&r)[4]) {
+  const uint32_t magic = 0x64006400u, bias = 0x64086408u;  // 1024, 1032
+  const __half2 sixteenth = u32_as_h2(0x2C002C00u), m72 = u32_as_h2(0xD480D480u);
+  const uint32_t y = x >> 8;
+  r[0] = hsub2_u(lop3_and_or(x, 0x000F000Fu, magic), bias);
+  r[1] = h2_as_u32(__hfma2(u32_as_h2(lop3_and_or(x, 0x00F000F0u, magic)), sixteenth, m72));
+  r[2] = hsub2_u(lop3_and_or(y, 0x000F000Fu, magic), bias);
+  r[3] = h2_as_u32(__hfma2(u32_as_h2(lop3_and_or(y, 0x00F000F0u, magic)), sixteenth, m72));
+}
+
+// Two fp32 at a time.
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Words of a query row: 8 dimensions from d0, zeros past head_dim.
+__device__ __forceinline__ void load_q8(const float* p, float (&e)[8]) {
+  const float4 a = load_act4(p), b = load_act4(p + 4);
+  e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
+  e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
+}
+__device__ __forceinline__ void load_q8(const __nv_bfloat16* p, float (&e)[8]) {
+  const float4 a = load_act4(p), b = load_act4(p + 4);
+  e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
+  e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  return h2_as_u32(__floats2half2_rn(lo, hi));
+}
+
+// G consecutive 32-bit words of memory.
+template <int G>
+__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[G]) {
+  if constexpr (G == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else if constexpr (G == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x, w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < G; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+}
+
+// One row's query elements of this lane, scaled by a power of two, as MMA A
+// words: word (w, i) = dims 32 w + 8 c + (i, i + 4). inv receives 2^-shift.
+template <int G, class T>
+__device__ __forceinline__ void load_query(const T* row, int head_dim, int c, bool split,
+                                           uint32_t (&hi)[G][4], uint32_t (&lo)[G][4],
+                                           float& inv) {
+  float e[G][8];
+  float amax = 0.0f;
+#pragma unroll
+  for (int w = 0; w < G; ++w) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[w][i] = 0.0f;
+    const int d0 = 32 * w + 8 * c;
+    if (row && d0 < head_dim) load_q8(row + d0, e[w]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(e[w][i]));
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const int ex = (int)(__float_as_uint(amax) >> 23);
+  // zero rows, subnormal rows and infinities stay as they are
+  const int sh = (ex == 0 || ex == 255) ? 0 : min(max(13 - (ex - 127), -126), 126);
+  const float sf = pow2(sh);
+  inv = pow2(-sh);
+#pragma unroll
+  for (int w = 0; w < G; ++w)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = e[w][i] * sf, y = e[w][i + 4] * sf;
+      hi[w][i] = pack_f16(x, y);
+      lo[w][i] = 0u;
+      if (split) {
+        const float2 h = __half22float2(u32_as_h2(hi[w][i]));
+        lo[w][i] = pack_f16(x - h.x, y - h.y);
+      }
+    }
+}
+
+// What a sequence asks for: its rows in tiles of tile_rows (token, head) rows, its
+// length in chunks of chunk_tokens. Lengths and offsets are cut to what the page
+// table and the call hold.
+struct SeqWork {
+  int len, n, row0, tiles, chunks;
+  long long cost;
+};
+
+__device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s, int tile_rows,
+                                            int chunk_tokens) {
+  SeqWork w;
+  const int cap = a.seqs.max_pages * a.cache.page_size;
+  w.len = min(max(a.seqs.seq_lens[s], 0), cap);
+  w.row0 = max(a.seqs.row_offsets[s], 0);
+  w.n = max(min(a.seqs.row_offsets[s + 1], a.seqs.n_rows) - w.row0, 0);
+  w.tiles = (int)(((long long)w.n * a.group + tile_rows - 1) / tile_rows);
+  w.chunks = max(1, (w.len + chunk_tokens - 1) / chunk_tokens);
+  w.cost = (long long)w.tiles * a.cache.kv * w.chunks;
+  return w;
+}
+
+// Inclusive block-wide scan of one value per thread; warp_sums: one per warp.
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) v += warp_sums[w];
+  __syncthreads();
+  return v;
+}
 #endif  // __CUDACC__
 
 }  // namespace mlb

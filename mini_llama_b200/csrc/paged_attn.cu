@@ -50,185 +50,22 @@ constexpr int kMaxSegs = 32;                  // segments of a run listed at a t
 // CTAs per SM: 128 registers a thread for one 8-row tile, 168 for two.
 __host__ __device__ constexpr int dec_ctas(int nt) { return nt > 1 ? 3 : 4; }
 
-struct DecArgs {
-  PagedCache cache;
-  PagedSeqs seqs;
-  const void* q;
-  void* out;
-  long long q_stride, out_stride;
-  int n_heads, group;
-  float scale_log2;  // scale * log2(e)
-  int4* split;       // per CTA: {parts, first record, row-tile key...} (two int4)
-  float* partial;    // per CTA two records of R x (32 G) + 2 R floats
-};
-
 // Part of a CTA's run: chunks [chunk0, chunk1) of one (sequence, KV head, row tile).
 struct Seg {
   int seq, head, tile, chunk0, chunk1, chunks, len, n, row0, record;
 };
 
-struct SeqWork {
-  int len, n, row0, tiles, chunks;
-  long long cost;
-};
-
-__device__ __forceinline__ SeqWork seq_work(const DecArgs& a, int s, int tile_rows) {
-  SeqWork w;
-  const int cap = a.seqs.max_pages * a.cache.page_size;
-  w.len = min(max(a.seqs.seq_lens[s], 0), cap);
-  w.row0 = max(a.seqs.row_offsets[s], 0);
-  w.n = max(min(a.seqs.row_offsets[s + 1], a.seqs.n_rows) - w.row0, 0);
-  w.tiles = (int)(((long long)w.n * a.group + tile_rows - 1) / tile_rows);
-  w.chunks = max(1, (w.len + kChunkTokens - 1) / kChunkTokens);
-  w.cost = (long long)w.tiles * a.cache.kv * w.chunks;
-  return w;
-}
-
-// Inclusive block-wide scan of one value per thread (kDecThreads threads).
-__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
-  if (lane == 31) warp_sums[warp] = v;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) v += warp_sums[w];
-  __syncthreads();
-  return v;
-}
-
 __device__ __forceinline__ long long run_begin(long long total, int i, int n) {
   return total * i / n;
-}
-
-// G consecutive 32-bit words of shared memory.
-template <int G>
-__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[G]) {
-  if constexpr (G == 4) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-  } else if constexpr (G == 2) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    w[0] = u.x, w[1] = u.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < G; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-  }
-}
-
-__device__ __forceinline__ uint32_t hsub2_u(uint32_t x, uint32_t y) {
-  return h2_as_u32(__hsub2(u32_as_h2(x), u32_as_h2(y)));
-}
-
-// Eight 4-bit codes of a word as fp16 pairs (nibble i, nibble i + 4), minus 8.
-// 1024 + q and 1024 + 16 q are exact fp16; the second form saves a shift.
-__device__ __forceinline__ void codes_f16(uint32_t x, uint32_t (&r)[4]) {
-  const uint32_t magic = 0x64006400u, bias = 0x64086408u;  // 1024, 1032
-  const __half2 sixteenth = u32_as_h2(0x2C002C00u), m72 = u32_as_h2(0xD480D480u);
-  const uint32_t y = x >> 8;
-  r[0] = hsub2_u(lop3_and_or(x, 0x000F000Fu, magic), bias);
-  r[1] = h2_as_u32(__hfma2(u32_as_h2(lop3_and_or(x, 0x00F000F0u, magic)), sixteenth, m72));
-  r[2] = hsub2_u(lop3_and_or(y, 0x000F000Fu, magic), bias);
-  r[3] = h2_as_u32(__hfma2(u32_as_h2(lop3_and_or(y, 0x00F000F0u, magic)), sixteenth, m72));
-}
-
-// Two fp32 at a time.
-__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
-  float2 r;
-  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
-      " mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
-  float2 r;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
-      " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
-  float2 r;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
-      " mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
 }
 
 // F of the largest V scale met so far: 2^F d < 2^14, and 2^F itself within fp16.
 __device__ __forceinline__ int shift_of(uint32_t d_bits) {
   return min(28 - max((int)(d_bits >> 10), 1), 15);
 }
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Words of a query row: 8 dimensions from d0, zeros past head_dim.
-__device__ __forceinline__ void load_q8(const float* p, float (&e)[8]) {
-  const float4 a = load_act4(p), b = load_act4(p + 4);
-  e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
-  e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
-}
-__device__ __forceinline__ void load_q8(const __nv_bfloat16* p, float (&e)[8]) {
-  const float4 a = load_act4(p), b = load_act4(p + 4);
-  e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
-  e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  return h2_as_u32(__floats2half2_rn(lo, hi));
-}
-
-// One row's query elements of this lane, scaled by a power of two, as MMA A
-// words: word (w, i) = dims 32 w + 8 c + (i, i + 4). inv receives 2^-shift.
-template <int G, class T>
-__device__ __forceinline__ void load_query(const T* row, int head_dim, int c, bool split,
-                                           uint32_t (&hi)[G][4], uint32_t (&lo)[G][4],
-                                           float& inv) {
-  float e[G][8];
-  float amax = 0.0f;
-#pragma unroll
-  for (int w = 0; w < G; ++w) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[w][i] = 0.0f;
-    const int d0 = 32 * w + 8 * c;
-    if (row && d0 < head_dim) load_q8(row + d0, e[w]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(e[w][i]));
-  }
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  const int ex = (int)(__float_as_uint(amax) >> 23);
-  // zero rows, subnormal rows and infinities stay as they are
-  const int sh = (ex == 0 || ex == 255) ? 0 : min(max(13 - (ex - 127), -126), 126);
-  const float sf = pow2(sh);
-  inv = pow2(-sh);
-#pragma unroll
-  for (int w = 0; w < G; ++w)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = e[w][i] * sf, y = e[w][i + 4] * sf;
-      hi[w][i] = pack_f16(x, y);
-      lo[w][i] = 0u;
-      if (split) {
-        const float2 h = __half22float2(u32_as_h2(hi[w][i]));
-        lo[w][i] = pack_f16(x - h.x, y - h.y);
-      }
-    }
-}
-
 // NT 8-row tiles per unit. SPLIT: queries and P dV as hi + lo pairs.
 template <int G, int NT, class T>
-__global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_kernel(DecArgs a) {
+__global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_kernel(PagedAttnArgs a) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int R = 8 * NT;
   constexpr int MT = SPLIT ? NT : (NT + 1) / 2;
@@ -251,10 +88,10 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
   long long total = 0;
   for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
     const int s = s0 + threadIdx.x;
-    total += s < a.seqs.n_seqs ? seq_work(a, s, R).cost : 0;
+    total += s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
   }
   {
-    const long long t = block_scan(total, warp_sums);
+    const long long t = block_scan<kDecThreads>(total, warp_sums);
     if (threadIdx.x == kDecThreads - 1) found_base = t;
     __syncthreads();
     total = found_base;
@@ -274,8 +111,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
     long long base = 0;
     for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
       const int s = s0 + threadIdx.x;
-      const long long cost = s < a.seqs.n_seqs ? seq_work(a, s, R).cost : 0;
-      const long long incl = block_scan(cost, warp_sums) + base;
+      const long long cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
+      const long long incl = block_scan<kDecThreads>(cost, warp_sums) + base;
       if (cost > 0 && begin >= incl - cost && begin < incl) {
         found_seq = s;
         found_base = incl - cost;
@@ -289,7 +126,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
   }
   int seq = found_seq;
   long long base = found_base;
-  SeqWork sw = seq_work(a, seq, R);
+  SeqWork sw = seq_work(a, seq, R, kChunkTokens);
   if (threadIdx.x == 0) split[0] = make_int4(0, 0, 0, 0);
 
   uint8_t* ring = smem + warp * (kStages * BLOCK);
@@ -302,7 +139,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
       while (at >= base + sw.cost) {  // next sequence with rows
         base += sw.cost;
         ++seq;
-        sw = seq_work(a, seq, R);
+        sw = seq_work(a, seq, R, kChunkTokens);
       }
       const long long u = (at - base) / sw.chunks;  // unit within the sequence
       const long long unit_begin = base + u * sw.chunks;
@@ -717,7 +554,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
 // of the unit whose second part CTA i holds. The warps take every fourth part,
 // so that up to 32 of them are on their way at a time, and join in order.
 template <int G, int NT, class T>
-__global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(DecArgs a) {
+__global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(PagedAttnArgs a) {
   constexpr int R = 8 * NT;
   constexpr int D = 32 * G;
   constexpr int REC = R * D + 2 * R;
@@ -728,7 +565,7 @@ __global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(DecArgs a)
   if (parts == 0) return;
   const int tile = a.split[2 * blockIdx.x + 1].x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y;
-  const SeqWork sw = seq_work(a, s0.z, R);
+  const SeqWork sw = seq_work(a, s0.z, R, kChunkTokens);
   const long long flat = (long long)tile * R + r;
   if (flat >= (long long)sw.n * a.group) return;
   const float* first = a.partial + ((size_t)(blockIdx.x - 1) * 2 + s0.y) * REC;
@@ -781,6 +618,11 @@ int dec_tiles(int n_rows, int n_seqs, int group) {
 
 int dec_grid(int sms, int nt) { return sms * dec_ctas(nt); }
 
+// The prompt form from 64 rows per sequence and KV head on average.
+bool prompt_form(int n_rows, int n_seqs, int group) {
+  return (long long)n_rows * group >= 64LL * n_seqs;
+}
+
 size_t dec_workspace(int grid, int groups, int nt) {
   const size_t rec = (size_t)8 * nt * 32 * groups + 16 * nt;
   return (size_t)grid * (2 * sizeof(int4) + 2 * rec * sizeof(float));
@@ -799,7 +641,7 @@ void allow_smem(K kernel, size_t bytes, int device_id) {
 }
 
 template <int G, int NT, class T>
-void launch_decode(const DecArgs& a, int grid, int device_id, cudaStream_t stream) {
+void launch_decode(const PagedAttnArgs& a, int grid, int device_id, cudaStream_t stream) {
   constexpr size_t smem = (size_t)kDecWarps * kStages * 576 * G;
   static_assert((8 * 16 * G + 16) * 4 <= 576 * G, "a record of 8 rows and half the dimensions fits a slot");
   allow_smem(paged_attn_decode_kernel<G, NT, T>, smem, device_id);
@@ -810,7 +652,7 @@ void launch_decode(const DecArgs& a, int grid, int device_id, cudaStream_t strea
 }
 
 template <class T>
-void decode_dispatch(const DecArgs& a, int groups, int nt, int grid, int device_id,
+void decode_dispatch(const PagedAttnArgs& a, int groups, int nt, int grid, int device_id,
                      cudaStream_t s) {
   switch (groups * 4 + nt) {
     case 4 + 1: return launch_decode<1, 1, T>(a, grid, device_id, s);
@@ -860,7 +702,7 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
                                    int device_id, void* stream) {
   return guarded([&] {
     const char* who = "CudaPagedAttention";
-    DecArgs a;
+    PagedAttnArgs a;
     a.cache = paged_cache(who, const_cast<void*>(pages), n_layers, n_pages, page_size, n_kv_heads,
                           head_dim, layer);
     a.seqs = paged_seqs(who, n_rows, n_seqs, row_offsets, seq_lens, page_table, max_pages,
@@ -896,6 +738,10 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
         ((long long)max_pages * page_size + kChunkTokens - 1) / kChunkTokens;
     const int grid = (int)std::min<long long>(most, tiles * n_kv_heads * chunks);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (prompt_form(n_rows, n_seqs, a.group)) {
+      paged_prompt_launch(a, act_type, device_id, s);
+      return;
+    }
     if (act_type == MLB_ACT_BF16)
       decode_dispatch<__nv_bfloat16>(a, groups, nt, grid, device_id, s);
     else

@@ -1,0 +1,644 @@
+// paged_prompt.cu — causal attention over the paged Q4_0 KV cache for many rows
+// per sequence, on the tcgen05 tensor cores.
+//
+// A CTA takes a tile of (token, head) rows of one sequence and KV head and goes
+// through the cache 128 tokens at a time:
+//
+//   S = Q K^T (128 x 128, fp32 in tensor memory), P = exp(S - ref) as fp16 over S,
+//   O += P V (fp32 in tensor memory)
+//
+// Here, unlike in the decode form, codes are widened to fp16 with their scales,
+// once for all rows of the tile: K is stored as d q / 16 (the shift keeps any
+// fp16 scale in range), V as d q (or d q / 16 for 16 tokens whose scales reach
+// 4096, with P times 16), each off by at most half an fp16 step (2^-11), P the
+// same. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
+// products that count. ref is the row's maximum as of the last time that it rose
+// by more than 2^4: only then is O brought to the new one.
+//
+// Roles (13 warps, one CTA per SM):
+//   warps 0..3    widen K and V into shared memory (fp32 calls: warps 8..11 too)
+//   warps 4..7    softmax of rows 0..127, one thread per row; epilogue
+//   warps 8..11   bf16 calls: the same for rows 128..255
+//   warp 12       tensor memory; one lane issues the products
+// bf16 calls keep two row tiles going, so that the tensor cores work on one while
+// the softmax of the other runs, with K and V double-buffered. fp32 calls have one
+// row tile and S double-buffered.
+//
+// Every wait is bounded: on a timeout the waiting thread records
+// MLB_ERR_TIMEOUT in the device's status word (mlb_paged_attention_status) and
+// raises the CTA's abort flag; all roles leave their loops, the products in flight
+// are waited for (bounded), tensor memory is released and the CTA exits.
+#include <map>
+#include <mutex>
+#include <utility>
+
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace mlb {
+
+namespace {
+
+constexpr int kTok = 128;  // tokens per step
+constexpr int kThreads = 13 * 32;
+constexpr int kMmaWarp = 12;
+constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
+// P = 2^(s - ref + kLift), and ref follows the row's maximum when that is kRise
+// above it: P up to 2^11, or 2^15 with the 16 of large V scales, and what fp16
+// loses below 2^-14 is 2^-32 of a token at ref.
+constexpr float kLift = 7.0f;
+constexpr float kRise = 4.0f;
+
+__device__ DeviceStatus g_status;
+
+// Shape of one instantiation: bytes of its parts of shared memory.
+template <int G, bool SPLIT>
+struct Plan {
+  static constexpr int D = 32 * G;
+  static constexpr int PT = SPLIT ? 2 : 1;      // hi, lo
+  static constexpr int NX = SPLIT ? 1 : 2;      // row tiles
+  static constexpr int NS = SPLIT ? 1 : 2;      // K and V buffers
+  static constexpr int ND = SPLIT ? 8 : 4;      // widening warps
+  static constexpr int ROWS = 128 * NX;
+  // operands: 8 x 16-byte core matrices, 128 bytes apart along the contraction
+  static constexpr int SBO_D = D / 8 * 128;     // rows of Q and K, contraction D
+  // rows of V^T, contraction tokens; 16 bytes more, so that the widening warps'
+  // 4-byte stores to four row groups fall into different banks
+  static constexpr int SBO_T = kTok / 8 * 128 + 16;
+  static constexpr int Q = 128 / 8 * SBO_D;     // one row tile, one part
+  static constexpr int K = kTok / 8 * SBO_D;
+  static constexpr int V = D / 8 * SBO_T;
+  static constexpr int Q0 = 0;
+  static constexpr int K0 = Q0 + NX * PT * Q;
+  static constexpr int V0 = K0 + NS * PT * K;
+  static constexpr int BYTES = V0 + NS * PT * V;
+  // tensor memory columns
+  static constexpr int O_COL = 0;               // + 128 x
+  static constexpr int S_COL = SPLIT ? 128 : 256;  // + 128 x (bf16), + 128 (step & 1) (fp32)
+  static constexpr int PLO_COL = 384;           // + 64 (step & 1)
+};
+
+struct Shared {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_done[2], drain;
+  long long warp_sums[13];
+  long long base;
+  int seq;
+  int abort_flag;
+  uint32_t tmem;
+  float row_scale[256];
+  // per step & 3, one byte per block: without a page; with large V scales
+  alignas(8) uint8_t absent[4][8];
+  alignas(8) uint8_t big[4][8];
+};
+
+// Bounded wait that also gives up when another thread did.
+__device__ __forceinline__ bool wait(Shared& sh, uint64_t* bar, int phase, int where) {
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, (uint32_t)phase & 1u)) {
+    if (*(volatile int*)&sh.abort_flag) return false;
+    if (clock64() - start > kWaitCycles) {
+      atomicExch(&g_status.code, MLB_ERR_TIMEOUT);
+      atomicExch(&g_status.where, where);
+      *(volatile int*)&sh.abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ uint64_t operand(uint32_t base, int offset, int sbo) {
+  return smem_desc(base + offset, sbo);
+}
+
+template <int G, class T>
+__global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs a) {
+  constexpr bool SPLIT = sizeof(T) == 4;
+  using P = Plan<G, SPLIT>;
+  constexpr int D = P::D, NX = P::NX, NS = P::NS, PT = P::PT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Shared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  // the sequence, KV head and row tile of this CTA; later tiles, which see more,
+  // come first
+  int seq = -1, head = 0, tile = 0;
+  SeqWork sw = {};
+  {
+    long long base = 0;
+    if (threadIdx.x == 0) sh.seq = -1;
+    __syncthreads();
+    for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kThreads) {
+      const int s = s0 + threadIdx.x;
+      long long units = 0;
+      if (s < a.seqs.n_seqs) {
+        const SeqWork w = seq_work(a, s, P::ROWS, kTok);
+        units = (long long)w.tiles * a.cache.kv;
+      }
+      const long long incl = block_scan<kThreads>(units, sh.warp_sums) + base;
+      if (blockIdx.x >= incl - units && blockIdx.x < incl) {
+        sh.seq = s;
+        sh.base = incl - units;
+      }
+      if (threadIdx.x == kThreads - 1) sh.warp_sums[0] = incl;
+      __syncthreads();
+      base = sh.warp_sums[0];
+      __syncthreads();
+      if (base > blockIdx.x) break;
+    }
+    seq = sh.seq;
+    if (seq < 0) return;
+    sw = seq_work(a, seq, P::ROWS, kTok);
+    const int u = (int)(blockIdx.x - sh.base);
+    head = u % a.cache.kv;
+    tile = sw.tiles - 1 - u / a.cache.kv;
+  }
+
+  // steps that each row tile needs: up to what its last row sees
+  const long long rows = (long long)sw.n * a.group, row0 = (long long)tile * P::ROWS;
+  int steps[2] = {0, 0};
+#pragma unroll
+  for (int x = 0; x < NX; ++x) {
+    const long long first = row0 + x * 128;
+    if (first < rows) {
+      const int tok = (int)(min(first + 127, rows - 1) / a.group);
+      steps[x] = (max(sw.len - sw.n + tok + 1, 0) + kTok - 1) / kTok;
+    }
+  }
+  const int n = max(steps[0], steps[1]);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.k_full[i], P::ND);
+      mbar_init(&sh.v_full[i], P::ND);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_done[i], 1);
+    }
+    mbar_init(&sh.drain, 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  // queries as operand tiles, 8 rows per warp and turn
+  {
+    const int g = lane >> 2, c = lane & 3;
+    const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+    for (int r0 = warp * 8; r0 < P::ROWS; r0 += 13 * 8) {
+      const long long flat = row0 + r0 + g;
+      const T* row = nullptr;
+      if (flat < rows) {
+        const int i = (int)(flat / a.group);
+        row = static_cast<const T*>(a.q) + (long long)(sw.row0 + i) * a.q_stride +
+              (size_t)(head * a.group + (int)(flat - (long long)i * a.group)) * a.cache.head_dim;
+      }
+      uint32_t hi[G][4], lo[G][4];
+      float inv;
+      load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
+      if (c == 0) sh.row_scale[r0 + g] = inv * sign * a.scale_log2 * 16.0f;
+      const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
+      uint8_t* at = smem + P::Q0 + (r0 / 128) * PT * P::Q + (r0 % 128) / 8 * P::SBO_D + g * 16;
+#pragma unroll
+      for (int w = 0; w < G; ++w) {
+        *reinterpret_cast<uint4*>(at + (4 * w + c) * 128) = make_uint4(
+            hi[w][0] ^ flip, hi[w][1] ^ flip, hi[w][2] ^ flip, hi[w][3] ^ flip);
+        if (SPLIT)
+          *reinterpret_cast<uint4*>(at + P::Q + (4 * w + c) * 128) = make_uint4(
+              lo[w][0] ^ flip, lo[w][1] ^ flip, lo[w][2] ^ flip, lo[w][3] ^ flip);
+      }
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < 4 || (SPLIT && warp >= 8 && warp < 12)) {
+    // ------------------------------------------------------------- widening
+    const int dw = warp < 4 ? warp : warp - 4;
+    const int g = lane >> 2, c = lane & 3;
+    const int bpp = a.cache.page_size / kPagedBlock;
+    constexpr int BLOCK = 576 * G;
+    constexpr int NB = 8 / P::ND;  // blocks per warp and step
+    const __half2 sixteenth = u32_as_h2(0x2C002C00u);
+    for (int j = 0; j < n; ++j) {
+      const int st = j % NS;
+      // this warp's blocks of the step, as they are in memory
+      uint32_t kw[NB][2][G], ks[NB][2][G], vw[NB][2][G], vs[NB][2][G];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int b = dw * NB + i, bl = j * 8 + b;
+        int page = -1;
+        if (bl * kPagedBlock < sw.len) {
+          const int p = bl / bpp;
+          page = a.seqs.table[(size_t)seq * a.seqs.max_pages + p];
+          if (page >= a.cache.n_pages) page = -1;
+          if (page >= 0) {
+            const uint8_t* block =
+                a.cache.layer +
+                (size_t)((page * a.cache.kv + head) * bpp + (bl - p * bpp)) * BLOCK;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              lds_words<G>(block + (h * 8 + g) * 16 * G + c * 4 * G, kw[i][h]);
+              lds_words<G>(block + (256 + 128 * h) * G + lane * 4 * G, vw[i][h]);
+              lds_words<G>(block + 512 * G + (h * 4 + (g >> 1)) * 4 * G, ks[i][h]);
+              lds_words<G>(block + 544 * G + (h * 4 + c) * 4 * G, vs[i][h]);
+            }
+          }
+        }
+        // scales of tokens that are not there: 0, whatever their codes
+        __half2 dmax = u32_as_h2(0u);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int left = page < 0 ? 0 : sw.len - bl * kPagedBlock - h * 8;
+          const bool kt = g < left, v0 = 2 * c < left, v1 = 2 * c + 1 < left;
+#pragma unroll
+          for (int w = 0; w < G; ++w) {
+            if (page < 0) kw[i][h][w] = vw[i][h][w] = 0u;
+            // K: the scale of token g in both halves, shifted by 2^-4
+            const uint32_t pair = __byte_perm(ks[i][h][w], 0, g & 1 ? 0x3232 : 0x1010);
+            ks[i][h][w] = kt ? h2_as_u32(__hmul2(u32_as_h2(pair), sixteenth)) : 0u;
+            vs[i][h][w] = (v0 ? vs[i][h][w] & 0xffffu : 0u) | (v1 ? vs[i][h][w] & 0xffff0000u : 0u);
+            dmax = __hmax2(dmax, u32_as_h2(vs[i][h][w]));
+          }
+        }
+        const uint32_t db = h2_as_u32(dmax);
+        const bool big = __any_sync(0xffffffffu, max(db & 0xffffu, db >> 16) >= 0x6C00u);
+        if (big) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int w = 0; w < G; ++w)
+              vs[i][h][w] = h2_as_u32(__hmul2(u32_as_h2(vs[i][h][w]), sixteenth));
+        }
+        if (lane == 0) {
+          sh.absent[j & 3][b] = page < 0;
+          sh.big[j & 3][b] = big;
+        }
+      }
+
+      if (j >= NS && !wait(sh, &sh.k_empty[st], j / NS - 1, 1001)) break;
+      uint8_t* k0 = smem + P::K0 + st * PT * P::K;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint8_t* at = k0 + ((dw * NB + i) * 2 + h) * P::SBO_D + c * 128 + g * 16;
+#pragma unroll
+          for (int w = 0; w < G; ++w) {
+            uint32_t r[4], x[4];
+            codes_f16(kw[i][h][w], r);
+            const __half2 d = u32_as_h2(ks[i][h][w]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = h2_as_u32(__hmul2(u32_as_h2(r[e]), d));
+            *reinterpret_cast<uint4*>(at + w * 512) = make_uint4(x[0], x[1], x[2], x[3]);
+            if (SPLIT) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                r[e] = h2_as_u32(__hfma2(u32_as_h2(r[e]), d, __hneg2(u32_as_h2(x[e]))));
+              *reinterpret_cast<uint4*>(at + P::K + w * 512) = make_uint4(r[0], r[1], r[2], r[3]);
+            }
+          }
+        }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.k_full[st]);
+
+      if (j >= NS && !wait(sh, &sh.v_empty[st], j / NS - 1, 1002)) break;
+      uint8_t* v0 = smem + P::V0 + st * PT * P::V;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint8_t* at = v0 + (g >> 1) * P::SBO_T + ((dw * NB + i) * 2 + h) * 128 +
+                        (g & 1) * 64 + 4 * c;
+#pragma unroll
+          for (int w = 0; w < G; ++w) {
+            uint32_t r[4];
+            codes_f16(vw[i][h][w], r);
+            const __half2 d = u32_as_h2(vs[i][h][w]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = h2_as_u32(__hmul2(u32_as_h2(r[e]), d));
+              *reinterpret_cast<uint32_t*>(at + w * 4 * P::SBO_T + e * 16) = x;
+              if (SPLIT)
+                *reinterpret_cast<uint32_t*>(at + P::V + w * 4 * P::SBO_T + e * 16) =
+                    h2_as_u32(__hfma2(u32_as_h2(r[e]), d, __hneg2(u32_as_h2(x))));
+            }
+          }
+        }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.v_full[st]);
+    }
+  } else if (warp < 12) {
+    // -------------------------------------------------------------- softmax
+    const int x = (warp - 4) / 4;
+    const int r = x * 128 + (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_at = tmem + lanes + P::O_COL + 128 * x;
+    const long long flat = row0 + r;
+    const bool live = flat < rows;
+    const int tok = live ? (int)(flat / a.group) : 0;
+    const int vis = live ? max(sw.len - sw.n + tok + 1, 0) : 0;
+    const float rs = sh.row_scale[r];
+    const int nx = steps[x];
+    float ref = -INFINITY;
+    float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
+    bool ok = true;
+    for (int j = 0; ok && j < nx; ++j) {
+      const int b = SPLIT ? j & 1 : x;
+      ok = wait(sh, &sh.s_full[b], SPLIT ? j >> 1 : j, 1003);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_at = tmem + lanes + P::S_COL + 128 * b;
+      const uint64_t absent = *reinterpret_cast<const volatile uint64_t*>(sh.absent[j & 3]);
+      const uint64_t big = *reinterpret_cast<const volatile uint64_t*>(sh.big[j & 3]);
+      const int left = vis - j * kTok;  // tokens of the step that the row sees
+      const bool whole = __all_sync(0xffffffffu, left >= kTok) && absent == 0;
+      // mask of 32 tokens: what the row sees of them
+      auto seen = [&](int ch) {
+        const int v = left - 32 * ch;
+        uint32_t m = v >= 32 ? 0xffffffffu : v <= 0 ? 0u : (1u << v) - 1u;
+        if (absent >> (16 * ch) & 0xff) m &= 0xffff0000u;
+        if (absent >> (16 * ch + 8) & 0xff) m &= 0x0000ffffu;
+        return m;
+      };
+
+      float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+      for (int ch = 0; ch < 4; ++ch) {
+        float v[32];
+        tmem_ld32(s_at + 32 * ch, v);
+        if (!whole) {
+          const uint32_t m = seen(ch);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = m >> i & 1 ? v[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          m0 = fmaxf(m0, v[i]);
+          m1 = fmaxf(m1, v[i + 1]);
+          m2 = fmaxf(m2, v[i + 2]);
+          m3 = fmaxf(m3, v[i + 3]);
+        }
+      }
+      const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      const float mx = top == -INFINITY ? top : top * rs;  // rs >= 0
+      if (ref == -INFINITY) {
+        ref = mx;  // nothing seen before: nothing to bring along
+      }
+      const bool rise = mx > ref + kRise;
+      if (__any_sync(0xffffffffu, rise) && j > 0) {
+        ok = wait(sh, &sh.o_done[x], j - 1, 1004);
+        if (!ok) break;
+        tc_fence_after();
+        const float f = rise ? ex2(ref - mx) : 1.0f;
+        l0 = mul2(l0, make_float2(f, f));
+        l1 = mul2(l1, make_float2(f, f));
+#pragma unroll
+        for (int ch = 0; ch < G; ++ch) {
+          float v[32];
+          tmem_ld32(o_at + 32 * ch, v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t u[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i] * f);
+            tmem_st16(o_at + 32 * ch + 16 * h, u);
+          }
+        }
+        tmem_wait_st();
+      }
+      if (rise) ref = mx;
+      const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
+
+#pragma unroll
+      for (int ch = 0; ch < 4; ++ch) {
+        float v[32];
+        tmem_ld32(s_at + 32 * ch, v);
+        const uint32_t m = whole ? 0xffffffffu : seen(ch);
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float2 p = fma2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(rs, rs),
+                          make_float2(neg, neg));
+          p.x = ex2(p.x);
+          p.y = ex2(p.y);
+          if (!whole) {
+            p.x = m >> (2 * i) & 1 ? p.x : 0.0f;
+            p.y = m >> (2 * i + 1) & 1 ? p.y : 0.0f;
+          }
+          if (i & 1)
+            l1 = add2(l1, p);
+          else
+            l0 = add2(l0, p);
+          if (big != 0 && (big >> (16 * ch + 8 * (i >> 3)) & 0xff))
+            p = mul2(p, make_float2(16.0f, 16.0f));
+          hi[i] = pack_f16(p.x, p.y);
+          if (SPLIT) {
+            const float2 h = __half22float2(u32_as_h2(hi[i]));
+            lo[i] = pack_f16(p.x - h.x, p.y - h.y);
+          }
+        }
+        tmem_st16(s_at + 16 * ch, hi);
+        if (SPLIT) tmem_st16(tmem + lanes + P::PLO_COL + 64 * b + 16 * ch, lo);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[x]);
+    }
+    if (ok && nx > 0) {
+      ok = wait(sh, &sh.o_done[x], nx - 1, 1005);
+      tc_fence_after();
+    }
+    if (ok) {
+      const float l = (l0.x + l0.y) + (l1.x + l1.y);
+      const float f = l == 0.0f ? 0.0f : 1.0f / l;
+      T* out = live ? static_cast<T*>(a.out) + (long long)(sw.row0 + tok) * a.out_stride +
+                          (size_t)(head * a.group + (int)(flat - (long long)tok * a.group)) *
+                              a.cache.head_dim
+                    : nullptr;
+#pragma unroll
+      for (int ch = 0; ch < G; ++ch) {
+        float v[32];
+        if (nx > 0) {
+          tmem_ld32(o_at + 32 * ch, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (32 * ch + i < a.cache.head_dim) {
+              store_act4(out + 32 * ch + i, make_float4(v[i] * f, v[i + 1] * f, v[i + 2] * f,
+                                                        v[i + 3] * f));
+              store_act4(out + 32 * ch + i + 4, make_float4(v[i + 4] * f, v[i + 5] * f,
+                                                            v[i + 6] * f, v[i + 7] * f));
+            }
+        }
+      }
+      tc_fence_before();
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------- products
+    const uint32_t base = smem_addr(smem);
+    const uint32_t id_s = idesc_f16(kTok), id_o = idesc_f16(D);
+    // S of row tile x, step j
+    auto scores = [&](int x, int j) {
+      const uint32_t d = tmem + P::S_COL + 128 * (SPLIT ? j & 1 : x);
+      const int q = P::Q0 + x * PT * P::Q, k = P::K0 + (j % NS) * PT * P::K;
+#pragma unroll
+      for (int part = 0; part < (SPLIT ? 3 : 1); ++part)  // hi hi, lo hi, hi lo
+#pragma unroll
+        for (int s = 0; s < 2 * G; ++s)
+          tc_mma_ss(d, operand(base, q + (part == 1 ? P::Q : 0) + s * 256, P::SBO_D),
+                    operand(base, k + (part == 2 ? P::K : 0) + s * 256, P::SBO_D), id_s,
+                    part > 0 || s > 0);
+    };
+    // O of row tile x += P V of step j
+    auto values = [&](int x, int j) {
+      const uint32_t d = tmem + P::O_COL + 128 * x;
+      const uint32_t hi = tmem + P::S_COL + 128 * (SPLIT ? j & 1 : x);
+      const uint32_t lo = tmem + P::PLO_COL + 64 * (j & 1);
+      const int v = P::V0 + (j % NS) * PT * P::V;
+#pragma unroll
+      for (int part = 0; part < (SPLIT ? 3 : 1); ++part)
+#pragma unroll
+        for (int s = 0; s < kTok / 16; ++s)
+          tc_mma_ts(d, (part == 1 ? lo : hi) + 8 * s,
+                    operand(base, v + (part == 2 ? P::V : 0) + s * 256, P::SBO_T), id_o,
+                    j > 0 || part > 0 || s > 0);
+    };
+    bool ok = n == 0 || wait(sh, &sh.k_full[0], 0, 1006);
+    if (ok && n > 0) {
+      tc_fence_after();
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+        if (steps[x] > 0) {
+          scores(x, 0);
+          tc_commit(&sh.s_full[x]);
+        }
+      tc_commit(&sh.k_empty[0]);
+    }
+    for (int j = 0; ok && j < n; ++j) {
+      const int st = j % NS, st1 = (j + 1) % NS;
+      if (SPLIT) {
+        if (j + 1 < n) {
+          ok = wait(sh, &sh.k_full[st1], (j + 1) / NS, 1007);
+          if (!ok) break;
+          tc_fence_after();
+          scores(0, j + 1);
+          tc_commit(&sh.s_full[(j + 1) & 1]);
+          tc_commit(&sh.k_empty[st1]);
+        }
+        ok = wait(sh, &sh.v_full[st], j / NS, 1008) && wait(sh, &sh.p_full[0], j, 1009);
+        if (!ok) break;
+        tc_fence_after();
+        values(0, j);
+        tc_commit(&sh.o_done[0]);
+        tc_commit(&sh.v_empty[st]);
+      } else {
+        ok = wait(sh, &sh.v_full[st], j / NS, 1008) &&
+             (j + 1 >= n || wait(sh, &sh.k_full[st1], (j + 1) / NS, 1007));
+        if (!ok) break;
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          if (j < steps[x]) {
+            ok = wait(sh, &sh.p_full[x], j, 1009);
+            if (!ok) break;
+            tc_fence_after();
+            values(x, j);
+            tc_commit(&sh.o_done[x]);
+          }
+          if (j + 1 < steps[x]) {
+            tc_fence_after();
+            scores(x, j + 1);  // over P of step j, which the product before it has read
+            tc_commit(&sh.s_full[x]);
+          }
+        }
+        if (!ok) break;
+        tc_commit(&sh.v_empty[st]);
+        if (j + 1 < n) tc_commit(&sh.k_empty[st1]);
+      }
+    }
+    // nothing is in flight when tensor and shared memory go
+    tc_commit(&sh.drain);
+    const long long start = clock64();
+    while (!mbar_try_wait(&sh.drain, 0) && clock64() - start < kWaitCycles) {
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int G, class T>
+void launch(const PagedAttnArgs& a, int device_id, cudaStream_t stream) {
+  using P = Plan<G, sizeof(T) == 4>;
+  static std::mutex mu;
+  static bool seen[64] = {};
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (device_id >= 64 || !seen[device_id]) {
+      MLB_CUDA(cudaFuncSetAttribute(paged_prompt_kernel<G, T>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES));
+      if (device_id < 64) seen[device_id] = true;
+    }
+  }
+  const long long tiles = (long long)a.seqs.n_rows * a.group / P::ROWS + a.seqs.n_seqs;
+  const long long grid = tiles * a.cache.kv;
+  if (grid > 0x7fffffffLL) invalid("CudaPagedAttention: too many rows");
+  paged_prompt_kernel<G, T><<<(unsigned)grid, kThreads, P::BYTES, stream>>>(a);
+  MLB_CUDA(cudaGetLastError());
+}
+
+template <class T>
+void dispatch(const PagedAttnArgs& a, int device_id, cudaStream_t stream) {
+  switch (paged_groups(a.cache.head_dim)) {
+    case 1: return launch<1, T>(a, device_id, stream);
+    case 2: return launch<2, T>(a, device_id, stream);
+    case 3: return launch<3, T>(a, device_id, stream);
+    default: return launch<4, T>(a, device_id, stream);
+  }
+}
+
+}  // namespace
+
+void paged_prompt_launch(const PagedAttnArgs& a, int act_type, int device_id,
+                         cudaStream_t stream) {
+  if (act_type == MLB_ACT_BF16)
+    dispatch<__nv_bfloat16>(a, device_id, stream);
+  else
+    dispatch<float>(a, device_id, stream);
+}
+
+}  // namespace mlb
+
+using namespace mlb;
+
+extern "C" int mlb_paged_attention_status(int device_id, int* code, int* where) {
+  return guarded([&] {
+    if (!code || !where) invalid("CudaPagedAttention: null output");
+    DeviceScope scope(device_id);
+    MLB_CUDA(cudaDeviceSynchronize());
+    DeviceStatus s;
+    MLB_CUDA(cudaMemcpyFromSymbol(&s, g_status, sizeof(s)));
+    const DeviceStatus none = {0, 0};
+    MLB_CUDA(cudaMemcpyToSymbol(g_status, &none, sizeof(none)));
+    *code = s.code;
+    *where = s.where;
+  });
+}

@@ -64,7 +64,12 @@ def attention(q, k, v, length, n, scale, absent=()):
             (top.transpose(0, 1)[..., None], v.abs().amax((0, 2))[None, :, None]))
 
 
-def attention_bound(out, vabs, top, length, dtype):
+def prompt_form(rows, n_seqs, group):
+    """Whether a call takes the prompt form (mlb_paged_attention's rule)."""
+    return rows * group >= 64 * n_seqs
+
+
+def attention_bound(out, vabs, top, length, dtype, prompt=False):
     """Largest error of the kernels. Scores: queries kept to 2^-22 and up to 16
     truncated adds of 2^-23 per product, so at most top * 2^-18 each, doubled by
     numerator and denominator; p: exp 2^-21, P dV kept to 2^-21 (bf16 calls: two
@@ -73,10 +78,20 @@ def attention_bound(out, vabs, top, length, dtype):
     2^F, the smaller of 2^15 and what brings the largest dV to at least 2^13, so
     that is the larger of 2^-40 and 2^-38 of the largest dV for each token, times
     codes up to 8 (the largest |v| is at most 8 dV, and at least 6 of them): per
-    token 2^-37 or 2^-35 / 6 of the largest |v|."""
+    token 2^-37 or 2^-35 / 6 of the largest |v|.
+
+    The prompt form adds: K and V in fp16, 2^-11 of each (fp32 calls: pairs that
+    hold them whole, three products, so 48 adds to a score and three per 16 tokens
+    to a sum), P in fp16, 2^-11, lifted by 2^7, so that what it loses below 2^-14
+    is 2^-32 of the largest |v| per token."""
     top, vmax = top
     floor = length * torch.clamp(vmax * 2.0 ** -35 / 6, min=2.0 ** -37)
     rel = top * 2.0 ** -17 + (16 + length / 32) * 2.0 ** -22
+    if prompt:
+        floor = floor + length * vmax * 2.0 ** -32
+        rel = top * 2.0 ** -16 + (16 + length / 8) * 2.0 ** -22
+        if dtype == torch.bfloat16:
+            rel = rel + (2 * top + 2) * 2.0 ** -11
     if dtype == torch.bfloat16:
         return vabs * (rel + 2.0 ** -10) + floor + out.abs() * 2.0 ** -8
     return vabs * rel + floor + out.abs() * 2.0 ** -24

@@ -17,6 +17,12 @@ from tests import paged_ref as R  # noqa: E402
 ROPE = {"normal": mlb.ROPE_NORMAL, "neox": mlb.ROPE_NEOX}
 
 
+@pytest.fixture(autouse=True)
+def no_timeouts():
+    yield
+    assert mlb.paged_attention_status() == (0, 0)
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
@@ -41,6 +47,7 @@ def filled(seqs, kv, hd, seed, layers=1, layer=0, pool=None):
 def check_attention(out, q, kk, vv, seqs, hd, dtype, scale=None):
     scale = 1 / math.sqrt(hd) if scale is None else scale
     row = at = 0
+    prompt = R.prompt_form(seqs.rows, len(seqs.new), q.shape[1] // kk.shape[1])
     for n, length in zip(seqs.new, seqs.lens):
         if n:
             m = min(n, length)  # rows before position 0 see nothing
@@ -49,7 +56,8 @@ def check_attention(out, q, kk, vv, seqs, hd, dtype, scale=None):
             want, vabs, top = R.attention(q[row + n - m:row + n], kk[at:at + length],
                                           vv[at:at + length], length, m, scale)
             got = out[row + n - m:row + n].double().cpu()
-            err, tol = (got - want).abs(), R.attention_bound(want, vabs, top, length, dtype)
+            err, tol = (got - want).abs(), R.attention_bound(want, vabs, top, length, dtype,
+                                                                      prompt)
             assert torch.isfinite(got).all()
             assert (err <= tol).all(), f"error {err.max():.3e}, worst ratio {(err / tol).max():.2f}"
         row, at = row + n, at + length
@@ -280,7 +288,8 @@ def test_pages_outside_the_pool_are_not_seen(cuda):
                                                 heads, kv, hd)
         want, vabs, top = R.attention(q, kk, vv, length, n, 1 / math.sqrt(hd), absent)
         err = (out.double().cpu() - want).abs()
-        assert (err <= R.attention_bound(want, vabs, top, length, dtype)).all()
+        prompt = R.prompt_form(n, 1, heads // kv)
+        assert (err <= R.attention_bound(want, vabs, top, length, dtype, prompt)).all()
         none = torch.full_like(table, -1)
         out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, seqs.offsets, seqs.seq_lens, none,
                                                 heads, kv, hd)
@@ -403,6 +412,39 @@ def test_offsets_past_32_bits(cuda):
         out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, s.offsets, s.seq_lens, table, heads,
                                                 kv, hd)
         check_attention(out, q, kk, vv, s, hd, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.5])
+@pytest.mark.parametrize("n", [1, 5, 100])
+def test_scale_of_any_sign(cuda, n, scale, dtype):
+    dtype = getattr(torch, dtype)
+    seqs = R.Seqs([n], [333], 16, seed=3)
+    cache, kk, vv = filled(seqs, 2, 64, 17)
+    q = randn(gen(4), n, 8, 64, dtype=dtype)
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, 64, scale=scale)
+    check_attention(out, q, kk, vv, seqs, 64, dtype, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_largest_values(cuda, dtype):
+    """Scales up to fp16's largest, next to ordinary ones."""
+    dtype = getattr(torch, dtype)
+    kv, hd, length = 2, 64, 300
+    g = gen(5)
+    k, v = randn(g, length, kv, hd), randn(g, length, kv, hd)
+    k[100:110] *= 3e4
+    v[40:50] *= 1e5
+    v[200, 0, 3] = 1e9  # past the format: kept at its largest scale
+    for n in (1, 70):
+        seqs = R.Seqs([n], [length], 32, seed=3)
+        cache = mlb.CudaPagedKvCache(1, seqs.n_pages, 32, kv, hd)
+        cache.AppendDevice(0, k, v, *seqs.whole(), rope_type=mlb.ROPE_NONE)
+        kk, vv = cache.ReadDevice(0, *seqs.whole(), length)
+        assert torch.isfinite(vv).all() and vv.max() == 7 * 65504
+        q = randn(g, n, 8, hd, dtype=dtype) * 1e-3
+        out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, kv, hd)
+        check_attention(out, q, kk, vv, seqs, hd, dtype)
 
 
 def test_nothing_to_do(cuda):
