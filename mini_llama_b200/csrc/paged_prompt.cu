@@ -13,7 +13,7 @@
 // 4096, with P times 16), each off by at most half an fp16 step (2^-11), P the
 // same. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
 // products that count. ref is the row's maximum as of the last time that it rose
-// by more than 2^4: only then is O brought to the new one.
+// by more than a constant: only then is O brought to the new one.
 //
 // Roles (13 warps, one CTA per SM):
 //   warps 0..3    widen K and V into shared memory (fp32 calls: warps 8..11 too)
@@ -28,9 +28,8 @@
 // MLB_ERR_TIMEOUT in the device's status word (mlb_paged_attention_status) and
 // raises the CTA's abort flag; all roles leave their loops, the products in flight
 // are waited for (bounded), tensor memory is released and the CTA exits.
-#include <map>
 #include <mutex>
-#include <utility>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -43,11 +42,13 @@ constexpr int kTok = 128;  // tokens per step
 constexpr int kThreads = 13 * 32;
 constexpr int kMmaWarp = 12;
 constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
-// P = 2^(s - ref + kLift), and ref follows the row's maximum when that is kRise
-// above it: P up to 2^11, or 2^15 with the 16 of large V scales, and what fp16
-// loses below 2^-14 is 2^-32 of a token at ref.
-constexpr float kLift = 7.0f;
-constexpr float kRise = 4.0f;
+// P = 2^(s - ref + lift), and ref follows the row's maximum when that is `rise`
+// above it. With P up to 2^11, and 2^15 with the 16 of large V scales, it stays
+// within fp16, and what fp16 loses below 2^-14 is 2^-(25 + lift) of a token at ref.
+// fp32 calls look for the maximum before they make P; bf16 calls make P in the
+// same pass and make it again when a row rises, which is dear, so they let it rise
+// further.
+constexpr float kRise = 4.0f, kRiseLate = 8.0f;
 
 __device__ DeviceStatus g_status;
 
@@ -116,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
   constexpr bool SPLIT = sizeof(T) == 4;
   using P = Plan<G, SPLIT>;
   constexpr int D = P::D, NX = P::NX, NS = P::NS, PT = P::PT;
+  constexpr float kLift = 11.0f - (SPLIT ? kRise : kRiseLate);
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -221,8 +223,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
 
   if (warp < 4 || (SPLIT && warp >= 8 && warp < 12)) {
     // ------------------------------------------------------------- widening
+    // K: token kg, chunk kc, so that eight lanes store 128 bytes in a row; V: row g,
+    // token pair c
     const int dw = warp < 4 ? warp : warp - 4;
-    const int g = lane >> 2, c = lane & 3;
+    const int kg = lane & 7, kc = lane >> 3, g = lane >> 2, c = lane & 3;
     const int bpp = a.cache.page_size / kPagedBlock;
     constexpr int BLOCK = 576 * G;
     constexpr int NB = 8 / P::ND;  // blocks per warp and step
@@ -245,9 +249,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
                 (size_t)((page * a.cache.kv + head) * bpp + (bl - p * bpp)) * BLOCK;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              lds_words<G>(block + (h * 8 + g) * 16 * G + c * 4 * G, kw[i][h]);
+              lds_words<G>(block + (h * 8 + kg) * 16 * G + kc * 4 * G, kw[i][h]);
               lds_words<G>(block + (256 + 128 * h) * G + lane * 4 * G, vw[i][h]);
-              lds_words<G>(block + 512 * G + (h * 4 + (g >> 1)) * 4 * G, ks[i][h]);
+              lds_words<G>(block + 512 * G + (h * 4 + (kg >> 1)) * 4 * G, ks[i][h]);
               lds_words<G>(block + 544 * G + (h * 4 + c) * 4 * G, vs[i][h]);
             }
           }
@@ -257,12 +261,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int left = page < 0 ? 0 : sw.len - bl * kPagedBlock - h * 8;
-          const bool kt = g < left, v0 = 2 * c < left, v1 = 2 * c + 1 < left;
+          const bool kt = kg < left, v0 = 2 * c < left, v1 = 2 * c + 1 < left;
 #pragma unroll
           for (int w = 0; w < G; ++w) {
             if (page < 0) kw[i][h][w] = vw[i][h][w] = 0u;
-            // K: the scale of token g in both halves, shifted by 2^-4
-            const uint32_t pair = __byte_perm(ks[i][h][w], 0, g & 1 ? 0x3232 : 0x1010);
+            // K: the scale of token kg in both halves, shifted by 2^-4
+            const uint32_t pair = __byte_perm(ks[i][h][w], 0, kg & 1 ? 0x3232 : 0x1010);
             ks[i][h][w] = kt ? h2_as_u32(__hmul2(u32_as_h2(pair), sixteenth)) : 0u;
             vs[i][h][w] = (v0 ? vs[i][h][w] & 0xffffu : 0u) | (v1 ? vs[i][h][w] & 0xffff0000u : 0u);
             dmax = __hmax2(dmax, u32_as_h2(vs[i][h][w]));
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint8_t* at = k0 + ((dw * NB + i) * 2 + h) * P::SBO_D + c * 128 + g * 16;
+          uint8_t* at = k0 + ((dw * NB + i) * 2 + h) * P::SBO_D + kc * 128 + kg * 16;
 #pragma unroll
           for (int w = 0; w < G; ++w) {
             uint32_t r[4], x[4];
@@ -371,38 +375,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         return m;
       };
 
-      float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+      // largest score of the step, scaled (rs >= 0)
+      auto step_max = [&]() {
+        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          float v[32];
+          tmem_ld32(s_at + 32 * ch, v);
+          const uint32_t m = whole ? 0xffffffffu : seen(ch);
 #pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        float v[32];
-        tmem_ld32(s_at + 32 * ch, v);
-        if (!whole) {
-          const uint32_t m = seen(ch);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = m >> i & 1 ? v[i] : -INFINITY;
+          for (int i = 0; i < 32; i += 2) {
+            m0 = fmaxf(m0, m >> i & 1 ? v[i] : -INFINITY);
+            m1 = fmaxf(m1, m >> (i + 1) & 1 ? v[i + 1] : -INFINITY);
+          }
         }
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          m0 = fmaxf(m0, v[i]);
-          m1 = fmaxf(m1, v[i + 1]);
-          m2 = fmaxf(m2, v[i + 2]);
-          m3 = fmaxf(m3, v[i + 3]);
-        }
-      }
-      const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-      const float mx = top == -INFINITY ? top : top * rs;  // rs >= 0
-      if (ref == -INFINITY) {
-        ref = mx;  // nothing seen before: nothing to bring along
-      }
-      const bool rise = mx > ref + kRise;
-      if (__any_sync(0xffffffffu, rise) && j > 0) {
-        ok = wait(sh, &sh.o_done[x], j - 1, 1004);
-        if (!ok) break;
+        const float top = fmaxf(m0, m1);
+        return top == -INFINITY ? top : top * rs;
+      };
+      // brings ref of the lanes that rise, their sums and O to mx
+      auto raise_to = [&](float mx, bool rise) {
+        const float f = !rise ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - mx);
+        if (rise) ref = mx;
+        if (j == 0) return true;  // no O yet
+        if (!wait(sh, &sh.o_done[x], j - 1, 1004)) return false;
         tc_fence_after();
-        const float f = rise ? ex2(ref - mx) : 1.0f;
         l0 = mul2(l0, make_float2(f, f));
         l1 = mul2(l1, make_float2(f, f));
-#pragma unroll
+#pragma unroll 1
         for (int ch = 0; ch < G; ++ch) {
           float v[32];
           tmem_ld32(o_at + 32 * ch, v);
@@ -415,40 +414,104 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           }
         }
         tmem_wait_st();
-      }
-      if (rise) ref = mx;
-      const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
+        return true;
+      };
 
+      if constexpr (SPLIT) {
+        // largest score first, then P as it is made
+        const float mx = step_max();
+        const bool rise = mx > ref + kRise;
+        if (__any_sync(0xffffffffu, rise)) ok = raise_to(mx, rise);
+        if (!ok) break;
+        const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          float v[32];
+          tmem_ld32(s_at + 32 * ch, v);
+          const uint32_t m = whole ? 0xffffffffu : seen(ch);
+          uint32_t hi[16], lo[16];
 #pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        float v[32];
-        tmem_ld32(s_at + 32 * ch, v);
-        const uint32_t m = whole ? 0xffffffffu : seen(ch);
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 p = fma2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(rs, rs),
-                          make_float2(neg, neg));
-          p.x = ex2(p.x);
-          p.y = ex2(p.y);
-          if (!whole) {
-            p.x = m >> (2 * i) & 1 ? p.x : 0.0f;
-            p.y = m >> (2 * i + 1) & 1 ? p.y : 0.0f;
-          }
-          if (i & 1)
-            l1 = add2(l1, p);
-          else
-            l0 = add2(l0, p);
-          if (big != 0 && (big >> (16 * ch + 8 * (i >> 3)) & 0xff))
-            p = mul2(p, make_float2(16.0f, 16.0f));
-          hi[i] = pack_f16(p.x, p.y);
-          if (SPLIT) {
+          for (int i = 0; i < 16; ++i) {
+            float2 p = fma2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(rs, rs),
+                            make_float2(neg, neg));
+            p.x = m >> (2 * i) & 1 ? ex2(p.x) : 0.0f;
+            p.y = m >> (2 * i + 1) & 1 ? ex2(p.y) : 0.0f;
+            if (i & 1)
+              l1 = add2(l1, p);
+            else
+              l0 = add2(l0, p);
+            const float up = big >> (16 * ch + 8 * (i >> 3)) & 0xff ? 16.0f : 1.0f;
+            p = mul2(p, make_float2(up, up));
+            hi[i] = pack_f16(p.x, p.y);
             const float2 h = __half22float2(u32_as_h2(hi[i]));
             lo[i] = pack_f16(p.x - h.x, p.y - h.y);
           }
+          tmem_st16(s_at + 16 * ch, hi);
+          tmem_st16(tmem + lanes + P::PLO_COL + 64 * b + 16 * ch, lo);
         }
-        tmem_st16(s_at + 16 * ch, hi);
-        if (SPLIT) tmem_st16(tmem + lanes + P::PLO_COL + 64 * b + 16 * ch, lo);
+      } else {
+        // P of the whole step in registers under the ref of the step before (one
+        // pass over S); again if a row has risen by more than P can hold
+        if (j == 0) raise_to(step_max(), true);
+        uint32_t hi[4][16];
+        while (true) {
+          const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
+          float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+          float top = -INFINITY;
+          auto pass = [&](auto plain_c) {
+            constexpr bool PLAIN = decltype(plain_c)::value;
+            uint32_t u[2][32];
+            tmem_ld32_start(s_at, u[0]);
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+              tmem_ld32_wait(u[ch & 1]);
+              if (ch < 3) tmem_ld32_start(s_at + 32 * (ch + 1), u[(ch + 1) & 1]);
+              const uint32_t m = PLAIN ? 0xffffffffu : seen(ch);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float vx = __uint_as_float(u[ch & 1][2 * i]);
+                float vy = __uint_as_float(u[ch & 1][2 * i + 1]);
+                if (!PLAIN) {
+                  vx = m >> (2 * i) & 1 ? vx : -INFINITY;
+                  vy = m >> (2 * i + 1) & 1 ? vy : -INFINITY;
+                }
+                top = fmaxf(fmaxf(top, vx), vy);
+                float2 p = fma2(make_float2(vx, vy), make_float2(rs, rs), make_float2(neg, neg));
+                p.x = ex2(p.x);
+                p.y = ex2(p.y);
+                if (!PLAIN) {  // -inf times rs = 0
+                  p.x = m >> (2 * i) & 1 ? p.x : 0.0f;
+                  p.y = m >> (2 * i + 1) & 1 ? p.y : 0.0f;
+                }
+                if (i & 1)
+                  s1 = add2(s1, p);
+                else
+                  s0 = add2(s0, p);
+                if (!PLAIN) {
+                  const float up = big >> (16 * ch + 8 * (i >> 3)) & 0xff ? 16.0f : 1.0f;
+                  p = mul2(p, make_float2(up, up));
+                }
+                hi[ch][i] = pack_f16(p.x, p.y);
+              }
+            }
+          };
+          if (whole && big == 0)
+            pass(std::true_type{});
+          else
+            pass(std::false_type{});
+          const float mx = top == -INFINITY ? top : top * rs;
+          const bool rise = mx > ref + kRiseLate;
+          if (!__any_sync(0xffffffffu, rise)) {
+            l0 = add2(l0, s0);
+            l1 = add2(l1, s1);
+            break;
+          }
+          ok = raise_to(mx, rise);
+          if (!ok) break;
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) tmem_st16(s_at + 16 * ch, hi[ch]);
       }
       tmem_wait_st();
       tc_fence_before();

@@ -98,9 +98,9 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t adesc, uint64_t b
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z)
       : "memory");
 }
-// 32 consecutive columns of this thread's lane, and the wait for the load.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t u[32];
+// 32 consecutive columns of this thread's lane, on their way; the wait that they
+// pass through (nothing reads them before it).
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&u)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
       "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
@@ -112,12 +112,18 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
         "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t (&u)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    asm volatile("" : "+r"(u[i])::"memory");  // nothing reads it before the wait
-    v[i] = __uint_as_float(u[i]);
-  }
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(u[i])::"memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t u[32];
+  tmem_ld32_start(taddr, u);
+  tmem_ld32_wait(u);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
 }
 
 #endif  // __CUDACC__

@@ -82,13 +82,13 @@ def attention_bound(out, vabs, top, length, dtype, prompt=False):
 
     The prompt form adds: K and V in fp16, 2^-11 of each (fp32 calls: pairs that
     hold them whole, three products, so 48 adds to a score and three per 16 tokens
-    to a sum), P in fp16, 2^-11, lifted by 2^7, so that what it loses below 2^-14
-    is 2^-32 of the largest |v| per token."""
+    to a sum), P in fp16, 2^-11, lifted by 2^7 (bf16 calls: 2^3), so that what it
+    loses below 2^-14 is 2^-32 (2^-28) of the largest |v| per token."""
     top, vmax = top
     floor = length * torch.clamp(vmax * 2.0 ** -35 / 6, min=2.0 ** -37)
     rel = top * 2.0 ** -17 + (16 + length / 32) * 2.0 ** -22
     if prompt:
-        floor = floor + length * vmax * 2.0 ** -32
+        floor = floor + length * vmax * 2.0 ** (-28 if dtype == torch.bfloat16 else -32)
         rel = top * 2.0 ** -16 + (16 + length / 8) * 2.0 ** -22
         if dtype == torch.bfloat16:
             rel = rel + (2 * top + 2) * 2.0 ** -11
