@@ -81,7 +81,7 @@ struct Plan {
 
 struct Shared {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_done[2], drain;
+  uint64_t s_full[2], p_full[2], o_done[2], o_last[2], drain;
   long long warp_sums[13];
   long long base;
   int seq;
@@ -95,6 +95,7 @@ struct Shared {
 
 // Bounded wait that also gives up when another thread did.
 __device__ __forceinline__ bool wait(Shared& sh, uint64_t* bar, int phase, int where) {
+  if (mbar_try_wait(bar, (uint32_t)phase & 1u)) return true;
   const long long start = clock64();
   while (!mbar_try_wait(bar, (uint32_t)phase & 1u)) {
     if (*(volatile int*)&sh.abort_flag) return false;
@@ -106,10 +107,6 @@ __device__ __forceinline__ bool wait(Shared& sh, uint64_t* bar, int phase, int w
     }
   }
   return true;
-}
-
-__device__ __forceinline__ uint64_t operand(uint32_t base, int offset, int sbo) {
-  return smem_desc(base + offset, sbo);
 }
 
 template <int G, class T>
@@ -178,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 4);
       mbar_init(&sh.o_done[i], 1);
+      mbar_init(&sh.o_last[i], 1);
     }
     mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
@@ -456,42 +454,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         uint32_t hi[4][16];
         while (true) {
           const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
-          float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-          float top = -INFINITY;
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          float top[2] = {-INFINITY, -INFINITY};
           auto pass = [&](auto plain_c) {
             constexpr bool PLAIN = decltype(plain_c)::value;
-            uint32_t u[2][32];
-            tmem_ld32_start(s_at, u[0]);
+            // 64 tokens on their way at a time
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-              tmem_ld32_wait(u[ch & 1]);
-              if (ch < 3) tmem_ld32_start(s_at + 32 * (ch + 1), u[(ch + 1) & 1]);
-              const uint32_t m = PLAIN ? 0xffffffffu : seen(ch);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t u[4][16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float vx = __uint_as_float(u[ch & 1][2 * i]);
-                float vy = __uint_as_float(u[ch & 1][2 * i + 1]);
-                if (!PLAIN) {
-                  vx = m >> (2 * i) & 1 ? vx : -INFINITY;
-                  vy = m >> (2 * i + 1) & 1 ? vy : -INFINITY;
+              for (int ch = 0; ch < 4; ++ch) tmem_ld16_start(s_at + 64 * h + 16 * ch, u[ch]);
+#pragma unroll
+              for (int ch = 0; ch < 4; ++ch) tmem_ld16_wait(u[ch]);
+#pragma unroll
+              for (int ch = 0; ch < 4; ++ch) {
+                const int b = 4 * h + ch;  // block of 16 tokens
+                const uint32_t m = PLAIN ? 0xffffffffu : seen(b >> 1) >> (16 * (b & 1));
+                const float up = !PLAIN && (big >> (8 * b) & 0xff) ? 16.0f : 1.0f;
+                float2 y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  y[i] = make_float2(__uint_as_float(u[ch][2 * i]), __uint_as_float(u[ch][2 * i + 1]));
+                  if (!PLAIN) {
+                    y[i].x = m >> (2 * i) & 1 ? y[i].x : -INFINITY;
+                    y[i].y = m >> (2 * i + 1) & 1 ? y[i].y : -INFINITY;
+                  }
+                  top[i & 1] = fmaxf(fmaxf(top[i & 1], y[i].x), y[i].y);
+                  y[i] = fma2(y[i], make_float2(rs, rs), make_float2(neg, neg));
                 }
-                top = fmaxf(fmaxf(top, vx), vy);
-                float2 p = fma2(make_float2(vx, vy), make_float2(rs, rs), make_float2(neg, neg));
-                p.x = ex2(p.x);
-                p.y = ex2(p.y);
-                if (!PLAIN) {  // -inf times rs = 0
-                  p.x = m >> (2 * i) & 1 ? p.x : 0.0f;
-                  p.y = m >> (2 * i + 1) & 1 ? p.y : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  y[i].x = ex2(y[i].x);
+                  y[i].y = ex2(y[i].y);
                 }
-                if (i & 1)
-                  s1 = add2(s1, p);
-                else
-                  s0 = add2(s0, p);
-                if (!PLAIN) {
-                  const float up = big >> (16 * ch + 8 * (i >> 3)) & 0xff ? 16.0f : 1.0f;
-                  p = mul2(p, make_float2(up, up));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  if (!PLAIN) {  // -inf times rs = 0
+                    y[i].x = m >> (2 * i) & 1 ? y[i].x : 0.0f;
+                    y[i].y = m >> (2 * i + 1) & 1 ? y[i].y : 0.0f;
+                  }
+                  sum[i & 1] = add2(sum[i & 1], y[i]);
+                  if (!PLAIN) y[i] = mul2(y[i], make_float2(up, up));
+                  hi[b >> 1][8 * (b & 1) + i] = pack_f16(y[i].x, y[i].y);
                 }
-                hi[ch][i] = pack_f16(p.x, p.y);
               }
             }
           };
@@ -499,11 +504,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             pass(std::true_type{});
           else
             pass(std::false_type{});
-          const float mx = top == -INFINITY ? top : top * rs;
+          const float t = fmaxf(top[0], top[1]);
+          const float mx = t == -INFINITY ? t : t * rs;
           const bool rise = mx > ref + kRiseLate;
           if (!__any_sync(0xffffffffu, rise)) {
-            l0 = add2(l0, s0);
-            l1 = add2(l1, s1);
+            l0 = add2(l0, sum[0]);
+            l1 = add2(l1, sum[1]);
             break;
           }
           ok = raise_to(mx, rise);
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       if (lane == 0) mbar_arrive(&sh.p_full[x]);
     }
     if (ok && nx > 0) {
-      ok = wait(sh, &sh.o_done[x], nx - 1, 1005);
+      ok = wait(sh, &sh.o_last[x], 0, 1005);
       tc_fence_after();
     }
     if (ok) {
@@ -551,35 +557,47 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       }
       tc_fence_before();
     }
-  } else if (lane == 0) {
+  } else if (warp == kMmaWarp && lane == 0) {
     // ------------------------------------------------------------- products
     const uint32_t base = smem_addr(smem);
     const uint32_t id_s = idesc_f16(kTok), id_o = idesc_f16(D);
+    // operand descriptors: the high words are alike, the low words step by bytes / 16
+    const uint64_t dq = smem_desc(base + P::Q0, P::SBO_D), dv = smem_desc(base + P::V0, P::SBO_T);
+    const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)smem_desc(base + P::K0, P::SBO_D);
+    const uint32_t v_lo = (uint32_t)dv;
+    const uint32_t hi_d = (uint32_t)(dq >> 32), hi_t = (uint32_t)(dv >> 32);
     // S of row tile x, step j
     auto scores = [&](int x, int j) {
       const uint32_t d = tmem + P::S_COL + 128 * (SPLIT ? j & 1 : x);
-      const int q = P::Q0 + x * PT * P::Q, k = P::K0 + (j % NS) * PT * P::K;
+      const uint32_t q = q_lo + x * (PT * P::Q / 16), k = k_lo + (j % NS) * (PT * P::K / 16);
 #pragma unroll
       for (int part = 0; part < (SPLIT ? 3 : 1); ++part)  // hi hi, lo hi, hi lo
 #pragma unroll
-        for (int s = 0; s < 2 * G; ++s)
-          tc_mma_ss(d, operand(base, q + (part == 1 ? P::Q : 0) + s * 256, P::SBO_D),
-                    operand(base, k + (part == 2 ? P::K : 0) + s * 256, P::SBO_D), id_s,
-                    part > 0 || s > 0);
+        for (int s = 0; s < 2 * G; ++s) {
+          const uint32_t aq = q + (part == 1 ? P::Q / 16 : 0) + s * 16;
+          const uint32_t bk = k + (part == 2 ? P::K / 16 : 0) + s * 16;
+          if (part == 0 && s == 0)
+            tc_mma_ss2<false>(d, aq, hi_d, bk, hi_d, id_s);
+          else
+            tc_mma_ss2<true>(d, aq, hi_d, bk, hi_d, id_s);
+        }
     };
     // O of row tile x += P V of step j
     auto values = [&](int x, int j) {
       const uint32_t d = tmem + P::O_COL + 128 * x;
       const uint32_t hi = tmem + P::S_COL + 128 * (SPLIT ? j & 1 : x);
       const uint32_t lo = tmem + P::PLO_COL + 64 * (j & 1);
-      const int v = P::V0 + (j % NS) * PT * P::V;
+      const uint32_t v = v_lo + (j % NS) * (PT * P::V / 16);
+      if (j == 0)
+        tc_mma_ts2<false>(d, hi, v, hi_t, id_o);
+      else
+        tc_mma_ts2<true>(d, hi, v, hi_t, id_o);
 #pragma unroll
       for (int part = 0; part < (SPLIT ? 3 : 1); ++part)
 #pragma unroll
-        for (int s = 0; s < kTok / 16; ++s)
-          tc_mma_ts(d, (part == 1 ? lo : hi) + 8 * s,
-                    operand(base, v + (part == 2 ? P::V : 0) + s * 256, P::SBO_T), id_o,
-                    j > 0 || part > 0 || s > 0);
+        for (int s = part == 0 ? 1 : 0; s < kTok / 16; ++s)
+          tc_mma_ts2<true>(d, (part == 1 ? lo : hi) + 8 * s,
+                           v + (part == 2 ? P::V / 16 : 0) + s * 16, hi_t, id_o);
     };
     bool ok = n == 0 || wait(sh, &sh.k_full[0], 0, 1006);
     if (ok && n > 0) {
@@ -595,8 +613,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     for (int j = 0; ok && j < n; ++j) {
       const int st = j % NS, st1 = (j + 1) % NS;
       if (SPLIT) {
-        if (j + 1 < n) {
-          ok = wait(sh, &sh.k_full[st1], (j + 1) / NS, 1007);
+        if (j + 1 < n) {  // over P of step j - 1: its product has to be done
+          ok = wait(sh, &sh.k_full[st1], (j + 1) / NS, 1007) &&
+               (j == 0 || wait(sh, &sh.o_done[0], j - 1, 1010));
           if (!ok) break;
           tc_fence_after();
           scores(0, j + 1);
@@ -609,6 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         values(0, j);
         tc_commit(&sh.o_done[0]);
         tc_commit(&sh.v_empty[st]);
+        if (j + 1 == n) tc_commit(&sh.o_last[0]);
       } else {
         ok = wait(sh, &sh.v_full[st], j / NS, 1008) &&
              (j + 1 >= n || wait(sh, &sh.k_full[st1], (j + 1) / NS, 1007));
@@ -621,10 +641,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             tc_fence_after();
             values(x, j);
             tc_commit(&sh.o_done[x]);
+            if (j + 1 == steps[x]) tc_commit(&sh.o_last[x]);
           }
           if (j + 1 < steps[x]) {
-            tc_fence_after();
-            scores(x, j + 1);  // over P of step j, which the product before it has read
+            // over P of step j: products of unlike accumulators need not run in the
+            // order of their issue
+            ok = wait(sh, &sh.o_done[x], j, 1010);
+            if (!ok) break;
+            scores(x, j + 1);
             tc_commit(&sh.s_full[x]);
           }
         }

@@ -88,42 +88,55 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// The same with A in shared memory.
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
-  const uint32_t z = 0u;
+// One product with A in shared memory (descriptors) or tensor memory; ACC = false
+// overwrites D. Descriptors as (low, high) words: the low word holds the address
+// in 16-byte units, so that a step along an operand is one addition.
+template <bool ACC>
+__device__ __forceinline__ void tc_mma_ss2(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                           uint32_t b_hi, uint32_t idesc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n"
+      " setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ACC ? 1 : 0)
       : "memory");
 }
-// 32 consecutive columns of this thread's lane, on their way; the wait that they
-// pass through (nothing reads them before it).
-__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&u)[32]) {
+template <bool ACC>
+__device__ __forceinline__ void tc_mma_ts2(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                           uint32_t idesc) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];"
+      "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n"
+      " setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+// 16 consecutive columns of this thread's lane, on their way; the wait that they
+// pass through (nothing reads them before it).
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&u)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
       : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
         "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
-        "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]),
-        "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]),
-        "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        "=r"(u[14]), "=r"(u[15])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld32_wait(uint32_t (&u)[32]) {
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t (&u)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(u[i])::"memory");
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(u[i])::"memory");
 }
+// 32 consecutive columns of this thread's lane, waited for.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t u[32];
-  tmem_ld32_start(taddr, u);
-  tmem_ld32_wait(u);
+  uint32_t u[2][16];
+  tmem_ld16_start(taddr, u[0]);
+  tmem_ld16_start(taddr + 16, u[1]);
+  tmem_ld16_wait(u[0]);
+  tmem_ld16_wait(u[1]);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i >> 4][i & 15]);
 }
 
 #endif  // __CUDACC__
