@@ -63,8 +63,8 @@ struct Plan {
   static constexpr int ROWS = 128 * NX;
   // operands: 8 x 16-byte core matrices, 128 bytes apart along the contraction
   static constexpr int SBO_D = D / 8 * 128;     // rows of Q and K, contraction D
-  // rows of V^T, contraction tokens; 16 bytes more, so that the widening warps'
-  // 4-byte stores to four row groups fall into different banks
+  // rows of V^T, contraction tokens; 16 bytes more, so that the eight rows of a
+  // stored matrix, two of each of four row groups, fall into different banks
   static constexpr int SBO_T = kTok / 8 * 128 + 16;
   static constexpr int Q = 128 / 8 * SBO_D;     // one row tile, one part
   static constexpr int K = kTok / 8 * SBO_D;
@@ -82,7 +82,7 @@ struct Plan {
 struct Shared {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_done[2], o_last[2], drain;
-  long long warp_sums[13];
+  long long warp_sums[kThreads / 32];
   long long base;
   int seq;
   int abort_flag;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
   {
     const int g = lane >> 2, c = lane & 3;
     const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    for (int r0 = warp * 8; r0 < P::ROWS; r0 += 13 * 8) {
+    for (int r0 = warp * 8; r0 < P::ROWS; r0 += kThreads / 32 * 8) {
       const long long flat = row0 + r0 + g;
       const T* row = nullptr;
       if (flat < rows) {
@@ -221,10 +221,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
 
   if (warp < 4 || (SPLIT && warp >= 8 && warp < 12)) {
     // ------------------------------------------------------------- widening
-    // K: token kg, chunk kc, so that eight lanes store 128 bytes in a row; V: row g,
-    // token pair c
+    // K: token kg, chunk kc, so that eight lanes store 128 bytes in a row; V: token
+    // pair c of row lane / 4
     const int dw = warp < 4 ? warp : warp - 4;
-    const int kg = lane & 7, kc = lane >> 3, g = lane >> 2, c = lane & 3;
+    const int kg = lane & 7, kc = lane >> 3, c = lane & 3;
     const int bpp = a.cache.page_size / kPagedBlock;
     constexpr int BLOCK = 576 * G;
     constexpr int NB = 8 / P::ND;  // blocks per warp and step
@@ -254,22 +254,34 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             }
           }
         }
-        // scales of tokens that are not there: 0, whatever their codes
+        // K: the scale of token kg in both halves, shifted by 2^-4
         __half2 dmax = u32_as_h2(0u);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int left = page < 0 ? 0 : sw.len - bl * kPagedBlock - h * 8;
-          const bool kt = kg < left, v0 = 2 * c < left, v1 = 2 * c + 1 < left;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int w = 0; w < G; ++w) {
-            if (page < 0) kw[i][h][w] = vw[i][h][w] = 0u;
-            // K: the scale of token kg in both halves, shifted by 2^-4
-            const uint32_t pair = __byte_perm(ks[i][h][w], 0, kg & 1 ? 0x3232 : 0x1010);
-            ks[i][h][w] = kt ? h2_as_u32(__hmul2(u32_as_h2(pair), sixteenth)) : 0u;
-            vs[i][h][w] = (v0 ? vs[i][h][w] & 0xffffu : 0u) | (v1 ? vs[i][h][w] & 0xffff0000u : 0u);
-            dmax = __hmax2(dmax, u32_as_h2(vs[i][h][w]));
+          for (int w = 0; w < G; ++w)
+            ks[i][h][w] = h2_as_u32(__hmul2(
+                u32_as_h2(__byte_perm(ks[i][h][w], 0, kg & 1 ? 0x3232 : 0x1010)), sixteenth));
+        // scales of tokens that are not there: 0, whatever their codes
+        if (page < 0 || (bl + 1) * kPagedBlock > sw.len) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int left = page < 0 ? 0 : sw.len - bl * kPagedBlock - h * 8;
+            const uint32_t kt = kg < left ? 0xffffffffu : 0u;
+            const uint32_t vt =
+                (2 * c < left ? 0xffffu : 0u) | (2 * c + 1 < left ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int w = 0; w < G; ++w) {
+              if (page < 0) kw[i][h][w] = vw[i][h][w] = ks[i][h][w] = vs[i][h][w] = 0u;
+              ks[i][h][w] &= kt;
+              vs[i][h][w] &= vt;
+            }
           }
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int w = 0; w < G; ++w) dmax = __hmax2(dmax, u32_as_h2(vs[i][h][w]));
         const uint32_t db = h2_as_u32(dmax);
         const bool big = __any_sync(0xffffffffu, max(db & 0xffffu, db >> 16) >= 0x6C00u);
         if (big) {
@@ -318,20 +330,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint8_t* at = v0 + (g >> 1) * P::SBO_T + ((dw * NB + i) * 2 + h) * 128 +
-                        (g & 1) * 64 + 4 * c;
+          // lane 8 e + k: row 4 k + e of a group of 32 dimensions
+          uint8_t* at = v0 + (kg >> 1) * P::SBO_T + ((dw * NB + i) * 2 + h) * 128 +
+                        (4 * (kg & 1) + kc) * 16;
 #pragma unroll
           for (int w = 0; w < G; ++w) {
-            uint32_t r[4];
+            uint32_t r[4], x[4];
             codes_f16(vw[i][h][w], r);
             const __half2 d = u32_as_h2(vs[i][h][w]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x = h2_as_u32(__hmul2(u32_as_h2(r[e]), d));
-              *reinterpret_cast<uint32_t*>(at + w * 4 * P::SBO_T + e * 16) = x;
-              if (SPLIT)
-                *reinterpret_cast<uint32_t*>(at + P::V + w * 4 * P::SBO_T + e * 16) =
-                    h2_as_u32(__hfma2(u32_as_h2(r[e]), d, __hneg2(u32_as_h2(x))));
+            for (int e = 0; e < 4; ++e) x[e] = h2_as_u32(__hmul2(u32_as_h2(r[e]), d));
+            store_matrices(at + w * 4 * P::SBO_T, x);
+            if (SPLIT) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                r[e] = h2_as_u32(__hfma2(u32_as_h2(r[e]), d, __hneg2(u32_as_h2(x[e]))));
+              store_matrices(at + P::V + w * 4 * P::SBO_T, r);
             }
           }
         }
@@ -458,45 +472,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           float top[2] = {-INFINITY, -INFINITY};
           auto pass = [&](auto plain_c) {
             constexpr bool PLAIN = decltype(plain_c)::value;
-            // 64 tokens on their way at a time
+            // 32 tokens on their way while 32 are worked on (products slow the loads
+            // down to about the time that this takes)
+            uint32_t u[2][32];
+            tmem_ld32_start(s_at, u[0]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t u[4][16];
+            for (int ch = 0; ch < 4; ++ch) {
+              tmem_ld32_wait(u[ch & 1]);
+              if (ch < 3) tmem_ld32_start(s_at + 32 * (ch + 1), u[(ch + 1) & 1]);
+              const uint32_t m = PLAIN ? 0xffffffffu : seen(ch);
 #pragma unroll
-              for (int ch = 0; ch < 4; ++ch) tmem_ld16_start(s_at + 64 * h + 16 * ch, u[ch]);
-#pragma unroll
-              for (int ch = 0; ch < 4; ++ch) tmem_ld16_wait(u[ch]);
-#pragma unroll
-              for (int ch = 0; ch < 4; ++ch) {
-                const int b = 4 * h + ch;  // block of 16 tokens
-                const uint32_t m = PLAIN ? 0xffffffffu : seen(b >> 1) >> (16 * (b & 1));
-                const float up = !PLAIN && (big >> (8 * b) & 0xff) ? 16.0f : 1.0f;
-                float2 y[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  y[i] = make_float2(__uint_as_float(u[ch][2 * i]), __uint_as_float(u[ch][2 * i + 1]));
-                  if (!PLAIN) {
-                    y[i].x = m >> (2 * i) & 1 ? y[i].x : -INFINITY;
-                    y[i].y = m >> (2 * i + 1) & 1 ? y[i].y : -INFINITY;
-                  }
-                  top[i & 1] = fmaxf(fmaxf(top[i & 1], y[i].x), y[i].y);
-                  y[i] = fma2(y[i], make_float2(rs, rs), make_float2(neg, neg));
+              for (int i = 0; i < 16; ++i) {
+                float vx = __uint_as_float(u[ch & 1][2 * i]);
+                float vy = __uint_as_float(u[ch & 1][2 * i + 1]);
+                if (!PLAIN) {
+                  vx = m >> (2 * i) & 1 ? vx : -INFINITY;
+                  vy = m >> (2 * i + 1) & 1 ? vy : -INFINITY;
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  y[i].x = ex2(y[i].x);
-                  y[i].y = ex2(y[i].y);
+                top[i & 1] = fmaxf(fmaxf(top[i & 1], vx), vy);
+                float2 p = fma2(make_float2(vx, vy), make_float2(rs, rs), make_float2(neg, neg));
+                p.x = ex2(p.x);
+                p.y = ex2(p.y);
+                if (!PLAIN) {  // -inf times rs = 0
+                  p.x = m >> (2 * i) & 1 ? p.x : 0.0f;
+                  p.y = m >> (2 * i + 1) & 1 ? p.y : 0.0f;
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  if (!PLAIN) {  // -inf times rs = 0
-                    y[i].x = m >> (2 * i) & 1 ? y[i].x : 0.0f;
-                    y[i].y = m >> (2 * i + 1) & 1 ? y[i].y : 0.0f;
-                  }
-                  sum[i & 1] = add2(sum[i & 1], y[i]);
-                  if (!PLAIN) y[i] = mul2(y[i], make_float2(up, up));
-                  hi[b >> 1][8 * (b & 1) + i] = pack_f16(y[i].x, y[i].y);
+                sum[i & 1] = add2(sum[i & 1], p);
+                if (!PLAIN) {
+                  const float up = big >> (16 * ch + 8 * (i >> 3)) & 0xff ? 16.0f : 1.0f;
+                  p = mul2(p, make_float2(up, up));
                 }
+                hi[ch][i] = pack_f16(p.x, p.y);
               }
             }
           };
@@ -630,9 +636,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         tc_commit(&sh.v_empty[st]);
         if (j + 1 == n) tc_commit(&sh.o_last[0]);
       } else {
-        ok = wait(sh, &sh.v_full[st], j / NS, 1008) &&
-             (j + 1 >= n || wait(sh, &sh.k_full[st1], (j + 1) / NS, 1007));
+        ok = wait(sh, &sh.v_full[st], j / NS, 1008);
         if (!ok) break;
+        bool k_seen = false;
 #pragma unroll
         for (int x = 0; x < NX; ++x) {
           if (j < steps[x]) {
@@ -646,8 +652,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           if (j + 1 < steps[x]) {
             // over P of step j: products of unlike accumulators need not run in the
             // order of their issue
-            ok = wait(sh, &sh.o_done[x], j, 1010);
+            ok = (k_seen || wait(sh, &sh.k_full[st1], (j + 1) / NS, 1007)) &&
+                 wait(sh, &sh.o_done[x], j, 1010);
             if (!ok) break;
+            k_seen = true;
+            tc_fence_after();
             scores(x, j + 1);
             tc_commit(&sh.s_full[x]);
           }

@@ -111,32 +111,43 @@ __device__ __forceinline__ void tc_mma_ts2(uint32_t d, uint32_t a, uint32_t b_lo
       "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ACC ? 1 : 0)
       : "memory");
 }
-// 16 consecutive columns of this thread's lane, on their way; the wait that they
-// pass through (nothing reads them before it).
-__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&u)[16]) {
+// Four 8 x 8 matrices of 16-bit elements, m[i] holding two neighbours of row
+// lane / 4 of matrix i, to shared memory; lane 8 i + r gives the address of row r
+// (16 bytes) of matrix i.
+__device__ __forceinline__ void store_matrices(void* row, const uint32_t (&m)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                   smem_addr(row)),
+               "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+               : "memory");
+}
+
+// 32 consecutive columns of this thread's lane, on their way; the wait that they
+// pass through (nothing reads them before it; it is for every load on its way).
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&u)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15}, [%16];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
-        "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
-        "=r"(u[14]), "=r"(u[15])
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, "
+      "%10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+      "%26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
+        "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]),
+        "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]),
+        "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
+        "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]),
+        "=r"(u[30]), "=r"(u[31])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld16_wait(uint32_t (&u)[16]) {
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t (&u)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(u[i])::"memory");
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(u[i])::"memory");
 }
-// 32 consecutive columns of this thread's lane, waited for.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t u[2][16];
-  tmem_ld16_start(taddr, u[0]);
-  tmem_ld16_start(taddr + 16, u[1]);
-  tmem_ld16_wait(u[0]);
-  tmem_ld16_wait(u[1]);
+  uint32_t u[32];
+  tmem_ld32_start(taddr, u);
+  tmem_ld32_wait(u);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i >> 4][i & 15]);
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
 }
 
 #endif  // __CUDACC__
