@@ -12,6 +12,7 @@
 // fp32: at position 1e5 an fp32 angle is off by up to 4e-3 rad, and a value next
 // to a code's border would fall on either side of it. Q4_0 codes then follow the
 // reference quantiser's fp32 steps bit for bit.
+#include <algorithm>
 #include <cmath>
 
 #include "paged.cuh"
@@ -25,7 +26,11 @@ struct RopeRates {
   double rate[kPagedMaxHeadDim / 2];  // theta^(-2j/D)
 };
 
-constexpr int kAppendThreads = 256;
+// Four warps: a prompt's rows bring enough CTAs, and every warp has several heads
+// to load one ahead of the other.
+constexpr int kAppendThreads = 128;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kAppendRows = kAppendWarps;  // rows per CTA at most: one warp looks up each
 
 template <class T>
 struct AppendArgs {
@@ -34,8 +39,29 @@ struct AppendArgs {
   const T *q, *k, *v;
   T* q_out;
   long long q_stride, k_stride, v_stride, q_out_stride;
-  int n_heads, rope_type;
+  int n_heads, rope_type, rows;
 };
+
+// A lane holds 8 consecutive dimensions of a head, so a head takes 4 G lanes and a
+// warp several heads.
+__device__ __forceinline__ int heads_per_warp(int g) { return 32 / (4 * g); }
+
+// The sequence and position of a row, and the page that holds it.
+struct RowPlace {
+  int pos, page, slot;  // pos < 0: of no sequence, or padded; page < 0: not stored
+};
+__device__ __forceinline__ RowPlace place_of(const PagedCache& c, const PagedSeqs& q, int row) {
+  RowPlace r = {-1, -1, 0};
+  const int s = q.n_seqs > 0 ? paged_find_seq(q, row) : -1;
+  if (s < 0 || s >= q.n_seqs) return r;
+  r.pos = q.seq_lens[s] - q.row_offsets[s + 1] + row;
+  if (r.pos < 0) return r;
+  const int logical = r.pos / c.page_size;
+  r.slot = r.pos - logical * c.page_size;
+  if (logical < q.max_pages) r.page = q.table[(size_t)s * q.max_pages + logical];
+  if (r.page >= c.n_pages) r.page = -1;
+  return r;
+}
 
 // Address of the 16-token block of (page, kv head) that holds `slot`.
 __device__ __forceinline__ uint8_t* block_at(const PagedCache& c, int page, int head, int slot) {
@@ -44,166 +70,249 @@ __device__ __forceinline__ uint8_t* block_at(const PagedCache& c, int page, int 
   return c.layer + (((size_t)page * c.kv + head) * bpp + slot / kPagedBlock) * bb;
 }
 
-// One row's four values of this lane -> codes and, in the first lane of each
-// group of 8, the scale.
-__device__ __forceinline__ void store_q4(uint8_t* block, bool value, int g, int tok, int lane,
-                                         const float4& x) {
-  float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  // a scale past fp16 stays its largest number: what is stored is always finite
-  const uint16_t d = min((int)synth::float_to_half_ref(__fdiv_rn(amax, 7.0f)), 0x7bff);
-  const float sd = synth::half_to_float(d);
-  const float inv = sd == 0.0f ? 0.0f : __fdiv_rn(1.0f, sd);
-  const float e[4] = {x.x, x.y, x.z, x.w};
-  uint32_t code = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int q = synth::clampi((int)roundf(__fadd_rn(__fmul_rn(e[i], inv), 8.0f)), 0, 15);
-    code |= (uint32_t)q << (4 * i);
-  }
-  const int w = lane >> 3;
-  if (w >= g) return;
-  uint8_t* at;
-  if (!value) {
-    at = block + (size_t)tok * 16 * g + ((lane & 7) >> 1) * 4 * g + w * 4 + (lane & 1) * 2;
-  } else {
-    at = block + 256 * g + (tok >> 3) * 128 * g + ((lane & 7) * 4 + ((tok & 7) >> 1)) * 4 * g +
-         w * 4 + (tok & 1) * 2;
-  }
-  *reinterpret_cast<uint16_t*>(at) = (uint16_t)code;
-  if ((lane & 7) == 0)
-    *reinterpret_cast<uint16_t*>(block + (value ? 544 : 512) * g + (tok >> 1) * 4 * g + w * 4 +
-                                 (tok & 1) * 2) = d;
+// Byte offsets in a block of what lane li of a head holds for token tok: K's word,
+// the first of V's two half words (the other is 16 G bytes on), the scales.
+__device__ __forceinline__ int k_word(int g, int tok, int li) {
+  return tok * 16 * g + (li & 3) * 4 * g + (li >> 2) * 4;
+}
+__device__ __forceinline__ int v_half(int g, int tok, int li) {
+  return 256 * g + (tok >> 3) * 128 * g + ((li & 3) * 8 + ((tok & 7) >> 1)) * 4 * g +
+         (li >> 2) * 4 + (tok & 1) * 2;
+}
+__device__ __forceinline__ int scale_half(int g, int tok, int li, bool value) {
+  return (value ? 544 : 512) * g + (tok >> 1) * 4 * g + (li >> 2) * 4 + (tok & 1) * 2;
 }
 
-// Rotation of this lane's dimensions 4 lane .. 4 lane + 3 with (cos, sin) pairs cs.
-__device__ __forceinline__ float4 rotate4(const float4& x, int rope_type, int head_dim, int lane,
-                                          const double2* cs) {
+// Eight elements as they are in memory (kept so while they are on their way).
+template <class T>
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void widen(float (&x)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x[4 * i] = __uint_as_float(u[i].x), x[4 * i + 1] = __uint_as_float(u[i].y);
+        x[4 * i + 2] = __uint_as_float(u[i].z), x[4 * i + 3] = __uint_as_float(u[i].w);
+      }
+    } else {
+      const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+};
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
+                                            pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+
+// Rotation of a lane's dimensions 8 li .. 8 li + 7 with (cos, sin) pairs cs; lane0 is
+// the first lane of the head. All lanes of the warp call it.
+__device__ __forceinline__ void rotate8(float (&x)[8], int rope_type, int head_dim, int lane0,
+                                        int li, const double2* cs) {
   if (rope_type == MLB_ROPE_NORMAL) {
-    if (4 * lane >= head_dim) return x;
-    const double2 a = cs[2 * lane], b = cs[2 * lane + 1];
-    const double x0 = x.x, x1 = x.y, x2 = x.z, x3 = x.w;
-    return make_float4((float)(x0 * a.x - x1 * a.y), (float)(x0 * a.y + x1 * a.x),
-                       (float)(x2 * b.x - x3 * b.y), (float)(x2 * b.y + x3 * b.x));
+    if (8 * li >= head_dim) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double2 t = cs[4 * li + i];
+      const double a = x[2 * i], b = x[2 * i + 1];
+      x[2 * i] = (float)(a * t.x - b * t.y);
+      x[2 * i + 1] = (float)(a * t.y + b * t.x);
+    }
+    return;
   }
-  // NeoX: dimension j pairs with j + D/2, D/8 lanes away
-  const int hl = head_dim / 8;
-  const bool first = lane < hl;
-  const int src = first ? lane + hl : lane - hl;
-  float4 o;
-  o.x = __shfl_sync(0xffffffffu, x.x, src);
-  o.y = __shfl_sync(0xffffffffu, x.y, src);
-  o.z = __shfl_sync(0xffffffffu, x.z, src);
-  o.w = __shfl_sync(0xffffffffu, x.w, src);
-  if (4 * lane >= head_dim) return x;
-  const double2* t = cs + 4 * (first ? lane : lane - hl);
-  const double sg = first ? -1.0 : 1.0;
-  return make_float4((float)(x.x * t[0].x + sg * o.x * t[0].y),
-                     (float)(x.y * t[1].x + sg * o.y * t[1].y),
-                     (float)(x.z * t[2].x + sg * o.z * t[2].y),
-                     (float)(x.w * t[3].x + sg * o.w * t[3].y));
+  // NeoX: dimension j pairs with j + D/2, element e of a lane with e, or with e ^ 4
+  // where D/2 is no multiple of 8
+  const int half = head_dim / 2;
+  const bool cross = half % 8 != 0;
+  float o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int d = 8 * li + e;
+    const int from = d < half ? d + half : d - half;
+    o[e] = __shfl_sync(0xffffffffu, cross ? x[e ^ 4] : x[e], lane0 + from / 8);
+  }
+  if (8 * li >= head_dim) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int d = 8 * li + e;
+    const bool first = d < half;
+    const double2 t = cs[first ? d : d - half];
+    const double a = x[e], b = o[e];
+    x[e] = (float)(a * t.x + (first ? -b : b) * t.y);
+  }
 }
 
-// One CTA per row (blockIdx.x) and share of the heads (blockIdx.y); one warp
-// per (row, head), four dimensions per lane.
+// One CTA per a.rows rows (blockIdx.x) and share of the heads (blockIdx.y). The
+// rows' places and rotations are made first, then the warps take (row, heads)
+// turns, two of them on their way ahead of the one at work.
 template <class T>
 __global__ void __launch_bounds__(kAppendThreads)
     paged_append_kernel(AppendArgs<T> a, RopeRates rates) {
-  __shared__ double2 cs[kPagedMaxHeadDim / 2];
+  __shared__ double2 cs[kAppendRows][kPagedMaxHeadDim / 2];
+  __shared__ RowPlace places[kAppendRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x;
-  const int D = a.cache.head_dim;
-  const int s = paged_find_seq(a.seqs, row);
-  if (s < 0 || s >= a.seqs.n_seqs) return;
-  const int pos = a.seqs.seq_lens[s] - a.seqs.row_offsets[s + 1] + row;
-  if (pos < 0) return;
+  const int row0 = blockIdx.x * a.rows, n_rows = min(a.rows, a.seqs.n_rows - row0);
+  const int D = a.cache.head_dim, g = paged_groups(D);
+  const int H = a.n_heads, KV = a.cache.kv, heads = H + 2 * KV;
+  const int hpw = heads_per_warp(g), hw = lane / (4 * g), li = lane - hw * 4 * g;
+  const bool on = hw < hpw && 8 * li < D;
+  const int turns = (heads + hpw - 1) / hpw, total = turns * n_rows;
+  const int step = gridDim.y * kAppendWarps;
+  int it = blockIdx.y * kAppendWarps + warp;
+  auto load = [&](int i, Raw8<T>& x) {
+    const int r = i / turns, h = (i - r * turns) * hpw + hw;
+    x.clear();
+    if (!on || i >= total || h >= heads) return;
+    const long long row = row0 + r;
+    const T* p = h < H        ? a.q + row * a.q_stride + (size_t)h * D
+                 : h < H + KV ? a.k + row * a.k_stride + (size_t)(h - H) * D
+                              : a.v + row * a.v_stride + (size_t)(h - H - KV) * D;
+    x.load(p + 8 * li);
+  };
+  Raw8<T> raw[2];
+  load(it, raw[0]);
+  load(it + step, raw[1]);
+
+  if (warp < n_rows) {
+    const RowPlace p = place_of(a.cache, a.seqs, row0 + warp);
+    if (lane == 0) places[warp] = p;
+  }
+  __syncthreads();
   if (a.rope_type != MLB_ROPE_NONE) {
-    for (int j = threadIdx.x; j < D / 2; j += kAppendThreads) {
+    for (int j = threadIdx.x; j < n_rows * (D / 2); j += kAppendThreads) {
+      const int r = j / (D / 2), i = j - r * (D / 2);
       double sn, c;
-      sincos((double)pos * rates.rate[j], &sn, &c);
-      cs[j] = make_double2(c, sn);
+      sincos((double)max(places[r].pos, 0) * rates.rate[i], &sn, &c);
+      cs[r][i] = make_double2(c, sn);
     }
     __syncthreads();
   }
-  const int logical = pos / a.cache.page_size;
-  const int slot = pos - logical * a.cache.page_size;
-  int page = -1;
-  if (logical < a.seqs.max_pages) page = a.seqs.table[(size_t)s * a.seqs.max_pages + logical];
-  const bool stored = page >= 0 && page < a.cache.n_pages;
-  const int g = paged_groups(D), tok = slot % kPagedBlock;
-  const int KV = a.cache.kv, heads = a.n_heads + 2 * KV;
-  const bool on = 4 * lane < D;
-  const int nw = kAppendThreads / 32;
-  for (int h = blockIdx.y * nw + warp; h < heads; h += gridDim.y * nw) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (h < a.n_heads) {
-      if (on) x = load_act4(a.q + row * a.q_stride + (size_t)h * D + 4 * lane);
-      if (a.rope_type != MLB_ROPE_NONE) x = rotate4(x, a.rope_type, D, lane, cs);
-      if (on) store_act4(a.q_out + row * a.q_out_stride + (size_t)h * D + 4 * lane, x);
-      continue;
+  for (; it < total; it += step) {
+    const int r = it / turns, h0 = (it - r * turns) * hpw, h = h0 + hw;
+    const long long row = row0 + r;
+    const RowPlace at = places[r];
+    float x[8];
+    raw[0].widen(x);
+    raw[0] = raw[1];
+    load(it + 2 * step, raw[1]);
+    if (at.pos < 0) continue;
+    const int tok = at.slot % kPagedBlock;
+    if (a.rope_type != MLB_ROPE_NONE && h0 < H + KV) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i];
+      rotate8(y, a.rope_type, D, hw * 4 * g, li, cs[r]);
+      if (h < H + KV) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i];
+      }
     }
-    if (!stored) continue;
-    const bool value = h >= a.n_heads + KV;
-    const int kh = h - a.n_heads - (value ? KV : 0);
-    if (on)
-      x = load_act4((value ? a.v + row * a.v_stride : a.k + row * a.k_stride) + (size_t)kh * D +
-                    4 * lane);
-    if (!value && a.rope_type != MLB_ROPE_NONE) x = rotate4(x, a.rope_type, D, lane, cs);
-    store_q4(block_at(a.cache, page, kh, slot), value, g, tok, lane, x);
+    if (h < H && on) store8(a.q_out + row * a.q_out_stride + (size_t)h * D + 8 * li, x);
+    if (h0 + hpw <= H || at.page < 0) continue;
+
+    // Q4_0 of the lane's quarter of a block of 32
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // a scale past fp16 stays its largest number: what is stored is always finite
+    const uint16_t d = min((int)synth::float_to_half_ref(__fdiv_rn(amax, 7.0f)), 0x7bff);
+    const float sd = synth::half_to_float(d);
+    const float inv = sd == 0.0f ? 0.0f : __fdiv_rn(1.0f, sd);
+    uint32_t code = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // round(v) of v = x / d + 8 with halves up, as floor(v + 1/2): 1.5 * 2^22 + 1/2 + v
+      // rounded down to a half leaves twice that in the low bits (v >= 0.99 unless the
+      // scale was cut, and then v below 0 counts as 0)
+      const float v = fminf(fmaxf(__fadd_rn(__fmul_rn(x[i], inv), 8.0f), 0.0f), 15.0f);
+      code |= (__float_as_uint(__fadd_rd(v, 6291456.5f)) >> 1 & 15u) << (4 * i);
+    }
+    if (h < H || h >= heads || hw >= hpw) continue;
+    const bool value = h >= H + KV;
+    uint8_t* block = block_at(a.cache, at.page, h - H - (value ? KV : 0), at.slot);
+    if (value) {
+      uint8_t* p = block + v_half(g, tok, li);
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)code;
+      *reinterpret_cast<uint16_t*>(p + 16 * g) = (uint16_t)(code >> 16);
+    } else {
+      *reinterpret_cast<uint32_t*>(block + k_word(g, tok, li)) = code;
+    }
+    if ((li & 3) == 0)
+      *reinterpret_cast<uint16_t*>(block + scale_half(g, tok, li, value)) = d;
   }
 }
 
 // Rows read back as the fp32 values their codes stand for; rows that are not
-// stored are zeros.
+// stored are zeros. One CTA per `rows` rows and share of the heads, as above.
 __global__ void __launch_bounds__(kAppendThreads)
-    paged_read_kernel(PagedCache c, PagedSeqs seqs, float* k_out, float* v_out) {
+    paged_read_kernel(PagedCache c, PagedSeqs seqs, int rows, float* k_out, float* v_out) {
+  __shared__ RowPlace places[kAppendRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x;
-  const int D = c.head_dim;
-  const int s = seqs.n_seqs > 0 ? paged_find_seq(seqs, row) : -1;
-  int page = -1, slot = 0;
-  if (s >= 0 && s < seqs.n_seqs) {
-    const int pos = seqs.seq_lens[s] - seqs.row_offsets[s + 1] + row;
-    const int logical = pos / c.page_size;
-    slot = pos - logical * c.page_size;
-    if (pos >= 0 && logical < seqs.max_pages)
-      page = seqs.table[(size_t)s * seqs.max_pages + logical];
+  const int row0 = blockIdx.x * rows, n_rows = min(rows, seqs.n_rows - row0);
+  const int D = c.head_dim, g = paged_groups(D);
+  const int hpw = heads_per_warp(g), hw = lane / (4 * g), li = lane - hw * 4 * g;
+  if (warp < n_rows) {
+    const RowPlace p = place_of(c, seqs, row0 + warp);
+    if (lane == 0) places[warp] = p;
   }
-  const bool stored = page >= 0 && page < c.n_pages;
-  const int g = paged_groups(D), tok = slot % kPagedBlock, w = lane >> 3;
-  const int nw = kAppendThreads / 32;
-  if (4 * lane >= D) return;
-  for (int h = blockIdx.y * nw + warp; h < 2 * c.kv; h += gridDim.y * nw) {
+  __syncthreads();
+  if (hw >= hpw || 8 * li >= D) return;
+  const int turns = (2 * c.kv + hpw - 1) / hpw, total = turns * n_rows;
+#pragma unroll 4
+  for (int it = blockIdx.y * kAppendWarps + warp; it < total; it += gridDim.y * kAppendWarps) {
+    const int r = it / turns, h = (it - r * turns) * hpw + hw;
+    if (h >= 2 * c.kv) continue;
+    const RowPlace at = places[r];
     const bool value = h >= c.kv;
-    const int kh = value ? h - c.kv : h;
-    float* out = (value ? v_out : k_out) + ((size_t)row * c.kv + kh) * D + 4 * lane;
-    if (!stored) {
-      store_act4(out, make_float4(0.f, 0.f, 0.f, 0.f));
-      continue;
+    const int kh = value ? h - c.kv : h, tok = at.slot % kPagedBlock;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+    if (at.pos >= 0 && at.page >= 0) {
+      const uint8_t* block = block_at(c, at.page, kh, at.slot);
+      uint32_t code;
+      if (value) {
+        const uint8_t* p = block + v_half(g, tok, li);
+        code = *reinterpret_cast<const uint16_t*>(p) |
+               (uint32_t) * reinterpret_cast<const uint16_t*>(p + 16 * g) << 16;
+      } else {
+        code = *reinterpret_cast<const uint32_t*>(block + k_word(g, tok, li));
+      }
+      const float d = __half2float(
+          *reinterpret_cast<const __half*>(block + scale_half(g, tok, li, value)));
+      // 2^23 + q as a float has q in its low bits
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = (__uint_as_float(0x4b000000u | (code >> (4 * i) & 15u)) - 8388616.0f) * d;
     }
-    const uint8_t* block = block_at(c, page, kh, slot);
-    const uint8_t* at =
-        value ? block + 256 * g + (tok >> 3) * 128 * g +
-                    ((lane & 7) * 4 + ((tok & 7) >> 1)) * 4 * g + w * 4 + (tok & 1) * 2
-              : block + (size_t)tok * 16 * g + ((lane & 7) >> 1) * 4 * g + w * 4 + (lane & 1) * 2;
-    const uint32_t code = *reinterpret_cast<const uint16_t*>(at);
-    const float d = __half2float(*reinterpret_cast<const __half*>(
-        block + (value ? 544 : 512) * g + (tok >> 1) * 4 * g + w * 4 + (tok & 1) * 2));
-    float4 x;
-    x.x = (float)((int)(code & 15) - 8) * d;
-    x.y = (float)((int)(code >> 4 & 15) - 8) * d;
-    x.z = (float)((int)(code >> 8 & 15) - 8) * d;
-    x.w = (float)((int)(code >> 12 & 15) - 8) * d;
-    store_act4(out, x);
+    store8((value ? v_out : k_out) + ((size_t)(row0 + r) * c.kv + kh) * D + 8 * li, x);
   }
 }
 
-// CTAs per row: one while the rows alone fill the GPU, more (down to one head
-// per warp) when they do not, so that a single token's heads run side by side.
-int head_shares(int rows, int heads, int sms) {
-  const int most = (heads + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-  return std::max(1, std::min(most, 4 * sms / std::max(rows, 1)));
+// CTAs per row: one while the rows alone fill the GPU, more (down to one turn per
+// warp) when they do not, so that a single token's heads run side by side.
+int head_shares(int rows, int heads, int head_dim, int sms) {
+  const int turn = kAppendWarps * (32 / (4 * paged_groups(head_dim)));
+  const int most = (heads + turn - 1) / turn;
+  return std::max(1, std::min(most, 8 * sms / std::max(rows, 1)));
 }
 
 template <class T>
@@ -228,8 +337,12 @@ void launch_append(const PagedCache& c, const PagedSeqs& s, const void* k, long 
   if (rope_type != MLB_ROPE_NONE)
     for (int j = 0; j < c.head_dim / 2; ++j)
       r.rate[j] = std::pow((double)theta, -2.0 * j / c.head_dim);
-  const int shares = head_shares(s.n_rows, n_heads + 2 * c.kv, sm_count(device_id));
-  paged_append_kernel<T><<<dim3(s.n_rows, shares), kAppendThreads, 0, stream>>>(a, r);
+  // several rows per CTA once that leaves every SM several CTAs
+  const int sms = sm_count(device_id);
+  a.rows = s.n_rows >= kAppendRows * 8 * sms ? kAppendRows : 1;
+  const int shares = head_shares(s.n_rows, n_heads + 2 * c.kv, c.head_dim, sms);
+  paged_append_kernel<T><<<dim3((s.n_rows + a.rows - 1) / a.rows, shares), kAppendThreads, 0,
+                           stream>>>(a, r);
   MLB_CUDA(cudaGetLastError());
 }
 
@@ -302,9 +415,11 @@ extern "C" int mlb_paged_kv_read(const void* pages, int n_layers, int n_pages, i
     }
     DeviceScope scope(device_id);
     if (n_rows == 0) return;
-    const int shares = head_shares(n_rows, 2 * n_kv_heads, sm_count(device_id));
-    paged_read_kernel<<<dim3(n_rows, shares), kAppendThreads, 0,
-                        static_cast<cudaStream_t>(stream)>>>(c, s, k_out, v_out);
+    const int sms = sm_count(device_id);
+    const int rows = n_rows >= kAppendRows * 8 * sms ? kAppendRows : 1;
+    const int shares = head_shares(n_rows, 2 * n_kv_heads, head_dim, sms);
+    paged_read_kernel<<<dim3((n_rows + rows - 1) / rows, shares), kAppendThreads, 0,
+                        static_cast<cudaStream_t>(stream)>>>(c, s, rows, k_out, v_out);
     MLB_CUDA(cudaGetLastError());
   });
 }
