@@ -12,13 +12,13 @@
 // -inf have probability 0.
 //
 // The k largest (ties: lower index first): 64-bit keys order value, then index.
-// Every thread knows the largest key of its own elements from the pass; the
-// k-th largest of those is a lower bound for the k-th largest of all, and every
-// key at or above it lies with the at most k threads whose own largest is at or
-// above it. So the row is not filtered while it streams: those few threads'
-// elements are looked at again and the survivors sorted. Rows that leave more
-// survivors than the buffer holds (long runs of repeated logits) are searched
-// key by key instead.
+// Every thread knows the largest key of its own elements from the pass. The k-th
+// largest of the largest keys of 32 groups of threads is a lower bound for the
+// k-th largest of all, and every key at or above it lies with a thread whose own
+// largest is. So the row is not filtered while it streams: those few threads'
+// elements are looked at again and the survivors (about k to 3 k) sorted. Rows that
+// leave more survivors than the buffer holds (long runs of repeated logits) are
+// searched key by key instead.
 //
 // A row is one CTA, or a cluster of up to 8 when there are too few rows to fill
 // the GPU; a cluster's CTAs take one slice each and rank 0 joins their sums and
@@ -47,12 +47,6 @@ struct LogprobArgs {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Sum of a set of elements: L, T relative to its largest element m.
 struct Sums {
   float m, l, t;
@@ -66,11 +60,26 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   r.m = fmaxf(a.m, b.m);
   const float da = a.m == r.m ? 0.0f : (a.m - r.m) * kLog2e;
   const float db = b.m == r.m ? 0.0f : (b.m - r.m) * kLog2e;
-  const float fa = exp2_approx(da), fb = exp2_approx(db);
+  const float fa = ex2(da), fb = ex2(db);
   r.l = fmaf(fa, a.l, fb * b.l);
   // a weight of 0 leaves nothing, whatever d is
   r.t = (fa == 0.0f ? 0.0f : fa * fmaf(da, a.l, a.t)) + (fb == 0.0f ? 0.0f : fb * fmaf(db, b.l, b.t));
   return r;
+}
+
+// The sums of N lanes (a power of two, from lane 0 on), in every one of them.
+template <int N>
+__device__ __forceinline__ Sums warp_join(Sums s) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) {
+    Sums u;
+    u.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+    u.l = __shfl_xor_sync(0xffffffffu, s.l, o);
+    u.t = __shfl_xor_sync(0xffffffffu, s.t, o);
+    s = lane & o ? join(u, s) : join(s, u);
+  }
+  return s;
 }
 
 // Keys: larger value first, then lower index. 0 is below every element's key.
@@ -106,6 +115,13 @@ __device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b_reversed) 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) k = exchange(k, o, (lane & o) == 0);
   return k;
+}
+
+// The largest of a warp's keys.
+__device__ __forceinline__ uint64_t warp_top(uint64_t k, uint32_t lanes = 0xffffffffu) {
+  const uint32_t hi = __reduce_max_sync(lanes, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(lanes, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (uint64_t)hi << 32 | lo;
 }
 
 // The 32 largest of one key per thread, descending, in lists[0..31]. Every
@@ -176,7 +192,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
   __shared__ uint64_t survivors[kMaxSurvivors];
   __shared__ Sums warp_sums[WARPS];
   __shared__ Sums slice_sums;
-  __shared__ int winners[kMaxTop];
+  __shared__ uint64_t groups[32];
+  __shared__ int winners[THREADS];
   __shared__ int n_winners, n_survivors;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -200,12 +217,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
   const uint4* vx = reinterpret_cast<const uint4*>(x + head_all) + v0;
   const int nv = v1 - v0, first = head_all + v0 * VEC;
 
+  // the given token's logit, on its way from the start
+  float chosen = __uint_as_float(0x7fc00000u);
+  if (rank == 0 && threadIdx.x == 0) {
+    const int t = a.tokens[row];
+    if (t >= 0 && t < a.vocab) chosen = to_f(x[t]);
+  }
+
   Sums s = {-INFINITY, 0.0f, 0.0f};
   float ref = 0.0f;  // s.m, or 0 while that is -inf
+  float2 l2 = make_float2(0.f, 0.f), t2 = l2;  // the vectors' sums, even and odd elements
   int at = -1;
   auto raise = [&](float top, int index) {
+    s.l += l2.x + l2.y;
+    s.t += t2.x + t2.y;
+    l2 = t2 = make_float2(0.f, 0.f);
     if (s.l != 0.0f) {
-      const float d = (s.m - top) * kLog2e, f = exp2_approx(d);
+      const float d = (s.m - top) * kLog2e, f = ex2(d);
       s.t = f == 0.0f ? 0.0f : f * fmaf(d, s.l, s.t);
       s.l *= f;
     }
@@ -214,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
     at = index;
   };
   auto add_one = [&](float e) {
-    const float y = (e - ref) * kLog2e, p = exp2_approx(y);
+    const float y = (e - ref) * kLog2e, p = ex2(y);
     s.l += p;
     s.t = fmaf(p, fmaxf(y, -1000.0f), s.t);
   };
@@ -235,7 +263,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
       raise(mx, first + v * VEC + i0);
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) add_one(e[i]);
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 y = mul2(add2(make_float2(e[i], e[i + 1]), make_float2(-ref, -ref)),
+                            make_float2(kLog2e, kLog2e));
+      const float2 p = make_float2(ex2(y.x), ex2(y.y));
+      l2 = add2(l2, p);
+      t2 = fma2(p, make_float2(fmaxf(y.x, -1000.0f), fmaxf(y.y, -1000.0f)), t2);
+    }
   };
 
   for (int j = threadIdx.x; j < singles_head; j += THREADS) add(to_f(x[j]), j);
@@ -255,15 +289,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
   }
 
   // sums of the slice
+  s.l += l2.x + l2.y;
+  s.t += t2.x + t2.y;
   const float best = s.m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums u;
-    u.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    u.l = __shfl_xor_sync(0xffffffffu, s.l, o);
-    u.t = __shfl_xor_sync(0xffffffffu, s.t, o);
-    s = lane & o ? join(u, s) : join(s, u);
-  }
+  s = warp_join<32>(s);
   if (lane == 0) warp_sums[warp] = s;
   if (threadIdx.x == 0) n_winners = n_survivors = 0;
 
@@ -273,15 +302,21 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
   if (k == 0) {
     __syncthreads();
   } else {
-    block_top32<WARPS>(own, lists);
+    // 32 groups of threads, each its largest
+    constexpr int GROUP = THREADS / 32;
+    static_assert(GROUP == 8 || GROUP == 16, "groups are parts of a warp");
+    const uint32_t part = ((1u << GROUP) - 1u) << (lane / GROUP * GROUP);
+    const uint64_t most = warp_top(own, part);
+    if (lane % GROUP == 0) groups[threadIdx.x / GROUP] = most;
+    __syncthreads();
+    const uint64_t mine = groups[lane];
     if (k == 1) {
-      top = lists[lane];
+      const uint64_t first_key = warp_top(mine);
+      top = lane == 0 ? first_key : 0;
     } else {
-      const uint64_t bound = lists[k - 1];  // 0: fewer threads than k hold elements
-      __syncthreads();
-      if (own != 0 && own >= bound) {
-        if (bound != 0) winners[atomicAdd(&n_winners, 1)] = threadIdx.x;
-      }
+      const uint64_t bound = __shfl_sync(0xffffffffu, warp_sort(mine), k - 1);  // 0: few elements
+      if (own != 0 && own >= bound && bound != 0)
+        winners[atomicAdd(&n_winners, 1)] = threadIdx.x;
       __syncthreads();
       auto push = [&](float e, int index) {
         if (!(e == e)) return;
@@ -308,7 +343,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
       }
       __syncthreads();
       const int n = n_survivors;
-      if (n <= kMaxSurvivors) {
+      if (n <= 4 * 32) {
+        if (warp == 0)
+          for (int j = 0; j < n; j += 32) {
+            const uint64_t sorted = warp_sort(j + lane < n ? survivors[j + lane] : 0);
+            top = j == 0 ? sorted
+                         : warp_merge(top, __shfl_sync(0xffffffffu, sorted, 31 - lane));
+          }
+      } else if (n <= kMaxSurvivors) {
         for (int j = 0; j < n; j += THREADS) {
           block_top32<WARPS>(j + threadIdx.x < n ? survivors[j + threadIdx.x] : 0, lists);
           if (warp == 0) top = j == 0 ? lists[lane] : warp_merge(top, lists[31 - lane]);
@@ -342,39 +384,37 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
     }
   }
 
-  if (threadIdx.x == 0) {
-    s = warp_sums[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) s = join(s, warp_sums[w]);
-    if (SLICES > 1) slice_sums = s;
+  if (warp == 0) {
+    s = warp_join<WARPS>(warp_sums[lane % WARPS]);
+    if (SLICES > 1 && lane == 0) slice_sums = s;
   }
   if (SLICES > 1) {
     __syncthreads();
     if (warp == 0) lists[lane] = top;
     cluster_sync();
     if (rank == 0 && warp == 0) {
-      for (int r = 1; r < SLICES; ++r) {
-        Sums u;
-        const uint32_t p = peer_addr(&slice_sums, r);
-        u.m = peer_f32(p);
-        u.l = peer_f32(p + 4);
-        u.t = peer_f32(p + 8);
-        s = join(s, u);
-        if (k > 0) top = warp_merge(top, peer_u64(peer_addr(lists + 31 - lane, r)));
-      }
+      // lane r joins slice r's sums; the lists come all at once
+      uint64_t peer[SLICES];
+#pragma unroll
+      for (int r = 1; r < SLICES; ++r)
+        peer[r] = k > 0 ? peer_u64(peer_addr(lists + 31 - lane, r)) : 0;
+      const uint32_t p = peer_addr(&slice_sums, lane % SLICES);
+      s.m = peer_f32(p);
+      s.l = peer_f32(p + 4);
+      s.t = peer_f32(p + 8);
+      s = warp_join<SLICES>(s);
+      if (k > 0)
+#pragma unroll
+        for (int r = 1; r < SLICES; ++r) top = warp_merge(top, peer[r]);
     }
     cluster_sync();  // a CTA's shared memory lives until rank 0 has read it
     if (rank != 0) return;
   }
   if (warp != 0) return;
-  s.m = __shfl_sync(0xffffffffu, s.m, 0);
-  s.l = __shfl_sync(0xffffffffu, s.l, 0);
-  s.t = __shfl_sync(0xffffffffu, s.t, 0);
   const float ln_l = logf(s.l);
   const float nan = __uint_as_float(0x7fc00000u);
   if (lane == 0) {
-    const int t = a.tokens[row];
-    a.logprob[row] = t >= 0 && t < a.vocab ? to_f(x[t]) - s.m - ln_l : nan;
+    a.logprob[row] = chosen - s.m - ln_l;
     a.entropy[row] = ln_l - kLn2 * (s.t / s.l);
   }
   if (lane < k) {
@@ -384,9 +424,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
   }
 }
 
-template <class T, int SLICES>
+template <class T, int THREADS, int SLICES>
 void launch(const LogprobArgs& a, cudaStream_t stream) {
-  constexpr int THREADS = 512;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * SLICES);
   cfg.blockDim = dim3(THREADS);
@@ -403,11 +442,14 @@ void launch(const LogprobArgs& a, cudaStream_t stream) {
 template <class T>
 void dispatch(const LogprobArgs& a, int slices, cudaStream_t s) {
   switch (slices) {
-    case 8: return launch<T, 8>(a, s);
-    case 4: return launch<T, 4>(a, s);
-    case 2: return launch<T, 2>(a, s);
-    default: return launch<T, 1>(a, s);
+    case 8: return launch<T, 512, 8>(a, s);
+    case 4: return launch<T, 512, 4>(a, s);
+    case 2: return launch<T, 512, 2>(a, s);
+    default: break;
   }
+  // many rows: 256 threads have twice the elements each against the same work at
+  // the end
+  return launch<T, 256, 1>(a, s);
 }
 
 }  // namespace

@@ -52,8 +52,12 @@ struct RowPlace {
 };
 __device__ __forceinline__ RowPlace place_of(const PagedCache& c, const PagedSeqs& q, int row) {
   RowPlace r = {-1, -1, 0};
-  const int s = q.n_seqs > 0 ? paged_find_seq(q, row) : -1;
-  if (s < 0 || s >= q.n_seqs) return r;
+  // while decoding, row s is sequence s: one look instead of a search
+  int s = row;
+  if (row >= q.n_seqs || q.row_offsets[row] != row || q.row_offsets[row + 1] != row + 1) {
+    s = q.n_seqs > 0 ? paged_find_seq(q, row) : -1;
+    if (s < 0 || s >= q.n_seqs) return r;
+  }
   r.pos = q.seq_lens[s] - q.row_offsets[s + 1] + row;
   if (r.pos < 0) return r;
   const int logical = r.pos / c.page_size;
@@ -158,9 +162,42 @@ __device__ __forceinline__ void rotate8(float (&x)[8], int rope_type, int head_d
   }
 }
 
+// Q4_0 of a lane's quarter of a block of 32: its eight codes and the block's scale
+// (fp16 bits). The reference quantiser's fp32 steps; its fp16 rounds halves up, which
+// for normal numbers is one addition.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& scale) {
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const float want = __fdiv_rn(amax, 7.0f);
+  float sd;
+  if (want >= 6.103515625e-05f) {  // 2^-14
+    // a scale past fp16 stays its largest number: what is stored is always finite
+    const uint32_t u = min((__float_as_uint(want) + 0x1000u) >> 13, 0x7bffu + (112u << 10));
+    scale = u - (112u << 10);
+    sd = __uint_as_float(u << 13);
+  } else {
+    scale = synth::float_to_half_ref(want);
+    sd = synth::half_to_float((uint16_t)scale);
+  }
+  const float inv = sd == 0.0f ? 0.0f : __frcp_rn(sd);
+  uint32_t code = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // round(v) of v = x / d + 8 with halves up, as floor(v + 1/2): 1.5 * 2^22 + 1/2 + v
+    // rounded down to a half leaves twice that in the low bits (v >= 0.99 unless the
+    // scale was cut, and then v below 0 counts as 0)
+    const float v = fminf(fmaxf(__fadd_rn(__fmul_rn(x[i], inv), 8.0f), 0.0f), 15.0f);
+    code |= (__float_as_uint(__fadd_rd(v, 6291456.5f)) >> 1 & 15u) << (4 * i);
+  }
+  return code;
+}
+
 // One CTA per a.rows rows (blockIdx.x) and share of the heads (blockIdx.y). The
-// rows' places and rotations are made first, then the warps take (row, heads)
-// turns, two of them on their way ahead of the one at work.
+// rows' places and rotations are made first, then the warps take turns of some heads
+// of q, k or v each, two of them on their way ahead of the one at work.
 template <class T>
 __global__ void __launch_bounds__(kAppendThreads)
     paged_append_kernel(AppendArgs<T> a, RopeRates rates) {
@@ -169,25 +206,31 @@ __global__ void __launch_bounds__(kAppendThreads)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row0 = blockIdx.x * a.rows, n_rows = min(a.rows, a.seqs.n_rows - row0);
   const int D = a.cache.head_dim, g = paged_groups(D);
-  const int H = a.n_heads, KV = a.cache.kv, heads = H + 2 * KV;
+  const int H = a.n_heads, KV = a.cache.kv;
   const int hpw = heads_per_warp(g), hw = lane / (4 * g), li = lane - hw * 4 * g;
   const bool on = hw < hpw && 8 * li < D;
-  const int turns = (heads + hpw - 1) / hpw, total = turns * n_rows;
-  const int step = gridDim.y * kAppendWarps;
-  int it = blockIdx.y * kAppendWarps + warp;
-  auto load = [&](int i, Raw8<T>& x) {
-    const int r = i / turns, h = (i - r * turns) * hpw + hw;
+  // a row's turns: q's, then k's, then v's
+  const int tq = (H + hpw - 1) / hpw, tk = (KV + hpw - 1) / hpw, turns = tq + 2 * tk;
+  const int step = gridDim.y * kAppendWarps, mine = hw * D + 8 * li, turn = hpw * D;
+  int lr = 0, lt = blockIdx.y * kAppendWarps + warp;  // next turn to load
+  auto load = [&](Raw8<T>& x) {
+    while (lt >= turns) {
+      lt -= turns;
+      ++lr;
+    }
     x.clear();
-    if (!on || i >= total || h >= heads) return;
-    const long long row = row0 + r;
-    const T* p = h < H        ? a.q + row * a.q_stride + (size_t)h * D
-                 : h < H + KV ? a.k + row * a.k_stride + (size_t)(h - H) * D
-                              : a.v + row * a.v_stride + (size_t)(h - H - KV) * D;
-    x.load(p + 8 * li);
+    if (lr < n_rows) {
+      const bool is_q = lt < tq, is_v = lt >= tq + tk;
+      const int t = is_q ? lt : is_v ? lt - tq - tk : lt - tq;
+      const T* p = (is_q ? a.q : is_v ? a.v : a.k) +
+                   (long long)(row0 + lr) * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride);
+      if (on && t * hpw + hw < (is_q ? H : KV)) x.load(p + t * turn + mine);
+    }
+    lt += step;
   };
   Raw8<T> raw[2];
-  load(it, raw[0]);
-  load(it + step, raw[1]);
+  load(raw[0]);
+  load(raw[1]);
 
   if (warp < n_rows) {
     const RowPlace p = place_of(a.cache, a.seqs, row0 + warp);
@@ -203,51 +246,32 @@ __global__ void __launch_bounds__(kAppendThreads)
     }
     __syncthreads();
   }
-  for (; it < total; it += step) {
-    const int r = it / turns, h0 = (it - r * turns) * hpw, h = h0 + hw;
-    const long long row = row0 + r;
-    const RowPlace at = places[r];
+  for (int r = 0, t = blockIdx.y * kAppendWarps + warp;; t += step) {
+    while (t >= turns) {
+      t -= turns;
+      ++r;
+    }
+    if (r >= n_rows) break;
     float x[8];
     raw[0].widen(x);
     raw[0] = raw[1];
-    load(it + 2 * step, raw[1]);
+    load(raw[1]);
+    const RowPlace at = places[r];
     if (at.pos < 0) continue;
-    const int tok = at.slot % kPagedBlock;
-    if (a.rope_type != MLB_ROPE_NONE && h0 < H + KV) {
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[i];
-      rotate8(y, a.rope_type, D, hw * 4 * g, li, cs[r]);
-      if (h < H + KV) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i];
-      }
+    if (t < tq + tk && a.rope_type != MLB_ROPE_NONE)
+      rotate8(x, a.rope_type, D, hw * 4 * g, li, cs[r]);
+    if (t < tq) {
+      if (on && t * hpw + hw < H)
+        store8(a.q_out + (long long)(row0 + r) * a.q_out_stride + t * turn + mine, x);
+      continue;
     }
-    if (h < H && on) store8(a.q_out + row * a.q_out_stride + (size_t)h * D + 8 * li, x);
-    if (h0 + hpw <= H || at.page < 0) continue;
-
-    // Q4_0 of the lane's quarter of a block of 32
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // a scale past fp16 stays its largest number: what is stored is always finite
-    const uint16_t d = min((int)synth::float_to_half_ref(__fdiv_rn(amax, 7.0f)), 0x7bff);
-    const float sd = synth::half_to_float(d);
-    const float inv = sd == 0.0f ? 0.0f : __fdiv_rn(1.0f, sd);
-    uint32_t code = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // round(v) of v = x / d + 8 with halves up, as floor(v + 1/2): 1.5 * 2^22 + 1/2 + v
-      // rounded down to a half leaves twice that in the low bits (v >= 0.99 unless the
-      // scale was cut, and then v below 0 counts as 0)
-      const float v = fminf(fmaxf(__fadd_rn(__fmul_rn(x[i], inv), 8.0f), 0.0f), 15.0f);
-      code |= (__float_as_uint(__fadd_rd(v, 6291456.5f)) >> 1 & 15u) << (4 * i);
-    }
-    if (h < H || h >= heads || hw >= hpw) continue;
-    const bool value = h >= H + KV;
-    uint8_t* block = block_at(a.cache, at.page, h - H - (value ? KV : 0), at.slot);
+    if (at.page < 0) continue;
+    uint32_t scale;
+    const uint32_t code = quantise8(x, scale);
+    const bool value = t >= tq + tk;
+    const int kh = (t - tq - (value ? tk : 0)) * hpw + hw, tok = at.slot % kPagedBlock;
+    if (kh >= KV || hw >= hpw) continue;
+    uint8_t* block = block_at(a.cache, at.page, kh, at.slot);
     if (value) {
       uint8_t* p = block + v_half(g, tok, li);
       *reinterpret_cast<uint16_t*>(p) = (uint16_t)code;
@@ -256,7 +280,7 @@ __global__ void __launch_bounds__(kAppendThreads)
       *reinterpret_cast<uint32_t*>(block + k_word(g, tok, li)) = code;
     }
     if ((li & 3) == 0)
-      *reinterpret_cast<uint16_t*>(block + scale_half(g, tok, li, value)) = d;
+      *reinterpret_cast<uint16_t*>(block + scale_half(g, tok, li, value)) = (uint16_t)scale;
   }
 }
 
