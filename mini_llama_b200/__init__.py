@@ -246,8 +246,11 @@ def _on_stream(call, device, stream):
         return call()
 
 
-def _raw_stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+def _raw_stream(index):
+    """torch's current stream on a device, without the 2 us of a Stream object."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
 
 
 def _act_type(who, t):
@@ -305,7 +308,7 @@ def CudaLogProbs(logits, tokens, top_k=0, stream=None):
     top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
     check(lib().mlb_logprobs(act, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), top_k,
                              logprob.data_ptr(), entropy.data_ptr(), ids.data_ptr(),
-                             top.data_ptr(), index, _raw_stream(dev)))
+                             top.data_ptr(), index, _raw_stream(index)))
     return logprob, entropy, ids, top
 
 

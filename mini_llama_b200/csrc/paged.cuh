@@ -131,7 +131,7 @@ struct PagedAttnArgs {
   long long q_stride, out_stride;
   int n_heads, group;
   float scale_log2;  // scale * log2(e)
-  int4* split;       // decode form, per CTA: {parts, first record, sequence, head}, {tile}
+  int4* split;       // decode form, per CTA: {parts, first record, head, tile}, {row0, rows}
   float* partial;    // decode form, per CTA: two records of R x (32 G) + 2 R floats
 };
 

@@ -84,19 +84,20 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
   const int g = lane >> 2, c = lane & 3;
   const int cta = blockIdx.x;
 
-  // total work and this CTA's run
-  long long total = 0;
+  // total work, this CTA's run, and the sequence that holds its begin (one look at
+  // the sequences where a block has a thread for each)
+  const bool few = a.seqs.n_seqs <= kDecThreads;
+  long long total = 0, cost = 0, incl = 0;
   for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
     const int s = s0 + threadIdx.x;
-    total += s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
+    cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
+    total += cost;
   }
-  {
-    const long long t = block_scan<kDecThreads>(total, warp_sums);
-    if (threadIdx.x == kDecThreads - 1) found_base = t;
-    __syncthreads();
-    total = found_base;
-    __syncthreads();
-  }
+  incl = block_scan<kDecThreads>(total, warp_sums);
+  if (threadIdx.x == kDecThreads - 1) found_base = incl;
+  __syncthreads();
+  total = found_base;
+  __syncthreads();
   const int nrun = (int)min((long long)gridDim.x, total);
   int4* split = a.split + 2 * cta;
   if (cta >= nrun) {
@@ -105,14 +106,18 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
   }
   const long long begin = run_begin(total, cta, nrun), end = run_begin(total, cta + 1, nrun);
   const long long prev = cta > 0 ? run_begin(total, cta - 1, nrun) : 0;
-
-  // the sequence that holds `begin`
-  {
+  if (few) {
+    if (cost > 0 && begin >= incl - cost && begin < incl) {
+      found_seq = threadIdx.x;
+      found_base = incl - cost;
+    }
+    __syncthreads();
+  } else {
     long long base = 0;
     for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
       const int s = s0 + threadIdx.x;
-      const long long cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
-      const long long incl = block_scan<kDecThreads>(cost, warp_sums) + base;
+      cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
+      incl = block_scan<kDecThreads>(cost, warp_sums) + base;
       if (cost > 0 && begin >= incl - cost && begin < incl) {
         found_seq = s;
         found_base = incl - cost;
@@ -161,8 +166,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
           // the last part is with the last run that begins before the unit ends
           const long long unit_end = unit_begin + sw.chunks;
           const int last = (int)((unit_end * nrun + total - 1) / total) - 1;
-          split[0] = make_int4(last - cta + 2, prev == unit_begin ? 0 : 1, seq, sg.head);
-          split[1] = make_int4(sg.tile, 0, 0, 0);
+          split[0] = make_int4(last - cta + 2, prev == unit_begin ? 0 : 1, sg.head, sg.tile);
+          split[1] = make_int4(sw.row0, sw.n, 0, 0);
         }
       }
       ++n_segs;
@@ -552,57 +557,79 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
 
 // Joins the parts of units that were cut between CTAs: block (i, y) joins row y
 // of the unit whose second part CTA i holds. The warps take every fourth part,
-// so that up to 32 of them are on their way at a time, and join in order.
+// so that up to 24 of them are on their way at a time; the order is fixed.
 template <int G, int NT, class T>
-__global__ void __launch_bounds__(kDecThreads) paged_attn_join_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kDecThreads, 8) paged_attn_join_kernel(PagedAttnArgs a) {
   constexpr int R = 8 * NT;
   constexpr int D = 32 * G;
   constexpr int REC = R * D + 2 * R;
-  __shared__ float xs[kDecWarps][D], sums[kDecWarps];
+  __shared__ float xs[kDecWarps][D], sums[kDecWarps], tops[kDecWarps];
   pdl_wait();
-  const int4 s0 = a.split[2 * blockIdx.x];
-  const int parts = s0.x;
+  const int4 s0 = a.split[2 * blockIdx.x], s1 = a.split[2 * blockIdx.x + 1];
+  const int parts = s0.x, head = s0.z, tile = s0.w, row0 = s1.x, n = s1.y;
   if (parts == 0) return;
-  const int tile = a.split[2 * blockIdx.x + 1].x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y;
-  const SeqWork sw = seq_work(a, s0.z, R, kChunkTokens);
   const long long flat = (long long)tile * R + r;
-  if (flat >= (long long)sw.n * a.group) return;
+  if (flat >= (long long)n * a.group) return;
   const float* first = a.partial + ((size_t)(blockIdx.x - 1) * 2 + s0.y) * REC;
   const float* rest = a.partial + (size_t)blockIdx.x * 2 * REC;  // part p >= 1: + 2 (p - 1) REC
   auto rec = [&](int p) { return p == 0 ? first : rest + (size_t)(p - 1) * 2 * REC; };
-  float mx = -INFINITY;
-  for (int p = lane; p < parts; p += 32) mx = fmaxf(mx, rec(p)[R * D + r]);
-  mx = warp_max(mx);
-  float sum = 0.0f, x[G];
+  // this warp's parts, six at a time (eight cost the registers of resident CTAs), each batch under the largest maximum so far
+  float mx = -INFINITY, sum = 0.0f, x[G];
 #pragma unroll
   for (int w = 0; w < G; ++w) x[w] = 0.0f;
-#pragma unroll 8
-  for (int p = warp; p < parts; p += kDecWarps) {
-    const float* q = rec(p);
-    const float mp = q[R * D + r];
-    const float f = mp == mx ? 1.0f : ex2(mp - mx);
-    sum = fmaf(f, q[R * D + R + r], sum);
+  for (int p0 = warp; p0 < parts; p0 += 6 * kDecWarps) {
+    float m[6], l[6], y[6][G];
 #pragma unroll
-    for (int w = 0; w < G; ++w) x[w] = fmaf(f, q[r * D + 32 * w + lane], x[w]);
+    for (int i = 0; i < 6; ++i) {
+      const int p = p0 + i * kDecWarps;
+      const float* q = rec(min(p, parts - 1));
+      m[i] = p < parts ? q[R * D + r] : -INFINITY;
+      l[i] = p < parts ? q[R * D + R + r] : 0.0f;
+#pragma unroll
+      for (int w = 0; w < G; ++w) y[i][w] = q[r * D + 32 * w + lane];
+    }
+    float top = mx;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) top = fmaxf(top, m[i]);
+    const float f0 = mx == top ? 1.0f : ex2(mx - top);
+    mx = top;
+    sum *= f0;
+#pragma unroll
+    for (int w = 0; w < G; ++w) x[w] *= f0;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      if (p0 + i * kDecWarps >= parts) continue;
+      const float f = m[i] == mx ? 1.0f : ex2(m[i] - mx);
+      sum = fmaf(f, l[i], sum);
+#pragma unroll
+      for (int w = 0; w < G; ++w) x[w] = fmaf(f, y[i][w], x[w]);
+    }
   }
 #pragma unroll
   for (int w = 0; w < G; ++w) xs[warp][32 * w + lane] = x[w];
-  if (lane == 0) sums[warp] = sum;
+  if (lane == 0) {
+    sums[warp] = sum;
+    tops[warp] = mx;
+  }
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= a.cache.head_dim) return;
   sum = 0.0f;
+  mx = -INFINITY;
   float y = 0.0f;
 #pragma unroll
+  for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, tops[w]);
+#pragma unroll
   for (int w = 0; w < kDecWarps; ++w) {
-    sum += sums[w];
-    y += xs[w][d];
+    const float f = tops[w] == mx ? 1.0f : ex2(tops[w] - mx);
+    sum = fmaf(f, sums[w], sum);
+    y = fmaf(f, xs[w][d], y);
   }
   y *= sum == 0.0f ? 0.0f : 1.0f / sum;
   const int tk = (int)(flat / a.group);
-  const int hq = s0.w * a.group + (int)(flat - (long long)tk * a.group);
-  T* out = static_cast<T*>(a.out) + (long long)(sw.row0 + tk) * a.out_stride +
+  const int hq = head * a.group + (int)(flat - (long long)tk * a.group);
+  T* out = static_cast<T*>(a.out) + (long long)(row0 + tk) * a.out_stride +
            (size_t)hq * a.cache.head_dim;
   if constexpr (sizeof(T) == 4)
     out[d] = y;
@@ -618,9 +645,22 @@ int dec_tiles(int n_rows, int n_seqs, int group) {
 
 int dec_grid(int sms, int nt) { return sms * dec_ctas(nt); }
 
-// The prompt form from 64 rows per sequence and KV head on average.
-bool prompt_form(int n_rows, int n_seqs, int group) {
-  return (long long)n_rows * group >= 64LL * n_seqs;
+// Whether a call takes the prompt form. Both forms' times grow with the length, so
+// what decides is the time per 64 tokens, from the average rows per sequence and KV
+// head: the decode form spreads row tiles of 16 over 3 CTAs per SM, 1.5 us each
+// (fp32: 2.05), the prompt form runs waves of one CTA per SM, 1.65 us for up to 256
+// rows (fp32: 2.1 for 128). Measured, decode / prompt us, bf16: 16 sequences of 4096
+// with 8 KV heads, 32 rows 72 / 90, 128 rows 225 / 86; one sequence of 4096, 512 rows
+// 72 / 93, 1024 rows 124 / 94; of 32768, 1024 rows 744 / 638.
+bool prompt_form(int act, int n_rows, int n_seqs, int kv, int group, int sms) {
+  const bool f32 = act == MLB_ACT_F32;
+  const long long units = (long long)n_seqs * kv;
+  const long long rows = ((long long)n_rows * group + n_seqs - 1) / n_seqs;
+  const long long per_cta = f32 ? 128 : 256;
+  const double decode = (double)(units * ((rows + 15) / 16)) * (f32 ? 2.05 : 1.5) / (3 * sms);
+  const long long ctas = units * ((rows + per_cta - 1) / per_cta);
+  const double prompt = (double)((ctas + sms - 1) / sms) * (f32 ? 2.1 : 1.65);
+  return prompt < decode;
 }
 
 size_t dec_workspace(int grid, int groups, int nt) {
@@ -738,7 +778,7 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
         ((long long)max_pages * page_size + kChunkTokens - 1) / kChunkTokens;
     const int grid = (int)std::min<long long>(most, tiles * n_kv_heads * chunks);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (prompt_form(n_rows, n_seqs, a.group)) {
+    if (prompt_form(act_type, n_rows, n_seqs, n_kv_heads, a.group, sm_count(device_id))) {
       paged_prompt_launch(a, act_type, device_id, s);
       return;
     }

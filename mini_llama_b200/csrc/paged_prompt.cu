@@ -362,7 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     const long long flat = row0 + r;
     const bool live = flat < rows;
     const int tok = live ? (int)(flat / a.group) : 0;
-    const int vis = live ? max(sw.len - sw.n + tok + 1, 0) : 0;
+    // rows of no one hide nothing, so that their warps need not mask
+    const int vis = live ? max(sw.len - sw.n + tok + 1, 0) : 0x40000000;
     const float rs = sh.row_scale[r];
     const int nx = steps[x];
     float ref = -INFINITY;

@@ -64,9 +64,14 @@ def attention(q, k, v, length, n, scale, absent=()):
             (top.transpose(0, 1)[..., None], v.abs().amax((0, 2))[None, :, None]))
 
 
-def prompt_form(rows, n_seqs, group):
+def prompt_form(rows, n_seqs, kv, group, dtype):
     """Whether a call takes the prompt form (mlb_paged_attention's rule)."""
-    return rows * group >= 64 * n_seqs
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    f32 = dtype == torch.float32
+    units, each = n_seqs * kv, -(-rows * group // n_seqs)
+    ctas = units * -(-each // (128 if f32 else 256))
+    return (-(-ctas // sms) * (2.1 if f32 else 1.65)
+            < units * -(-each // 16) * (2.05 if f32 else 1.5) / (3 * sms))
 
 
 def attention_bound(out, vabs, top, length, dtype, prompt=False):

@@ -47,7 +47,8 @@ def filled(seqs, kv, hd, seed, layers=1, layer=0, pool=None):
 def check_attention(out, q, kk, vv, seqs, hd, dtype, scale=None):
     scale = 1 / math.sqrt(hd) if scale is None else scale
     row = at = 0
-    prompt = R.prompt_form(seqs.rows, len(seqs.new), q.shape[1] // kk.shape[1])
+    kv = kk.shape[1]
+    prompt = R.prompt_form(seqs.rows, len(seqs.new), kv, q.shape[1] // kv, dtype)
     for n, length in zip(seqs.new, seqs.lens):
         if n:
             m = min(n, length)  # rows before position 0 see nothing
@@ -206,6 +207,27 @@ def test_long_and_many(cuda, new, lens, heads, kv, dtype):
     check_attention(out, q, kk, vv, seqs, 128, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new,lens,heads,kv,hd", [
+    ([600], [600], 32, 8, 128), ([300, 200, 7, 0, 130], [300, 333, 900, 4, 128], 32, 16, 128),
+    ([257] * 6, [257, 300, 640, 257, 1000, 200], 24, 24, 96),
+    ([128] * 20, [128 + 37 * i for i in range(20)], 16, 8, 64), ([1000], [1000], 40, 40, 40),
+    ([90] * 40, [90] * 40, 16, 4, 32)])
+def test_prompts(cuda, new, lens, heads, kv, hd, dtype):
+    """Calls that take the prompt form: row tiles that end inside a token, tiles whose
+    second half is empty, lengths on both sides of its steps, more rows than length."""
+    dtype = getattr(torch, dtype)
+    seqs = R.Seqs(new, lens, 32, seed=len(new))
+    assert R.prompt_form(seqs.rows, len(new), kv, heads // kv, dtype)
+    cache, kk, vv = filled(seqs, kv, hd, 19, pool=255)
+    q = randn(gen(23), seqs.rows, heads, hd, dtype=dtype) * 2
+    q[0] *= 30  # scores that rise by far more than a step allows for
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), heads, kv, hd)
+    check_attention(out, q, kk, vv, seqs, hd, dtype)
+    again = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), heads, kv, hd)
+    assert torch.equal(out, again)
+
+
 def test_many_sequences(cuda):
     lens = [1 + (i * 37) % 90 for i in range(400)]
     new = [(i % 5 != 3) * 1 for i in range(400)]
@@ -240,12 +262,12 @@ def test_small_scales_keep_their_precision(cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("n", [1, 6, 90])
+@pytest.mark.parametrize("n", [1, 6, 90, 700])
 def test_what_a_row_does_not_see_has_no_say(cuda, n, dtype):
     """Infinite and NaN values past a row, and in pages and slots of no one."""
     dtype = getattr(torch, dtype)
     kv, hd, page, heads = 2, 64, 32, 8
-    length = 200
+    length = 200 if n < 200 else 750
     seqs = R.Seqs([n], [length], page, seed=4)
     g = gen(6)
     k, v = randn(g, length, kv, hd), randn(g, length, kv, hd)
@@ -274,8 +296,9 @@ def test_what_a_row_does_not_see_has_no_say(cuda, n, dtype):
 
 def test_pages_outside_the_pool_are_not_seen(cuda):
     kv, hd, page, heads = 2, 128, 16, 8
-    for n, dtype in ((1, torch.float32), (3, torch.bfloat16), (64, torch.float32)):
-        length = 300
+    for n, dtype in ((1, torch.float32), (3, torch.bfloat16), (64, torch.float32),
+                     (1100, torch.float32), (1100, torch.bfloat16)):
+        length = max(300, n)
         seqs = R.Seqs([n], [length], page, seed=8)
         cache, kk, vv = filled(seqs, kv, hd, 4)
         q = randn(gen(5), n, heads, hd, dtype=dtype)
@@ -288,7 +311,7 @@ def test_pages_outside_the_pool_are_not_seen(cuda):
                                                 heads, kv, hd)
         want, vabs, top = R.attention(q, kk, vv, length, n, 1 / math.sqrt(hd), absent)
         err = (out.double().cpu() - want).abs()
-        prompt = R.prompt_form(n, 1, heads // kv)
+        prompt = R.prompt_form(n, 1, kv, heads // kv, dtype)
         assert (err <= R.attention_bound(want, vabs, top, length, dtype, prompt)).all()
         none = torch.full_like(table, -1)
         out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, seqs.offsets, seqs.seq_lens, none,
@@ -339,13 +362,14 @@ def test_rows_behind_the_last_sequence_are_left_alone(cuda):
         assert (out[seqs.rows:] == 3).all() and (out[:seqs.rows] != 3).any()
 
 
-@pytest.mark.parametrize("n,dtype", [(1, "float32"), (3, "bfloat16"), (100, "bfloat16")])
+@pytest.mark.parametrize("n,dtype", [(1, "float32"), (3, "bfloat16"), (900, "bfloat16"),
+                                     (900, "float32")])
 def test_graph_replay_with_new_lengths(cuda, n, dtype):
     """A captured step follows the lengths and tables that its buffers hold when
     it is replayed, on another stream, and twice gives the same bits."""
     dtype = getattr(torch, dtype)
     heads, kv, hd, page = 8, 2, 128, 16
-    seqs = R.Seqs([n, n], [400, 310], page, seed=12)
+    seqs = R.Seqs([n, n], [max(n, 400), n + 310], page, seed=12)
     cache, kk, vv = filled(seqs, kv, hd, 3)
     q = randn(gen(2), seqs.rows, heads, hd, dtype=dtype)
     lens = seqs.seq_lens.clone()
@@ -416,10 +440,10 @@ def test_offsets_past_32_bits(cuda):
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1.5])
-@pytest.mark.parametrize("n", [1, 5, 100])
+@pytest.mark.parametrize("n", [1, 5, 1200])
 def test_scale_of_any_sign(cuda, n, scale, dtype):
     dtype = getattr(torch, dtype)
-    seqs = R.Seqs([n], [333], 16, seed=3)
+    seqs = R.Seqs([n], [max(n, 333)], 16, seed=3)
     cache, kk, vv = filled(seqs, 2, 64, 17)
     q = randn(gen(4), n, 8, 64, dtype=dtype)
     out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, 64, scale=scale)
@@ -430,13 +454,13 @@ def test_scale_of_any_sign(cuda, n, scale, dtype):
 def test_largest_values(cuda, dtype):
     """Scales up to fp16's largest, next to ordinary ones."""
     dtype = getattr(torch, dtype)
-    kv, hd, length = 2, 64, 300
+    kv, hd, length = 2, 64, 1500
     g = gen(5)
     k, v = randn(g, length, kv, hd), randn(g, length, kv, hd)
     k[100:110] *= 3e4
     v[40:50] *= 1e5
     v[200, 0, 3] = 1e9  # past the format: kept at its largest scale
-    for n in (1, 70):
+    for n in (1, 70, 1300):
         seqs = R.Seqs([n], [length], 32, seed=3)
         cache = mlb.CudaPagedKvCache(1, seqs.n_pages, 32, kv, hd)
         cache.AppendDevice(0, k, v, *seqs.whole(), rope_type=mlb.ROPE_NONE)
