@@ -81,7 +81,7 @@ struct Plan {
 
 struct Shared {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_done[2], o_last[2], drain;
+  uint64_t s_full[2], p_full[2], o_done[2], o_last[2], q_full, drain;
   long long warp_sums[kThreads / 32];
   long long base;
   int seq;
@@ -123,7 +123,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
   // come first
   int seq = -1, head = 0, tile = 0;
   SeqWork sw = {};
-  {
+  if (a.seqs.n_seqs == 1) {  // nothing to look through
+    sw = seq_work(a, 0, P::ROWS, kTok);
+    if (blockIdx.x >= (long long)sw.tiles * a.cache.kv) return;
+    seq = 0;
+    head = blockIdx.x % a.cache.kv;
+    tile = sw.tiles - 1 - blockIdx.x / a.cache.kv;
+  } else {
     long long base = 0;
     if (threadIdx.x == 0) sh.seq = -1;
     __syncthreads();
@@ -177,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       mbar_init(&sh.o_done[i], 1);
       mbar_init(&sh.o_last[i], 1);
     }
+    mbar_init(&sh.q_full, 4 * NX);
     mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
     fence_mbar_init();
@@ -184,35 +191,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
   if (warp == kMmaWarp) {
     tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
-  }
-  // queries as operand tiles, 8 rows per warp and turn
-  {
-    const int g = lane >> 2, c = lane & 3;
-    const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    for (int r0 = warp * 8; r0 < P::ROWS; r0 += kThreads / 32 * 8) {
-      const long long flat = row0 + r0 + g;
-      const T* row = nullptr;
-      if (flat < rows) {
-        const int i = (int)(flat / a.group);
-        row = static_cast<const T*>(a.q) + (long long)(sw.row0 + i) * a.q_stride +
-              (size_t)(head * a.group + (int)(flat - (long long)i * a.group)) * a.cache.head_dim;
-      }
-      uint32_t hi[G][4], lo[G][4];
-      float inv;
-      load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
-      if (c == 0) sh.row_scale[r0 + g] = inv * sign * a.scale_log2 * 16.0f;
-      const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
-      uint8_t* at = smem + P::Q0 + (r0 / 128) * PT * P::Q + (r0 % 128) / 8 * P::SBO_D + g * 16;
-#pragma unroll
-      for (int w = 0; w < G; ++w) {
-        *reinterpret_cast<uint4*>(at + (4 * w + c) * 128) = make_uint4(
-            hi[w][0] ^ flip, hi[w][1] ^ flip, hi[w][2] ^ flip, hi[w][3] ^ flip);
-        if (SPLIT)
-          *reinterpret_cast<uint4*>(at + P::Q + (4 * w + c) * 128) = make_uint4(
-              lo[w][0] ^ flip, lo[w][1] ^ flip, lo[w][2] ^ flip, lo[w][3] ^ flip);
-      }
-    }
-    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
@@ -355,6 +333,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     }
   } else if (warp < 12) {
     // -------------------------------------------------------------- softmax
+    // first the queries as operand tiles, 8 rows per warp and turn
+    {
+      const int g = lane >> 2, c = lane & 3;
+      const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;
+      for (int r0 = (warp - 4) * 8; r0 < P::ROWS; r0 += 4 * NX * 8) {
+        const long long flat = row0 + r0 + g;
+        const T* row = nullptr;
+        if (flat < rows) {
+          const int i = (int)(flat / a.group);
+          row = static_cast<const T*>(a.q) + (long long)(sw.row0 + i) * a.q_stride +
+                (size_t)(head * a.group + (int)(flat - (long long)i * a.group)) * a.cache.head_dim;
+        }
+        uint32_t hi[G][4], lo[G][4];
+        float inv;
+        load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
+        if (c == 0) sh.row_scale[r0 + g] = inv * sign * a.scale_log2 * 16.0f;
+        const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
+        uint8_t* at = smem + P::Q0 + (r0 / 128) * PT * P::Q + (r0 % 128) / 8 * P::SBO_D + g * 16;
+#pragma unroll
+        for (int w = 0; w < G; ++w) {
+          *reinterpret_cast<uint4*>(at + (4 * w + c) * 128) = make_uint4(
+              hi[w][0] ^ flip, hi[w][1] ^ flip, hi[w][2] ^ flip, hi[w][3] ^ flip);
+          if (SPLIT)
+            *reinterpret_cast<uint4*>(at + P::Q + (4 * w + c) * 128) = make_uint4(
+                lo[w][0] ^ flip, lo[w][1] ^ flip, lo[w][2] ^ flip, lo[w][3] ^ flip);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
+      asm volatile("bar.sync 1, %0;" ::"n"(4 * NX * 32) : "memory");  // row_scale
+    }
     const int x = (warp - 4) / 4;
     const int r = x * 128 + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -606,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           tc_mma_ts2<true>(d, (part == 1 ? lo : hi) + 8 * s,
                            v + (part == 2 ? P::V / 16 : 0) + s * 16, hi_t, id_o);
     };
-    bool ok = n == 0 || wait(sh, &sh.k_full[0], 0, 1006);
+    bool ok = wait(sh, &sh.q_full, 0, 1011) && (n == 0 || wait(sh, &sh.k_full[0], 0, 1006));
     if (ok && n > 0) {
       tc_fence_after();
 #pragma unroll
