@@ -42,13 +42,13 @@ constexpr int kTok = 128;  // tokens per step
 constexpr int kThreads = 13 * 32;
 constexpr int kMmaWarp = 12;
 constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
-// P = 2^(s - ref + lift), and ref follows the row's maximum when that is `rise`
-// above it. With P up to 2^11, and 2^15 with the 16 of large V scales, it stays
-// within fp16, and what fp16 loses below 2^-14 is 2^-(25 + lift) of a token at ref.
-// fp32 calls look for the maximum before they make P; bf16 calls make P in the
-// same pass and make it again when a row rises, which is dear, so they let it rise
-// further.
-constexpr float kRise = 4.0f, kRiseLate = 8.0f;
+// P = 2^(s - ref + lift). With P up to 2^11, and 2^15 with the 16 of large V scales,
+// it stays within fp16, and what fp16 loses below 2^-14 is 2^-(25 + lift) of a token
+// at ref. fp32 calls look for the row's maximum first, and ref follows it when that
+// is more than kRise above. bf16 calls make P in one pass and, when the step's sum
+// exceeds 2^11 (128 tokens at ref come to 2^10), look for the maximum, raise ref to
+// it and make P again.
+constexpr float kRise = 4.0f, kMostP = 2048.0f;
 
 __device__ DeviceStatus g_status;
 
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
   constexpr bool SPLIT = sizeof(T) == 4;
   using P = Plan<G, SPLIT>;
   constexpr int D = P::D, NX = P::NX, NS = P::NS, PT = P::PT;
-  constexpr float kLift = 11.0f - (SPLIT ? kRise : kRiseLate);
+  constexpr float kLift = SPLIT ? 11.0f - kRise : 3.0f;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -474,13 +474,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         }
       } else {
         // P of the whole step in registers under the ref of the step before (one
-        // pass over S); again if a row has risen by more than P can hold
-        if (j == 0) raise_to(step_max(), true);
+        // pass over S); again if a row's P have become too large
+        // rows that see something for the first time have no ref yet
+        if (__any_sync(0xffffffffu, ref == -INFINITY && left > 0)) {
+          const float mx = step_max();
+          ok = raise_to(mx, ref == -INFINITY && mx > ref);
+          if (!ok) break;
+        }
         uint32_t hi[4][16];
         while (true) {
           const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          float top[2] = {-INFINITY, -INFINITY};
           auto pass = [&](auto plain_c) {
             constexpr bool PLAIN = decltype(plain_c)::value;
             // 32 tokens on their way while 32 are worked on (products slow the loads
@@ -500,7 +504,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
                   vx = m >> (2 * i) & 1 ? vx : -INFINITY;
                   vy = m >> (2 * i + 1) & 1 ? vy : -INFINITY;
                 }
-                top[i & 1] = fmaxf(fmaxf(top[i & 1], vx), vy);
                 float2 p = fma2(make_float2(vx, vy), make_float2(rs, rs), make_float2(neg, neg));
                 p.x = ex2(p.x);
                 p.y = ex2(p.y);
@@ -521,15 +524,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             pass(std::true_type{});
           else
             pass(std::false_type{});
-          const float t = fmaxf(top[0], top[1]);
-          const float mx = t == -INFINITY ? t : t * rs;
-          const bool rise = mx > ref + kRiseLate;
-          if (!__any_sync(0xffffffffu, rise)) {
+          // no P above the sum, so none that fp16 does not hold; looking for the maximum
+          // as well would cost a sixth of the pass
+          const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          if (!__any_sync(0xffffffffu, all > kMostP)) {
             l0 = add2(l0, sum[0]);
             l1 = add2(l1, sum[1]);
             break;
           }
-          ok = raise_to(mx, rise);
+          const float mx = step_max();
+          ok = raise_to(mx, mx > ref);
           if (!ok) break;
         }
         if (!ok) break;

@@ -320,6 +320,31 @@ def test_pages_outside_the_pool_are_not_seen(cuda):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [1, 20, 1200])
+def test_first_pages_missing(cuda, n, dtype):
+    """Rows whose first sight of the cache comes late, at scores far below zero."""
+    dtype = getattr(torch, dtype)
+    kv, hd, page, heads, length = 2, 64, 16, 8, 1300
+    seqs = R.Seqs([n], [length], page, seed=8)
+    g = gen(14)
+    cache = mlb.CudaPagedKvCache(1, seqs.n_pages, page, kv, hd)
+    k, v = randn(g, length, kv, hd) * 0.3 + 1.0, randn(g, length, kv, hd)
+    cache.AppendDevice(0, k, v, *seqs.whole(), rope_type=mlb.ROPE_NONE)
+    kk, vv = cache.ReadDevice(0, *seqs.whole(), length)
+    q = (randn(g, n, heads, hd) - 25.0).to(dtype)  # scores near -200
+    table = seqs.table.clone()
+    table[0, :30] = -1
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, seqs.offsets, seqs.seq_lens, table, heads,
+                                            kv, hd)
+    absent = list(range(30 * page))
+    want, vabs, top = R.attention(q, kk, vv, length, n, 1 / math.sqrt(hd), absent)
+    prompt = R.prompt_form(n, 1, kv, heads // kv, dtype)
+    err = (out.double().cpu() - want).abs()
+    assert (err <= R.attention_bound(want, vabs, top, length, dtype, prompt)).all()
+    assert n == 1 or (out[:max(0, n - (length - 30 * page))] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_strided_and_unaligned_rows(cuda, dtype):
     """Rows cut out of one projection's output, and at odd addresses."""
     dtype = getattr(torch, dtype)
