@@ -268,13 +268,12 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[G]) {
   }
 }
 
-// One row's query elements of this lane, scaled by a power of two, as MMA A
-// words: word (w, i) = dims 32 w + 8 c + (i, i + 4). inv receives 2^-shift.
+// One row's query elements of this lane, dims 32 w + 8 c + 0..7 (zeros past head_dim
+// and without a row); returns the exponent of the power of two that brings the row's
+// largest element near 2^13.
 template <int G, class T>
-__device__ __forceinline__ void load_query(const T* row, int head_dim, int c, bool split,
-                                           uint32_t (&hi)[G][4], uint32_t (&lo)[G][4],
-                                           float& inv) {
-  float e[G][8];
+__device__ __forceinline__ int load_query_row(const T* row, int head_dim, int c,
+                                              float (&e)[G][8]) {
   float amax = 0.0f;
 #pragma unroll
   for (int w = 0; w < G; ++w) {
@@ -289,21 +288,23 @@ __device__ __forceinline__ void load_query(const T* row, int head_dim, int c, bo
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   const int ex = (int)(__float_as_uint(amax) >> 23);
   // zero rows, subnormal rows and infinities stay as they are
-  const int sh = (ex == 0 || ex == 255) ? 0 : min(max(13 - (ex - 127), -126), 126);
-  const float sf = pow2(sh);
-  inv = pow2(-sh);
+  return (ex == 0 || ex == 255) ? 0 : min(max(13 - (ex - 127), -126), 126);
+}
+
+// Eight elements times sf as fp16 words, word i = elements (i, i + 4), and for split
+// what they leave.
+__device__ __forceinline__ void query_words(const float (&e)[8], float sf, bool split,
+                                            uint32_t (&hi)[4], uint32_t (&lo)[4]) {
 #pragma unroll
-  for (int w = 0; w < G; ++w)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = e[w][i] * sf, y = e[w][i + 4] * sf;
-      hi[w][i] = pack_f16(x, y);
-      lo[w][i] = 0u;
-      if (split) {
-        const float2 h = __half22float2(u32_as_h2(hi[w][i]));
-        lo[w][i] = pack_f16(x - h.x, y - h.y);
-      }
+  for (int i = 0; i < 4; ++i) {
+    const float x = e[i] * sf, y = e[i + 4] * sf;
+    hi[i] = pack_f16(x, y);
+    lo[i] = 0u;
+    if (split) {
+      const float2 h = __half22float2(u32_as_h2(hi[i]));
+      lo[i] = pack_f16(x - h.x, y - h.y);
     }
+  }
 }
 
 // What a sequence asks for: its rows in tiles of tile_rows (token, head) rows, its

@@ -55,8 +55,13 @@ struct Seg {
   int seq, head, tile, chunk0, chunk1, chunks, len, n, row0, record;
 };
 
+// a / b of non-negative numbers; 32-bit division where that will do (a quarter of the
+// instructions, and every warp does a few per segment).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
 __device__ __forceinline__ long long run_begin(long long total, int i, int n) {
-  return total * i / n;
+  return quotient(total * i, n);
 }
 
 // F of the largest V scale met so far: 2^F d < 2^14, and 2^F itself within fp16.
@@ -146,11 +151,11 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
         ++seq;
         sw = seq_work(a, seq, R, kChunkTokens);
       }
-      const long long u = (at - base) / sw.chunks;  // unit within the sequence
+      const long long u = quotient(at - base, sw.chunks);  // unit within the sequence
       const long long unit_begin = base + u * sw.chunks;
       Seg sg;
       sg.seq = seq;
-      sg.head = (int)(u / sw.tiles);
+      sg.head = (int)quotient(u, sw.tiles);
       sg.tile = (int)(u - (long long)sg.head * sw.tiles);
       sg.chunk0 = (int)(at - unit_begin);
       sg.chunk1 = (int)min((long long)sw.chunks, end - unit_begin);
@@ -165,7 +170,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
           // this CTA holds the second part of a unit that an earlier one began;
           // the last part is with the last run that begins before the unit ends
           const long long unit_end = unit_begin + sw.chunks;
-          const int last = (int)((unit_end * nrun + total - 1) / total) - 1;
+          const int last = (int)quotient(unit_end * nrun + total - 1, total) - 1;
           split[0] = make_int4(last - cta + 2, prev == unit_begin ? 0 : 1, sg.head, sg.tile);
           split[1] = make_int4(sw.row0, sw.n, 0, 0);
         }
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
       for (int t = 0; t < NT; ++t) {
         const long long flat = (long long)sg.tile * R + t * 8 + g;
         const bool live = flat < (long long)sg.n * a.group;
-        const int i = live ? (int)(flat / a.group) : 0;
+        const int i = live ? (int)quotient(flat, a.group) : 0;
         const int hq = sg.head * a.group + (live ? (int)(flat - (long long)i * a.group) : 0);
         vis[t] = live ? max(sg.len - sg.n + i + 1, 0) : 0;
         if (live) vis_min = min(vis_min, vis[t]);
@@ -234,27 +239,29 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
         const T* row = live ? static_cast<const T*>(a.q) + (long long)(sg.row0 + i) * a.q_stride +
                                   (size_t)hq * a.cache.head_dim
                             : nullptr;
-        uint32_t hi[G][4], lo[G][4];
-        float inv;
-        load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
-        rs[t] = inv * a.scale_log2;
-        // the warps share the tile; each writes its part of the words
+        float e[G][8];
+        const int sh = load_query_row<G, T>(row, a.cache.head_dim, c, e);
+        rs[t] = pow2(-sh) * a.scale_log2;
+        // the warps share the tile; each makes and writes its part of the words
+        const float sf = pow2(sh);
 #pragma unroll
-        for (int w = 0; w < G; ++w) {
-          if (w % kDecWarps != warp) continue;
+        for (int w = 0; w < G; ++w)
+          if (w % kDecWarps == warp) {
+            uint32_t hi[4], lo[4];
+            query_words(e[w], sf, SPLIT, hi, lo);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint4& q = queries[(((SPLIT ? t : t / 2) * G + w) * 2 + k) * 32 + lane];
-            if (SPLIT) {
-              q = make_uint4(hi[w][2 * k], lo[w][2 * k], hi[w][2 * k + 1], lo[w][2 * k + 1]);
-            } else if (t & 1) {
-              q.y = hi[w][2 * k];
-              q.w = hi[w][2 * k + 1];
-            } else {
-              q = make_uint4(hi[w][2 * k], 0u, hi[w][2 * k + 1], 0u);
+            for (int k = 0; k < 2; ++k) {
+              uint4& q = queries[(((SPLIT ? t : t / 2) * G + w) * 2 + k) * 32 + lane];
+              if (SPLIT) {
+                q = make_uint4(hi[2 * k], lo[2 * k], hi[2 * k + 1], lo[2 * k + 1]);
+              } else if (t & 1) {
+                q.y = hi[2 * k];
+                q.w = hi[2 * k + 1];
+              } else {
+                q = make_uint4(hi[2 * k], 0u, hi[2 * k + 1], 0u);
+              }
             }
           }
-        }
       }
       vis_min = __reduce_min_sync(0xffffffffu, vis_min);
       vis_max = __reduce_max_sync(0xffffffffu, vis_max);
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
             if (complete) {
               const long long flat = (long long)sg.tile * R + t * 8 + r;
               if (flat < (long long)sg.n * a.group && d0 < a.cache.head_dim) {
-                const int tk = (int)(flat / a.group);
+                const int tk = (int)quotient(flat, a.group);
                 const int hq = sg.head * a.group + (int)(flat - (long long)tk * a.group);
                 const float f = all == 0.0f ? 0.0f : 1.0f / all;  // sees nothing: zeros
                 store_act2(static_cast<T*>(a.out) + (long long)(sg.row0 + tk) * a.out_stride +

@@ -345,19 +345,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           row = static_cast<const T*>(a.q) + (long long)(sw.row0 + i) * a.q_stride +
                 (size_t)(head * a.group + (int)(flat - (long long)i * a.group)) * a.cache.head_dim;
         }
-        uint32_t hi[G][4], lo[G][4];
-        float inv;
-        load_query<G, T>(row, a.cache.head_dim, c, SPLIT, hi, lo, inv);
-        if (c == 0) sh.row_scale[r0 + g] = inv * sign * a.scale_log2 * 16.0f;
-        const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
+        float e[G][8];
+        const int sh2 = load_query_row<G, T>(row, a.cache.head_dim, c, e);
+        if (c == 0) sh.row_scale[r0 + g] = pow2(-sh2) * sign * a.scale_log2 * 16.0f;
+        const float sf = pow2(sh2) * sign;
         uint8_t* at = smem + P::Q0 + (r0 / 128) * PT * P::Q + (r0 % 128) / 8 * P::SBO_D + g * 16;
 #pragma unroll
         for (int w = 0; w < G; ++w) {
-          *reinterpret_cast<uint4*>(at + (4 * w + c) * 128) = make_uint4(
-              hi[w][0] ^ flip, hi[w][1] ^ flip, hi[w][2] ^ flip, hi[w][3] ^ flip);
+          uint32_t hi[4], lo[4];
+          query_words(e[w], sf, SPLIT, hi, lo);
+          *reinterpret_cast<uint4*>(at + (4 * w + c) * 128) =
+              make_uint4(hi[0], hi[1], hi[2], hi[3]);
           if (SPLIT)
-            *reinterpret_cast<uint4*>(at + P::Q + (4 * w + c) * 128) = make_uint4(
-                lo[w][0] ^ flip, lo[w][1] ^ flip, lo[w][2] ^ flip, lo[w][3] ^ flip);
+            *reinterpret_cast<uint4*>(at + P::Q + (4 * w + c) * 128) =
+                make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
       fence_proxy_async_smem();
