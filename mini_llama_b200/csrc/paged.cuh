@@ -269,21 +269,26 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[G]) {
 }
 
 // One row's query elements of this lane, dims 32 w + 8 c + 0..7 (zeros past head_dim
-// and without a row); returns the exponent of the power of two that brings the row's
-// largest element near 2^13.
+// and without a row).
 template <int G, class T>
-__device__ __forceinline__ int load_query_row(const T* row, int head_dim, int c,
-                                              float (&e)[G][8]) {
-  float amax = 0.0f;
+__device__ __forceinline__ void load_query_elements(const T* row, int head_dim, int c,
+                                                    float (&e)[G][8]) {
 #pragma unroll
   for (int w = 0; w < G; ++w) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[w][i] = 0.0f;
     const int d0 = 32 * w + 8 * c;
     if (row && d0 < head_dim) load_q8(row + d0, e[w]);
+  }
+}
+// The exponent of the power of two that brings the row's largest element near 2^13.
+template <int G>
+__device__ __forceinline__ int query_shift(const float (&e)[G][8]) {
+  float amax = 0.0f;
+#pragma unroll
+  for (int w = 0; w < G; ++w)
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(e[w][i]));
-  }
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   const int ex = (int)(__float_as_uint(amax) >> 23);
@@ -308,7 +313,8 @@ __device__ __forceinline__ void query_words(const float (&e)[8], float sf, bool 
 }
 
 // What a sequence asks for: its rows in tiles of tile_rows (token, head) rows, its
-// length in chunks of chunk_tokens. Lengths and offsets are cut to what the page
+// length in chunks of chunk_tokens, and their number with unit_slots more per (KV
+// head, tile). Lengths and offsets are cut to what the page
 // table and the call hold.
 struct SeqWork {
   int len, n, row0, tiles, chunks;
@@ -316,7 +322,7 @@ struct SeqWork {
 };
 
 __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s, int tile_rows,
-                                            int chunk_tokens) {
+                                            int chunk_tokens, int unit_slots) {
   SeqWork w;
   const int cap = a.seqs.max_pages * a.cache.page_size;
   w.len = min(max(a.seqs.seq_lens[s], 0), cap);
@@ -324,7 +330,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s, int t
   w.n = max(min(a.seqs.row_offsets[s + 1], a.seqs.n_rows) - w.row0, 0);
   w.tiles = (int)(((long long)w.n * a.group + tile_rows - 1) / tile_rows);
   w.chunks = max(1, (w.len + chunk_tokens - 1) / chunk_tokens);
-  w.cost = (long long)w.tiles * a.cache.kv * w.chunks;
+  w.cost = (long long)w.tiles * a.cache.kv * (w.chunks + unit_slots);
   return w;
 }
 

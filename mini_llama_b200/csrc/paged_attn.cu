@@ -45,6 +45,9 @@ constexpr int kDecWarps = 4;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kChunkTokens = kPagedBlock * kDecWarps;  // one block per warp
 constexpr int kStages = 5;                    // blocks on their way per warp, and in use
+// A unit counts for this many chunks more than it has: its queries, the join of its
+// warps and its result take a CTA about as long as one chunk.
+constexpr int kUnitSlots = 1;
 constexpr int kMaxSegs = 32;                  // segments of a run listed at a time
 
 // CTAs per SM: 128 registers a thread for one 8-row tile, 168 for two.
@@ -95,7 +98,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
   long long total = 0, cost = 0, incl = 0;
   for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
     const int s = s0 + threadIdx.x;
-    cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
+    cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens, kUnitSlots).cost : 0;
     total += cost;
   }
   incl = block_scan<kDecThreads>(total, warp_sums);
@@ -121,7 +124,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
     long long base = 0;
     for (int s0 = 0; s0 < a.seqs.n_seqs; s0 += kDecThreads) {
       const int s = s0 + threadIdx.x;
-      cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens).cost : 0;
+      cost = s < a.seqs.n_seqs ? seq_work(a, s, R, kChunkTokens, kUnitSlots).cost : 0;
       incl = block_scan<kDecThreads>(cost, warp_sums) + base;
       if (cost > 0 && begin >= incl - cost && begin < incl) {
         found_seq = s;
@@ -136,7 +139,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
   }
   int seq = found_seq;
   long long base = found_base;
-  SeqWork sw = seq_work(a, seq, R, kChunkTokens);
+  SeqWork sw = seq_work(a, seq, R, kChunkTokens, kUnitSlots);
   if (threadIdx.x == 0) split[0] = make_int4(0, 0, 0, 0);
 
   uint8_t* ring = smem + warp * (kStages * BLOCK);
@@ -149,10 +152,15 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
       while (at >= base + sw.cost) {  // next sequence with rows
         base += sw.cost;
         ++seq;
-        sw = seq_work(a, seq, R, kChunkTokens);
+        sw = seq_work(a, seq, R, kChunkTokens, kUnitSlots);
       }
-      const long long u = quotient(at - base, sw.chunks);  // unit within the sequence
-      const long long unit_begin = base + u * sw.chunks;
+      const int slots = sw.chunks + kUnitSlots;
+      const long long u = quotient(at - base, slots);  // unit within the sequence
+      const long long unit_begin = base + u * slots;
+      if (at - unit_begin >= sw.chunks) {  // the slots past its chunks stand for its ends
+        at = unit_begin + slots;
+        continue;
+      }
       Seg sg;
       sg.seq = seq;
       sg.head = (int)quotient(u, sw.tiles);
@@ -178,6 +186,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
       ++n_segs;
       at = unit_begin + sg.chunk1;
     }
+    if (n_segs == 0) break;
     __syncthreads();
 
     // copies, running ahead of the arithmetic across segments: block 4 chunk + warp
@@ -216,8 +225,6 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
       }
       cp_async_commit();
     };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue();
     int slot = 0;
 
     for (int si = 0; si < n_segs; ++si) {
@@ -240,7 +247,16 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
                                   (size_t)hq * a.cache.head_dim
                             : nullptr;
         float e[G][8];
-        const int sh = load_query_row<G, T>(row, a.cache.head_dim, c, e);
+        if (si == 0 && t == 0) {
+          // the first queries are asked for before the copies that would be ahead of
+          // them in the memory's queue
+          load_query_elements<G, T>(row, a.cache.head_dim, c, e);
+#pragma unroll
+          for (int i = 0; i < kStages - 1; ++i) issue();
+        } else {
+          load_query_elements<G, T>(row, a.cache.head_dim, c, e);
+        }
+        const int sh = query_shift<G>(e);
         rs[t] = pow2(-sh) * a.scale_log2;
         // the warps share the tile; each makes and writes its part of the words
         const float sf = pow2(sh);

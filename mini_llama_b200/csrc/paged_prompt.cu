@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
   int seq = -1, head = 0, tile = 0;
   SeqWork sw = {};
   if (a.seqs.n_seqs == 1) {  // nothing to look through
-    sw = seq_work(a, 0, P::ROWS, kTok);
+    sw = seq_work(a, 0, P::ROWS, kTok, 0);
     if (blockIdx.x >= (long long)sw.tiles * a.cache.kv) return;
     seq = 0;
     head = blockIdx.x % a.cache.kv;
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       const int s = s0 + threadIdx.x;
       long long units = 0;
       if (s < a.seqs.n_seqs) {
-        const SeqWork w = seq_work(a, s, P::ROWS, kTok);
+        const SeqWork w = seq_work(a, s, P::ROWS, kTok, 0);
         units = (long long)w.tiles * a.cache.kv;
       }
       const long long incl = block_scan<kThreads>(units, sh.warp_sums) + base;
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     }
     seq = sh.seq;
     if (seq < 0) return;
-    sw = seq_work(a, seq, P::ROWS, kTok);
+    sw = seq_work(a, seq, P::ROWS, kTok, 0);
     const int u = (int)(blockIdx.x - sh.base);
     head = u % a.cache.kv;
     tile = sw.tiles - 1 - u / a.cache.kv;
@@ -346,7 +346,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
                 (size_t)(head * a.group + (int)(flat - (long long)i * a.group)) * a.cache.head_dim;
         }
         float e[G][8];
-        const int sh2 = load_query_row<G, T>(row, a.cache.head_dim, c, e);
+        load_query_elements<G, T>(row, a.cache.head_dim, c, e);
+        const int sh2 = query_shift<G>(e);
         if (c == 0) sh.row_scale[r0 + g] = pow2(-sh2) * sign * a.scale_log2 * 16.0f;
         const float sf = pow2(sh2) * sign;
         uint8_t* at = smem + P::Q0 + (r0 / 128) * PT * P::Q + (r0 % 128) / 8 * P::SBO_D + g * 16;
