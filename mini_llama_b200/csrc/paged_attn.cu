@@ -46,8 +46,9 @@ constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kChunkTokens = kPagedBlock * kDecWarps;  // one block per warp
 constexpr int kStages = 5;                    // blocks on their way per warp, and in use
 // A unit counts for this many chunks more than it has: its queries, the join of its
-// warps and its result take a CTA about as long as one chunk.
-constexpr int kUnitSlots = 1;
+// warps and its result take a CTA about as long as three (64 uneven sequences: 1: 80 us,
+// 2: 76, 3: 73, 5: 73).
+constexpr int kUnitSlots = 3;
 constexpr int kMaxSegs = 32;                  // segments of a run listed at a time
 
 // CTAs per SM: 128 registers a thread for one 8-row tile, 168 for two.
