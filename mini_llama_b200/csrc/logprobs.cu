@@ -185,7 +185,7 @@ __device__ __forceinline__ float peer_f32(uint32_t a) {
 }
 
 template <class T, int THREADS, int SLICES>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(LogprobArgs a) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 2) logprob_kernel(LogprobArgs a) {
   constexpr int WARPS = THREADS / 32;
   constexpr int VEC = 16 / sizeof(T);
   __shared__ uint64_t lists[WARPS * 32];
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_kernel(Logpro
   };
 
   for (int j = threadIdx.x; j < singles_head; j += THREADS) add(to_f(x[j]), j);
-  constexpr int UNROLL = 4;
+  constexpr int UNROLL = THREADS == 256 ? 2 : 4;  // vectors on their way per thread
   int v = threadIdx.x;
   for (; v + (UNROLL - 1) * THREADS < nv; v += UNROLL * THREADS) {
     uint4 u[UNROLL];

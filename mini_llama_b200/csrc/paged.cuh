@@ -26,7 +26,10 @@
 
 #include <cuda_bf16.h>
 
+#include <map>
+#include <mutex>
 #include <string>
+#include <utility>
 
 #include "common.cuh"
 
@@ -120,6 +123,18 @@ inline void paged_check_rows(const char* who, const char* name, const void* p, l
 inline void paged_check_act(const char* who, int act) {
   if (act != MLB_ACT_F32 && act != MLB_ACT_BF16)
     invalid(std::string(who) + ": unknown activation type " + std::to_string(act));
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.
+template <class K>
+inline void allow_smem(K kernel, size_t bytes, int device_id) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, bool> seen;
+  std::lock_guard<std::mutex> lock(mu);
+  bool& s = seen[{reinterpret_cast<const void*>(kernel), device_id}];
+  if (s) return;
+  MLB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  s = true;
 }
 
 // Arguments of the attention kernels.

@@ -30,10 +30,7 @@
 // timing.
 #include <algorithm>
 #include <cmath>
-#include <map>
-#include <mutex>
 #include <type_traits>
-#include <utility>
 
 #include "paged.cuh"
 
@@ -690,18 +687,6 @@ bool prompt_form(int act, int n_rows, int n_seqs, int kv, int group, int sms) {
 size_t dec_workspace(int grid, int groups, int nt) {
   const size_t rec = (size_t)8 * nt * 32 * groups + 16 * nt;
   return (size_t)grid * (2 * sizeof(int4) + 2 * rec * sizeof(float));
-}
-
-// Lets a kernel use `bytes` of dynamic shared memory, once per kernel and device.
-template <class K>
-void allow_smem(K kernel, size_t bytes, int device_id) {
-  static std::mutex mu;
-  static std::map<std::pair<const void*, int>, bool> seen;
-  std::lock_guard<std::mutex> lock(mu);
-  bool& s = seen[{reinterpret_cast<const void*>(kernel), device_id}];
-  if (s) return;
-  MLB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  s = true;
 }
 
 template <int G, int NT, class T>

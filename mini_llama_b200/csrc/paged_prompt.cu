@@ -28,7 +28,6 @@
 // MLB_ERR_TIMEOUT in the device's status word (mlb_paged_attention_status) and
 // raises the CTA's abort flag; all roles leave their loops, the products in flight
 // are waited for (bounded), tensor memory is released and the CTA exits.
-#include <mutex>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -701,16 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
 template <int G, class T>
 void launch(const PagedAttnArgs& a, int device_id, cudaStream_t stream) {
   using P = Plan<G, sizeof(T) == 4>;
-  static std::mutex mu;
-  static bool seen[64] = {};
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (device_id >= 64 || !seen[device_id]) {
-      MLB_CUDA(cudaFuncSetAttribute(paged_prompt_kernel<G, T>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES));
-      if (device_id < 64) seen[device_id] = true;
-    }
-  }
+  allow_smem(paged_prompt_kernel<G, T>, P::BYTES, device_id);
   const long long tiles = (long long)a.seqs.n_rows * a.group / P::ROWS + a.seqs.n_seqs;
   const long long grid = tiles * a.cache.kv;
   if (grid > 0x7fffffffLL) invalid("CudaPagedAttention: too many rows");

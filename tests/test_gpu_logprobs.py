@@ -100,6 +100,22 @@ def test_masked_logits(cuda):
         -math.inf, device="cuda"))
 
 
+@pytest.mark.parametrize("vocab", [300, 40000])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_extreme_logits_next_to_masked_ones(cuda, dtype, vocab):
+    dtype = getattr(torch, dtype)
+    x = torch.full((3, vocab), -math.inf, device="cuda", dtype=dtype)
+    x[0, :8], x[1, 5:7] = 2e38, 3e38
+    x[1, ::2], x[2, 1::3] = torch.finfo(dtype).min, torch.finfo(dtype).min
+    tok = torch.tensor([3, 5, 1], dtype=torch.int32, device="cuda")
+    lp, ent, ids, _ = mlb.CudaLogProbs(x, tok, top_k=4)
+    # 8 equal logits; one or two of 3e38 (index 6 is even: the lowest); every third
+    want = [math.log(8), 0.0, math.log(len(range(1, vocab, 3)))]
+    for r in range(3):
+        assert abs(lp[r] + want[r]) < 1e-5 and abs(ent[r] - want[r]) < 1e-5
+    assert ids.tolist() == [[0, 1, 2, 3], [5, 0, 2, 4], [1, 4, 7, 10]]
+
+
 def test_rows_without_a_number(cuda):
     x = torch.zeros(4, 3000, device="cuda")
     x[0] = -math.inf
