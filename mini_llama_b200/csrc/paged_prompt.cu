@@ -12,7 +12,9 @@
 // fp16 scale in range), V as d q (or d q / 16 for 16 tokens whose scales reach
 // 4096, with P times 16), each off by at most half an fp16 step (2^-11), P the
 // same. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
-// products that count. ref is the row's maximum as of the last time that it rose
+// products that count; the tensor cores cut what falls below the sum's last bit off, so
+// O takes only hi hi, one cut per 16 tokens, and the small products have a sum of their
+// own (a single sum was off by 1.5e-6 after 2000 tokens, this by 5e-7). ref is the row's maximum as of the last time that it rose
 // by more than a constant: only then is O brought to the new one.
 //
 // Roles (13 warps, one CTA per SM):
@@ -75,7 +77,9 @@ struct Plan {
   // tensor memory columns
   static constexpr int O_COL = 0;               // + 128 x
   static constexpr int S_COL = SPLIT ? 128 : 256;  // + 128 x (bf16), + 128 (step & 1) (fp32)
-  static constexpr int PLO_COL = 384;           // + 64 (step & 1)
+  static constexpr int OLO_COL = 384;           // fp32: the small products of O
+  // P over S: 32 tokens' hi in 16 columns; fp32: their lo in the 16 after them
+  static constexpr int P_STEP = SPLIT ? 32 : 16;
 };
 
 struct Shared {
@@ -370,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     const int r = x * 128 + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_at = tmem + lanes + P::O_COL + 128 * x;
+    const uint32_t olo_at = tmem + lanes + P::OLO_COL;  // fp32
     const long long flat = row0 + r;
     const bool live = flat < rows;
     const int tok = live ? (int)(flat / a.group) : 0;
@@ -426,15 +431,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         l0 = mul2(l0, make_float2(f, f));
         l1 = mul2(l1, make_float2(f, f));
 #pragma unroll 1
-        for (int ch = 0; ch < G; ++ch) {
+        for (int ch = 0; ch < PT * G; ++ch) {
+          const uint32_t at = ch < G ? o_at + 32 * ch : olo_at + 32 * (ch - G);
           float v[32];
-          tmem_ld32(o_at + 32 * ch, v);
+          tmem_ld32(at, v);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t u[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i] * f);
-            tmem_st16(o_at + 32 * ch + 16 * h, u);
+            tmem_st16(at + 16 * h, u);
           }
         }
         tmem_wait_st();
@@ -470,8 +476,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             const float2 h = __half22float2(u32_as_h2(hi[i]));
             lo[i] = pack_f16(p.x - h.x, p.y - h.y);
           }
-          tmem_st16(s_at + 16 * ch, hi);
-          tmem_st16(tmem + lanes + P::PLO_COL + 64 * b + 16 * ch, lo);
+          tmem_st16(s_at + P::P_STEP * ch, hi);
+          tmem_st16(s_at + P::P_STEP * ch + 16, lo);
         }
       } else {
         // P of the whole step in registers under the ref of the step before (one
@@ -539,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         }
         if (!ok) break;
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) tmem_st16(s_at + 16 * ch, hi[ch]);
+        for (int ch = 0; ch < 4; ++ch) tmem_st16(s_at + P::P_STEP * ch, hi[ch]);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -562,6 +568,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         float v[32];
         if (nx > 0) {
           tmem_ld32(o_at + 32 * ch, v);
+          if (SPLIT) {
+            float u[32];
+            tmem_ld32(olo_at + 32 * ch, u);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += u[i];
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0.0f;
@@ -592,13 +604,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     auto scores = [&](int x, int j) {
       const uint32_t d = tmem + P::S_COL + 128 * (SPLIT ? j & 1 : x);
       const uint32_t q = q_lo + x * (PT * P::Q / 16), k = k_lo + (j % NS) * (PT * P::K / 16);
+      // fp32: lo hi and hi lo first, while the sum is small
 #pragma unroll
-      for (int part = 0; part < (SPLIT ? 3 : 1); ++part)  // hi hi, lo hi, hi lo
+      for (int part = SPLIT ? 2 : 0; part >= 0; --part)
 #pragma unroll
         for (int s = 0; s < 2 * G; ++s) {
           const uint32_t aq = q + (part == 1 ? P::Q / 16 : 0) + s * 16;
           const uint32_t bk = k + (part == 2 ? P::K / 16 : 0) + s * 16;
-          if (part == 0 && s == 0)
+          if (part == (SPLIT ? 2 : 0) && s == 0)
             tc_mma_ss2<false>(d, aq, hi_d, bk, hi_d, id_s);
           else
             tc_mma_ss2<true>(d, aq, hi_d, bk, hi_d, id_s);
@@ -606,20 +619,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     };
     // O of row tile x += P V of step j
     auto values = [&](int x, int j) {
-      const uint32_t d = tmem + P::O_COL + 128 * x;
-      const uint32_t hi = tmem + P::S_COL + 128 * (SPLIT ? j & 1 : x);
-      const uint32_t lo = tmem + P::PLO_COL + 64 * (j & 1);
+      const uint32_t p = tmem + P::S_COL + 128 * (SPLIT ? j & 1 : x);
       const uint32_t v = v_lo + (j % NS) * (PT * P::V / 16);
-      if (j == 0)
-        tc_mma_ts2<false>(d, hi, v, hi_t, id_o);
-      else
-        tc_mma_ts2<true>(d, hi, v, hi_t, id_o);
 #pragma unroll
-      for (int part = 0; part < (SPLIT ? 3 : 1); ++part)
+      for (int part = 0; part < (SPLIT ? 3 : 1); ++part) {
+        const uint32_t d = tmem + (part == 0 ? P::O_COL + 128 * x : P::OLO_COL);
 #pragma unroll
-        for (int s = part == 0 ? 1 : 0; s < kTok / 16; ++s)
-          tc_mma_ts2<true>(d, (part == 1 ? lo : hi) + 8 * s,
-                           v + (part == 2 ? P::V / 16 : 0) + s * 16, hi_t, id_o);
+        for (int s = 0; s < kTok / 16; ++s) {
+          const uint32_t ap = p + P::P_STEP * (s / 2) + 8 * (s % 2) + (part == 1 ? 16 : 0);
+          const uint32_t bv = v + (part == 2 ? P::V / 16 : 0) + s * 16;
+          if (part < 2 && s == 0 && j == 0)
+            tc_mma_ts2<false>(d, ap, bv, hi_t, id_o);
+          else
+            tc_mma_ts2<true>(d, ap, bv, hi_t, id_o);
+        }
+      }
     };
     bool ok = wait(sh, &sh.q_full, 0, 1011) && (n == 0 || wait(sh, &sh.k_full[0], 0, 1006));
     if (ok && n > 0) {
