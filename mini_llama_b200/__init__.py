@@ -420,7 +420,7 @@ def _aligned_rows(t):
     return t, stride
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=4096)
 def _paged_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim, device_id):
     n = ctypes.c_size_t()
     check(lib().mlb_paged_attention_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim,
@@ -594,7 +594,8 @@ def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offs
     """Attention of q [rows, n_heads, head_dim] (fp32 or bf16), each row over the
     positions of its sequence up to its own (mlb_paged_attention): one row per
     sequence while decoding, a few to check drafted tokens, many for a prompt.
-    scale defaults to 1 / sqrt(head_dim). A row that sees nothing gets zeros."""
+    scale defaults to 1 / sqrt(head_dim). A row that sees nothing gets zeros. out
+    must not share memory with q."""
     torch = _torch()
     who = "CudaPagedAttention"
     kv_cache._layer(who, layer)

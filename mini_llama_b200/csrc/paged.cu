@@ -58,8 +58,9 @@ __device__ __forceinline__ RowPlace place_of(const PagedCache& c, const PagedSeq
     s = q.n_seqs > 0 ? paged_find_seq(q, row) : -1;
     if (s < 0 || s >= q.n_seqs) return r;
   }
-  r.pos = q.seq_lens[s] - q.row_offsets[s + 1] + row;
-  if (r.pos < 0) return r;
+  const long long pos = (long long)q.seq_lens[s] - q.row_offsets[s + 1] + row;
+  if (pos < 0 || pos > 0x7fffffff) return r;  // more: offsets that decrease
+  r.pos = (int)pos;
   const int logical = r.pos / c.page_size;
   r.slot = r.pos - logical * c.page_size;
   if (logical < q.max_pages) r.page = q.table[(size_t)s * q.max_pages + logical];

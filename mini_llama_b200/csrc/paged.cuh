@@ -245,7 +245,6 @@ __device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -329,20 +328,26 @@ __device__ __forceinline__ void query_words(const float (&e)[8], float sf, bool 
 
 // What a sequence asks for: its rows in tiles of tile_rows (token, head) rows, its
 // length in chunks of chunk_tokens, and their number with unit_slots more per (KV
-// head, tile). Lengths and offsets are cut to what the page
-// table and the call hold.
+// head, tile). Lengths and offsets are cut to what the page table and the call hold;
+// pos0, the position of row row0, is not.
 struct SeqWork {
   int len, n, row0, tiles, chunks;
-  long long cost;
+  long long pos0, cost;
 };
+// Positions that row row0 + i sees.
+__device__ __forceinline__ int seen_by(long long pos0, int i, int len) {
+  return (int)max(min(pos0 + i + 1, (long long)len), 0LL);
+}
 
 __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s, int tile_rows,
                                             int chunk_tokens, int unit_slots) {
   SeqWork w;
   const int cap = a.seqs.max_pages * a.cache.page_size;
-  w.len = min(max(a.seqs.seq_lens[s], 0), cap);
+  const int len = a.seqs.seq_lens[s], row1 = a.seqs.row_offsets[s + 1];
+  w.len = min(max(len, 0), cap);
   w.row0 = max(a.seqs.row_offsets[s], 0);
-  w.n = max(min(a.seqs.row_offsets[s + 1], a.seqs.n_rows) - w.row0, 0);
+  w.n = max(min(row1, a.seqs.n_rows) - w.row0, 0);
+  w.pos0 = (long long)len - row1 + w.row0;
   w.tiles = (int)(((long long)w.n * a.group + tile_rows - 1) / tile_rows);
   w.chunks = max(1, (w.len + chunk_tokens - 1) / chunk_tokens);
   w.cost = (long long)w.tiles * a.cache.kv * (w.chunks + unit_slots);

@@ -54,6 +54,7 @@ __host__ __device__ constexpr int dec_ctas(int nt) { return nt > 1 ? 3 : 4; }
 // Part of a CTA's run: chunks [chunk0, chunk1) of one (sequence, KV head, row tile).
 struct Seg {
   int seq, head, tile, chunk0, chunk1, chunks, len, n, row0, record;
+  long long pos0;
 };
 
 // a / b of non-negative numbers; 32-bit division where that will do (a quarter of the
@@ -71,7 +72,8 @@ __device__ __forceinline__ int shift_of(uint32_t d_bits) {
 }
 // NT 8-row tiles per unit. SPLIT: queries and P dV as hi + lo pairs.
 template <int G, int NT, class T>
-__global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kDecThreads, dec_ctas(NT))
+    paged_attn_decode_kernel(PagedAttnArgs a) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int R = 8 * NT;
   constexpr int MT = SPLIT ? NT : (NT + 1) / 2;
@@ -169,6 +171,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
       sg.len = sw.len;
       sg.n = sw.n;
       sg.row0 = sw.row0;
+      sg.pos0 = sw.pos0;
       sg.record = at == begin ? 0 : 1;
       if (threadIdx.x == 0) {
         segs[n_segs] = sg;
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT)) paged_attn_decode_k
         const bool live = flat < (long long)sg.n * a.group;
         const int i = live ? (int)quotient(flat, a.group) : 0;
         const int hq = sg.head * a.group + (live ? (int)(flat - (long long)i * a.group) : 0);
-        vis[t] = live ? max(sg.len - sg.n + i + 1, 0) : 0;
+        vis[t] = live ? seen_by(sg.pos0, i, sg.len) : 0;
         if (live) vis_min = min(vis_min, vis[t]);
         vis_max = max(vis_max, vis[t]);
         const T* row = live ? static_cast<const T*>(a.q) + (long long)(sg.row0 + i) * a.q_stride +
@@ -595,7 +598,8 @@ __global__ void __launch_bounds__(kDecThreads, 8) paged_attn_join_kernel(PagedAt
   const float* first = a.partial + ((size_t)(blockIdx.x - 1) * 2 + s0.y) * REC;
   const float* rest = a.partial + (size_t)blockIdx.x * 2 * REC;  // part p >= 1: + 2 (p - 1) REC
   auto rec = [&](int p) { return p == 0 ? first : rest + (size_t)(p - 1) * 2 * REC; };
-  // this warp's parts, six at a time (eight cost the registers of resident CTAs), each batch under the largest maximum so far
+  // this warp's parts, six at a time (eight cost the registers of resident CTAs), each
+  // batch under the largest maximum so far
   float mx = -INFINITY, sum = 0.0f, x[G];
 #pragma unroll
   for (int w = 0; w < G; ++w) x[w] = 0.0f;
@@ -762,6 +766,7 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
     if (n_rows > 0) {
       paged_check_rows(who, "q", q, q_stride, n_heads, head_dim, act_type);
       paged_check_rows(who, "out", out, out_stride, n_heads, head_dim, act_type);
+      if (q == out) invalid("CudaPagedAttention: q and out must not overlap");
     }
     DeviceScope scope(device_id);
     if (n_rows == 0 || n_seqs == 0) return;

@@ -12,10 +12,11 @@
 // fp16 scale in range), V as d q (or d q / 16 for 16 tokens whose scales reach
 // 4096, with P times 16), each off by at most half an fp16 step (2^-11), P the
 // same. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
-// products that count; the tensor cores cut what falls below the sum's last bit off, so
-// O takes only hi hi, one cut per 16 tokens, and the small products have a sum of their
-// own (a single sum was off by 1.5e-6 after 2000 tokens, this by 5e-7). ref is the row's maximum as of the last time that it rose
-// by more than a constant: only then is O brought to the new one.
+// products that count. The tensor cores cut off what falls below a sum's last bit,
+// so O takes only hi hi, one cut per 16 tokens, and the small products have a sum
+// of their own (with one sum the result was off by 1.5e-6 after 2000 tokens, now
+// by 5e-7). ref is the row's maximum as of the last time that it rose by more than
+// a constant: only then is O brought to the new one.
 //
 // Roles (13 warps, one CTA per SM):
 //   warps 0..3    widen K and V into shared memory (fp32 calls: warps 8..11 too)
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     const long long first = row0 + x * 128;
     if (first < rows) {
       const int tok = (int)(min(first + 127, rows - 1) / a.group);
-      steps[x] = (max(sw.len - sw.n + tok + 1, 0) + kTok - 1) / kTok;
+      steps[x] = (seen_by(sw.pos0, tok, sw.len) + kTok - 1) / kTok;
     }
   }
   const int n = max(steps[0], steps[1]);
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     const bool live = flat < rows;
     const int tok = live ? (int)(flat / a.group) : 0;
     // rows of no one hide nothing, so that their warps need not mask
-    const int vis = live ? max(sw.len - sw.n + tok + 1, 0) : 0x40000000;
+    const int vis = live ? seen_by(sw.pos0, tok, sw.len) : 0x40000000;
     const float rs = sh.row_scale[r];
     const int nx = steps[x];
     float ref = -INFINITY;

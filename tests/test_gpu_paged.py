@@ -345,6 +345,28 @@ def test_first_pages_missing(cuda, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,over", [(1, 1), (9, 4), (9, 40), (1200, 700)])
+def test_lengths_past_the_page_table(cuda, n, over, dtype):
+    """Rows keep their positions when the sequence has outgrown its table: they
+    see what the table holds up to their own."""
+    dtype = getattr(torch, dtype)
+    heads, kv, hd, page, held = 32, 4, 64, 32, 1600
+    seqs = R.Seqs([n], [held], page, seed=n)
+    cache, kk, vv = filled(seqs, kv, hd, over)
+    q = randn(gen(n), n, heads, hd, dtype=dtype)
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, seqs.offsets, seqs.seq_lens + over,
+                                            seqs.table, heads, kv, hd)
+    more = torch.zeros(over, kv, hd, device="cuda")
+    length = held + over
+    want, vabs, top = R.attention(q, torch.cat((kk, more)), torch.cat((vv, more)), length, n,
+                                  1 / math.sqrt(hd), absent=range(held, length))
+    prompt = R.prompt_form(n, 1, kv, heads // kv, dtype)
+    err = (out.double().cpu() - want).abs()
+    tol = R.attention_bound(want, vabs, top, length, dtype, prompt)
+    assert (err <= tol).all(), f"error {err.max():.3e}, worst ratio {(err / tol).max():.2f}"
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_strided_and_unaligned_rows(cuda, dtype):
     """Rows cut out of one projection's output, and at odd addresses."""
     dtype = getattr(torch, dtype)
@@ -545,6 +567,7 @@ def test_refusals(cuda):
     refused("does not match attention shape", lambda: A(q, cache, 0, *at, 4, 1, 64))
     refused("expected q", lambda: A(q, cache, 0, *at, 2, 2, 64))
     refused("out must be", lambda: A(q, cache, 0, *at, 4, 2, 64, out=q.bfloat16()))
+    refused("must not overlap", lambda: A(q, cache, 0, *at, 4, 2, 64, out=q))
     refused("scale must be finite", lambda: A(q, cache, 0, *at, 4, 2, 64, scale=math.inf))
     refused("cache is empty", lambda: A(q, mlb.CudaPagedKvCache(), 0, *at, 4, 2, 64))
     refused("multiple of 16", lambda: mlb.CudaPagedKvCache(1, 4, 24, 2, 64))

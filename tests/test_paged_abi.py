@@ -79,6 +79,7 @@ def test_attention_is_refused():
     err(attend(heads=0), "n_heads must be positive")
     err(attend(scale=float("inf")), "scale must be finite")
     err(attend(out=None), "null out")
+    err(attend(out=P), "must not overlap")
     err(attend(qs=255), "row stride of q is smaller than a row")
     err(attend(table=None), "page_table")
     err(attend(layer=9), "layer out of range", -2)
