@@ -264,10 +264,12 @@ int mlb_paged_kv_read(const void* pages_dev, int n_layers, int n_pages, int page
  * ragged sequences; GQA head map h / (n_heads / n_kv_heads)): one row per
  * sequence while decoding, a few to check drafted tokens, many for a prompt. A
  * row that sees nothing gets zeros. q and out may not overlap. The workspace
- * (16-byte aligned, mlb_paged_attention_workspace bytes, contents irrelevant)
- * belongs to the call until it has finished on the device. */
+ * (16-byte aligned, mlb_paged_attention_workspace bytes, contents irrelevant;
+ * null where that is 0) belongs to the call until it has finished on the
+ * device. */
 int mlb_paged_attention_workspace(int act_type, int n_rows, int n_seqs, int n_heads,
-                                  int n_kv_heads, int head_dim, int device_id, size_t* bytes);
+                                  int n_kv_heads, int head_dim, int page_size, int max_pages,
+                                  int device_id, size_t* bytes);
 int mlb_paged_attention(const void* pages_dev, int n_layers, int n_pages, int page_size,
                         int n_kv_heads, int head_dim, int layer, int act_type, const void* q_dev,
                         long long q_stride, int n_heads, int n_rows, int n_seqs,

@@ -301,11 +301,12 @@ def CudaLogProbs(logits, tokens, top_k=0, stream=None):
     stride = logits.stride(0) if rows > 1 else vocab
     if logits.stride(1) != 1 or stride < vocab:
         logits, stride = logits.contiguous(), vocab
-    dev = logits.device
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    # made like tensors at hand: torch.empty with a shape, a type and a device takes
+    # twice the time, and a row's call is bound by its time on the host
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    ids = tokens.new_empty(rows, top_k)
+    top = logprob.new_empty(rows, top_k)
     check(lib().mlb_logprobs(act, logits.data_ptr(), stride, rows, vocab, tokens.data_ptr(), top_k,
                              logprob.data_ptr(), entropy.data_ptr(), ids.data_ptr(),
                              top.data_ptr(), index, _raw_stream(index)))
@@ -421,10 +422,11 @@ def _aligned_rows(t):
 
 
 @functools.lru_cache(maxsize=4096)
-def _paged_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim, device_id):
+def _paged_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, max_pages,
+                     device_id):
     n = ctypes.c_size_t()
     check(lib().mlb_paged_attention_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim,
-                                              device_id, ctypes.byref(n)))
+                                              page_size, max_pages, device_id, ctypes.byref(n)))
     return n.value
 
 
@@ -536,7 +538,7 @@ class CudaPagedKvCache:
             _on_device(who, "q", q, self.device_id)
             heads = q.shape[1]
             if q_out is None:
-                q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = q.new_empty(rows, heads, dim)
                 qos = heads * dim
             else:
                 _on_device(who, "q_out", q_out, self.device_id)
@@ -570,8 +572,8 @@ class CudaPagedKvCache:
             return _on_stream(lambda: self.ReadDevice(layer, row_offsets, seq_lens, page_table,
                                                       n_rows), self.pages.device, stream)
         n_layers, n_pages, page_size, kv, dim = self._shape
-        k = torch.empty((n_rows, kv, dim), dtype=torch.float32, device=self.pages.device)
-        v = torch.empty((n_rows, kv, dim), dtype=torch.float32, device=self.pages.device)
+        k = self.pages.new_empty(n_rows, kv, dim, dtype=torch.float32)
+        v = torch.empty_like(k)
         check(lib().mlb_paged_kv_read(
             self.pages.data_ptr(), n_layers, n_pages, page_size, kv, dim, layer, n_rows, n_seqs,
             row_offsets.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), max_pages,
@@ -596,7 +598,6 @@ def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offs
     sequence while decoding, a few to check drafted tokens, many for a prompt.
     scale defaults to 1 / sqrt(head_dim). A row that sees nothing gets zeros. out
     must not share memory with q."""
-    torch = _torch()
     who = "CudaPagedAttention"
     kv_cache._layer(who, layer)
     n_layers, n_pages, page_size, kv, dim = kv_cache._shape
@@ -616,7 +617,7 @@ def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offs
             scale, out), q.device, stream)
     rows = q.shape[0]
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(rows, n_heads, head_dim)
         out_stride = n_heads * head_dim
     else:
         _on_device(who, "out", out, index)
@@ -624,13 +625,15 @@ def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offs
         if out_stride == 0:
             raise MlbError(-1, f"{who}: out must be shaped like q, with 16-byte aligned rows")
     q, q_stride = _aligned_rows(q)
-    size = _paged_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim, index)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    size = _paged_workspace(act, rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size,
+                            max_pages, index)
+    ws = kv_cache.pages.new_empty(size) if size else None
     check(lib().mlb_paged_attention(
         kv_cache.pages.data_ptr(), n_layers, n_pages, page_size, kv, dim, layer, act, q.data_ptr(),
         q_stride, n_heads, rows, n_seqs, row_offsets.data_ptr(), seq_lens.data_ptr(),
         page_table.data_ptr(), max_pages, head_dim ** -0.5 if scale is None else scale,
-        out.data_ptr(), out_stride, ws.data_ptr(), size, index, _raw_stream(index)))
+        out.data_ptr(), out_stride, ws.data_ptr() if size else None, size, index,
+        _raw_stream(index)))
     return out
 
 

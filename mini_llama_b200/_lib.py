@@ -71,7 +71,8 @@ SIGNATURES = [
     ("mlb_paged_kv_read", _c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                    _c_int, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp]),
     ("mlb_paged_attention_workspace", _c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                                               _c_int, ctypes.POINTER(_c_size_t)]),
+                                               _c_int, _c_int, _c_int,
+                                               ctypes.POINTER(_c_size_t)]),
     ("mlb_paged_attention", _c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                      _vp, _c_ll, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int,
                                      _c_float, _vp, _c_ll, _vp, _c_size_t, _c_int, _vp]),

@@ -146,6 +146,7 @@ struct PagedAttnArgs {
   long long q_stride, out_stride;
   int n_heads, group;
   float scale_log2;  // scale * log2(e)
+  bool whole;        // decode form: no unit is cut between CTAs (and neither of these is used)
   int4* split;       // decode form, per CTA: {parts, first record, head, tile}, {row0, rows}
   float* partial;    // decode form, per CTA: two records of R x (32 G) + 2 R floats
 };
@@ -327,11 +328,12 @@ __device__ __forceinline__ void query_words(const float (&e)[8], float sf, bool 
 }
 
 // What a sequence asks for: its rows in tiles of tile_rows (token, head) rows, its
-// length in chunks of chunk_tokens, and their number with unit_slots more per (KV
-// head, tile). Lengths and offsets are cut to what the page table and the call hold;
-// pos0, the position of row row0, is not.
+// length in chunks of chunk_tokens, and what its units, one per (KV head, tile), take
+// up in the runs: their chunks and unit_slots more, or 1 where they stay whole.
+// Lengths and offsets are cut to what the page table and the call hold; pos0, the
+// position of row row0, is not.
 struct SeqWork {
-  int len, n, row0, tiles, chunks;
+  int len, n, row0, tiles, chunks, slots;
   long long pos0, cost;
 };
 // Positions that row row0 + i sees.
@@ -350,7 +352,8 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s, int t
   w.pos0 = (long long)len - row1 + w.row0;
   w.tiles = (int)(((long long)w.n * a.group + tile_rows - 1) / tile_rows);
   w.chunks = max(1, (w.len + chunk_tokens - 1) / chunk_tokens);
-  w.cost = (long long)w.tiles * a.cache.kv * (w.chunks + unit_slots);
+  w.slots = a.whole ? 1 : w.chunks + unit_slots;
+  w.cost = (long long)w.tiles * a.cache.kv * w.slots;
   return w;
 }
 

@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT))
   const int nrun = (int)min((long long)gridDim.x, total);
   int4* split = a.split + 2 * cta;
   if (cta >= nrun) {
-    if (threadIdx.x == 0) split[0] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0 && !a.whole) split[0] = make_int4(0, 0, 0, 0);
     return;
   }
   const long long begin = run_begin(total, cta, nrun), end = run_begin(total, cta + 1, nrun);
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT))
   int seq = found_seq;
   long long base = found_base;
   SeqWork sw = seq_work(a, seq, R, kChunkTokens, kUnitSlots);
-  if (threadIdx.x == 0) split[0] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0 && !a.whole) split[0] = make_int4(0, 0, 0, 0);
 
   uint8_t* ring = smem + warp * (kStages * BLOCK);
   const int bpp = a.cache.page_size / kPagedBlock;
@@ -154,11 +154,10 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT))
         ++seq;
         sw = seq_work(a, seq, R, kChunkTokens, kUnitSlots);
       }
-      const int slots = sw.chunks + kUnitSlots;
-      const long long u = quotient(at - base, slots);  // unit within the sequence
-      const long long unit_begin = base + u * slots;
+      const long long u = quotient(at - base, sw.slots);  // unit within the sequence
+      const long long unit_begin = base + u * sw.slots;
       if (at - unit_begin >= sw.chunks) {  // the slots past its chunks stand for its ends
-        at = unit_begin + slots;
+        at = unit_begin + sw.slots;
         continue;
       }
       Seg sg;
@@ -166,7 +165,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT))
       sg.head = (int)quotient(u, sw.tiles);
       sg.tile = (int)(u - (long long)sg.head * sw.tiles);
       sg.chunk0 = (int)(at - unit_begin);
-      sg.chunk1 = (int)min((long long)sw.chunks, end - unit_begin);
+      sg.chunk1 = a.whole ? sw.chunks : (int)min((long long)sw.chunks, end - unit_begin);
       sg.chunks = sw.chunks;
       sg.len = sw.len;
       sg.n = sw.n;
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas(NT))
         }
       }
       ++n_segs;
-      at = unit_begin + sg.chunk1;
+      at = unit_begin + (a.whole ? 1 : sg.chunk1);
     }
     if (n_segs == 0) break;
     __syncthreads();
@@ -688,6 +687,16 @@ bool prompt_form(int act, int n_rows, int n_seqs, int kv, int group, int sms) {
   return prompt < decode;
 }
 
+// Whether units stay whole, so that the second kernel and the workspace fall away:
+// where the page table holds 256 tokens, or 512 and there are 64 units. A CTA takes
+// about 13 us per 1000 tokens of a unit. Measured, whole / cut us, fp32, 32 heads over 8
+// KV heads, one row each: 1 sequence of 128 tokens 7.4 / 9.5, of 256 9.3 / 9.5, of 500
+// 12.6 / 9.6; 8 sequences of 500 13.1 / 13.5, of 1000 19.9 / 13.8; 64 of 500 21.0 / 26.6.
+bool whole_units(int max_pages, int page_size, int n_seqs, int kv) {
+  const long long tokens = (long long)max_pages * page_size;
+  return tokens <= 256 || (tokens <= 512 && (long long)n_seqs * kv >= 64);
+}
+
 size_t dec_workspace(int grid, int groups, int nt) {
   const size_t rec = (size_t)8 * nt * 32 * groups + 16 * nt;
   return (size_t)grid * (2 * sizeof(int4) + 2 * rec * sizeof(float));
@@ -700,6 +709,7 @@ void launch_decode(const PagedAttnArgs& a, int grid, int device_id, cudaStream_t
   allow_smem(paged_attn_decode_kernel<G, NT, T>, smem, device_id);
   paged_attn_decode_kernel<G, NT, T><<<grid, kDecThreads, smem, stream>>>(a);
   MLB_CUDA(cudaGetLastError());
+  if (a.whole) return;
   launch_pdl(paged_attn_join_kernel<G, NT, T>, dim3(grid, 8 * NT), dim3(kDecThreads), 0, stream,
              true, a);
 }
@@ -731,18 +741,23 @@ void check_heads(const char* who, int n_heads, int kv) {
 using namespace mlb;
 
 extern "C" int mlb_paged_attention_workspace(int act_type, int n_rows, int n_seqs, int n_heads,
-                                             int n_kv_heads, int head_dim, int device_id,
-                                             size_t* bytes) {
+                                             int n_kv_heads, int head_dim, int page_size,
+                                             int max_pages, int device_id, size_t* bytes) {
   return guarded([&] {
     const char* who = "CudaPagedAttention";
     if (!bytes) invalid("CudaPagedAttention: null output");
     paged_check_act(who, act_type);
-    paged_check_shape(who, kPagedBlock, n_kv_heads, head_dim);
+    paged_check_shape(who, page_size, n_kv_heads, head_dim);
     check_heads(who, n_heads, n_kv_heads);
     if (n_rows < 0 || n_seqs < 0) invalid("CudaPagedAttention: negative row or sequence count");
+    if (max_pages <= 0) invalid("CudaPagedAttention: page_table must have at least one column");
     DeviceScope scope(device_id);
-    const int nt = dec_tiles(n_rows, n_seqs, n_heads / n_kv_heads);
-    *bytes = dec_workspace(dec_grid(sm_count(device_id), nt), paged_groups(head_dim), nt);
+    const int group = n_heads / n_kv_heads, sms = sm_count(device_id);
+    const int nt = dec_tiles(n_rows, n_seqs, group);
+    *bytes = n_rows == 0 || n_seqs == 0 || whole_units(max_pages, page_size, n_seqs, n_kv_heads) ||
+                     prompt_form(act_type, n_rows, n_seqs, n_kv_heads, group, sms)
+                 ? 0
+                 : dec_workspace(dec_grid(sms, nt), paged_groups(head_dim), nt);
   });
 }
 
@@ -777,25 +792,32 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
     a.n_heads = n_heads;
     a.group = n_heads / n_kv_heads;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const int groups = paged_groups(head_dim);
-    const int nt = dec_tiles(n_rows, n_seqs, a.group);
-    const int most = dec_grid(sm_count(device_id), nt);
-    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
-        workspace_bytes < dec_workspace(most, groups, nt))
-      invalid("CudaPagedAttention: workspace is null, unaligned or too small");
-    a.split = static_cast<int4*>(workspace);
-    a.partial = reinterpret_cast<float*>(a.split + 2 * (size_t)most);
-    // no more CTAs than chunks that the page table and the rows can make
-    const long long tiles =
-        ((long long)n_rows * a.group + 8 * nt - 1) / (8 * nt) + n_seqs;
-    const long long chunks =
-        ((long long)max_pages * page_size + kChunkTokens - 1) / kChunkTokens;
-    const int grid = (int)std::min<long long>(most, tiles * n_kv_heads * chunks);
+    a.whole = false;
+    a.split = nullptr;
+    a.partial = nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (prompt_form(act_type, n_rows, n_seqs, n_kv_heads, a.group, sm_count(device_id))) {
+    const int sms = sm_count(device_id);
+    if (prompt_form(act_type, n_rows, n_seqs, n_kv_heads, a.group, sms)) {
       paged_prompt_launch(a, act_type, device_id, s);
       return;
     }
+    const int groups = paged_groups(head_dim);
+    const int nt = dec_tiles(n_rows, n_seqs, a.group);
+    const int most = dec_grid(sms, nt);
+    a.whole = whole_units(max_pages, page_size, n_seqs, n_kv_heads);
+    if (!a.whole) {
+      if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+          workspace_bytes < dec_workspace(most, groups, nt))
+        invalid("CudaPagedAttention: workspace is null, unaligned or too small");
+      a.split = static_cast<int4*>(workspace);
+      a.partial = reinterpret_cast<float*>(a.split + 2 * (size_t)most);
+    }
+    // no more CTAs than units or chunks that the page table and the rows can make
+    const long long tiles =
+        ((long long)n_rows * a.group + 8 * nt - 1) / (8 * nt) + n_seqs;
+    const long long chunks =
+        a.whole ? 1 : ((long long)max_pages * page_size + kChunkTokens - 1) / kChunkTokens;
+    const int grid = (int)std::min<long long>(most, tiles * n_kv_heads * chunks);
     if (act_type == MLB_ACT_BF16)
       decode_dispatch<__nv_bfloat16>(a, groups, nt, grid, device_id, s);
     else

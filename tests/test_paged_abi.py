@@ -85,9 +85,11 @@ def test_attention_is_refused():
     err(attend(layer=9), "layer out of range", -2)
     n = ctypes.c_size_t()
     f = _lib.lib().mlb_paged_attention_workspace
-    err(f(0, 1, 1, 4, 2, 64, 0, None), "null output")
-    err(f(5, 1, 1, 4, 2, 64, 0, ctypes.byref(n)), "unknown activation type")
-    err(f(0, -1, 1, 4, 2, 64, 0, ctypes.byref(n)), "negative row or sequence count")
+    err(f(0, 1, 1, 4, 2, 64, 16, 8, 0, None), "null output")
+    err(f(5, 1, 1, 4, 2, 64, 16, 8, 0, ctypes.byref(n)), "unknown activation type")
+    err(f(0, 1, 1, 4, 2, 64, 16, 0, 0, ctypes.byref(n)), "page_table")
+    err(f(0, 1, 1, 4, 2, 64, 24, 8, 0, ctypes.byref(n)), "multiple of 16")
+    err(f(0, -1, 1, 4, 2, 64, 16, 8, 0, ctypes.byref(n)), "negative row or sequence count")
 
 
 def read(**kw):
