@@ -117,6 +117,37 @@ def test_append_one_token_at_a_time_is_the_same_cache(cuda):
     assert torch.equal(one.pages, whole.pages)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rope", ["normal", "neox", "none"])
+@pytest.mark.parametrize("heads,kv,hd", [(5, 2, 128), (3, 3, 40), (7, 1, 8), (2, 3, 96),
+                                         (6, 6, 48)])
+def test_append_of_many_rows_is_that_of_few(cuda, heads, kv, hd, rope, dtype):
+    """More rows than 8 per SM go another way: the same bits as in calls of 400,
+    rows of no position among them."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n, page = 8 * sms + 37, 32
+    seqs = R.Seqs([n], [n - 3], page, seed=heads)  # three rows are before position 0
+    g = gen(hd)
+    dtype = getattr(torch, dtype)
+    rope = {**ROPE, "none": mlb.ROPE_NONE}[rope]
+    rows = n + 5  # and five behind the last sequence
+    q, k, v = (randn(g, rows, h, hd, dtype=dtype) for h in (heads, kv, kv))
+    table = seqs.table.clone()
+    table[0, 3] = seqs.n_pages  # not in the pool
+    many, few = (mlb.CudaPagedKvCache(1, seqs.n_pages, page, kv, hd) for _ in range(2))
+    out = torch.full_like(q, 7.0)
+    many.AppendDevice(0, k, v, seqs.offsets, seqs.seq_lens, table, rope_type=rope, q=q, q_out=out)
+    assert (out[:3] == 7).all() and (out[n:] == 7).all()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for r in range(0, n, 400):
+        e = min(r + 400, n)
+        part = few.AppendDevice(0, k[r:e], v[r:e], torch.tensor([0, e - r], **i32),
+                                torch.tensor([e - 3], **i32), table, rope_type=rope, q=q[r:e])
+        first = 3 if r == 0 else 0
+        assert torch.equal(out[r + first:e], part[first:])
+    assert torch.equal(many.pages, few.pages)
+
+
 def test_rows_that_belong_to_no_position_are_left_alone(cuda):
     """Rows behind the last sequence, at negative positions, past the table and
     on pages outside the pool."""
