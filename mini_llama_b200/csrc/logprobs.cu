@@ -23,6 +23,13 @@
 // A row is one CTA, or a cluster of up to 8 when there are too few rows to fill
 // the GPU; a cluster's CTAs take one slice each and rank 0 joins their sums and
 // lists through distributed shared memory, in rank order.
+//
+// Measured: 4095 bf16 rows of 32000, k = 1: 73 us, 3.6 TB/s; 64 fp32 rows of 152064,
+// k = 5: 14.8 us, 2.6 TB/s; one fp32 row of 128256, k = 20: 10.5 us. Of the first,
+// 20 us are what ends a row (joins, candidates), the rest the pass at 4.7 TB/s, bound
+// by issue: about six instructions per element, one of them an exponential. Short calls
+// are a chain of latencies: launch, load, join, candidates, cluster. A ring of
+// asynchronous copies in place of loads to registers was slower (82 us).
 #include <algorithm>
 
 #include "paged.cuh"

@@ -27,6 +27,13 @@
 // the softmax of the other runs, with K and V double-buffered. fp32 calls have one
 // row tile and S double-buffered.
 //
+// Measured: 4096 rows of 32 heads over 8 KV heads of 128 (bf16, one sequence): 186 us,
+// 740 TFLOP/s of the products that the mask leaves. A step of 2 x 128 rows x 128 tokens takes
+// 4650 cycles where its products alone take 2880: the rest is the softmax, 2050
+// cycles per row tile (exponentials, rounding and the loads from tensor memory),
+// which two tiles do not hide whole. Steps of 64 tokens (242 us), two threads per row
+// (227) and registers moved to the softmax warps (215) were slower.
+//
 // Every wait is bounded: on a timeout the waiting thread records
 // MLB_ERR_TIMEOUT in the device's status word (mlb_paged_attention_status) and
 // raises the CTA's abort flag; all roles leave their loops, the products in flight

@@ -259,6 +259,23 @@ def test_prompts(cuda, new, lens, heads, kv, hd, dtype):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (6, 6, 48), (4, 4, 96), (10, 2, 8)])
+@pytest.mark.parametrize("rows", [1, 5, 20])
+def test_short_tables(cuda, rows, heads, kv, hd, dtype):
+    """Tables of at most 256 or 512 tokens keep units whole; wider ones do not."""
+    dtype = getattr(torch, dtype)
+    for lens in ([5, 1, 250, 256, 16, 130, 20], [500, 37, 512] + list(range(20, 490, 13))):
+        seqs = R.Seqs([rows] * len(lens), lens, 16, seed=rows)
+        cache, kk, vv = filled(seqs, kv, hd, heads, pool=255)
+        q = randn(gen(hd), seqs.rows, heads, hd, dtype=dtype)
+        wide = torch.cat((seqs.table, torch.full_like(seqs.table, -1)), 1)
+        for table in (seqs.table, wide):
+            out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, seqs.offsets, seqs.seq_lens,
+                                                    table, heads, kv, hd)
+            check_attention(out, q, kk, vv, seqs, hd, dtype)
+
+
 def test_many_sequences(cuda):
     lens = [1 + (i * 37) % 90 for i in range(400)]
     new = [(i % 5 != 3) * 1 for i in range(400)]
