@@ -28,6 +28,9 @@ struct RopeRates {
 };
 
 constexpr int kAppendThreads = 128;
+// CTAs per SM: 64 registers, or the 96 that a NeoX key's eight pairs need (left to the
+// compiler, 80 to 128 registers: 256 rows 7.1 us instead of 5.7, 15878 rows 82 instead of 78).
+constexpr int append_ctas(bool neox) { return neox ? 5 : 8; }
 constexpr int kAppendWarps = kAppendThreads / 32;
 constexpr int kAppendRows = kAppendWarps;  // rows per CTA of a read at most: one warp looks up each
 
@@ -267,7 +270,7 @@ __device__ __forceinline__ void store_codes(uint8_t* block, int g, int tok, int 
 // the one at work and ahead of the row's place and rotation. Bound by that chain of
 // latencies: 3.7 us for one row (a launch alone takes 2.5), 5 to 6 us for 64.
 template <class T, bool NEOX>
-__global__ void __launch_bounds__(kAppendThreads, 5)
+__global__ void __launch_bounds__(kAppendThreads, append_ctas(NEOX))
     paged_append_kernel(AppendArgs<T> a, RopeRates rates) {
   __shared__ double2 cs[kPagedMaxHeadDim / 2];
   __shared__ RowPlace place;
@@ -346,12 +349,12 @@ __global__ void __launch_bounds__(kAppendThreads, 5)
 }
 
 // Many rows: one warp per row, so that its place and a lane's rotation are made once
-// for all heads, and every address is a step from the one before. 20480 bf16 rows of
-// 32 + 8 + 8 heads of 128: 82 us, 3.4 TB/s (the form for few rows with four rows per
-// CTA: 119 us). Bound by instruction issue and the conversions to and from 64 bits
-// (four per pair of dimensions, 16 a cycle per SM, 47 us of the 82).
+// for all heads, and every address is a step from the one before. 15878 bf16 rows of
+// 32 + 8 + 8 heads of 128: 78 us, 3.9 TB/s (the form for few rows with four rows per
+// CTA: 119 us). Bound by latency and the conversions to and from 64 bits (four per pair
+// of dimensions, 16 a cycle per SM: half of the time on their unit; issue slots 53 %).
 template <class T, bool NEOX>
-__global__ void __launch_bounds__(kAppendThreads)
+__global__ void __launch_bounds__(kAppendThreads, append_ctas(NEOX))
     paged_append_rows_kernel(AppendArgs<T> a, RopeRates rates) {
   constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2;  // 64 bytes per lane on their way
   __shared__ double2 cs[kAppendWarps][kPagedMaxHeadDim / 2];
