@@ -14,8 +14,8 @@
 // same. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
 // products that count. The tensor cores cut off what falls below a sum's last bit,
 // so O takes only hi hi, one cut per 16 tokens, and the small products have a sum
-// of their own (with one sum the result was off by 1.5e-6 after 2000 tokens, now
-// by 5e-7). ref is the row's maximum as of the last time that it rose by more than
+// of their own (with one sum results over 700 tokens were off by 1.5e-6, now by
+// 5e-7). ref is the row's maximum as of the last time that it rose by more than
 // a constant: only then is O brought to the new one.
 //
 // Roles (13 warps, one CTA per SM):
