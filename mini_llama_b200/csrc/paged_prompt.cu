@@ -51,13 +51,19 @@ constexpr int kTok = 128;  // tokens per step
 constexpr int kThreads = 13 * 32;
 constexpr int kMmaWarp = 12;
 constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
-// P = 2^(s - ref + lift). With P up to 2^11, and 2^15 with the 16 of large V scales,
-// it stays within fp16, and what fp16 loses below 2^-14 is 2^-(25 + lift) of a token
-// at ref. fp32 calls look for the row's maximum first, and ref follows it when that
-// is more than kRise above. bf16 calls make P in one pass and, when the step's sum
-// exceeds 2^11 (128 tokens at ref come to 2^10), look for the maximum, raise ref to
-// it and make P again.
-constexpr float kRise = 4.0f, kMostP = 2048.0f;
+// P = 2^((S - ref) rs + lift), rs >= 0 the row's scale. With P up to 2^11, and 2^15
+// with the 16 of large V scales, it stays within fp16, and what fp16 loses below 2^-14
+// is 2^-(25 + lift) of a token at ref. fp32 calls look for the row's maximum first, and
+// ref follows it when that is more than kRise above. bf16 calls make P in one pass and,
+// when the step's sum exceeds 2^11 (128 tokens at ref come to 2^10), look for the
+// maximum, raise ref to it and make P once more.
+// ref is a value of S, and the difference comes before the product: no P is above
+// 2^lift at ref's own value, however large the scores are. As S rs - ref rs with the
+// second product rounded P is off by up to half a step of ref rs, and from scores of
+// 2^28 on 2^11 and more. Below kFar that is 2^-12 of P: there one fused multiply-add
+// does, which spares the main path of bf16 calls an addition per two scores (4096 rows
+// of 32 heads: 189 us, 193 with it).
+constexpr float kRise = 4.0f, kMostP = 2048.0f, kFar = 8192.0f;
 
 __device__ DeviceStatus g_status;
 
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         return m;
       };
 
-      // largest score of the step, scaled (rs >= 0)
+      // largest S of the step
       auto step_max = [&]() {
         float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll 1
@@ -426,12 +432,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             m1 = fmaxf(m1, m >> (i + 1) & 1 ? v[i + 1] : -INFINITY);
           }
         }
-        const float top = fmaxf(m0, m1);
-        return top == -INFINITY ? top : top * rs;
+        return fmaxf(m0, m1);
       };
       // brings ref of the lanes that rise, their sums and O to mx
       auto raise_to = [&](float mx, bool rise) {
-        const float f = !rise ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - mx);
+        const float f = !rise ? 1.0f : ref == -INFINITY ? 0.0f : ex2((ref - mx) * rs);
         if (rise) ref = mx;
         if (j == 0) return true;  // no O yet
         if (!wait(sh, &sh.o_done[x], j - 1, 1004)) return false;
@@ -458,10 +463,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       if constexpr (SPLIT) {
         // largest score first, then P as it is made
         const float mx = step_max();
-        const bool rise = mx > ref + kRise;
+        const bool rise = ref == -INFINITY ? mx > ref : (mx - ref) * rs > kRise;
         if (__any_sync(0xffffffffu, rise)) ok = raise_to(mx, rise);
         if (!ok) break;
-        const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
+        const float from = ref == -INFINITY ? 0.0f : -ref;
 #pragma unroll 1
         for (int ch = 0; ch < 4; ++ch) {
           float v[32];
@@ -470,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 p = fma2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(rs, rs),
-                            make_float2(neg, neg));
+            float2 p = fma2(add2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(from, from)),
+                            make_float2(rs, rs), make_float2(kLift, kLift));
             p.x = m >> (2 * i) & 1 ? ex2(p.x) : 0.0f;
             p.y = m >> (2 * i + 1) & 1 ? ex2(p.y) : 0.0f;
             if (i & 1)
@@ -496,14 +501,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           ok = raise_to(mx, ref == -INFINITY && mx > ref);
           if (!ok) break;
         }
+        // nothing to mask, and no ref so large that its product's rounding would tell
+        bool plain = whole && big == 0 && __all_sync(0xffffffffu, fabsf(ref * rs) < kFar);
         uint32_t hi[4][16];
-        while (true) {
-          const float neg = ref == -INFINITY ? 0.0f : kLift - ref;
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+          const float neg = fmaf(-ref, rs, kLift);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           auto pass = [&](auto plain_c) {
             constexpr bool PLAIN = decltype(plain_c)::value;
             // 32 tokens on their way while 32 are worked on (products slow the loads
             // down to about the time that this takes)
+            const float from = ref == -INFINITY ? 0.0f : -ref;
             uint32_t u[2][32];
             tmem_ld32_start(s_at, u[0]);
 #pragma unroll
@@ -519,10 +528,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
                   vx = m >> (2 * i) & 1 ? vx : -INFINITY;
                   vy = m >> (2 * i + 1) & 1 ? vy : -INFINITY;
                 }
-                float2 p = fma2(make_float2(vx, vy), make_float2(rs, rs), make_float2(neg, neg));
+                float2 p = make_float2(vx, vy);
+                if (PLAIN)
+                  p = fma2(p, make_float2(rs, rs), make_float2(neg, neg));
+                else
+                  p = fma2(add2(p, make_float2(from, from)), make_float2(rs, rs),
+                           make_float2(kLift, kLift));
                 p.x = ex2(p.x);
                 p.y = ex2(p.y);
-                if (!PLAIN) {  // -inf times rs = 0
+                if (!PLAIN) {  // -inf times rs = 0, or less ref = -inf
                   p.x = m >> (2 * i) & 1 ? p.x : 0.0f;
                   p.y = m >> (2 * i + 1) & 1 ? p.y : 0.0f;
                 }
@@ -535,14 +549,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
               }
             }
           };
-          if (whole && big == 0)
+          if (plain)
             pass(std::true_type{});
           else
             pass(std::false_type{});
           // no P above the sum, so none that fp16 does not hold; looking for the maximum
-          // as well would cost a sixth of the pass
+          // as well would cost a sixth of the pass. One more pass at most: after it ref is
+          // the maximum, and what is still too large is infinite or no number
           const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          if (!__any_sync(0xffffffffu, all > kMostP)) {
+          if (again || !__any_sync(0xffffffffu, all > kMostP)) {
             l0 = add2(l0, sum[0]);
             l1 = add2(l1, sum[1]);
             break;
@@ -550,6 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
           const float mx = step_max();
           ok = raise_to(mx, mx > ref);
           if (!ok) break;
+          plain = false;
         }
         if (!ok) break;
 #pragma unroll

@@ -1,0 +1,110 @@
+"""Paged attention where its number formats end: scores far past what an fp32 exponent
+resolves. Both forms of the kernel, against 64-bit attention within the bound that
+paged_ref derives."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+import mini_llama_b200 as mlb  # noqa: E402
+from tests import paged_ref as R  # noqa: E402
+from tests.test_gpu_paged import gen, randn  # noqa: E402
+
+
+@pytest.fixture(autouse=True)
+def no_timeouts():
+    yield
+    assert mlb.paged_attention_status() == (0, 0)
+
+
+def stored(seqs, k, v):
+    """A cache that holds k and v, and the values its codes stand for."""
+    cache = mlb.CudaPagedKvCache(1, seqs.n_pages, seqs.page, k.shape[1], k.shape[2])
+    cache.AppendDevice(0, k, v, *seqs.whole(), rope_type=mlb.ROPE_NONE)
+    return (cache, *cache.ReadDevice(0, *seqs.whole(), seqs.total))
+
+
+# rows of a call whose 8 heads over 2 KV heads take the decode form (1, 6) or the prompt form
+ROWS = [1, 6, 1200]
+
+
+def both_forms(n, dtype):
+    assert R.prompt_form(n, 1, 2, 4, dtype) == (n == 1200)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e7, 1e8, 3e9, 1e12, 1e25])
+def test_scores_of_any_size(cuda, size, n, dtype):
+    """A query is one dimension, so a score is one product, exact in fp32, and equal
+    keys tie exactly. Scores of unlike keys are hundreds apart or more: a row is the
+    mean of the values whose keys tie at the top, whatever the scores' size."""
+    dtype = getattr(torch, dtype)
+    both_forms(n, dtype)
+    hd, length = 64, 1300
+    seqs = R.Seqs([n], [length], 32, seed=n)
+    g = gen(53)
+    # keys of one scale (7 in every block), so integers, each token with its twin
+    k = torch.randint(-5, 6, (length // 2, 2, hd), device="cuda", generator=g).float()
+    k[:, :, 1::32] = 7.0
+    top = torch.rand(length // 2, device="cuda", generator=g) < 0.01
+    k[:, :, 0] = torch.where(top[:, None], 7.0, k[:, :, 0])
+    k = k.repeat(2, 1, 1)
+    cache, kk, vv = stored(seqs, k, randn(g, length, 2, hd))
+    assert torch.equal(kk, k)
+    q = torch.zeros(n, 8, hd, device="cuda")
+    q[:, :, 0] = (1 + torch.rand(n, 8, device="cuda", generator=g)) * size
+    q[:, ::3, 0] *= -1
+    q = q.bfloat16().to(dtype)
+    scale = 1.7
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, hd, scale=scale)
+    want, vabs, (_, vmax) = R.attention(q, kk, vv, length, n, scale)
+    # scores bring no error: neither the tied ones' differences, 0, nor the others' p, 0
+    none = torch.zeros(n, 8, 1, dtype=torch.float64)
+    tol = R.attention_bound(want, vabs, (none, vmax), length, dtype, n == 1200)
+    err = (out.double().cpu() - want).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), f"error {err.max():.3e}, worst ratio {(err / tol).max():.2f}"
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("size,scale", [(1e6, 0.1), (1e9, 0.1), (1.0, 1e10), (1e30, 1e-20)])
+def test_outputs_stay_within_the_values(cuda, size, scale, n, dtype):
+    """Whatever the scores, a row's result is a mean of the values that it sees."""
+    dtype = getattr(torch, dtype)
+    hd, length = 128, 1300
+    seqs = R.Seqs([n], [length], 32, seed=n)
+    g = gen(54)
+    cache, _, vv = stored(seqs, randn(g, length, 2, hd), randn(g, length, 2, hd))
+    q = (randn(g, n, 8, hd) * size).to(dtype)
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, hd, scale=scale)
+    low, high = (getattr(vv, f)(0)[None].repeat_interleave(4, 1) for f in ("amin", "amax"))
+    # P and V are rounded to fp16 at worst, the sum cut once per 16 tokens, the result
+    # rounded to its type
+    slack = vv.abs().max() * (2.0 ** -11 + 2.0 ** -11 + 82 * 2.0 ** -23 + 2.0 ** -8)
+    assert (out >= low - slack).all() and (out <= high + slack).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", ROWS[1:])
+def test_rows_that_are_no_numbers_keep_to_themselves(cuda, n, dtype):
+    """Infinite and NaN queries: the call ends, and other rows are what they were."""
+    dtype = getattr(torch, dtype)
+    hd, length = 128, 1300
+    seqs = R.Seqs([n], [length], 32, seed=n)
+    g = gen(55)
+    cache, kk, vv = stored(seqs, randn(g, length, 2, hd), randn(g, length, 2, hd))
+    q = randn(g, n, 8, hd, dtype=dtype)
+    want, vabs, top = R.attention(q, kk, vv, length, n, 0.1)
+    good = torch.ones(n, 8, dtype=torch.bool)
+    for row, head, dim, x in ((0, 0, 3, "inf"), (2, 1, 127, "-inf"), (n - 1, 7, 0, "nan"),
+                              (n // 2, 4, slice(None), "inf"), (n // 2, 5, slice(None), "nan")):
+        q[row, head, dim] = float(x)
+        good[row, head] = False
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, hd, scale=0.1)
+    tol = R.attention_bound(want, vabs, top, length, dtype, n == 1200)
+    err = (out.double().cpu() - want).abs()
+    assert (err <= tol)[good].all()
+    assert not torch.isfinite(out.cpu()[~good]).any()
