@@ -8,10 +8,11 @@
 //   O += P V (fp32 in tensor memory)
 //
 // Here, unlike in the decode form, codes are widened to fp16 with their scales,
-// once for all rows of the tile: K is stored as d q / 16 (the shift keeps any
-// fp16 scale in range), V as d q (or d q / 16 for 16 tokens whose scales reach
-// 4096, with P times 16), each off by at most half an fp16 step (2^-11), P the
-// same. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
+// once for all rows of the tile, as d q. That is a whole multiple of 2^-24, so small
+// scales lose nothing, and off by at most half an fp16 step (2^-11) otherwise. d q / 16
+// where a scale reaches 4096: for K by token, with its S times 16 (a group of such a
+// token whose scale is below 2^-10 is off by up to 2^-36 of the token's largest key), for
+// V by 16 tokens, with their P times 16. P is off by half a step, too. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
 // products that count. The tensor cores cut off what falls below a sum's last bit,
 // so O takes only hi hi, one cut per 16 tokens, and the small products have a sum
 // of their own (with one sum results over 700 tokens were off by 1.5e-6, now by
@@ -65,6 +66,9 @@ constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
 // of 32 heads: 189 us, 193 with it).
 constexpr float kRise = 4.0f, kMostP = 2048.0f, kFar = 8192.0f;
 
+constexpr uint32_t kBigV = 1, kBigK = 2;
+constexpr uint32_t kLargeScale = 0x6C00u;  // 4096 as fp16
+
 __device__ DeviceStatus g_status;
 
 // Shape of one instantiation: bytes of its parts of shared memory.
@@ -105,9 +109,11 @@ struct Shared {
   int abort_flag;
   uint32_t tmem;
   float row_scale[256];
-  // per step & 3, one byte per block: without a page; with large V scales
+  // per step & 3, one byte per block: without a page; kBigV with large V scales, kBigK
+  // with large K scales, whose tokens are the bits of k_big
   alignas(8) uint8_t absent[4][8];
   alignas(8) uint8_t big[4][8];
+  alignas(4) uint16_t k_big[4][8];
 };
 
 // Bounded wait that also gives up when another thread did.
@@ -249,14 +255,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             }
           }
         }
-        // K: the scale of token kg in both halves, shifted by 2^-4
-        __half2 dmax = u32_as_h2(0u);
+        // K: the scale of token kg in both halves
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int w = 0; w < G; ++w)
-            ks[i][h][w] = h2_as_u32(__hmul2(
-                u32_as_h2(__byte_perm(ks[i][h][w], 0, kg & 1 ? 0x3232 : 0x1010)), sixteenth));
+            ks[i][h][w] = __byte_perm(ks[i][h][w], 0, kg & 1 ? 0x3232 : 0x1010);
         // scales of tokens that are not there: 0, whatever their codes
         if (page < 0 || (bl + 1) * kPagedBlock > sw.len) {
 #pragma unroll
@@ -273,22 +277,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             }
           }
         }
+        // large scales: a vote for all of them, the rest only where there are some
+        __half2 top = u32_as_h2(0u);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int w = 0; w < G; ++w) dmax = __hmax2(dmax, u32_as_h2(vs[i][h][w]));
-        const uint32_t db = h2_as_u32(dmax);
-        const bool big = __any_sync(0xffffffffu, max(db & 0xffffu, db >> 16) >= 0x6C00u);
-        if (big) {
+          for (int w = 0; w < G; ++w)
+            top = __hmax2(top, __hmax2(u32_as_h2(ks[i][h][w]), u32_as_h2(vs[i][h][w])));
+        const uint32_t tb = h2_as_u32(top);
+        uint32_t big = 0, k_big = 0;
+        if (__any_sync(0xffffffffu, max(tb & 0xffffu, tb >> 16) >= kLargeScale)) {
+          __half2 v_top = u32_as_h2(0u);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            uint32_t k_top = 0;
 #pragma unroll
-            for (int w = 0; w < G; ++w)
-              vs[i][h][w] = h2_as_u32(__hmul2(u32_as_h2(vs[i][h][w]), sixteenth));
+            for (int w = 0; w < G; ++w) {
+              k_top = max(k_top, ks[i][h][w]);
+              v_top = __hmax2(v_top, u32_as_h2(vs[i][h][w]));
+            }
+            const bool large = k_top >= kLargeScale << 16;
+            // lanes 0..7 stand for eight tokens
+            k_big |= (__ballot_sync(0xffffffffu, large) & 0xffu) << (8 * h);
+            if (large) {
+#pragma unroll
+              for (int w = 0; w < G; ++w)
+                ks[i][h][w] = h2_as_u32(__hmul2(u32_as_h2(ks[i][h][w]), sixteenth));
+            }
+          }
+          if (k_big) big |= kBigK;
+          const uint32_t vb = h2_as_u32(v_top);
+          if (__any_sync(0xffffffffu, max(vb & 0xffffu, vb >> 16) >= kLargeScale)) {
+            big |= kBigV;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int w = 0; w < G; ++w)
+                vs[i][h][w] = h2_as_u32(__hmul2(u32_as_h2(vs[i][h][w]), sixteenth));
+          }
         }
         if (lane == 0) {
           sh.absent[j & 3][b] = page < 0;
-          sh.big[j & 3][b] = big;
+          sh.big[j & 3][b] = (uint8_t)big;
+          sh.k_big[j & 3][b] = (uint16_t)k_big;
         }
       }
 
@@ -365,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         float e[G][8];
         load_query_elements<G, T>(row, a.cache.head_dim, c, e);
         const int sh2 = query_shift<G>(e);
-        if (c == 0) sh.row_scale[r0 + g] = pow2(-sh2) * sign * a.scale_log2 * 16.0f;
+        if (c == 0) sh.row_scale[r0 + g] = pow2(-sh2) * sign * a.scale_log2;
         const float sf = pow2(sh2) * sign;
         uint8_t* at = smem + P::Q0 + (r0 / 128) * PT * P::Q + (r0 % 128) / 8 * P::SBO_D + g * 16;
 #pragma unroll
@@ -418,8 +449,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         return m;
       };
 
+      // S of keys stored as d q / 16 times 16, once before anything looks at it (called
+      // where steps with large scales come by: in the main path the branch alone took 3 %)
+      bool s_done = (big & 0x0101010101010101ull * kBigK) == 0;
+      auto scale_s = [&]() {
+        if (s_done) return;
+        s_done = true;
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          const uint32_t k16 =
+              *reinterpret_cast<const volatile uint32_t*>(&sh.k_big[j & 3][2 * ch]);
+          float v[32];
+          tmem_ld32(s_at + 32 * ch, v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t u[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              u[i] = __float_as_uint(v[16 * h + i] * (k16 >> (16 * h + i) & 1 ? 16.0f : 1.0f));
+            tmem_st16(s_at + 32 * ch + 16 * h, u);
+          }
+        }
+        tmem_wait_st();
+      };
+
       // largest S of the step
       auto step_max = [&]() {
+        scale_s();
         float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll 1
         for (int ch = 0; ch < 4; ++ch) {
@@ -483,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
               l1 = add2(l1, p);
             else
               l0 = add2(l0, p);
-            const float up = big >> (16 * ch + 8 * (i >> 3)) & 0xff ? 16.0f : 1.0f;
+            const float up = big >> (16 * ch + 8 * (i >> 3)) & kBigV ? 16.0f : 1.0f;
             p = mul2(p, make_float2(up, up));
             hi[i] = pack_f16(p.x, p.y);
             const float2 h = __half22float2(u32_as_h2(hi[i]));
@@ -542,17 +598,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
                 }
                 sum[i & 1] = add2(sum[i & 1], p);
                 if (!PLAIN) {
-                  const float up = big >> (16 * ch + 8 * (i >> 3)) & 0xff ? 16.0f : 1.0f;
+                  const float up = big >> (16 * ch + 8 * (i >> 3)) & kBigV ? 16.0f : 1.0f;
                   p = mul2(p, make_float2(up, up));
                 }
                 hi[ch][i] = pack_f16(p.x, p.y);
               }
             }
           };
-          if (plain)
+          if (plain) {
             pass(std::true_type{});
-          else
+          } else {
+            scale_s();
             pass(std::false_type{});
+          }
           // no P above the sum, so none that fp16 does not hold; looking for the maximum
           // as well would cost a sixth of the pass. One more pass at most: after it ref is
           // the maximum, and what is still too large is infinite or no number

@@ -1,6 +1,6 @@
-"""Paged attention where its number formats end: scores far past what an fp32 exponent
-resolves. Both forms of the kernel, against 64-bit attention within the bound that
-paged_ref derives."""
+"""Paged attention where its number formats end: keys and queries of very different
+sizes, scores far past what an fp32 exponent resolves. Both forms of the kernel, against
+64-bit attention within the bound that paged_ref derives."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -9,7 +9,7 @@ torch = pytest.importorskip("torch")
 
 import mini_llama_b200 as mlb  # noqa: E402
 from tests import paged_ref as R  # noqa: E402
-from tests.test_gpu_paged import gen, randn  # noqa: E402
+from tests.test_gpu_paged import check_attention, gen, randn  # noqa: E402
 
 
 @pytest.fixture(autouse=True)
@@ -31,6 +31,41 @@ ROWS = [1, 6, 1200]
 
 def both_forms(n, dtype):
     assert R.prompt_form(n, 1, 2, 4, dtype) == (n == 1200)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4, 1e-6, 5e4])
+def test_keys_of_any_size(cuda, size, n, dtype):
+    """Queries are as large as keys are small, so that scores stay ordinary."""
+    dtype = getattr(torch, dtype)
+    both_forms(n, dtype)
+    seqs = R.Seqs([n], [1300], 32, seed=n)
+    g = gen(51)
+    cache, kk, vv = stored(seqs, randn(g, 1300, 2, 128) * size, randn(g, 1300, 2, 128))
+    q = (randn(g, n, 8, 128) * (2 / size)).to(dtype)
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, 128)
+    check_attention(out, q, kk, vv, seqs, 128, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("sizes", [(1e-2, 1e-3, 1e-4, 1e-5), (3e4, 3e3, 6e4, 5e2)])
+def test_keys_of_many_sizes_in_one_sequence(cuda, sizes, n, dtype):
+    """A token has keys in one of four groups of 32 dimensions, each group's of another
+    size and its queries to match: every score is ordinary whichever the token's size,
+    within a tile of tokens and within 16 neighbours."""
+    dtype = getattr(torch, dtype)
+    seqs = R.Seqs([n], [1300], 32, seed=n)
+    g = gen(52)
+    k = randn(g, 1300, 2, 4, 32)
+    group = torch.randint(4, (1300,), device="cuda", generator=g)
+    k *= torch.nn.functional.one_hot(group, 4)[:, None, :, None]
+    each = torch.tensor(sizes, device="cuda")[:, None]
+    cache, kk, vv = stored(seqs, (k * each).flatten(2), randn(g, 1300, 2, 128))
+    q = (randn(g, n, 8, 4, 32) * 4 / each).flatten(2).to(dtype)
+    out = mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, 128)
+    check_attention(out, q, kk, vv, seqs, 128, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
