@@ -348,7 +348,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s, int t
   const int len = a.seqs.seq_lens[s], row1 = a.seqs.row_offsets[s + 1];
   w.len = min(max(len, 0), cap);
   w.row0 = max(a.seqs.row_offsets[s], 0);
-  w.n = max(min(row1, a.seqs.n_rows) - w.row0, 0);
+  w.n = max(min(max(row1, 0), a.seqs.n_rows) - w.row0, 0);  // no difference wraps
   w.pos0 = (long long)len - row1 + w.row0;
   w.tiles = (int)(((long long)w.n * a.group + tile_rows - 1) / tile_rows);
   w.chunks = max(1, (w.len + chunk_tokens - 1) / chunk_tokens);

@@ -143,3 +143,35 @@ def test_rows_that_are_no_numbers_keep_to_themselves(cuda, n, dtype):
     err = (out.double().cpu() - want).abs()
     assert (err <= tol)[good].all()
     assert not torch.isfinite(out.cpu()[~good]).any()
+
+
+BOTTOM, TOP = -2 ** 31, 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [5, 4800])
+@pytest.mark.parametrize("offsets", [
+    (0, 3, TOP, -2, 5), (TOP, BOTTOM, TOP, -1, TOP), (-5, 2, BOTTOM, TOP, 3), (9, 7, 7, -1, -2)])
+@pytest.mark.parametrize("lens", [(40, 41, 42, 43), (BOTTOM, TOP, -1, 0)])
+@pytest.mark.parametrize("width", [3, 48])
+def test_offsets_and_lengths_of_any_value(cuda, width, lens, offsets, n, dtype):
+    """Nothing past the call's rows is written, whatever the arrays hold."""
+    dtype = getattr(torch, dtype)
+    kv, hd, page, heads = 2, 32, 16, 8
+    assert R.prompt_form(n, 4, kv, heads // kv, dtype) == (n > 5)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    where = (torch.tensor(offsets, **i32), torch.tensor(lens, **i32),
+             (torch.arange(4 * width, **i32) % 16).view(4, width))  # 12 .. 15: not in the pool
+    g = gen(56)
+    q, k, v = (randn(g, n, h, hd, dtype=dtype) for h in (heads, kv, kv))
+    cache = mlb.CudaPagedKvCache(3, 12, page, kv, hd)
+    cache.pages.fill_(85)
+    cache.pages[1] = 0
+    wide = torch.full((n + 64, heads, hd), 3.0, dtype=dtype, device="cuda")
+    out = wide[32:32 + n]
+    mlb.CudaPagedAttentionDeviceInput(q, cache, 1, *where, heads, kv, hd, out=out)
+    cache.AppendDevice(1, k, v, *where, q=q, q_out=out)
+    for x in cache.ReadDevice(1, *where, n):
+        assert torch.isfinite(x).all()
+    assert (wide[:32] == 3).all() and (wide[32 + n:] == 3).all()
+    assert (cache.pages[0] == 85).all() and (cache.pages[2] == 85).all()
