@@ -278,10 +278,18 @@ int mlb_paged_attention(const void* pages_dev, int n_layers, int n_pages, int pa
                         long long out_stride, void* workspace_dev, size_t workspace_bytes,
                         int device_id, void* stream);
 
-/* Waits in the prompt form of mlb_paged_attention are bounded; one that gave up
- * leaves its rows unwritten. Waits for the device, returns the last such
- * (MLB_ERR_TIMEOUT, site) since the call before, or (0, 0), and clears it. */
+/* Waits in the prompt form of mlb_paged_attention are bounded; where one gave up
+ * rows without a result become NaN. Waits for the device, returns the last such
+ * (MLB_ERR_TIMEOUT, site) since the call before, or (0, 0), and clears it; there is
+ * one such word per device, for all its streams. */
 int mlb_paged_attention_status(int device_id, int* code, int* where);
+/* Failure-detection self-test (as mlb_wait_selftest): runs the prompt form on 8 rows
+ * of its own with a barrier that never completes and waits of limit_ms (0 < limit_ms
+ * <= 1000). Writes the status recorded (MLB_ERR_TIMEOUT and a site, cleared as by
+ * mlb_paged_attention_status) and how many of the 8 rows are NaN; the device stays
+ * usable. Synchronous. */
+int mlb_paged_attention_wait_selftest(int device_id, int act_type, double limit_ms, int* code,
+                                      int* where, int* nan_rows);
 
 /* --------------------------------------------------------- prepared weights
  * A weight repacked once into the B200 GEMV layout (what the decode path

@@ -37,7 +37,7 @@ __all__ = [
     "CudaElementwiseAddDeviceInput", "CudaSoftmax", "CudaEmbeddingLookupDeviceWeight",
     "CudaRopeDeviceInput", "CudaArgMax", "CudaLogProbs", "CudaKvCache",
     "CudaAttentionDecodeDeviceInput", "CudaPagedKvCache", "CudaPagedAttentionDeviceInput",
-    "paged_attention_status",
+    "paged_attention_status", "paged_attention_wait_selftest",
     "QMatrix", "CudaModel", "Context", "Batch", "ForwardToken", "configs", "tp_plan", "nccl_unique_id",
 ]
 
@@ -584,10 +584,22 @@ class CudaPagedKvCache:
 def paged_attention_status(device_id=0):
     """(status code, site) of the last bounded wait that gave up in the prompt
     form of CudaPagedAttentionDeviceInput since the last call, (0, 0) if none
-    did (mlb_paged_attention_status). Waits for the device."""
+    did (mlb_paged_attention_status); rows without a result are NaN. Waits for
+    the device."""
     code, where = ctypes.c_int(0), ctypes.c_int(0)
     check(lib().mlb_paged_attention_status(device_id, ctypes.byref(code), ctypes.byref(where)))
     return code.value, where.value
+
+
+def paged_attention_wait_selftest(bf16=False, limit_ms: float = 1.0, device_id: int = 0):
+    """Runs the prompt form on 8 rows with a barrier that never completes and returns
+    (status code, site, rows that became NaN): (MLB_ERR_TIMEOUT, 1001 .. 1011, 8) when
+    its waits gave up after limit_ms (mlb_paged_attention_wait_selftest)."""
+    code, where, rows = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
+    check(lib().mlb_paged_attention_wait_selftest(device_id, int(bool(bf16)), float(limit_ms),
+                                                  ctypes.byref(code), ctypes.byref(where),
+                                                  ctypes.byref(rows)))
+    return code.value, where.value, rows.value
 
 
 def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offsets, seq_lens,

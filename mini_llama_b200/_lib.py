@@ -77,6 +77,8 @@ SIGNATURES = [
                                      _vp, _c_ll, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int,
                                      _c_float, _vp, _c_ll, _vp, _c_size_t, _c_int, _vp]),
     ("mlb_paged_attention_status", _c_int, [_c_int, _ip, _ip]),
+    ("mlb_paged_attention_wait_selftest", _c_int, [_c_int, _c_int, ctypes.c_double, _ip, _ip,
+                                                   _ip]),
     ("mlb_qmatrix_create", _c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _c_int,
                                     ctypes.POINTER(_vp)]),
     ("mlb_qmatrix_synthesize", _c_int, [_c_int, _c_int, _c_int, _c_u64, _c_u64, _c_int, _c_int,

@@ -149,6 +149,8 @@ struct PagedAttnArgs {
   bool whole;        // decode form: no unit is cut between CTAs (and neither of these is used)
   int4* split;       // decode form, per CTA: {parts, first record, head, tile}, {row0, rows}
   float* partial;    // decode form, per CTA: two records of R x (32 G) + 2 R floats
+  long long wait_cycles;  // prompt form: limit of a wait
+  int never;              // prompt form: arrivals that K's barriers wait for in vain (self-test)
 };
 
 // Prompt form (paged_prompt.cu): many rows per sequence.

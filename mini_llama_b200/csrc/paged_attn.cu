@@ -802,6 +802,8 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
     a.whole = false;
     a.split = nullptr;
     a.partial = nullptr;
+    a.wait_cycles = 0;
+    a.never = 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int sms = sm_count(device_id);
     if (prompt_form(act_type, n_rows, n_seqs, n_kv_heads, a.group, sms)) {

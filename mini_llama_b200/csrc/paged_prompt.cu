@@ -9,14 +9,15 @@
 //
 // Here, unlike in the decode form, codes are widened to fp16 with their scales,
 // once for all rows of the tile, as d q. That is a whole multiple of 2^-24, so small
-// scales lose nothing, and off by at most half an fp16 step (2^-11) otherwise. d q / 16
-// where a scale reaches 4096: for K by token, with its S times 16 (a group of such a
-// token whose scale is below 2^-10 is off by up to 2^-36 of the token's largest key), for
-// V by 16 tokens, with their P times 16. P is off by half a step, too. fp32 calls keep queries, K, V and P as hi + lo pairs and add the three
-// products that count. The tensor cores cut off what falls below a sum's last bit,
-// so O takes only hi hi, one cut per 16 tokens, and the small products have a sum
-// of their own (with one sum results over 700 tokens were off by 1.5e-6, now by
-// 5e-7). ref is the row's maximum as of the last time that it rose by more than
+// scales lose nothing, and is off by at most half an fp16 step (2^-11) otherwise.
+// Where a scale reaches 4096 it is d q / 16: for K by token, with its S times 16 (a
+// group of such a token whose own scale is below 2^-10 is off by up to 2^-32 of the
+// token's largest key), for V by 16 tokens, with their P times 16. P is off by at most
+// half a step, too. fp32 calls keep queries, K, V and P as hi + lo pairs and add the
+// three products that count. The tensor cores cut off what falls below a sum's last
+// bit, so O takes only hi hi, one cut per 16 tokens, and the small products have a sum
+// of their own (with one sum results over 700 tokens were off by 1.5e-6, now by 5e-7).
+// ref is the row's maximum as of the last time that it rose by more than
 // a constant: only then is O brought to the new one.
 //
 // Roles (13 warps, one CTA per SM):
@@ -37,11 +38,14 @@
 //
 // Every wait is bounded: on a timeout the waiting thread records
 // MLB_ERR_TIMEOUT in the device's status word (mlb_paged_attention_status) and
-// raises the CTA's abort flag; all roles leave their loops, the products in flight
-// are waited for (bounded), tensor memory is released and the CTA exits.
+// raises the CTA's abort flag; all roles leave their loops, a warp's lanes together,
+// rows without a result become NaN, the products in flight are waited for (bounded),
+// tensor memory is released and the CTA exits.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.cuh"
+#include "runtime.cuh"
 #include "tcgen05.cuh"
 
 namespace mlb {
@@ -105,6 +109,7 @@ struct Shared {
   uint64_t s_full[2], p_full[2], o_done[2], o_last[2], q_full, drain;
   long long warp_sums[kThreads / 32];
   long long base;
+  long long wait_cycles;
   int seq;
   int abort_flag;
   uint32_t tmem;
@@ -116,13 +121,13 @@ struct Shared {
   alignas(4) uint16_t k_big[4][8];
 };
 
-// Bounded wait that also gives up when another thread did.
+// Bounded wait of one thread that also gives up when another one did.
 __device__ __forceinline__ bool wait(Shared& sh, uint64_t* bar, int phase, int where) {
   if (mbar_try_wait(bar, (uint32_t)phase & 1u)) return true;
   const long long start = clock64();
   while (!mbar_try_wait(bar, (uint32_t)phase & 1u)) {
     if (*(volatile int*)&sh.abort_flag) return false;
-    if (clock64() - start > kWaitCycles) {
+    if (clock64() - start > sh.wait_cycles) {
       atomicExch(&g_status.code, MLB_ERR_TIMEOUT);
       atomicExch(&g_status.where, where);
       *(volatile int*)&sh.abort_flag = 1;
@@ -130,6 +135,17 @@ __device__ __forceinline__ bool wait(Shared& sh, uint64_t* bar, int phase, int w
     }
   }
   return true;
+}
+
+// The same for a warp: its lanes go on or give up together, for what follows is for
+// whole warps. Out of line where the first try fails: inside, the bf16 softmax lost
+// registers to it (4096 rows of 32 heads 198 us, so 194).
+__device__ __noinline__ bool wait_longer(Shared& sh, uint64_t* bar, int phase, int where) {
+  return __all_sync(0xffffffffu, wait(sh, bar, phase, where));
+}
+__device__ __forceinline__ bool wait_warp(Shared& sh, uint64_t* bar, int phase, int where) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, (uint32_t)phase & 1u))) return true;
+  return wait_longer(sh, bar, phase, where);
 }
 
 template <int G, class T>
@@ -197,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.k_full[i], P::ND);
+      mbar_init(&sh.k_full[i], P::ND + a.never);
       mbar_init(&sh.v_full[i], P::ND);
       mbar_init(&sh.k_empty[i], 1);
       mbar_init(&sh.v_empty[i], 1);
@@ -209,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     mbar_init(&sh.q_full, 4 * NX);
     mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
+    sh.wait_cycles = a.wait_cycles;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -323,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         }
       }
 
-      if (j >= NS && !wait(sh, &sh.k_empty[st], j / NS - 1, 1001)) break;
+      if (j >= NS && !wait_warp(sh, &sh.k_empty[st], j / NS - 1, 1001)) break;
       uint8_t* k0 = smem + P::K0 + st * PT * P::K;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
@@ -350,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.k_full[st]);
 
-      if (j >= NS && !wait(sh, &sh.v_empty[st], j / NS - 1, 1002)) break;
+      if (j >= NS && !wait_warp(sh, &sh.v_empty[st], j / NS - 1, 1002)) break;
       uint8_t* v0 = smem + P::V0 + st * PT * P::V;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
@@ -432,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     bool ok = true;
     for (int j = 0; ok && j < nx; ++j) {
       const int b = SPLIT ? j & 1 : x;
-      ok = wait(sh, &sh.s_full[b], SPLIT ? j >> 1 : j, 1003);
+      ok = wait_warp(sh, &sh.s_full[b], SPLIT ? j >> 1 : j, 1003);
       if (!ok) break;
       tc_fence_after();
       const uint32_t s_at = tmem + lanes + P::S_COL + 128 * b;
@@ -495,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         const float f = !rise ? 1.0f : ref == -INFINITY ? 0.0f : ex2((ref - mx) * rs);
         if (rise) ref = mx;
         if (j == 0) return true;  // no O yet
-        if (!wait(sh, &sh.o_done[x], j - 1, 1004)) return false;
+        if (!wait_warp(sh, &sh.o_done[x], j - 1, 1004)) return false;
         tc_fence_after();
         l0 = mul2(l0, make_float2(f, f));
         l1 = mul2(l1, make_float2(f, f));
@@ -635,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
       if (lane == 0) mbar_arrive(&sh.p_full[x]);
     }
     if (ok && nx > 0) {
-      ok = wait(sh, &sh.o_last[x], 0, 1005);
+      ok = wait_warp(sh, &sh.o_last[x], 0, 1005);
       tc_fence_after();
     }
     if (ok) {
@@ -672,6 +689,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         }
       }
       tc_fence_before();
+    } else if (live) {  // no result
+      const float nan = __uint_as_float(0x7fc00000u);
+      T* out = static_cast<T*>(a.out) + (long long)(sw.row0 + tok) * a.out_stride +
+               (size_t)(head * a.group + (int)(flat - (long long)tok * a.group)) *
+                   a.cache.head_dim;
+      for (int d = 0; d < a.cache.head_dim; d += 4)
+        store_act4(out + d, make_float4(nan, nan, nan, nan));
     }
   } else if (warp == kMmaWarp && lane == 0) {
     // ------------------------------------------------------------- products
@@ -781,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     // nothing is in flight when tensor and shared memory go
     tc_commit(&sh.drain);
     const long long start = clock64();
-    while (!mbar_try_wait(&sh.drain, 0) && clock64() - start < kWaitCycles) {
+    while (!mbar_try_wait(&sh.drain, 0) && clock64() - start < sh.wait_cycles) {
     }
   }
   __syncwarp();
@@ -791,6 +815,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// The last wait of the device that gave up, and forgets it.
+DeviceStatus take_status() {
+  MLB_CUDA(cudaDeviceSynchronize());
+  DeviceStatus s;
+  MLB_CUDA(cudaMemcpyFromSymbol(&s, g_status, sizeof(s)));
+  const DeviceStatus none = {0, 0};
+  MLB_CUDA(cudaMemcpyToSymbol(g_status, &none, sizeof(none)));
+  return s;
 }
 
 template <int G, class T>
@@ -816,8 +850,10 @@ void dispatch(const PagedAttnArgs& a, int device_id, cudaStream_t stream) {
 
 }  // namespace
 
-void paged_prompt_launch(const PagedAttnArgs& a, int act_type, int device_id,
+void paged_prompt_launch(const PagedAttnArgs& args, int act_type, int device_id,
                          cudaStream_t stream) {
+  PagedAttnArgs a = args;
+  if (a.wait_cycles == 0) a.wait_cycles = kWaitCycles;
   if (act_type == MLB_ACT_BF16)
     dispatch<__nv_bfloat16>(a, device_id, stream);
   else
@@ -832,12 +868,55 @@ extern "C" int mlb_paged_attention_status(int device_id, int* code, int* where) 
   return guarded([&] {
     if (!code || !where) invalid("CudaPagedAttention: null output");
     DeviceScope scope(device_id);
-    MLB_CUDA(cudaDeviceSynchronize());
-    DeviceStatus s;
-    MLB_CUDA(cudaMemcpyFromSymbol(&s, g_status, sizeof(s)));
-    const DeviceStatus none = {0, 0};
-    MLB_CUDA(cudaMemcpyToSymbol(g_status, &none, sizeof(none)));
+    const DeviceStatus s = take_status();
     *code = s.code;
     *where = s.where;
+  });
+}
+
+extern "C" int mlb_paged_attention_wait_selftest(int device_id, int act_type, double limit_ms,
+                                                 int* code, int* where, int* nan_rows) {
+  return guarded([&] {
+    const char* who = "CudaPagedAttention";
+    if (!code || !where || !nan_rows) invalid("CudaPagedAttention: null output");
+    paged_check_act(who, act_type);
+    if (!(limit_ms > 0.0) || limit_ms > 1000.0)
+      invalid("CudaPagedAttention: limit_ms must be in (0, 1000]");
+    DeviceScope scope(device_id);
+    int khz = 0;
+    MLB_CUDA(cudaDeviceGetAttribute(&khz, cudaDevAttrClockRate, device_id));
+    // one sequence of kRows rows over one page of zeros, one head of 32
+    constexpr int kRows = 8, kDim = 32, kPage = kPagedBlock;
+    const size_t page = paged_page_bytes(kPage, 1, kDim), rows = kRows * kDim * sizeof(float);
+    const int seqs[4] = {0, kRows, kRows, 0};  // row offsets, length, page table
+    const size_t at_q = page, at_out = at_q + rows, at_seqs = at_out + rows;
+    DevBuf buf(at_seqs + sizeof(seqs));
+    uint8_t* p = static_cast<uint8_t*>(buf.p);
+    zero_now(p, at_seqs);
+    copy_to_device_now(p + at_seqs, seqs, sizeof(seqs));
+    const int* s = reinterpret_cast<const int*>(p + at_seqs);
+    PagedAttnArgs a = {};
+    a.cache = paged_cache(who, p, 1, 1, kPage, 1, kDim, 0);
+    a.seqs = paged_seqs(who, kRows, 1, s, s + 2, s + 3, 1, kPage);
+    a.q = p + at_q;
+    a.out = p + at_out;
+    a.q_stride = a.out_stride = kDim;
+    a.n_heads = a.group = 1;
+    a.scale_log2 = 1.0f;
+    a.wait_cycles = std::max(1LL, (long long)(limit_ms * (double)khz));
+    a.never = 1;
+    paged_prompt_launch(a, act_type, device_id, nullptr);
+    const DeviceStatus st = take_status();
+    uint32_t out[kRows * kDim];
+    MLB_CUDA(cudaMemcpy(out, p + at_out, rows, cudaMemcpyDeviceToHost));
+    // a row's elements are NaN if every word holds one (bf16: two, in half the words)
+    const int words = act_type == MLB_ACT_BF16 ? kDim / 2 : kDim;
+    const uint32_t nan = act_type == MLB_ACT_BF16 ? 0x7fc07fc0u : 0x7fc00000u;
+    *nan_rows = 0;
+    for (int r = 0; r < kRows; ++r)
+      *nan_rows += std::all_of(out + r * words, out + (r + 1) * words,
+                               [&](uint32_t w) { return (w & nan) == nan; });
+    *code = st.code;
+    *where = st.where;
   });
 }

@@ -175,3 +175,14 @@ def test_offsets_and_lengths_of_any_value(cuda, width, lens, offsets, n, dtype):
         assert torch.isfinite(x).all()
     assert (wide[:32] == 3).all() and (wide[32 + n:] == 3).all()
     assert (cache.pages[0] == 85).all() and (cache.pages[2] == 85).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_wait_that_gives_up_is_told(cuda, bf16):
+    """A barrier that never completes: every role of the prompt form gives up, the
+    status word says so once, no row keeps what the buffer held, and the next call on
+    the device is right."""
+    code, where, rows = mlb.paged_attention_wait_selftest(bf16)
+    assert code == mlb.ERR_TIMEOUT and 1001 <= where <= 1011 and rows == 8
+    assert mlb.paged_attention_status() == (0, 0)
+    test_keys_of_any_size(cuda, 1.0, 1200, "bfloat16" if bf16 else "float32")
