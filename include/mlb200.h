@@ -263,7 +263,8 @@ int mlb_paged_kv_read(const void* pages_dev, int n_layers, int n_pages, int page
  * (CudaAttentionDecodeDeviceInput, include/mini_llama/cuda_attention.h:13, for
  * ragged sequences; GQA head map h / (n_heads / n_kv_heads)): one row per
  * sequence while decoding, a few to check drafted tokens, many for a prompt. A
- * row that sees nothing gets zeros. q and out may not overlap. The workspace
+ * row that sees nothing gets zeros. Rows of q and out may not overlap (side by side
+ * in one buffer they do not). The workspace
  * (16-byte aligned, mlb_paged_attention_workspace bytes, contents irrelevant;
  * null where that is 0) belongs to the call until it has finished on the
  * device. */

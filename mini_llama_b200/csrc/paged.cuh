@@ -120,6 +120,29 @@ inline void paged_check_rows(const char* who, const char* name, const void* p, l
     invalid(w + ": rows of " + name + " must be 16-byte aligned");
 }
 
+// Whether two sets of n rows share a byte: rows of a_bytes (b_bytes), a_stride (b_stride)
+// apart, at least a row. Rows side by side in one buffer do not.
+inline bool rows_overlap(const void* a, long long a_stride, long long a_bytes, const void* b,
+                         long long b_stride, long long b_bytes, int n) {
+  using wide = __int128;  // strides are the caller's
+  const wide d = (wide)reinterpret_cast<uintptr_t>(b) - (wide)reinterpret_cast<uintptr_t>(a);
+  const auto floor_div = [](wide x, wide y) { return x / y - (x % y < 0 ? 1 : 0); };
+  // rows of b that row i of a meets: those with i a_stride - j b_stride - d in (-a_bytes, b_bytes)
+  const auto meets = [&](wide at, wide j0, wide j1) {
+    const wide lo = floor_div(at - d - b_bytes, b_stride) + 1;
+    const wide hi = floor_div(at - d + a_bytes - 1, b_stride);
+    return (lo > j0 ? lo : j0) <= (hi < j1 ? hi : j1);
+  };
+  if (n <= 0) return false;
+  // of equal strides only the difference of the rows counts
+  if (a_stride == b_stride) return meets(0, -(wide)(n - 1), n - 1);
+  if (d >= (wide)(n - 1) * a_stride + a_bytes || -d >= (wide)(n - 1) * b_stride + b_bytes)
+    return false;
+  for (int i = 0; i < n; ++i)
+    if (meets((wide)i * a_stride, 0, n - 1)) return true;
+  return false;
+}
+
 inline void paged_check_act(const char* who, int act) {
   if (act != MLB_ACT_F32 && act != MLB_ACT_BF16)
     invalid(std::string(who) + ": unknown activation type " + std::to_string(act));

@@ -186,3 +186,19 @@ def test_a_wait_that_gives_up_is_told(cuda, bf16):
     assert code == mlb.ERR_TIMEOUT and 1001 <= where <= 1011 and rows == 8
     assert mlb.paged_attention_status() == (0, 0)
     test_keys_of_any_size(cuda, 1.0, 1200, "bfloat16" if bf16 else "float32")
+
+
+@pytest.mark.parametrize("n", ROWS)
+def test_queries_and_outputs_side_by_side(cuda, n):
+    """Rows of one buffer in turn: not an overlap, and what separate buffers give."""
+    seqs = R.Seqs([n], [1300], 32, seed=n)
+    g = gen(57)
+    cache, _, _ = stored(seqs, randn(g, 1300, 2, 64), randn(g, 1300, 2, 64))
+    both = randn(g, n, 16, 64)
+    q, out = both[:, :8], both[:, 8:]
+    want = mlb.CudaPagedAttentionDeviceInput(q.clone(), cache, 0, *seqs.where(), 8, 2, 64)
+    mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, 64, out=out)
+    assert torch.equal(out, want)
+    with pytest.raises(mlb.MlbError, match="must not overlap"):
+        mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, 64,
+                                          out=both[:, 1:9])

@@ -1,6 +1,7 @@
 """Refusals of the paged attention's entry points that need no GPU: the checks come
 before any device call."""
 import ctypes
+import random
 
 import pytest
 
@@ -11,6 +12,61 @@ from mini_llama_b200 import _lib
 def err(rc, text, code=-1):
     assert rc == code, (rc, _lib.lib().mlb_last_error())
     assert text.encode() in _lib.lib().mlb_last_error(), _lib.lib().mlb_last_error()
+
+
+P = 1 << 20  # never dereferenced: a call that passes these checks is refused for its workspace
+
+
+def attend(q=0, out=0, qs=256, outs=256, rows=3, act=0):
+    n = _lib.lib().mlb_paged_attention(
+        P, 2, 4, 16, 2, 64, 0, act, P + q, qs, 4, rows, 1, P, P, P, 64, 0.1, P + out, outs, None, 0,
+        0, None)
+    assert n != 0
+    return b"must not overlap" in _lib.lib().mlb_last_error()
+
+
+def shares(q=0, out=0, qs=256, outs=256, rows=3, act=0):
+    """Whether a byte belongs to a row of both (4 heads of 64), row by row."""
+    es = 2 if act else 4
+    n = 256 * es
+    return any(abs(q + i * qs * es - out - j * outs * es) < n
+               for i in range(rows) for j in range(rows))
+
+
+@pytest.mark.parametrize("call", [
+    dict(out=0), dict(out=16), dict(q=16), dict(out=1008), dict(out=1024), dict(out=2048),
+    dict(q=3056), dict(out=2048 + 1008), dict(out=512, qs=512), dict(out=2048, qs=512, rows=2),
+    dict(out=1024, outs=512), dict(q=512, qs=512, outs=384), dict(q=8192, outs=2048),
+    dict(act=1, out=496), dict(act=1, out=1408, qs=512, outs=512, rows=4),
+    dict(q=2048 * 100 + 1008, qs=260, outs=512, rows=300)])
+def test_attention_refuses_outputs_over_queries(call):
+    assert shares(**call) and attend(**call)
+
+
+@pytest.mark.parametrize("call", [
+    dict(out=3072), dict(q=3072), dict(out=1024, qs=512, outs=512), dict(q=1024, qs=512, outs=512),
+    dict(out=1024, rows=1), dict(out=1024, qs=512, outs=768, rows=2), dict(q=4096, outs=2048),
+    dict(act=1, out=512, qs=512, outs=512), dict(act=1, out=512, rows=1, qs=512, outs=264),
+    dict(act=1, out=1536, qs=512, outs=512, rows=4),
+    dict(out=1024 + 512, qs=768, outs=768, rows=300), dict(q=P, qs=1 << 40, outs=1 << 41)])
+def test_attention_takes_rows_side_by_side(call):
+    assert not shares(**call) and not attend(**call)
+
+
+def test_any_two_sets_of_rows():
+    rng = random.Random(1)
+    seen = [0, 0]
+    for _ in range(3000):
+        act = rng.randrange(2)
+        unit = 8 if act else 4  # elements in 16 bytes
+        qs = 256 + unit * rng.randrange(0, 200)
+        call = dict(act=act, qs=qs, outs=rng.choice([qs, 256 + unit * rng.randrange(0, 200)]),
+                    rows=rng.randrange(1, 12), q=16 * rng.randrange(0, 600),
+                    out=16 * rng.randrange(0, 600))
+        want = shares(**call)
+        assert attend(**call) == want, call
+        seen[want] += 1
+    assert min(seen) > 300
 
 
 def test_wait_selftest_refuses_bad_arguments():
