@@ -242,7 +242,8 @@ int mlb_attention_decode_noalloc(const float* q_dev, const float* keys_dev,
 int mlb_paged_kv_page_bytes(int page_size, int n_kv_heads, int head_dim, size_t* bytes);
 /* Stores the rows of k and v [n_rows, n_kv_heads, head_dim] at their positions,
  * k rotated first (rope_type MLB_ROPE_*), and writes q [n_rows, n_heads,
- * head_dim] rotated to q_out (may be q itself; n_heads = 0: no queries). Angles
+ * head_dim] rotated to q_out (q itself, or no byte of q, k or v; n_heads = 0: no
+ * queries). Angles
  * and rotation are computed in 64 bits and rounded once; mlb_rope's fp32
  * angles differ from that by up to pos * 2^-24. */
 int mlb_paged_kv_append(void* pages_dev, int n_layers, int n_pages, int page_size, int n_kv_heads,

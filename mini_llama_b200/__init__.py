@@ -507,7 +507,8 @@ class CudaPagedKvCache:
                      rope_type=ROPE_NORMAL, q=None, q_out=None, stream=None):
         """Stores k and v [rows, n_kv_heads, head_dim] (fp32 or bf16) at their
         positions, k rotated on the way, and returns q [rows, n_heads, head_dim]
-        rotated to the same positions, in q_out if given (q itself: in place).
+        rotated to the same positions, in q_out if given (q itself: in place;
+        otherwise no part of q, k or v).
         rope_type ROPE_NONE stores k and returns q as they are."""
         who = "CudaPagedKvCache"
         self._layer(who, layer)

@@ -202,3 +202,27 @@ def test_queries_and_outputs_side_by_side(cuda, n):
     with pytest.raises(mlb.MlbError, match="must not overlap"):
         mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 8, 2, 64,
                                           out=both[:, 1:9])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [1, 7, 1500])
+def test_append_in_one_buffer(cuda, n, dtype):
+    """q, k and v cut out of one projection's rows, q rotated in place or into the same
+    rows' spare part: what separate buffers give, k and v left as they were."""
+    dtype = getattr(torch, dtype)
+    seqs = R.Seqs([n], [n + 9], 32, seed=n)
+    g = gen(58)
+    fused = randn(g, n, 8 + 2 + 2 + 8, 64, dtype=dtype)
+    caches = [mlb.CudaPagedKvCache(1, seqs.n_pages, 32, 2, 64) for _ in range(3)]
+    want = caches[0].AppendDevice(0, fused[:, 8:10].clone(), fused[:, 10:12].clone(),
+                                  *seqs.where(), q=fused[:, :8].clone())
+    for cache, at in ((caches[1], 0), (caches[2], 12)):
+        x = fused.clone()
+        q, k, v = x[:, :8], x[:, 8:10], x[:, 10:12]
+        out = cache.AppendDevice(0, k, v, *seqs.where(), q=q, q_out=x[:, at:at + 8])
+        assert torch.equal(out, want) and torch.equal(cache.pages, caches[0].pages)
+        assert torch.equal(x[:, 8:12], fused[:, 8:12])
+        with pytest.raises(mlb.MlbError, match="q_out must not overlap k or v"):
+            cache.AppendDevice(0, k, v, *seqs.where(), q=fused[:, :8], q_out=x[:, 9:17])
+        with pytest.raises(mlb.MlbError, match="q_out must be q itself or not overlap it"):
+            cache.AppendDevice(0, k, v, *seqs.where(), q=x[:, 12:20], q_out=x[:, 11:19])

@@ -69,6 +69,36 @@ def test_any_two_sets_of_rows():
     assert min(seen) > 300
 
 
+def append(q=0, qo=1 << 16, k=1 << 17, v=1 << 18, qs=256, qos=256, ks=128, vs=128, rows=3):
+    n = _lib.lib().mlb_paged_kv_append(
+        P, 2, 4, 16, 2, 64, 0, 0, P + k, ks, P + v, vs, P + q, qs, 4, P + qo, qos, rows, 1, P, P, P,
+        2, 1e4, 0, 0, None)
+    assert n == -1
+    return _lib.lib().mlb_last_error().decode()
+
+
+# every one of these is refused: a call that is not would launch on addresses of no one
+@pytest.mark.parametrize("call", [
+    dict(qo=16), dict(qo=1024), dict(q=3056, qo=0), dict(qo=0, qos=512), dict(qo=0, qs=512),
+    dict(qo=512, qs=512, qos=512)])
+def test_append_refuses_queries_out_over_queries(call):
+    assert "q_out must be q itself or not overlap it" in append(**call)
+
+
+@pytest.mark.parametrize("call", [
+    dict(qo=1 << 17), dict(k=4096, qo=4096 + 1520), dict(q=4096, qo=4096, v=4096),
+    dict(k=8192, ks=640, qo=8192 + 256, qos=640), dict(k=1 << 14, ks=512, v=1 << 15, qo=(1 << 15) - 512)])
+def test_append_refuses_queries_out_over_keys_or_values(call):
+    assert "q_out must not overlap k or v" in append(**call)
+
+
+def test_read_refuses_values_over_keys():
+    for k, v in ((0, 0), (0, 1520), (1024, 0)):  # three rows of 512 bytes
+        n = _lib.lib().mlb_paged_kv_read(P, 2, 4, 16, 2, 64, 0, 3, 1, P, P, P, 2, P + k, P + v, 0,
+                                         None)
+        assert n == -1 and b"k_out and v_out must not overlap" in _lib.lib().mlb_last_error()
+
+
 def test_wait_selftest_refuses_bad_arguments():
     f = _lib.lib().mlb_paged_attention_wait_selftest
     a, b, c = (ctypes.byref(ctypes.c_int()) for _ in range(3))
