@@ -456,10 +456,12 @@ class CudaPagedKvCache:
                 raise MlbError(-1, f"CudaPagedKvCache: {name} must be positive")
         n = ctypes.c_size_t()
         check(lib().mlb_paged_kv_page_bytes(page_size, n_kv_heads, head_dim, ctypes.byref(n)))
+        # empty until there is a pool of the new shape: the old one makes room for it
+        self.pages, self._shape = None, (0, 0, 0, 0, 0)
         self.device_id = device_id
-        self._shape = (n_layers, n_pages, page_size, n_kv_heads, head_dim)
         self.pages = torch.zeros((n_layers, n_pages, n.value), dtype=torch.uint8,
                                  device=torch.device("cuda", device_id))
+        self._shape = (n_layers, n_pages, page_size, n_kv_heads, head_dim)
 
     def Clear(self):
         if self.pages is not None:

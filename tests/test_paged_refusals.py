@@ -108,3 +108,27 @@ def test_wait_selftest_refuses_bad_arguments():
     for limit in (0.0, -1.0, 1001.0, float("nan")):
         with pytest.raises(mlb.MlbError, match="limit_ms"):
             mlb.paged_attention_wait_selftest(limit_ms=limit)
+
+
+def test_reset_that_fails_leaves_an_empty_cache(monkeypatch):
+    """Not the old pool under the new shape, which every later call would overrun."""
+    torch = pytest.importorskip("torch")
+    made = []
+
+    def zeros(shape, **kw):
+        if made:
+            raise RuntimeError("out of memory")
+        made.append(shape)
+        return torch.empty(1)
+
+    monkeypatch.setattr(torch, "zeros", zeros)
+    cache = mlb.CudaPagedKvCache(1, 2, 16, 2, 64)
+    assert not cache.empty() and cache.n_pages() == 2
+    with pytest.raises(mlb.MlbError, match="multiple of 16"):
+        cache.Reset(1, 4, 24, 2, 64)
+    assert cache.n_pages() == 2  # refused before anything changed
+    with pytest.raises(RuntimeError, match="out of memory"):
+        cache.Reset(1, 2000, 16, 2, 64)
+    assert cache.empty() and cache.n_pages() == 0 and cache.bytes() == 0
+    with pytest.raises(mlb.MlbError, match="paged KV cache is empty"):
+        cache.ReadDevice(0, None, None, None, 1)
