@@ -58,16 +58,16 @@ constexpr int kMmaWarp = 12;
 constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
 // P = 2^((S - ref) rs + lift), rs >= 0 the row's scale. With P up to 2^11, and 2^15
 // with the 16 of large V scales, it stays within fp16, and what fp16 loses below 2^-14
-// is 2^-(25 + lift) of a token at ref. fp32 calls look for the row's maximum first, and
-// ref follows it when that is more than kRise above. bf16 calls make P in one pass and,
-// when the step's sum exceeds 2^11 (128 tokens at ref come to 2^10), look for the
-// maximum, raise ref to it and make P once more.
+// is 2^-(25 + lift) of a token at ref. A step looks for each row's maximum first, and
+// ref follows it when that is more than kRise above. bf16 calls first make P in one pass
+// under the ref that there is, and leave it at that unless the step's sum exceeds 2^11
+// (128 tokens at ref come to 2^10) or there is something to mask.
 // ref is a value of S, and the difference comes before the product: no P is above
 // 2^lift at ref's own value, however large the scores are. As S rs - ref rs with the
 // second product rounded P is off by up to half a step of ref rs, and from scores of
 // 2^28 on 2^11 and more. Below kFar that is 2^-12 of P: there one fused multiply-add
 // does, which spares the main path of bf16 calls an addition per two scores (4096 rows
-// of 32 heads: 189 us, 193 with it).
+// of 32 heads: 186.6 us, 187.8 with it; 4500 of 8 heads of 64: 47.7, 49.2).
 constexpr float kRise = 4.0f, kMostP = 2048.0f, kFar = 8192.0f;
 
 constexpr uint32_t kBigV = 1, kBigK = 2;
@@ -139,7 +139,7 @@ __device__ __forceinline__ bool wait(Shared& sh, uint64_t* bar, int phase, int w
 
 // The same for a warp: its lanes go on or give up together, for what follows is for
 // whole warps. Out of line where the first try fails: inside, the bf16 softmax lost
-// registers to it (4096 rows of 32 heads 198 us, so 194).
+// registers to it (4096 rows of 32 heads 192.7 us, so 186.6).
 __device__ __noinline__ bool wait_longer(Shared& sh, uint64_t* bar, int phase, int where) {
   return __all_sync(0xffffffffu, wait(sh, bar, phase, where));
 }
@@ -466,33 +466,67 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
         return m;
       };
 
-      // S of keys stored as d q / 16 times 16, once before anything looks at it (called
-      // where steps with large scales come by: in the main path the branch alone took 3 %)
-      bool s_done = (big & 0x0101010101010101ull * kBigK) == 0;
-      auto scale_s = [&]() {
-        if (s_done) return;
-        s_done = true;
-#pragma unroll 1
-        for (int ch = 0; ch < 4; ++ch) {
-          const uint32_t k16 =
-              *reinterpret_cast<const volatile uint32_t*>(&sh.k_big[j & 3][2 * ch]);
-          float v[32];
-          tmem_ld32(s_at + 32 * ch, v);
+      // bf16, nothing to mask, no large scale, and no ref so large that its product's
+      // rounding would tell: P of the whole step in registers under the ref that there is,
+      // in one pass over S; not taken if a row's P have become too large
+      bool done = false, tried = false;
+      if constexpr (!SPLIT) {
+        tried = whole && big == 0 && __all_sync(0xffffffffu, fabsf(ref * rs) < kFar);
+        if (tried) {
+          const float neg = fmaf(-ref, rs, kLift);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          // 32 tokens on their way while 32 are worked on (products slow the loads
+          // down to about the time that this takes)
+          uint32_t u[2][32], hi[4][16];
+          tmem_ld32_start(s_at, u[0]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t u[16];
+          for (int ch = 0; ch < 4; ++ch) {
+            tmem_ld32_wait(u[ch & 1]);
+            if (ch < 3) tmem_ld32_start(s_at + 32 * (ch + 1), u[(ch + 1) & 1]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              u[i] = __float_as_uint(v[16 * h + i] * (k16 >> (16 * h + i) & 1 ? 16.0f : 1.0f));
-            tmem_st16(s_at + 32 * ch + 16 * h, u);
+            for (int i = 0; i < 16; ++i) {
+              float2 p = make_float2(__uint_as_float(u[ch & 1][2 * i]),
+                                     __uint_as_float(u[ch & 1][2 * i + 1]));
+              p = fma2(p, make_float2(rs, rs), make_float2(neg, neg));
+              p.x = ex2(p.x);
+              p.y = ex2(p.y);
+              sum[i & 1] = add2(sum[i & 1], p);
+              hi[ch][i] = pack_f16(p.x, p.y);
+            }
+          }
+          // no P above the sum, so none that fp16 does not hold; looking for the maximum
+          // as well would cost a sixth of the pass
+          done = !__any_sync(0xffffffffu, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y) > kMostP);
+          if (done) {
+            l0 = add2(l0, sum[0]);
+            l1 = add2(l1, sum[1]);
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) tmem_st16(s_at + P::P_STEP * ch, hi[ch]);
           }
         }
-        tmem_wait_st();
-      };
+      }
 
-      // largest S of the step
-      auto step_max = [&]() {
-        scale_s();
+      // otherwise the largest S first, then P as it is made
+      if (!done) {
+        if (big & 0x0101010101010101ull * kBigK) {  // S of keys stored as d q / 16
+#pragma unroll 1
+          for (int ch = 0; ch < 4; ++ch) {
+            const uint32_t k16 =
+                *reinterpret_cast<const volatile uint32_t*>(&sh.k_big[j & 3][2 * ch]);
+            float v[32];
+            tmem_ld32(s_at + 32 * ch, v);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t u[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                u[i] = __float_as_uint(v[16 * h + i] * (k16 >> (16 * h + i) & 1 ? 16.0f : 1.0f));
+              tmem_st16(s_at + 32 * ch + 16 * h, u);
+            }
+          }
+          tmem_wait_st();
+        }
+
         float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll 1
         for (int ch = 0; ch < 4; ++ch) {
@@ -505,40 +539,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             m1 = fmaxf(m1, m >> (i + 1) & 1 ? v[i + 1] : -INFINITY);
           }
         }
-        return fmaxf(m0, m1);
-      };
-      // brings ref of the lanes that rise, their sums and O to mx
-      auto raise_to = [&](float mx, bool rise) {
-        const float f = !rise ? 1.0f : ref == -INFINITY ? 0.0f : ex2((ref - mx) * rs);
-        if (rise) ref = mx;
-        if (j == 0) return true;  // no O yet
-        if (!wait_warp(sh, &sh.o_done[x], j - 1, 1004)) return false;
-        tc_fence_after();
-        l0 = mul2(l0, make_float2(f, f));
-        l1 = mul2(l1, make_float2(f, f));
+        // ref of the rows that rise, their sums and O go to the maximum
+        const float mx = fmaxf(m0, m1);
+        const bool rise =
+            ref == -INFINITY ? mx > ref : tried ? mx > ref : (mx - ref) * rs > kRise;
+        if (__any_sync(0xffffffffu, rise)) {
+          const float f = !rise ? 1.0f : ref == -INFINITY ? 0.0f : ex2((ref - mx) * rs);
+          if (rise) ref = mx;
+          if (j > 0) {  // there is an O
+            ok = wait_warp(sh, &sh.o_done[x], j - 1, 1004);
+            if (!ok) break;
+            tc_fence_after();
+            l0 = mul2(l0, make_float2(f, f));
+            l1 = mul2(l1, make_float2(f, f));
 #pragma unroll 1
-        for (int ch = 0; ch < PT * G; ++ch) {
-          const uint32_t at = ch < G ? o_at + 32 * ch : olo_at + 32 * (ch - G);
-          float v[32];
-          tmem_ld32(at, v);
+            for (int ch = 0; ch < PT * G; ++ch) {
+              const uint32_t at = ch < G ? o_at + 32 * ch : olo_at + 32 * (ch - G);
+              float v[32];
+              tmem_ld32(at, v);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t u[16];
+              for (int h = 0; h < 2; ++h) {
+                uint32_t u[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i] * f);
-            tmem_st16(at + 16 * h, u);
+                for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i] * f);
+                tmem_st16(at + 16 * h, u);
+              }
+            }
+            tmem_wait_st();
           }
         }
-        tmem_wait_st();
-        return true;
-      };
 
-      if constexpr (SPLIT) {
-        // largest score first, then P as it is made
-        const float mx = step_max();
-        const bool rise = ref == -INFINITY ? mx > ref : (mx - ref) * rs > kRise;
-        if (__any_sync(0xffffffffu, rise)) ok = raise_to(mx, rise);
-        if (!ok) break;
         const float from = ref == -INFINITY ? 0.0f : -ref;
 #pragma unroll 1
         for (int ch = 0; ch < 4; ++ch) {
@@ -559,92 +589,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(PagedAttnArgs
             const float up = big >> (16 * ch + 8 * (i >> 3)) & kBigV ? 16.0f : 1.0f;
             p = mul2(p, make_float2(up, up));
             hi[i] = pack_f16(p.x, p.y);
-            const float2 h = __half22float2(u32_as_h2(hi[i]));
-            lo[i] = pack_f16(p.x - h.x, p.y - h.y);
-          }
-          tmem_st16(s_at + P::P_STEP * ch, hi);
-          tmem_st16(s_at + P::P_STEP * ch + 16, lo);
-        }
-      } else {
-        // P of the whole step in registers under the ref of the step before (one
-        // pass over S); again if a row's P have become too large
-        // rows that see something for the first time have no ref yet
-        if (__any_sync(0xffffffffu, ref == -INFINITY && left > 0)) {
-          const float mx = step_max();
-          ok = raise_to(mx, ref == -INFINITY && mx > ref);
-          if (!ok) break;
-        }
-        // nothing to mask, and no ref so large that its product's rounding would tell
-        bool plain = whole && big == 0 && __all_sync(0xffffffffu, fabsf(ref * rs) < kFar);
-        uint32_t hi[4][16];
-#pragma unroll 1
-        for (bool again = false;; again = true) {
-          const float neg = fmaf(-ref, rs, kLift);
-          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          auto pass = [&](auto plain_c) {
-            constexpr bool PLAIN = decltype(plain_c)::value;
-            // 32 tokens on their way while 32 are worked on (products slow the loads
-            // down to about the time that this takes)
-            const float from = ref == -INFINITY ? 0.0f : -ref;
-            uint32_t u[2][32];
-            tmem_ld32_start(s_at, u[0]);
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-              tmem_ld32_wait(u[ch & 1]);
-              if (ch < 3) tmem_ld32_start(s_at + 32 * (ch + 1), u[(ch + 1) & 1]);
-              const uint32_t m = PLAIN ? 0xffffffffu : seen(ch);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float vx = __uint_as_float(u[ch & 1][2 * i]);
-                float vy = __uint_as_float(u[ch & 1][2 * i + 1]);
-                if (!PLAIN) {
-                  vx = m >> (2 * i) & 1 ? vx : -INFINITY;
-                  vy = m >> (2 * i + 1) & 1 ? vy : -INFINITY;
-                }
-                float2 p = make_float2(vx, vy);
-                if (PLAIN)
-                  p = fma2(p, make_float2(rs, rs), make_float2(neg, neg));
-                else
-                  p = fma2(add2(p, make_float2(from, from)), make_float2(rs, rs),
-                           make_float2(kLift, kLift));
-                p.x = ex2(p.x);
-                p.y = ex2(p.y);
-                if (!PLAIN) {  // -inf times rs = 0, or less ref = -inf
-                  p.x = m >> (2 * i) & 1 ? p.x : 0.0f;
-                  p.y = m >> (2 * i + 1) & 1 ? p.y : 0.0f;
-                }
-                sum[i & 1] = add2(sum[i & 1], p);
-                if (!PLAIN) {
-                  const float up = big >> (16 * ch + 8 * (i >> 3)) & kBigV ? 16.0f : 1.0f;
-                  p = mul2(p, make_float2(up, up));
-                }
-                hi[ch][i] = pack_f16(p.x, p.y);
-              }
+            if (SPLIT) {
+              const float2 h = __half22float2(u32_as_h2(hi[i]));
+              lo[i] = pack_f16(p.x - h.x, p.y - h.y);
             }
-          };
-          if (plain) {
-            pass(std::true_type{});
-          } else {
-            scale_s();
-            pass(std::false_type{});
           }
-          // no P above the sum, so none that fp16 does not hold; looking for the maximum
-          // as well would cost a sixth of the pass. One more pass at most: after it ref is
-          // the maximum, and what is still too large is infinite or no number
-          const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          if (again || !__any_sync(0xffffffffu, all > kMostP)) {
-            l0 = add2(l0, sum[0]);
-            l1 = add2(l1, sum[1]);
-            break;
-          }
-          const float mx = step_max();
-          ok = raise_to(mx, mx > ref);
-          if (!ok) break;
-          plain = false;
+          tmem_st16(s_at + P::P_STEP * ch, hi);  // over S that has been read
+          if (SPLIT) tmem_st16(s_at + P::P_STEP * ch + 16, lo);
         }
-        if (!ok) break;
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) tmem_st16(s_at + P::P_STEP * ch, hi[ch]);
       }
       tmem_wait_st();
       tc_fence_before();
