@@ -231,9 +231,9 @@ int mlb_attention_decode_noalloc(const float* q_dev, const float* keys_dev,
  * calls are asynchronous on `stream` and can be captured in a CUDA graph that
  * is replayed with new lengths and tables. What the device arrays hold is
  * checked where it is used, and never followed out of bounds: rows at or past
- * row_offsets[n_seqs] and rows at a negative position are left as they were, a
- * position past the table or on a page outside [0, n_pages) is not stored, and
- * attention does not see it. Rows of activations are contiguous [heads,
+ * row_offsets[n_seqs] are left as they were, rows at a negative position too by
+ * append (read and attention give zeros), a position past the table or on a page
+ * outside [0, n_pages) is not stored, and attention does not see it. Rows of activations are contiguous [heads,
  * head_dim], 16-byte aligned, a row stride (in elements) apart; act_type is
  * MLB_ACT_F32 or MLB_ACT_BF16. What is stored is finite: a block's scale ends
  * at fp16's largest number, and non-finite inputs leave some finite values in
@@ -263,7 +263,10 @@ int mlb_paged_kv_read(const void* pages_dev, int n_layers, int n_pages, int page
 /* out = softmax(scale q K^T) V of every row over the positions up to its own
  * (CudaAttentionDecodeDeviceInput, include/mini_llama/cuda_attention.h:13, for
  * ragged sequences; GQA head map h / (n_heads / n_kv_heads)): one row per
- * sequence while decoding, a few to check drafted tokens, many for a prompt. A
+ * sequence while decoding, a few to check drafted tokens, many for a prompt. All
+ * rows of a call go one way, chosen from their average number per sequence: long
+ * sequences that decode are served faster by a call of their own than beside a
+ * prompt. A
  * row that sees nothing gets zeros. Rows of q and out may not overlap (side by side
  * in one buffer they do not). The workspace
  * (16-byte aligned, mlb_paged_attention_workspace bytes, contents irrelevant;

@@ -610,7 +610,8 @@ def CudaPagedAttentionDeviceInput(q, kv_cache: CudaPagedKvCache, layer, row_offs
                                   stream=None):
     """Attention of q [rows, n_heads, head_dim] (fp32 or bf16), each row over the
     positions of its sequence up to its own (mlb_paged_attention): one row per
-    sequence while decoding, a few to check drafted tokens, many for a prompt.
+    sequence while decoding, a few to check drafted tokens, many for a prompt
+    (long decoding sequences in a call of their own: beside a prompt they are slow).
     scale defaults to 1 / sqrt(head_dim). A row that sees nothing gets zeros. Rows of
     out must not overlap rows of q (side by side in one buffer they do not)."""
     who = "CudaPagedAttention"

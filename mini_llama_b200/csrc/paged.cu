@@ -9,9 +9,10 @@
 //   x0' = x0 cos a - x1 sin a,  x1' = x0 sin a + x1 cos a,  a = p theta^(-2j/D)
 //
 // Angle, sine, cosine and rotation are kept in 64 bits and rounded once to
-// fp32: at position 1e5 an fp32 angle is off by up to 4e-3 rad, and a value next
-// to a code's border would fall on either side of it. Q4_0 codes then follow the
-// reference quantiser's fp32 steps bit for bit.
+// fp32: at position 1e5 an fp32 angle is off by up to 4e-3 rad, and a key next to a
+// code's border would fall on either side of it. Queries, which have no codes, take the
+// same angles and the same rotation. Q4_0 codes then follow the reference quantiser's
+// fp32 steps bit for bit.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -278,12 +278,8 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Words of a query row: 8 dimensions from d0, zeros past head_dim.
-__device__ __forceinline__ void load_q8(const float* p, float (&e)[8]) {
-  const float4 a = load_act4(p), b = load_act4(p + 4);
-  e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
-  e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
-}
-__device__ __forceinline__ void load_q8(const __nv_bfloat16* p, float (&e)[8]) {
+template <class T>
+__device__ __forceinline__ void load_q8(const T* p, float (&e)[8]) {
   const float4 a = load_act4(p), b = load_act4(p + 4);
   e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w;
   e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;

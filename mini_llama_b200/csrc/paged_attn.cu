@@ -21,7 +21,8 @@
 // fp32 calls keep both as hi + lo pairs, off by at most 2^-21 of the value, or
 // 2^-25 2^-F where that is larger; bf16 queries are exact in one fp16 (down to
 // 2^-27 of the row's largest), and p 2^F and its product with dV in one fp16
-// each are off by at most 2^-10, a quarter of the bf16 output's own half step.
+// each are off by at most 2^-10, a quarter of the bf16 output's own half step, or
+// 2^-25 2^-F where that is larger: 2^-38 of the largest dV that the row's tile sees.
 //
 // Work: the blocks of all (sequence, KV head, row tile) units are laid end to
 // end in chunks of 64 tokens and cut into equal runs, one per CTA, so uneven
@@ -32,9 +33,10 @@
 // Measured: one fp32 sequence of 131072 tokens, 64 heads over 8 of 128: 58 us, 2.6
 // TB/s of cache; 64 bf16 sequences of 512 to 8192: 72 us, 3.0 TB/s; 16 fp32 sequences
 // of up to 4096 with 5 rows and 32 KV heads: 51 us. The main loop alone runs at 3.7
-// TB/s, bound by instruction issue (about 400 instructions for a warp's 16 tokens of
-// 128, most of them the widening of codes, at 55 to 60 % of the issue slots); before
-// it come 4.6 us until the first block is there, after it 4 to 6 us for the join.
+// TB/s: about 400 instructions for a warp's 16 tokens of 128, a third of them the
+// widening of codes, at 55 to 60 % of the issue slots. The rest is waiting: 16 warps per
+// SM, each in a chain of products, two shuffles, votes, exponentials and products again.
+// Before it come 4.6 us until the first block is there, after it 4 to 6 us for the join.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -682,7 +684,11 @@ int dec_grid(int sms, int nt) { return sms * dec_ctas(nt); }
 // (fp32: 2.05), the prompt form runs waves of one CTA per SM, 1.65 us for up to 256
 // rows (fp32: 2.1 for 128). Measured, decode / prompt us, bf16: 16 sequences of 4096
 // with 8 KV heads, 32 rows 72 / 90, 128 rows 225 / 86; one sequence of 4096, 512 rows
-// 72 / 93, 1024 rows 124 / 94; of 32768, 1024 rows 744 / 638.
+// 72 / 93, 1024 rows 124 / 94; of 32768, 1024 rows 744 / 638. All at head_dim 128.
+// Averages do not see a long sequence with a row beside a prompt: the prompt form cuts
+// no tile's length, so such a call is as long as its longest sequence (bf16, 32 heads
+// over 8: 512 rows of a prompt and one row over 131072 tokens 2645 us, as two calls
+// 25 + 54; 2048 rows and 63 rows over 512 to 7952 tokens 479, as two 67 + 93).
 bool prompt_form(int act, int n_rows, int n_seqs, int kv, int group, int sms) {
   const bool f32 = act == MLB_ACT_F32;
   const long long units = (long long)n_seqs * kv;
@@ -699,6 +705,7 @@ bool prompt_form(int act, int n_rows, int n_seqs, int kv, int group, int sms) {
 // about 13 us per 1000 tokens of a unit. Measured, whole / cut us, fp32, 32 heads over 8
 // KV heads, one row each: 1 sequence of 128 tokens 7.4 / 9.5, of 256 9.3 / 9.5, of 500
 // 12.6 / 9.6; 8 sequences of 500 13.1 / 13.5, of 1000 19.9 / 13.8; 64 of 500 21.0 / 26.6.
+// All at head_dim 128.
 bool whole_units(int max_pages, int page_size, int n_seqs, int kv) {
   const long long tokens = (long long)max_pages * page_size;
   return tokens <= 256 || (tokens <= 512 && (long long)n_seqs * kv >= 64);

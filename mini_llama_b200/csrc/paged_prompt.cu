@@ -17,8 +17,8 @@
 // three products that count. The tensor cores cut off what falls below a sum's last
 // bit, so O takes only hi hi, one cut per 16 tokens, and the small products have a sum
 // of their own (with one sum results over 700 tokens were off by 1.5e-6, now by 5e-7).
-// ref is the row's maximum as of the last time that it rose by more than
-// a constant: only then is O brought to the new one.
+// ref is the row's maximum as of the last time that it was looked for and had risen
+// by more than a constant: only then is O brought to the new one.
 //
 // Roles (13 warps, one CTA per SM):
 //   warps 0..3    widen K and V into shared memory (fp32 calls: warps 8..11 too)
@@ -29,8 +29,8 @@
 // the softmax of the other runs, with K and V double-buffered. fp32 calls have one
 // row tile and S double-buffered.
 //
-// Measured: 4096 rows of 32 heads over 8 KV heads of 128 (bf16, one sequence): 186 us,
-// 740 TFLOP/s of the products that the mask leaves. A step of 2 x 128 rows x 128 tokens takes
+// Measured: 4096 rows of 32 heads over 8 KV heads of 128 (bf16, one sequence): 187 us,
+// 735 TFLOP/s of the products that the mask leaves. A step of 2 x 128 rows x 128 tokens takes
 // 4650 cycles where its products alone take 2880: the rest is the softmax, 2050
 // cycles per row tile (exponentials, rounding and the loads from tensor memory),
 // which two tiles do not hide whole. Steps of 64 tokens (242 us), two threads per row
@@ -67,7 +67,8 @@ constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
 // second product rounded P is off by up to half a step of ref rs, and from scores of
 // 2^28 on 2^11 and more. Below kFar that is 2^-12 of P: there one fused multiply-add
 // does, which spares the main path of bf16 calls an addition per two scores (4096 rows
-// of 32 heads: 186.6 us, 187.8 with it; 4500 of 8 heads of 64: 47.7, 49.2).
+// of 32 heads: 186.6 us, 187.8 with it; 2945 of 8 heads of 64
+// behind prefixes: 47.7, 49.2).
 constexpr float kRise = 4.0f, kMostP = 2048.0f, kFar = 8192.0f;
 
 constexpr uint32_t kBigV = 1, kBigK = 2;
