@@ -573,14 +573,13 @@ extern "C" int mlb_paged_kv_append(void* pages, int n_layers, int n_pages, int p
         paged_check_rows(who, "q", q, q_stride, n_heads, head_dim, act_type);
         paged_check_rows(who, "q_out", q_out, q_out_stride, n_heads, head_dim, act_type);
         // a row's q is read by the lanes that write it; other rows have no such order
-        const int es = act_type == MLB_ACT_BF16 ? 2 : 4;
-        const long long row = (long long)n_heads * head_dim * es, qo = q_out_stride * es;
-        const long long kv_row = (long long)n_kv_heads * head_dim * es;
+        const long long row = (long long)n_heads * head_dim;
+        const long long kv_row = (long long)n_kv_heads * head_dim;
         const bool in_place = q == q_out && (q_stride == q_out_stride || n_rows == 1);
-        if (!in_place && rows_overlap(q, q_stride * es, row, q_out, qo, row, n_rows))
+        if (!in_place && rows_overlap(q, q_stride, row, q_out, q_out_stride, row, n_rows, act_type))
           invalid("CudaPagedKvCache: q_out must be q itself or not overlap it");
-        if (rows_overlap(k, k_stride * es, kv_row, q_out, qo, row, n_rows) ||
-            rows_overlap(v, v_stride * es, kv_row, q_out, qo, row, n_rows))
+        if (rows_overlap(k, k_stride, kv_row, q_out, q_out_stride, row, n_rows, act_type) ||
+            rows_overlap(v, v_stride, kv_row, q_out, q_out_stride, row, n_rows, act_type))
           invalid("CudaPagedKvCache: q_out must not overlap k or v");
       }
     }
@@ -607,7 +606,7 @@ extern "C" int mlb_paged_kv_read(const void* pages, int n_layers, int n_pages, i
       const long long stride = (long long)n_kv_heads * head_dim;
       paged_check_rows(who, "k_out", k_out, stride, n_kv_heads, head_dim, MLB_ACT_F32);
       paged_check_rows(who, "v_out", v_out, stride, n_kv_heads, head_dim, MLB_ACT_F32);
-      if (rows_overlap(k_out, 4 * stride, 4 * stride, v_out, 4 * stride, 4 * stride, n_rows))
+      if (rows_overlap(k_out, stride, stride, v_out, stride, stride, n_rows, MLB_ACT_F32))
         invalid("CudaPagedKvCache: k_out and v_out must not overlap");
     }
     DeviceScope scope(device_id);

@@ -116,15 +116,18 @@ inline void paged_check_rows(const char* who, const char* name, const void* p, l
   if (!p) invalid(w + ": null " + name);
   if (stride < (long long)heads * head_dim)
     invalid(w + ": row stride of " + name + " is smaller than a row");
-  if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || (stride * es) % 16 != 0)
+  if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || stride % (16 / es) != 0)
     invalid(w + ": rows of " + name + " must be 16-byte aligned");
 }
 
-// Whether two sets of n rows share a byte: rows of a_bytes (b_bytes), a_stride (b_stride)
-// apart, at least a row. Rows side by side in one buffer do not.
-inline bool rows_overlap(const void* a, long long a_stride, long long a_bytes, const void* b,
-                         long long b_stride, long long b_bytes, int n) {
+// Whether two sets of n rows share a byte: rows of a_row (b_row) elements,
+// a_row_stride (b_row_stride) apart, at least a row. Rows side by side in one buffer do not.
+inline bool rows_overlap(const void* a, long long a_row_stride, long long a_row, const void* b,
+                         long long b_row_stride, long long b_row, int n, int act) {
   using wide = __int128;  // strides are the caller's
+  const int es = act == MLB_ACT_BF16 ? 2 : 4;
+  const wide a_stride = (wide)a_row_stride * es, b_stride = (wide)b_row_stride * es;
+  const wide a_bytes = (wide)a_row * es, b_bytes = (wide)b_row * es;
   const wide d = (wide)reinterpret_cast<uintptr_t>(b) - (wide)reinterpret_cast<uintptr_t>(a);
   const auto floor_div = [](wide x, wide y) { return x / y - (x % y < 0 ? 1 : 0); };
   // rows of b that row i of a meets: those with i a_stride - j b_stride - d in (-a_bytes, b_bytes)

@@ -795,9 +795,8 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
     if (n_rows > 0) {
       paged_check_rows(who, "q", q, q_stride, n_heads, head_dim, act_type);
       paged_check_rows(who, "out", out, out_stride, n_heads, head_dim, act_type);
-      const int es = act_type == MLB_ACT_BF16 ? 2 : 4;
-      const long long row = (long long)n_heads * head_dim * es;
-      if (rows_overlap(q, q_stride * es, row, out, out_stride * es, row, n_rows))
+      const long long row = (long long)n_heads * head_dim;
+      if (rows_overlap(q, q_stride, row, out, out_stride, row, n_rows, act_type))
         invalid("CudaPagedAttention: q and out must not overlap");
     }
     DeviceScope scope(device_id);

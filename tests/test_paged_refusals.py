@@ -53,6 +53,16 @@ def test_attention_takes_rows_side_by_side(call):
     assert not shares(**call) and not attend(**call)
 
 
+@pytest.mark.parametrize("stride", [1 << 60, 1 << 61, 1 << 62, (1 << 63) - 8])
+def test_strides_whose_bytes_pass_64_bits(stride):
+    for act in (0, 1):
+        for rows in (1, 3):
+            assert not attend(out=2048, qs=stride, act=act, rows=rows)
+            assert not attend(q=2048, outs=stride, act=act, rows=rows)
+            assert attend(qs=stride, outs=stride, act=act, rows=rows)
+            assert attend(q=16, qs=stride, act=act, rows=rows)
+
+
 def test_any_two_sets_of_rows():
     rng = random.Random(1)
     seen = [0, 0]
