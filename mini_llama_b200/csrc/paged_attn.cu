@@ -791,7 +791,8 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
                         page_size);
     paged_check_act(who, act_type);
     check_heads(who, n_heads, n_kv_heads);
-    if (!std::isfinite(scale)) invalid("CudaPagedAttention: scale must be finite");
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) invalid("CudaPagedAttention: scale must be finite");
     if (n_rows > 0) {
       paged_check_rows(who, "q", q, q_stride, n_heads, head_dim, act_type);
       paged_check_rows(who, "out", out, out_stride, n_heads, head_dim, act_type);
@@ -807,7 +808,7 @@ extern "C" int mlb_paged_attention(const void* pages, int n_layers, int n_pages,
     a.out_stride = out_stride;
     a.n_heads = n_heads;
     a.group = n_heads / n_kv_heads;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     a.whole = false;
     a.split = nullptr;
     a.partial = nullptr;

@@ -79,6 +79,14 @@ def test_any_two_sets_of_rows():
     assert min(seen) > 300
 
 
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38, float("nan"), float("-inf")])
+def test_scales_past_the_exponent_range_are_refused(scale):
+    """Scores are taken in powers of two: scale log2(e) has to be a number."""
+    n = _lib.lib().mlb_paged_attention(P, 2, 4, 16, 2, 64, 0, 0, P, 256, 4, 3, 1, P, P, P, 64, scale,
+                                       P + 4096, 256, None, 0, 0, None)
+    assert n == -1 and b"scale must be finite" in _lib.lib().mlb_last_error()
+
+
 def append(q=0, qo=1 << 16, k=1 << 17, v=1 << 18, qs=256, qos=256, ks=128, vs=128, rows=3):
     n = _lib.lib().mlb_paged_kv_append(
         P, 2, 4, 16, 2, 64, 0, 0, P + k, ks, P + v, vs, P + q, qs, 4, P + qo, qos, rows, 1, P, P, P,
