@@ -77,3 +77,25 @@ def test_more_prompts_than_threads(cuda, dtype):
     ([512, 1], [512, 9000]), ([1, 700, 1, 3], [5000, 900, 17, 6001])])
 def test_prompts_beside_decoding_sequences(cuda, new, lens, dtype):
     attend(new, lens, 32, 8, 128, dtype, prompt=True, page=64)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("hd", [32, 128])
+def test_prompts_on_two_streams(cuda, hd, dtype):
+    """Calls that overlap share the SMs' tensor memory, which one CTA takes whole."""
+    dtype = getattr(torch, dtype)
+    seqs = R.Seqs([400, 300, 350], [400, 700, 360], 32, seed=3)
+    cache, _, _ = filled(seqs, 4, hd, 63)
+    qs = [randn(gen(i), seqs.rows, 16, hd, dtype=dtype) for i in range(2)]
+    assert R.prompt_form(seqs.rows, 3, 4, 4, dtype)
+    want = [mlb.CudaPagedAttentionDeviceInput(q, cache, 0, *seqs.where(), 16, 4, hd) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            got[i].append(mlb.CudaPagedAttentionDeviceInput(
+                qs[i], cache, 0, *seqs.where(), 16, 4, hd, stream=streams[i].cuda_stream))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
