@@ -44,7 +44,7 @@ def test_attention_refuses_outputs_over_queries(call):
 
 
 @pytest.mark.parametrize("call", [
-    dict(out=3072), dict(q=3072), dict(out=1024, qs=512, outs=512), dict(q=1024, qs=512, outs=512),
+    dict(out=4096, rows=4), dict(q=4096, rows=4), dict(out=1024, qs=512, outs=512), dict(q=1024, qs=512, outs=512),
     dict(out=1024, rows=1), dict(out=1024, qs=512, outs=768, rows=2), dict(q=4096, outs=2048),
     dict(act=1, out=512, qs=512, outs=512), dict(act=1, out=512, rows=1, qs=512, outs=264),
     dict(act=1, out=1536, qs=512, outs=512, rows=4),
