@@ -45,6 +45,12 @@ extern "C" {
 #define MLB_ROPE_NEOX 1
 #define MLB_ROPE_NONE (-1) /* mlb_paged_kv_append: rows stored as they are */
 
+/* How mlb_rope_frequencies scales rotary frequencies for long contexts. */
+#define MLB_ROPE_SCALING_NONE 0
+#define MLB_ROPE_SCALING_LINEAR 1
+#define MLB_ROPE_SCALING_LLAMA3 2
+#define MLB_ROPE_SCALING_YARN 3
+
 /* Element type of activations where an entry point takes more than fp32. */
 #define MLB_ACT_F32 0
 #define MLB_ACT_BF16 1
@@ -156,6 +162,37 @@ int mlb_embedding(const float* table_dev, int vocab, int dim, int token,
 int mlb_rope(float* q_dev, float* k_dev, int n_heads, int n_kv_heads,
              int head_dim, int pos, float theta, int rope_type, int device_id,
              void* stream);
+/* Rotary frequencies, in radians per position, of the rotary_dim / 2 pairs (2 to
+ * 1024 dimensions), in host memory, and the amplitude that mlb_rope_rows multiplies
+ * sine and cosine with: theta^(-2 i / rotary_dim), and scaled (MLB_ROPE_SCALING_*)
+ *   LINEAR  divided by factor
+ *   LLAMA3  divided by factor where a pair makes fewer than low_freq_factor turns
+ *           over original_len positions, kept above high_freq_factor, between both
+ *           in proportion to its turns
+ *   YARN    kept up to the pair that makes beta_fast turns over original_len,
+ *           divided by factor from the one that makes beta_slow on, in proportion to
+ *           the pair's index between them (both rounded outwards); amplitude
+ *           0.1 ln(factor) + 1 for factors above 1, else 1
+ * (arguments that a scaling does not name are ignored). Host only. The reference has
+ * NONE, computed anew at each call (src/ops.cc:143-178). */
+int mlb_rope_frequencies(int rotary_dim, double theta, int scaling, double factor,
+                         double original_len, double low_freq_factor, double high_freq_factor,
+                         double beta_fast, double beta_slow, double* frequencies_host,
+                         double* amplitude);
+/* RoPE of many rows, each at positions_dev[row] (any int32): the first rotary_dim
+ * of every head's head_dim dimensions (both even, head_dim up to 1024) turned by
+ * position * frequencies_dev[pair] (64 bits, rotary_dim / 2), sine and cosine times
+ * amplitude; the other dimensions as they are. q [n_rows, n_heads, head_dim] and k
+ * [n_rows, n_kv_heads, head_dim] (0 heads: none) of act_type, a row stride (in
+ * elements) apart, any alignment, go to q_out and k_out: q and k themselves (in
+ * place), or no byte of what the call reads or of the other output. Asynchronous on
+ * `stream`. CudaRopeDeviceInput (cuda_ops.h:37) for rows. */
+int mlb_rope_rows(int act_type, const void* q_dev, long long q_stride, int n_heads,
+                  const void* k_dev, long long k_stride, int n_kv_heads, int head_dim,
+                  int rotary_dim, const int* positions_dev, const double* frequencies_dev,
+                  float amplitude, int rope_type, int n_rows, void* q_out_dev,
+                  long long q_out_stride, void* k_out_dev, long long k_out_stride, int device_id,
+                  void* stream);
 /* Index of the largest logit, lowest index on ties (ArgMax, src/ops.cc:220). */
 int mlb_argmax(const float* x_dev, int n, int* index_host, int device_id, void* stream);
 
@@ -172,6 +209,65 @@ int mlb_logprobs(int logits_type, const void* logits_dev, long long row_stride, 
                  int vocab, const int* tokens_dev, int top_k, float* logprob_dev,
                  float* entropy_dev, int* top_ids_dev, float* top_logprob_dev, int device_id,
                  void* stream);
+
+/* ------------------------------------------- rows in 8-bit integers, their product
+ * A row of values t is held as int8 codes in [-127, 127] with one fp32 scale:
+ *   A = max |t|,  code = rint(127 t / A) (ties to even),  scale = A / 127
+ * computed as if in 64 bits; A = 0 gives codes and scale 0. A row with a NaN or an
+ * infinity among its values, or a scale past fp32's largest number, gets the scale
+ * NaN: every product of it is NaN, whatever its codes. Rows of codes are 16-byte
+ * aligned, a row stride (in codes, a multiple of 16) apart; rows of activations
+ * (act_type) have any stride and alignment. Codes and scales may not overlap what a
+ * call reads. Calls are asynchronous on `stream`, need no workspace and can be
+ * captured in a CUDA graph. No reference counterpart (its 8-bit form is Q8_0, blocks
+ * of 32 of weights only, src/quant.cc:106-168). */
+/* t = x: weights (a row is an output channel), attention outputs. */
+int mlb_int8_quantize(int act_type, const void* x_dev, long long x_stride, int rows, int n,
+                      int8_t* codes_dev, long long codes_stride, float* scales_dev, int device_id,
+                      void* stream);
+/* t = h w / sqrt(mean(h^2) + eps) with fp32 weights w [n] and h = x, or with a
+ * residual h = x + residual rounded to act_type, which goes to sum (x or residual
+ * itself, or no byte of what the call reads). CudaRmsNormDeviceWeight (cuda_ops.h:27)
+ * and CudaElementwiseAddDeviceInput (cuda_ops.h:33) for rows, as the input of
+ * mlb_int8_linear. */
+int mlb_rmsnorm_int8(int act_type, const void* x_dev, long long x_stride,
+                     const void* residual_dev, long long residual_stride, const float* w_dev,
+                     int rows, int n, float eps, void* sum_dev, long long sum_stride,
+                     int8_t* codes_dev, long long codes_stride, float* scales_dev, int device_id,
+                     void* stream);
+/* t = gate / (1 + e^-gate) up: CudaSiluDeviceInput and CudaElementwiseMulDeviceInput
+ * (cuda_ops.h:29,31) for rows; gate and up may be halves of one buffer's rows. */
+int mlb_silu_mul_int8(int act_type, const void* gate_dev, long long gate_stride,
+                      const void* up_dev, long long up_stride, int rows, int n,
+                      int8_t* codes_dev, long long codes_stride, float* scales_dev, int device_id,
+                      void* stream);
+/* code * scale of every row, to out [rows, n] (fp32, or rounded to bf16). */
+int mlb_int8_dequantize(const int8_t* codes_dev, long long codes_stride, const float* scales_dev,
+                        int rows, int n, int out_type, void* out_dev, long long out_stride,
+                        int device_id, void* stream);
+/* out[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n] + bias[n] of codes x
+ * [rows, in_features] and w [out_features, in_features] (any int8, -128 too;
+ * in_features up to 131071), bias [out_features] fp32 or null, to out [rows,
+ * out_features] (out_type MLB_ACT_*, any stride and alignment, no byte of an input).
+ * The sum is exact, so a row's results depend on neither the rows beside it nor the
+ * run. CudaQ80LinearDeviceInput (include/mini_llama/cuda_quant.h:18) with 8-bit
+ * activations. */
+int mlb_int8_linear(const int8_t* x_dev, long long x_stride, const float* x_scale_dev, int rows,
+                    int in_features, const int8_t* w_dev, long long w_stride,
+                    const float* w_scale_dev, int out_features, const float* bias_dev,
+                    int out_type, void* out_dev, long long out_stride, int device_id,
+                    void* stream);
+/* Waits in mlb_int8_linear are bounded; results that one left undone become NaN.
+ * Waits for the device, returns the last wait that gave up (MLB_ERR_TIMEOUT, site)
+ * since the call before, or (0, 0), and clears it; one such word per device. */
+int mlb_int8_linear_status(int device_id, int* code, int* where);
+/* Failure-detection self-test (as mlb_wait_selftest): a product of `rows` (1 to 1024)
+ * rows of its own with a barrier that never completes and waits of limit_ms (0 <
+ * limit_ms <= 1000). Writes the status recorded (MLB_ERR_TIMEOUT and a site, cleared as
+ * by mlb_int8_linear_status) and how many rows are NaN; the device stays usable.
+ * Synchronous. */
+int mlb_int8_linear_wait_selftest(int device_id, int rows, double limit_ms, int* code, int* where,
+                                  int* nan_rows);
 
 /* ------------------------------------------------------ KV cache + attention
  * The cache is two fp32 arrays [n_layers][max_seq_len][n_kv_heads][head_dim]

@@ -23,6 +23,7 @@ from .configs import (F32, Q4_0, Q4_1, Q8_0, W_BK, W_BQ, W_BV, W_DOWN, W_FFN_NOR
                       W_WQ, W_WV, W_ATTENTION_NORM)
 
 ROPE_NORMAL, ROPE_NEOX = 0, 1
+ROPE_SCALING_NONE, ROPE_SCALING_LINEAR, ROPE_SCALING_LLAMA3, ROPE_SCALING_YARN = 0, 1, 2, 3
 ROPE_NONE = -1  # MLB_ROPE_NONE: CudaPagedKvCache.AppendDevice stores rows as they are
 ATTN_CPU_COMPAT, ATTN_STANDARD = 0, 1
 KV_F32, KV_BF16 = 0, 1  # MLB_KV_F32, MLB_KV_BF16: KV cache element type of a Batch
@@ -35,7 +36,11 @@ __all__ = [
     "CudaLinearDeviceInput", "CudaQ80Linear", "CudaQ40Linear", "CudaQ41Linear", "CudaLinear",
     "CudaRmsNormDeviceWeight", "CudaSiluDeviceInput", "CudaElementwiseMulDeviceInput",
     "CudaElementwiseAddDeviceInput", "CudaSoftmax", "CudaEmbeddingLookupDeviceWeight",
-    "CudaRopeDeviceInput", "CudaArgMax", "CudaLogProbs", "CudaKvCache",
+    "CudaRopeDeviceInput", "RopeTable", "CudaRopeRowsDeviceInput", "ROPE_SCALING_NONE",
+    "ROPE_SCALING_LINEAR", "ROPE_SCALING_LLAMA3", "ROPE_SCALING_YARN", "CudaArgMax",
+    "CudaLogProbs", "CudaInt8QuantizeDeviceInput", "CudaRmsNormInt8DeviceWeight",
+    "CudaSiluMulInt8DeviceInput", "CudaInt8DequantizeDeviceInput", "CudaInt8LinearDeviceInput",
+    "int8_linear_status", "int8_linear_wait_selftest", "CudaKvCache",
     "CudaAttentionDecodeDeviceInput", "CudaPagedKvCache", "CudaPagedAttentionDeviceInput",
     "paged_attention_status", "paged_attention_wait_selftest",
     "QMatrix", "CudaModel", "Context", "Batch", "ForwardToken", "configs", "tp_plan", "nccl_unique_id",
@@ -311,6 +316,348 @@ def CudaLogProbs(logits, tokens, top_k=0, stream=None):
                              logprob.data_ptr(), entropy.data_ptr(), ids.data_ptr(),
                              top.data_ptr(), index, _raw_stream(index)))
     return logprob, entropy, ids, top
+
+
+# ------------------------------------------- rows in 8-bit integers, their product
+
+def _act_rows(who, name, t, shape=None, index=None):
+    """Row stride of t [rows, n] (fp32 or bf16) as the kernels read it; t itself, or a
+    copy where its elements do not follow one another."""
+    if t.dim() != 2 or (shape is not None and t.shape != shape):
+        want = "[rows, n]" if shape is None else list(shape)
+        raise MlbError(-1, f"{who}: expected {name} {want}, got {list(t.shape)}")
+    if index is None:
+        if not t.is_cuda:
+            raise MlbError(-1, f"{who}: {name} must be on a CUDA device")
+    else:
+        _on_device(who, name, t, index)
+    rows, n = t.shape
+    stride, one = t.stride()
+    if (one != 1 and n > 1) or (stride < n and rows > 1):
+        return t.contiguous(), n
+    return t, stride if rows > 1 else n
+
+
+def _new_codes(like, rows, n):
+    """Room for codes [rows, n], rows 16-byte aligned, and their scales."""
+    torch = _torch()
+    width = (n + 15) // 16 * 16
+    codes = like.new_empty(rows, width, dtype=torch.int8)
+    return codes, width, like.new_empty(rows, dtype=torch.float32)
+
+
+def CudaInt8QuantizeDeviceInput(x, stream=None):
+    """Rows of x [rows, n] (fp32 or bf16) as int8 codes with a scale per row
+    (mlb_int8_quantize): returns (codes int8 [rows, n], rows 16-byte aligned, scales
+    fp32 [rows]). Of a weight [out_features, in_features]: a scale per channel."""
+    who = "Int8Quantize"
+    act = _act_type(who, x)
+    x, stride = _act_rows(who, "x", x)
+    rows, n = x.shape
+    if n == 0:
+        raise MlbError(-1, f"{who}: rows must have at least one element")
+    index = x.get_device()
+    if stream is not None:
+        return _on_stream(lambda: CudaInt8QuantizeDeviceInput(x), x.device, stream)
+    codes, width, scales = _new_codes(x, rows, n)
+    check(lib().mlb_int8_quantize(act, x.data_ptr(), stride, rows, n, codes.data_ptr(), width,
+                                  scales.data_ptr(), index, _raw_stream(index)))
+    return codes if width == n else codes[:, :n], scales
+
+
+def CudaRmsNormInt8DeviceWeight(x, w, eps, residual=None, sum_out=None, stream=None):
+    """RMSNorm of rows x [rows, n] (fp32 or bf16) with weights w [n] (fp32) as int8
+    codes with a scale per row (mlb_rmsnorm_int8): returns (codes, scales), or with a
+    residual, which is added first, (codes, scales, sum). The sum is in x's type, in
+    sum_out if given: x or residual itself, or no part of them. For one row: x [n]."""
+    who = "RmsNormInt8"
+    act = _act_type(who, x)
+    if x.dim() == 1:
+        x = x[None]
+        residual = residual[None] if residual is not None and residual.dim() == 1 else residual
+        sum_out = sum_out[None] if sum_out is not None and sum_out.dim() == 1 else sum_out
+    x_in = x
+    x, stride = _act_rows(who, "x", x)
+    rows, n = x.shape
+    if n == 0:
+        raise MlbError(-1, f"{who}: rows must have at least one element")
+    index = x.get_device()
+    if w.dtype is not _torch().float32 or w.shape != (n,) or not w.is_contiguous():
+        raise MlbError(-1, f"{who}: expected contiguous float32 weights [{n}], got {w.dtype} "
+                           f"{list(w.shape)}")
+    _on_device(who, "w", w, index)
+    if residual is None and sum_out is not None:
+        raise MlbError(-1, f"{who}: sum_out without a residual")
+    if residual is not None and residual.dtype is not x.dtype:
+        raise MlbError(-1, f"{who}: x and residual differ in type")
+    if stream is not None:
+        return _on_stream(lambda: CudaRmsNormInt8DeviceWeight(x_in, w, eps, residual, sum_out),
+                          x.device, stream)
+    r_at = s_at = None
+    r_stride = s_stride = n
+    if residual is not None:
+        r, r_stride = _act_rows(who, "residual", residual, x.shape, index)
+        r_at = r.data_ptr()
+        if sum_out is None:
+            sum_out = x.new_empty(rows, n)
+        else:
+            _on_device(who, "sum_out", sum_out, index)
+            s_stride = sum_out.stride(0) if sum_out.dim() == 2 and rows > 1 else n
+            if (sum_out.shape != x.shape or sum_out.dtype is not x.dtype
+                    or (sum_out.stride(1) != 1 and n > 1) or s_stride < n):
+                raise MlbError(-1, f"{who}: sum_out must be shaped like x, with elements that "
+                                   "follow one another")
+        s_at = sum_out.data_ptr()
+    codes, width, scales = _new_codes(x, rows, n)
+    check(lib().mlb_rmsnorm_int8(act, x.data_ptr(), stride, r_at, r_stride, w.data_ptr(), rows, n,
+                                 eps, s_at, s_stride, codes.data_ptr(), width, scales.data_ptr(),
+                                 index, _raw_stream(index)))
+    if width != n:
+        codes = codes[:, :n]
+    return (codes, scales) if residual is None else (codes, scales, sum_out)
+
+
+def CudaSiluMulInt8DeviceInput(gate, up, stream=None):
+    """SiLU(gate) * up of rows [rows, n] (fp32 or bf16; halves of one product's rows
+    as they are) as int8 codes with a scale per row (mlb_silu_mul_int8): returns
+    (codes, scales)."""
+    who = "SiluMulInt8"
+    act = _act_type(who, gate)
+    gate, g_stride = _act_rows(who, "gate", gate)
+    rows, n = gate.shape
+    if n == 0:
+        raise MlbError(-1, f"{who}: rows must have at least one element")
+    index = gate.get_device()
+    if up.dtype is not gate.dtype:
+        raise MlbError(-1, f"{who}: gate and up differ in type")
+    up, u_stride = _act_rows(who, "up", up, gate.shape, index)
+    if stream is not None:
+        return _on_stream(lambda: CudaSiluMulInt8DeviceInput(gate, up), gate.device, stream)
+    codes, width, scales = _new_codes(gate, rows, n)
+    check(lib().mlb_silu_mul_int8(act, gate.data_ptr(), g_stride, up.data_ptr(), u_stride, rows, n,
+                                  codes.data_ptr(), width, scales.data_ptr(), index,
+                                  _raw_stream(index)))
+    return codes if width == n else codes[:, :n], scales
+
+
+def _code_rows(who, name, t, index=None):
+    """codes [rows, n] with 16-byte aligned rows (t itself, or a copy) and their stride."""
+    torch = _torch()
+    if t.dtype is not torch.int8 or t.dim() != 2 or t.shape[1] == 0:
+        raise MlbError(-1, f"{who}: expected int8 {name} [rows, n], got {t.dtype} {list(t.shape)}")
+    if index is None:
+        if not t.is_cuda:
+            raise MlbError(-1, f"{who}: {name} must be on a CUDA device")
+    else:
+        _on_device(who, name, t, index)
+    rows, n = t.shape
+    width = (n + 15) // 16 * 16
+    stride, one = t.stride()
+    if rows <= 1:
+        stride = width
+    if (one != 1 and n > 1) or stride < n or stride % 16 or t.data_ptr() % 16:
+        padded = t.new_empty(rows, width)
+        padded[:, :n] = t
+        return padded, width
+    return t, stride
+
+
+def _scale_vector(who, name, t, n, index):
+    if t.dtype is not _torch().float32 or t.shape != (n,) or not t.is_contiguous():
+        raise MlbError(-1, f"{who}: expected contiguous float32 {name} [{n}], got {t.dtype} "
+                           f"{list(t.shape)}")
+    _on_device(who, name, t, index)
+
+
+def _out_type(who, dtype):
+    torch = _torch()
+    if dtype is None or dtype is torch.float32:
+        return torch.float32, 0
+    if dtype is torch.bfloat16:
+        return dtype, 1
+    raise MlbError(-1, f"{who}: expected float32 or bfloat16, got {dtype}")
+
+
+def CudaInt8DequantizeDeviceInput(codes, scales, out_dtype=None, stream=None):
+    """The values [rows, n] that codes with a scale per row stand for, fp32 or rounded
+    to bf16 (mlb_int8_dequantize)."""
+    who = "Int8Dequantize"
+    dtype, act = _out_type(who, out_dtype)
+    if stream is not None and codes.is_cuda:
+        return _on_stream(lambda: CudaInt8DequantizeDeviceInput(codes, scales, out_dtype),
+                          codes.device, stream)
+    c, stride = _code_rows(who, "codes", codes)
+    rows, n = codes.shape
+    index = c.get_device()
+    _scale_vector(who, "scales", scales, rows, index)
+    out = scales.new_empty(rows, n, dtype=dtype)
+    check(lib().mlb_int8_dequantize(c.data_ptr(), stride, scales.data_ptr(), rows, n, act,
+                                    out.data_ptr(), n, index, _raw_stream(index)))
+    return out
+
+
+def CudaInt8LinearDeviceInput(x, x_scale, w, w_scale, bias=None, out_dtype=None, out=None,
+                              stream=None):
+    """Product of int8 codes x [rows, in_features] and w [out_features, in_features]
+    with a scale per row of each, plus bias [out_features] (fp32): (x w^T) x_scale
+    w_scale + bias as fp32 or bf16 [rows, out_features] (mlb_int8_linear), in out if
+    given (of any row stride). Codes whose rows are not 16-byte aligned are copied at
+    every call: CudaInt8QuantizeDeviceInput makes aligned ones."""
+    who = "Int8Linear"
+    torch = _torch()
+    if out is not None and out_dtype is None:
+        out_dtype = out.dtype
+    dtype, act = _out_type(who, out_dtype)
+    if stream is not None and x.is_cuda:
+        return _on_stream(lambda: CudaInt8LinearDeviceInput(x, x_scale, w, w_scale, bias,
+                                                            out_dtype, out), x.device, stream)
+    if x.dim() == 1:
+        x = x[None]
+    xc, x_stride = _code_rows(who, "x", x)
+    index = xc.get_device()
+    wc, w_stride = _code_rows(who, "w", w, index)
+    rows, k = x.shape
+    n = w.shape[0]
+    if w.shape[1] != k:
+        raise MlbError(-1, f"{who}: dimension mismatch x={list(x.shape)} weight={list(w.shape)}")
+    _scale_vector(who, "x_scale", x_scale, rows, index)
+    _scale_vector(who, "w_scale", w_scale, n, index)
+    if bias is not None:
+        _scale_vector(who, "bias", bias, n, index)
+    if out is None:
+        out = x_scale.new_empty(rows, n, dtype=dtype)
+        out_stride = n
+    else:
+        _on_device(who, "out", out, index)
+        if (out.shape != (rows, n) or out.dtype is not dtype or (n > 1 and out.stride(1) != 1)
+                or (rows > 1 and out.stride(0) < n)):
+            raise MlbError(-1, f"{who}: out must be {dtype} [{rows}, {n}] with elements that "
+                               "follow one another")
+        out_stride = out.stride(0) if rows > 1 else n
+    check(lib().mlb_int8_linear(xc.data_ptr(), x_stride, x_scale.data_ptr(), rows, k,
+                                wc.data_ptr(), w_stride, w_scale.data_ptr(), n,
+                                None if bias is None else bias.data_ptr(), act, out.data_ptr(),
+                                out_stride, index, _raw_stream(index)))
+    return out
+
+
+def int8_linear_status(device_id=0):
+    """(status code, site) of the last bounded wait that gave up in
+    CudaInt8LinearDeviceInput since the last call, (0, 0) if none did
+    (mlb_int8_linear_status); results that it left undone are NaN. Waits for the
+    device."""
+    code, where = ctypes.c_int(0), ctypes.c_int(0)
+    check(lib().mlb_int8_linear_status(device_id, ctypes.byref(code), ctypes.byref(where)))
+    return code.value, where.value
+
+
+def int8_linear_wait_selftest(rows=8, limit_ms: float = 1.0, device_id: int = 0):
+    """Runs a product of `rows` rows with a barrier that never completes and returns
+    (status code, site, rows that became NaN): (MLB_ERR_TIMEOUT, 1101 .., rows) when its
+    waits gave up after limit_ms (mlb_int8_linear_wait_selftest)."""
+    code, where, nan = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
+    check(lib().mlb_int8_linear_wait_selftest(device_id, rows, float(limit_ms),
+                                              ctypes.byref(code), ctypes.byref(where),
+                                              ctypes.byref(nan)))
+    return code.value, where.value, nan.value
+
+
+# ------------------------------------------------------------ rotation of rows
+
+class RopeTable:
+    """Rotary frequencies of rotary_dim dimensions on a device, as CudaRopeRowsDeviceInput
+    reads them (mlb_rope_frequencies): theta^(-2 i / rotary_dim), scaled for long
+    contexts by ROPE_SCALING_LINEAR (factor), ROPE_SCALING_LLAMA3 (factor, original_len,
+    low_freq_factor, high_freq_factor) or ROPE_SCALING_YARN (factor, original_len,
+    beta_fast, beta_slow; sine and cosine times `amplitude`). `factors` [rotary_dim / 2]
+    divides each pair's frequency instead (what a checkpoint's table of factors holds)."""
+
+    def __init__(self, rotary_dim, theta=10000.0, scaling=ROPE_SCALING_NONE, factor=1.0,
+                 original_len=0, low_freq_factor=1.0, high_freq_factor=4.0, beta_fast=32.0,
+                 beta_slow=1.0, factors=None, device_id=0):
+        torch = _torch()
+        half = max(0, rotary_dim // 2)
+        values = np.zeros(max(half, 1), np.float64)
+        amplitude = ctypes.c_double(1.0)
+        check(lib().mlb_rope_frequencies(
+            rotary_dim, theta, scaling, factor, original_len, low_freq_factor, high_freq_factor,
+            beta_fast, beta_slow, values.ctypes.data_as(ctypes.POINTER(ctypes.c_double)),
+            ctypes.byref(amplitude)))
+        if factors is not None:
+            f = np.asarray(factors, np.float64)
+            if f.shape != (half,) or not (np.isfinite(f) & (f > 0)).all():
+                raise MlbError(-1, f"RopeTable: expected {half} finite positive factors")
+            values = values / f
+        self.rotary_dim = rotary_dim
+        self.amplitude = amplitude.value
+        self.device_id = device_id
+        self.frequencies = torch.from_numpy(values).to(torch.device("cuda", device_id))
+
+
+def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NORMAL, q_out=None,
+                            k_out=None, stream=None):
+    """RoPE of rows at positions of their own (mlb_rope_rows): q [rows, n_heads,
+    head_dim] and k [rows, n_kv_heads, head_dim] (fp32 or bf16, any row stride; one of
+    them may be None) turned to positions [rows] (int32) in their first table.rotary_dim
+    dimensions. Returns (q_out, k_out): new tensors, or those given (q and k themselves
+    for in place, otherwise no part of either)."""
+    who = "RopeRows"
+    first = q if q is not None else k
+    if first is None:
+        raise MlbError(-1, f"{who}: neither q nor k")
+    if first.dim() != 3:
+        raise MlbError(-1, f"{who}: expected rows [rows, heads, head_dim], got "
+                           f"{list(first.shape)}")
+    act = _act_type(who, first)
+    rows, _, dim = first.shape
+    index = table.device_id
+    _int_tensor(who, "positions", positions, (rows,), index)
+    for name, t, given in (("q", q, q_out), ("k", k, k_out)):
+        if t is None:
+            if given is not None:
+                raise MlbError(-1, f"{who}: {name}_out without {name}")
+            continue
+        _on_device(who, name, t, index)
+        if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim or t.dtype is not first.dtype:
+            raise MlbError(-1, f"{who}: expected {name} [{rows}, heads, {dim}] of "
+                               f"{first.dtype}, got {t.dtype} {list(t.shape)}")
+        if given is not None:
+            _on_device(who, f"{name}_out", given, index)
+            if given.shape != t.shape or given.dtype is not t.dtype or not _whole_rows(given):
+                raise MlbError(-1, f"{who}: {name}_out must be shaped like {name}, its rows' "
+                                   "elements following one another")
+    if stream is not None:
+        return _on_stream(lambda: CudaRopeRowsDeviceInput(q, k, positions, table, rope_type,
+                                                          q_out, k_out), first.device, stream)
+    args, outs, held = [], [], []
+    for t, given in ((q, q_out), (k, k_out)):
+        if t is None:
+            args.append((None, 0, 0, None, 0))
+            outs.append(None)
+            continue
+        heads = t.shape[1]
+        if given is None:
+            given = t.new_empty(rows, heads, dim)
+        if not _whole_rows(t):
+            t = t.contiguous()
+            held.append(t)
+        width = heads * dim
+        args.append((t.data_ptr(), t.stride(0) if rows > 1 else width, heads, given.data_ptr(),
+                     given.stride(0) if rows > 1 else width))
+        outs.append(given)
+    (qp, qs, qh, qo, qos), (kp, ks, kh, ko, kos) = args
+    check(lib().mlb_rope_rows(act, qp, qs, qh, kp, ks, kh, dim, table.rotary_dim,
+                              positions.data_ptr(), table.frequencies.data_ptr(), table.amplitude,
+                              rope_type, rows, qo, qos, ko, kos, index, _raw_stream(index)))
+    return outs[0], outs[1]
+
+
+def _whole_rows(t):
+    """Whether each row of t [rows, heads, dim] is one run of elements, apart from others."""
+    rows, heads, dim = t.shape
+    stride, head, one = t.stride()
+    return ((one == 1 or dim == 1) and (head == dim or heads == 1)
+            and (stride >= heads * dim or rows <= 1))
 
 
 # -------------------------------------------------------- KV cache, attention

@@ -13,7 +13,7 @@ from . import build as _build
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 _c_int, _c_size_t, _c_float, _c_u64 = ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_uint64
-_c_ll = ctypes.c_longlong
+_c_ll, _c_double = ctypes.c_longlong, ctypes.c_double
 _vp, _fp = ctypes.c_void_p, ctypes.POINTER(ctypes.c_float)
 _ip = ctypes.POINTER(ctypes.c_int)
 
@@ -54,6 +54,11 @@ SIGNATURES = [
     ("mlb_softmax", _c_int, [_vp, _c_int, _vp, _c_int, _vp]),
     ("mlb_embedding", _c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
     ("mlb_rope", _c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _vp]),
+    ("mlb_rope_frequencies", _c_int, [_c_int, _c_double, _c_int] + [_c_double] * 6 + [
+        ctypes.POINTER(_c_double), ctypes.POINTER(_c_double)]),
+    ("mlb_rope_rows", _c_int, [_c_int, _vp, _c_ll, _c_int, _vp, _c_ll, _c_int, _c_int, _c_int, _vp,
+                               _vp, _c_float, _c_int, _c_int, _vp, _c_ll, _vp, _c_ll, _c_int,
+                               _vp]),
     ("mlb_argmax", _c_int, [_vp, _c_int, _ip, _c_int, _vp]),
     ("mlb_kv_write", _c_int, [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp,
                               _c_int, _vp]),
@@ -63,6 +68,18 @@ SIGNATURES = [
                                               _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp]),
     ("mlb_logprobs", _c_int, [_c_int, _vp, _c_ll, _c_int, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp,
                               _c_int, _vp]),
+    ("mlb_int8_quantize", _c_int, [_c_int, _vp, _c_ll, _c_int, _c_int, _vp, _c_ll, _vp, _c_int,
+                                   _vp]),
+    ("mlb_rmsnorm_int8", _c_int, [_c_int, _vp, _c_ll, _vp, _c_ll, _vp, _c_int, _c_int, _c_float,
+                                  _vp, _c_ll, _vp, _c_ll, _vp, _c_int, _vp]),
+    ("mlb_silu_mul_int8", _c_int, [_c_int, _vp, _c_ll, _vp, _c_ll, _c_int, _c_int, _vp, _c_ll, _vp,
+                                   _c_int, _vp]),
+    ("mlb_int8_dequantize", _c_int, [_vp, _c_ll, _vp, _c_int, _c_int, _c_int, _vp, _c_ll, _c_int,
+                                     _vp]),
+    ("mlb_int8_linear", _c_int, [_vp, _c_ll, _vp, _c_int, _c_int, _vp, _c_ll, _vp, _c_int, _vp,
+                                 _c_int, _vp, _c_ll, _c_int, _vp]),
+    ("mlb_int8_linear_status", _c_int, [_c_int, _ip, _ip]),
+    ("mlb_int8_linear_wait_selftest", _c_int, [_c_int, _c_int, _c_double, _ip, _ip, _ip]),
     ("mlb_paged_kv_page_bytes", _c_int, [_c_int, _c_int, _c_int, ctypes.POINTER(_c_size_t)]),
     ("mlb_paged_kv_append", _c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                      _vp, _c_ll, _vp, _c_ll, _vp, _c_ll, _c_int, _vp, _c_ll,

@@ -1,0 +1,464 @@
+// int8_gemm.cu — product of int8 rows with a scale for each token and each channel, on
+// the tcgen05 tensor cores.
+//
+//   y[m, n] = (sum_k x[m, k] w[n, k]) sx[m] sw[n] + bias[n]
+//
+// Sums are exact in 32-bit integers (131071 products of two codes of at most 128 are
+// below 2^31), in any order: a row's result does not depend on the rows beside it, on
+// how the work is split or on the run. Then three fp32 steps, each rounded once, and
+// one rounding to bf16 where that is asked for.
+//
+// A CTA takes 128 channels by NT tokens and a share of K: one lane loads tiles of
+// 128 bytes along K by TMA (what lies past the matrices' edges arrives as zeros) into a
+// ring, one lane issues the products, channels as the rows of D, so that few tokens fill
+// the tensor cores' other side and a warp stores consecutive channels. Where the tiles
+// alone leave SMs idle, a cluster of CTAs shares K and joins its sums through
+// distributed shared memory: no workspace, one launch.
+//
+// Few tokens are bound by HBM (the weights are read once), many by the tensor cores.
+//
+// Every wait is bounded: on a timeout the waiting thread records MLB_ERR_TIMEOUT in the
+// device's status word (mlb_int8_linear_status) and raises the CTA's abort flag, copies
+// and products in flight are waited for (bounded), the results of the cluster's tile
+// become NaN, tensor memory is released and the CTA exits.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "paged.cuh"
+#include "runtime.cuh"
+#include "rows.cuh"
+#include "tcgen05.cuh"
+
+namespace mlb {
+
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kTileK = 128;      // bytes along K of a tile
+constexpr int kChannels = 128;   // channels of a CTA
+constexpr int kMaxStages = 8;
+constexpr int kMaxSplit = 8;
+constexpr int kMaxK = 131071;
+constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
+
+__device__ DeviceStatus g_status;
+
+struct LinearArgs {
+  const float* x_scale;
+  const float* w_scale;
+  const float* bias;
+  void* out;
+  long long out_stride;
+  int rows, n, tiles_k, channel_tiles, split, stages;
+  long long wait_cycles;  // limit of a wait
+  int never;              // arrivals that the first barrier waits for in vain (self-test)
+};
+
+struct Shared {
+  uint64_t full[kMaxStages], empty[kMaxStages], done, drain;
+  int abort_flag;
+  uint32_t tmem;
+};
+
+__device__ __forceinline__ bool wait(Shared& sh, const LinearArgs& a, uint64_t* bar,
+                                     uint32_t parity, int where) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*(volatile int*)&sh.abort_flag) return false;
+    if (clock64() - start > a.wait_cycles) {
+      atomicExch(&g_status.code, MLB_ERR_TIMEOUT);
+      atomicExch(&g_status.where, where);
+      *(volatile int*)&sh.abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+// The last wait for what is in flight, after which there is nothing more to be done.
+__device__ __forceinline__ void drain_wait(const LinearArgs& a, uint64_t* bar, uint32_t parity) {
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - start < a.wait_cycles) {
+  }
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ int peer_int(uint32_t address) {
+  int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Grid: ((token tile * channel tiles) + channel tile) * split + share of K, the shares of
+// a tile being a cluster.
+template <int NT, class T>
+__global__ void __launch_bounds__(kThreads)
+    int8_linear_kernel(const __grid_constant__ CUtensorMap w_map,
+                       const __grid_constant__ CUtensorMap x_map, const LinearArgs a) {
+  constexpr int COLS = NT < 32 ? 32 : NT;
+  constexpr int W_BYTES = kChannels * kTileK, X_BYTES = NT * kTileK;
+  constexpr int STAGE = W_BYTES + X_BYTES;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ Shared sh;
+  uint8_t* smem = dynamic + (-smem_addr(dynamic) & 1023u);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int share = blockIdx.x % a.split, tile = blockIdx.x / a.split;
+  const int token_tile = tile / a.channel_tiles;
+  const int channel0 = (tile - token_tile * a.channel_tiles) * kChannels;
+  const int token0 = token_tile * NT;
+  // the CTA's tiles along K; a share has one at least
+  const int k0 = (int)((long long)a.tiles_k * share / a.split);
+  const int count = (int)((long long)a.tiles_k * (share + 1) / a.split) - k0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(&sh.full[i], 1 + a.never);
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.done, 1);
+    mbar_init(&sh.drain, 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem, COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  int issued = 0;
+  if (warp == 0 && lane == 0) {
+    for (; issued < count; ++issued) {
+      const int s = issued % a.stages, turn = issued / a.stages;
+      if (turn > 0 && !wait(sh, a, &sh.empty[s], (uint32_t)(turn - 1) & 1u, 1101)) break;
+      uint8_t* stage = smem + s * STAGE;
+      mbar_arrive_expect_tx(&sh.full[s], STAGE);
+      tma_load(stage, &w_map, (k0 + issued) * kTileK, channel0, &sh.full[s]);
+      tma_load(stage + W_BYTES, &x_map, (k0 + issued) * kTileK, token0, &sh.full[s]);
+    }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = idesc_i8(kChannels, NT);
+    for (int i = 0; i < count; ++i) {
+      const int s = i % a.stages, turn = i / a.stages;
+      if (!wait(sh, a, &sh.full[s], (uint32_t)turn & 1u, 1102)) break;
+      tc_fence_after();
+      const uint64_t w = smem_desc_sw128(smem_addr(smem + s * STAGE));
+      const uint64_t x = smem_desc_sw128(smem_addr(smem + s * STAGE + W_BYTES));
+#pragma unroll
+      for (int k = 0; k < kTileK / 32; ++k)
+        tc_mma_i8(tmem, w + 2 * k, x + 2 * k, idesc, i > 0 || k > 0);
+      tc_commit(&sh.empty[s]);
+      if (i == count - 1) tc_commit(&sh.done);
+    }
+  }
+  __syncwarp();
+  bool ok = __syncthreads_and(wait(sh, a, &sh.done, 0, 1103));
+  if (!ok) {
+    // nothing is in flight when shared and tensor memory go
+    if (threadIdx.x == 0)
+      for (int j = max(0, issued - a.stages); j < issued; ++j)
+        drain_wait(a, &sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u);
+    if (warp == 1 && lane == 0) {
+      tc_commit(&sh.drain);
+      drain_wait(a, &sh.drain, 0);
+    }
+    __syncthreads();
+  }
+  tc_fence_after();
+
+  const int tokens = min(NT, a.rows - token0);
+  const int channel = channel0 + threadIdx.x;
+  const bool inside = channel < a.n;
+  const float sw = inside ? a.w_scale[channel] : 0.0f;
+  const float bias = inside && a.bias ? a.bias[channel] : 0.0f;
+  T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel;
+  const auto finish = [&](int sum, int t, bool good) {
+    float y = (float)sum * a.x_scale[token0 + t];
+    y = a.bias ? fmaf(y, sw, bias) : y * sw;
+    put(out + (long long)t * a.out_stride, good ? y : nanf(""));
+  };
+  const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  if (a.split == 1) {
+#pragma unroll 1
+    for (int c = 0; c < tokens; c += 8) {
+      uint32_t d[8];
+      tmem_ld8(lanes + c, d);
+      if (inside) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < tokens) finish((int)d[i], c + i, ok);
+      }
+    }
+  } else {
+    // every share leaves its sums, tokens apart, over the ring that it no longer needs;
+    // tokens are finished by the shares in turn
+    int* sums = reinterpret_cast<int*>(smem);
+#pragma unroll 1
+    for (int c = 0; c < tokens; c += 8) {
+      uint32_t d[8];
+      tmem_ld8(lanes + c, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sums[(c + i) * kChannels + threadIdx.x] = (int)d[i];
+    }
+    if (threadIdx.x == 0) sh.abort_flag = !ok;
+    cluster_sync_all();
+    for (int r = 0; r < a.split; ++r) ok = ok && peer_int(peer_address(&sh.abort_flag, r)) == 0;
+    for (int t = share; t < tokens; t += a.split) {
+      const int* mine = sums + t * kChannels + threadIdx.x;
+      int v[kMaxSplit];
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        v[r] = r < a.split ? peer_int(peer_address(mine, r)) : 0;
+      int sum = 0;
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r) sum += v[r];
+      if (inside) finish(sum, t, ok);
+    }
+    __syncwarp();
+    cluster_sync_all();  // a CTA's shared memory lives until the others have read it
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, COLS);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static const EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    MLB_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !p)
+      fail(MLB_ERR_CUDA, "Int8Linear: the driver has no tensor maps");
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return f;
+}
+
+// Tiles of 128 bytes by `box_rows` of a byte matrix; past its edges lie zeros.
+CUtensorMap tile_map(const void* p, long long stride, int rows, int k, int box_rows) {
+  CUtensorMap m;
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows};
+  const cuuint32_t unit[2] = {1, 1};
+  const CUresult r = encode_tiled()(
+      &m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, unit,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    fail(MLB_ERR_CUDA, "Int8Linear: no tensor map for " + std::to_string(rows) + " rows of " +
+                           std::to_string(k) + " (error " + std::to_string((int)r) + ")");
+  return m;
+}
+
+struct Operands {
+  const int8_t* x;
+  long long x_stride;
+  const int8_t* w;
+  long long w_stride;
+  int k;
+};
+
+template <int NT, class T>
+void launch(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream) {
+  constexpr int STAGE = (kChannels + NT) * kTileK;
+  a.tiles_k = (o.k + kTileK - 1) / kTileK;
+  a.channel_tiles = (a.n + kChannels - 1) / kChannels;
+  const long long tiles = (long long)a.channel_tiles * ((a.rows + NT - 1) / NT);
+  // shares of K: double while the tiles leave SMs without their two CTAs and a share
+  // keeps at least 4 tiles of K
+  a.split = 1;
+  while (a.split < kMaxSplit && tiles * a.split * 2 <= 2 * sm_count(device_id) &&
+         a.tiles_k / (a.split * 2) >= 4)
+    a.split *= 2;
+  const int share = (a.tiles_k + a.split - 1) / a.split;
+  // half of an SM's shared memory, for two CTAs
+  constexpr int kMost = std::min(kMaxStages, 110 * 1024 / STAGE);
+  a.stages = std::min(kMost, share);
+  // the ring, or the sums of all tokens
+  const int bytes = std::max(a.stages * STAGE, a.split > 1 ? NT * kChannels * 4 : 0) + 1024;
+  constexpr int kMostBytes = std::max(kMost * STAGE, NT * kChannels * 4) + 1024;
+  static_assert(kMostBytes <= 227 * 1024);
+  allow_smem(int8_linear_kernel<NT, T>, kMostBytes, device_id);
+  if (tiles * a.split > 0x7fffffffLL) invalid("Int8Linear: too many rows");
+  const CUtensorMap w_map = tile_map(o.w, o.w_stride, a.n, o.k, kChannels);
+  const CUtensorMap x_map = tile_map(o.x, o.x_stride, a.rows, o.k, NT);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * a.split));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  MLB_CUDA(cudaLaunchKernelEx(&cfg, int8_linear_kernel<NT, T>, w_map, x_map, a));
+}
+
+template <class T>
+void dispatch(const Operands& o, const LinearArgs& a, int device_id, cudaStream_t stream) {
+  if (a.rows <= 16) return launch<16, T>(o, a, device_id, stream);
+  if (a.rows <= 32) return launch<32, T>(o, a, device_id, stream);
+  if (a.rows <= 64) return launch<64, T>(o, a, device_id, stream);
+  if (a.rows <= 128) return launch<128, T>(o, a, device_id, stream);
+  return launch<256, T>(o, a, device_id, stream);
+}
+
+void run(const Operands& o, LinearArgs a, int out_type, int device_id, cudaStream_t stream) {
+  if (a.wait_cycles == 0) a.wait_cycles = kWaitCycles;
+  if (out_type == MLB_ACT_BF16)
+    dispatch<__nv_bfloat16>(o, a, device_id, stream);
+  else
+    dispatch<float>(o, a, device_id, stream);
+}
+
+// The last wait of the device that gave up, and forgets it.
+DeviceStatus take_status() {
+  MLB_CUDA(cudaDeviceSynchronize());
+  DeviceStatus s;
+  MLB_CUDA(cudaMemcpyFromSymbol(&s, g_status, sizeof(s)));
+  const DeviceStatus none = {0, 0};
+  MLB_CUDA(cudaMemcpyToSymbol(g_status, &none, sizeof(none)));
+  return s;
+}
+
+void check_codes(const std::string& who, const char* name, const void* p, long long stride, int k) {
+  if (!p) invalid(who + ": null " + name);
+  if (stride < k) invalid(who + ": row stride of " + name + " is smaller than a row");
+  if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || stride % 16 != 0)
+    invalid(who + ": rows of " + name + " must be 16-byte aligned");
+  if (stride >= (1LL << 40)) invalid(who + ": row stride of " + name + " must be below 2^40");
+}
+void check_floats(const std::string& who, const char* name, const void* p) {
+  if (!p) invalid(who + ": null " + name);
+  if (reinterpret_cast<uintptr_t>(p) % 4 != 0) invalid(who + ": " + name + " is unaligned");
+}
+
+}  // namespace
+
+}  // namespace mlb
+
+using namespace mlb;
+
+extern "C" int mlb_int8_linear(const int8_t* x, long long x_stride, const float* x_scale, int rows,
+                               int in_features, const int8_t* w, long long w_stride,
+                               const float* w_scale, int out_features, const float* bias,
+                               int out_type, void* out, long long out_stride, int device_id,
+                               void* stream) {
+  return guarded([&] {
+    const std::string who = "Int8Linear";
+    paged_check_act("Int8Linear", out_type);
+    if (rows < 0) invalid(who + ": negative row count");
+    if (in_features <= 0 || in_features > kMaxK)
+      invalid(who + ": in_features must be 1 to 131071, got " + std::to_string(in_features));
+    if (out_features <= 0 || out_features > (1 << 28))
+      invalid(who + ": out_features must be 1 to 2^28, got " + std::to_string(out_features));
+    if (rows > 0) {
+      check_codes(who, "x", x, x_stride, in_features);
+      check_codes(who, "w", w, w_stride, in_features);
+      check_floats(who, "x_scale", x_scale);
+      check_floats(who, "w_scale", w_scale);
+      if (bias) check_floats(who, "bias", bias);
+      if (!out) invalid(who + ": null out");
+      const int es = out_type == MLB_ACT_BF16 ? 2 : 4;
+      if (reinterpret_cast<uintptr_t>(out) % es != 0) invalid(who + ": out is unaligned");
+      if (out_stride < out_features) invalid(who + ": row stride of out is smaller than a row");
+      const auto apart = [&](const char* name, const void* p, wide_int stride, wide_int bytes,
+                             int n) {
+        if (byte_rows_overlap(out, (wide_int)out_stride * es, (wide_int)out_features * es, rows, p,
+                              stride, bytes, n))
+          invalid(who + ": out must not overlap " + name);
+      };
+      apart("x", x, x_stride, in_features, rows);
+      apart("w", w, w_stride, in_features, out_features);
+      apart("x_scale", x_scale, (wide_int)rows * 4, (wide_int)rows * 4, 1);
+      apart("w_scale", w_scale, (wide_int)out_features * 4, (wide_int)out_features * 4, 1);
+      if (bias) apart("bias", bias, (wide_int)out_features * 4, (wide_int)out_features * 4, 1);
+    }
+    DeviceScope scope(device_id);
+    if (rows == 0) return;
+    LinearArgs a = {};
+    a.x_scale = x_scale, a.w_scale = w_scale, a.bias = bias;
+    a.out = out, a.out_stride = out_stride, a.rows = rows, a.n = out_features;
+    run({x, x_stride, w, w_stride, in_features}, a, out_type, device_id,
+        static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int mlb_int8_linear_status(int device_id, int* code, int* where) {
+  return guarded([&] {
+    if (!code || !where) invalid("Int8Linear: null output");
+    DeviceScope scope(device_id);
+    const DeviceStatus s = take_status();
+    *code = s.code;
+    *where = s.where;
+  });
+}
+
+extern "C" int mlb_int8_linear_wait_selftest(int device_id, int rows, double limit_ms, int* code,
+                                             int* where, int* nan_rows) {
+  return guarded([&] {
+    if (!code || !where || !nan_rows) invalid("Int8Linear: null output");
+    if (rows < 1 || rows > 1024) invalid("Int8Linear: rows must be 1 to 1024");
+    if (!(limit_ms > 0.0) || limit_ms > 1000.0)
+      invalid("Int8Linear: limit_ms must be in (0, 1000]");
+    DeviceScope scope(device_id);
+    int khz = 0;
+    MLB_CUDA(cudaDeviceGetAttribute(&khz, cudaDevAttrClockRate, device_id));
+    // zeros times zeros, with scales of zero
+    constexpr int kIn = 2048, kOut = 256;
+    const size_t codes = (size_t)(rows + kOut) * kIn, scales = (size_t)(rows + kOut) * sizeof(float);
+    const size_t results = (size_t)rows * kOut * sizeof(float);
+    const size_t at_scales = codes, at_out = (at_scales + scales + 15) / 16 * 16;
+    DevBuf buf(at_out + results);
+    uint8_t* p = static_cast<uint8_t*>(buf.p);
+    zero_now(p, at_out + results);
+    LinearArgs a = {};
+    a.x_scale = reinterpret_cast<const float*>(p + at_scales);
+    a.w_scale = a.x_scale + rows;
+    a.out = p + at_out;
+    a.out_stride = kOut, a.rows = rows, a.n = kOut;
+    a.wait_cycles = std::max(1LL, (long long)(limit_ms * (double)khz));
+    a.never = 1;
+    const int8_t* x = reinterpret_cast<const int8_t*>(p);
+    run({x, kIn, x + (size_t)rows * kIn, kIn, kIn}, a, MLB_ACT_F32, device_id, nullptr);
+    const DeviceStatus st = take_status();
+    std::vector<float> out((size_t)rows * kOut);
+    MLB_CUDA(cudaMemcpy(out.data(), p + at_out, results, cudaMemcpyDeviceToHost));
+    *nan_rows = 0;
+    for (int r = 0; r < rows; ++r)
+      *nan_rows += std::all_of(out.begin() + (size_t)r * kOut, out.begin() + (size_t)(r + 1) * kOut,
+                               [](float v) { return v != v; });
+    *code = st.code;
+    *where = st.where;
+  });
+}

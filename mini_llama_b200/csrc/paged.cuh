@@ -32,6 +32,7 @@
 #include <utility>
 
 #include "common.cuh"
+#include "rows.cuh"
 
 namespace mlb {
 
@@ -124,26 +125,9 @@ inline void paged_check_rows(const char* who, const char* name, const void* p, l
 // a_row_stride (b_row_stride) apart, at least a row. Rows side by side in one buffer do not.
 inline bool rows_overlap(const void* a, long long a_row_stride, long long a_row, const void* b,
                          long long b_row_stride, long long b_row, int n, int act) {
-  using wide = __int128;  // strides are the caller's
   const int es = act == MLB_ACT_BF16 ? 2 : 4;
-  const wide a_stride = (wide)a_row_stride * es, b_stride = (wide)b_row_stride * es;
-  const wide a_bytes = (wide)a_row * es, b_bytes = (wide)b_row * es;
-  const wide d = (wide)reinterpret_cast<uintptr_t>(b) - (wide)reinterpret_cast<uintptr_t>(a);
-  const auto floor_div = [](wide x, wide y) { return x / y - (x % y < 0 ? 1 : 0); };
-  // rows of b that row i of a meets: those with i a_stride - j b_stride - d in (-a_bytes, b_bytes)
-  const auto meets = [&](wide at, wide j0, wide j1) {
-    const wide lo = floor_div(at - d - b_bytes, b_stride) + 1;
-    const wide hi = floor_div(at - d + a_bytes - 1, b_stride);
-    return (lo > j0 ? lo : j0) <= (hi < j1 ? hi : j1);
-  };
-  if (n <= 0) return false;
-  // of equal strides only the difference of the rows counts
-  if (a_stride == b_stride) return meets(0, -(wide)(n - 1), n - 1);
-  if (d >= (wide)(n - 1) * a_stride + a_bytes || -d >= (wide)(n - 1) * b_stride + b_bytes)
-    return false;
-  for (int i = 0; i < n; ++i)
-    if (meets((wide)i * a_stride, 0, n - 1)) return true;
-  return false;
+  return byte_rows_overlap(a, (wide_int)a_row_stride * es, (wide_int)a_row * es, n, b,
+                           (wide_int)b_row_stride * es, (wide_int)b_row * es, n);
 }
 
 inline void paged_check_act(const char* who, int act) {
