@@ -85,15 +85,6 @@ __device__ __forceinline__ void drain_wait(const LinearArgs& a, uint64_t* bar, u
   }
 }
 
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
-}
-__device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
-  return r;
-}
 __device__ __forceinline__ int peer_int(uint32_t address) {
   int v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
@@ -219,19 +210,18 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (threadIdx.x == 0) sh.abort_flag = !ok;
     cluster_sync_all();
-    for (int r = 0; r < a.split; ++r) ok = ok && peer_int(peer_address(&sh.abort_flag, r)) == 0;
+    for (int r = 0; r < a.split; ++r) ok = ok && peer_int(cluster_address(&sh.abort_flag, r)) == 0;
     for (int t = share; t < tokens; t += a.split) {
       const int* mine = sums + t * kChannels + threadIdx.x;
       int v[kMaxSplit];
 #pragma unroll
       for (int r = 0; r < kMaxSplit; ++r)
-        v[r] = r < a.split ? peer_int(peer_address(mine, r)) : 0;
+        v[r] = r < a.split ? peer_int(cluster_address(mine, r)) : 0;
       int sum = 0;
 #pragma unroll
       for (int r = 0; r < kMaxSplit; ++r) sum += v[r];
       if (inside) finish(sum, t, ok);
     }
-    __syncwarp();
     cluster_sync_all();  // a CTA's shared memory lives until the others have read it
   }
   tc_fence_before();
@@ -239,6 +229,262 @@ __global__ void __launch_bounds__(kThreads)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, COLS);
+  }
+}
+
+// ------------------------------------------------------------ many tokens
+// A pair of CTAs takes 256 tokens by N channels at a time, tokens as the rows of D: each
+// CTA loads its 128 tokens and half of the channels, and the tensor cores of both read
+// both halves. Two accumulators in tensor memory: the products of a tile run while the
+// one before is scaled, turned in shared memory and stored, 128 bytes of a row at once.
+// Pairs take tiles in turn, tokens first in groups of kGroup tiles, so that the pairs at
+// work share few tiles of either matrix in L2.
+//
+// Roles (6 warps): 0 loads, 1 tensor memory and (first CTA) products, 2..5 epilogue.
+
+constexpr int kPairThreads = 192;
+constexpr int kPairTokens = 256;
+constexpr int kGroup = 16;
+constexpr int kMaxPairStages = 6;
+constexpr int kTurnWords = 36;  // a row of 32 words, its 16-byte pieces in unlike banks
+
+struct PairShared {
+  uint64_t full[kMaxPairStages], empty[kMaxPairStages], sum_full[2], sum_empty[2], drain;
+  int abort_flag;
+  uint32_t tmem;
+  alignas(16) float scale[2][256];
+  alignas(16) float bias[2][256];
+};
+
+template <int N>
+struct PairPlan {
+  static constexpr int A = 128 * kTileK, B = N / 2 * kTileK;
+  static constexpr int STAGE = A + B;
+  static constexpr int STAGES = kMaxPairStages;
+  static constexpr int TURN = 32 * kTurnWords * 4;  // per epilogue warp
+  static constexpr int BYTES = STAGES * STAGE + 4 * TURN + 1024;
+};
+
+__device__ __forceinline__ bool wait_pair(PairShared& sh, const LinearArgs& a, uint64_t* bar,
+                                          uint32_t parity, int where) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const long long start = clock64();
+  while (!mbar_try_wait_cluster(bar, parity)) {
+    if (*(volatile int*)&sh.abort_flag) return false;
+    if (clock64() - start > a.wait_cycles) {
+      atomicExch(&g_status.code, MLB_ERR_TIMEOUT);
+      atomicExch(&g_status.where, where);
+      *(volatile int*)&sh.abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+template <int N, class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    int8_linear_pair_kernel(const __grid_constant__ CUtensorMap x_map,
+                            const __grid_constant__ CUtensorMap w_map, const LinearArgs a) {
+  using P = PairPlan<N>;
+  extern __shared__ uint8_t dynamic[];
+  __shared__ PairShared sh;
+  uint8_t* smem = dynamic + (-smem_addr(dynamic) & 1023u);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int token_tiles = (a.rows + kPairTokens - 1) / kPairTokens;
+  const int tiles = token_tiles * a.channel_tiles;
+  const auto place = [&](int tile, int& token0, int& channel0) {
+    const int group = tile / (kGroup * a.channel_tiles);
+    const int in_group = min(kGroup, token_tiles - group * kGroup);
+    const int r = tile - group * kGroup * a.channel_tiles;
+    channel0 = r / in_group * N;
+    token0 = (group * kGroup + r % in_group) * kPairTokens + rank * 128;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < P::STAGES; ++i) {
+      mbar_init(&sh.full[i], 1 + a.never);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.sum_full[i], 1);
+      mbar_init(&sh.sum_empty[i], 8);  // four warps of each CTA
+    }
+    mbar_init(&sh.drain, 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&sh.tmem, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the other CTA's barriers are there
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  int issued = 0;
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int tile = pair; ok && tile < tiles; tile += pairs) {
+        int token0, channel0;
+        place(tile, token0, channel0);
+        for (int k = 0; k < a.tiles_k; ++k, ++issued) {
+          const int s = issued % P::STAGES, turn = issued / P::STAGES;
+          if (turn > 0 && !wait_pair(sh, a, &sh.empty[s], (uint32_t)(turn - 1) & 1u, 1111)) {
+            ok = false;
+            break;
+          }
+          // the first CTA's barrier counts the bytes of both
+          if (rank == 0) mbar_arrive_expect_tx(&sh.full[s], 2 * P::STAGE);
+          const uint32_t bar = cluster_address(&sh.full[s], 0);
+          uint8_t* stage = smem + s * P::STAGE;
+          tma_load_pair(stage, &x_map, k * kTileK, token0, bar);
+          tma_load_pair(stage + P::A, &w_map, k * kTileK, channel0 + rank * (N / 2), bar);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      const uint32_t idesc = idesc_i8(kPairTokens, N);
+      int i = 0, done = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < tiles; tile += pairs, ++done) {
+        const int b = done & 1, turn = done >> 1;
+        if (turn > 0) ok = wait_pair(sh, a, &sh.sum_empty[b], (uint32_t)(turn - 1) & 1u, 1112);
+        if (!ok) break;
+        tc_fence_after();
+        for (int k = 0; k < a.tiles_k; ++k, ++i) {
+          const int s = i % P::STAGES;
+          ok = wait_pair(sh, a, &sh.full[s], (uint32_t)(i / P::STAGES) & 1u, 1113);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t x = smem_desc_sw128(smem_addr(smem + s * P::STAGE));
+          const uint64_t w = smem_desc_sw128(smem_addr(smem + s * P::STAGE + P::A));
+#pragma unroll
+          for (int j = 0; j < kTileK / 32; ++j)
+            tc_mma_i8_pair(tmem + b * N, x + 2 * j, w + 2 * j, idesc, k > 0 || j > 0);
+          tc_commit_pair(&sh.empty[s]);
+        }
+        if (ok) tc_commit_pair(&sh.sum_full[b]);
+      }
+    }
+  } else {
+    const int quarter = warp & 3, thread = threadIdx.x - 64;
+    float* turn_buf = reinterpret_cast<float*>(smem + P::STAGES * P::STAGE) +
+                      quarter * 32 * kTurnWords;
+    constexpr int COLS = 128 / (int)sizeof(T);  // channels of 128 bytes of a row
+    const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 &&
+                      a.out_stride % (16 / (int)sizeof(T)) == 0;
+    bool ok = true;
+    int done = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++done) {
+      int token0, channel0;
+      place(tile, token0, channel0);
+      const int b = done & 1;
+      token0 += quarter * 32;
+      // the tile's scales and biases, while its products run; the warps are at most a
+      // tile apart, so the buffer of the tile before the last is free
+      for (int c = thread; c < N; c += 128) {
+        const bool inside = channel0 + c < a.n;
+        sh.scale[b][c] = inside ? a.w_scale[channel0 + c] : 0.0f;
+        sh.bias[b][c] = inside && a.bias ? a.bias[channel0 + c] : 0.0f;
+      }
+      const float sx = token0 + lane < a.rows ? a.x_scale[token0 + lane] : 0.0f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      ok = __all_sync(0xffffffffu,
+                      ok && wait_pair(sh, a, &sh.sum_full[b], (uint32_t)(done >> 1) & 1u, 1114));
+      tc_fence_after();
+      const uint32_t sums = tmem + b * N + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c0 = 0; c0 < N; c0 += COLS) {
+        if (channel0 + c0 >= a.n) break;
+        float y[32];
+#pragma unroll
+        for (int part = 0; part < COLS / 32; ++part) {
+          uint32_t d[32];
+          if (ok) {
+            tmem_ld32_start(sums + c0 + part * 32, d);
+            tmem_ld32_wait(d);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(&sh.scale[b][c0 + part * 32 + j]);
+            const float4 z = *reinterpret_cast<const float4*>(&sh.bias[b][c0 + part * 32 + j]);
+            const float sv[4] = {s.x, s.y, s.z, s.w}, zv[4] = {z.x, z.y, z.z, z.w};
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[e] = ok ? (float)(int)d[j + e] * sx : nanf("");
+              v[e] = a.bias ? fmaf(v[e], sv[e], zv[e]) : v[e] * sv[e];
+            }
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[j + e] = v[e];
+            } else {
+              y[part * 16 + j / 2] = __uint_as_float(pack_bf16(v[0], v[1]));
+              y[part * 16 + j / 2 + 1] = __uint_as_float(pack_bf16(v[2], v[3]));
+            }
+          }
+        }
+        if (c0 + COLS >= N || channel0 + c0 + COLS >= a.n) {  // the last read of these sums
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(cluster_address(&sh.sum_empty[b], 0));
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(turn_buf + lane * kTurnWords + j) =
+              make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+        __syncwarp();
+        T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel0 + c0;
+        const int rows = min(32, a.rows - token0), cols = min(COLS, a.n - channel0 - c0);
+        if (wide && cols == COLS) {
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 4) {
+            const int r = r0 + lane / 8;
+            const float4 v =
+                *reinterpret_cast<const float4*>(turn_buf + r * kTurnWords + lane % 8 * 4);
+            if (r < rows)
+              *reinterpret_cast<float4*>(out + r * a.out_stride + lane % 8 * (16 / sizeof(T))) = v;
+          }
+        } else {
+          for (int r = 0; r < rows; ++r)
+            for (int c = lane; c < cols; c += 32)
+              out[r * a.out_stride + c] =
+                  reinterpret_cast<const T*>(turn_buf + r * kTurnWords)[c];
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  __syncwarp();
+  __syncthreads();
+  if (*(volatile int*)&sh.abort_flag) {
+    // nothing is in flight when shared and tensor memory go; the second CTA's copies are
+    // counted by the first alone, so it gives them the time that a copy takes at most
+    if (rank == 0 && threadIdx.x == 0)
+      for (int j = max(0, issued - P::STAGES); j < issued; ++j)
+        drain_wait(a, &sh.full[j % P::STAGES], (uint32_t)(j / P::STAGES) & 1u);
+    if (rank == 0 && threadIdx.x == 32) {
+      tc_commit_pair(&sh.drain);
+      drain_wait(a, &sh.drain, 0);
+    }
+    if (rank == 1 && threadIdx.x == 0) {
+      const long long start = clock64();
+      while (clock64() - start < 2000000) {
+      }
+    }
+    __syncthreads();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // neither CTA's memory goes while the other one's products read it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -324,8 +570,25 @@ void launch(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream)
   MLB_CUDA(cudaLaunchKernelEx(&cfg, int8_linear_kernel<NT, T>, w_map, x_map, a));
 }
 
+template <int N, class T>
+void launch_pair(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream) {
+  using P = PairPlan<N>;
+  static_assert(P::BYTES + sizeof(PairShared) <= 227 * 1024);
+  a.tiles_k = (o.k + kTileK - 1) / kTileK;
+  a.channel_tiles = (a.n + N - 1) / N;
+  const long long tiles = (long long)a.channel_tiles * ((a.rows + kPairTokens - 1) / kPairTokens);
+  if (tiles * a.tiles_k > 0x7fffffffLL) invalid("Int8Linear: too many rows");
+  allow_smem(int8_linear_pair_kernel<N, T>, P::BYTES, device_id);
+  const CUtensorMap x_map = tile_map(o.x, o.x_stride, a.rows, o.k, 128);
+  const CUtensorMap w_map = tile_map(o.w, o.w_stride, a.n, o.k, N / 2);
+  const int pairs = (int)std::min<long long>(tiles, sm_count(device_id) / 2);
+  int8_linear_pair_kernel<N, T><<<2 * pairs, kPairThreads, P::BYTES, stream>>>(x_map, w_map, a);
+  MLB_CUDA(cudaGetLastError());
+}
+
 template <class T>
 void dispatch(const Operands& o, const LinearArgs& a, int device_id, cudaStream_t stream) {
+  if (a.rows > 256) return launch_pair<256, T>(o, a, device_id, stream);
   if (a.rows <= 16) return launch<16, T>(o, a, device_id, stream);
   if (a.rows <= 32) return launch<32, T>(o, a, device_id, stream);
   if (a.rows <= 64) return launch<64, T>(o, a, device_id, stream);
