@@ -61,6 +61,9 @@ struct Shared {
   uint64_t full[kMaxStages], empty[kMaxStages], done, drain;
   int abort_flag;
   uint32_t tmem;
+  float x_scale[256];
+  alignas(16) float w_scale[kChannels];
+  alignas(16) float bias[kChannels];
 };
 
 __device__ __forceinline__ bool wait(Shared& sh, const LinearArgs& a, uint64_t* bar,
@@ -87,12 +90,31 @@ __device__ __forceinline__ void drain_wait(const LinearArgs& a, uint64_t* bar, u
 
 __device__ __forceinline__ int peer_int(uint32_t address) {
   int v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address));
+  return v;
+}
+__device__ __forceinline__ int4 peer_int4(uint32_t address) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(address));
   return v;
 }
 
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put4(float* p, const float4& v) {
+  *reinterpret_cast<float4*>(p) = v;
+}
+__device__ __forceinline__ void put4(__nv_bfloat16* p, const float4& v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+// A sum with its scales and bias: three roundings, two without a bias.
+__device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias, bool biased) {
+  const float y = (float)sum * sx;
+  return biased ? fmaf(y, sw, bias) : y * sw;
+}
 
 // Grid: ((token tile * channel tiles) + channel tile) * split + share of K, the shares of
 // a tile being a cluster.
@@ -115,7 +137,10 @@ __global__ void __launch_bounds__(kThreads)
   const int k0 = (int)((long long)a.tiles_k * share / a.split);
   const int count = (int)((long long)a.tiles_k * (share + 1) / a.split) - k0;
 
+  pdl_launch_dependents();
   if (threadIdx.x == 0) {
+    prefetch_map(&w_map);
+    prefetch_map(&x_map);
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(&sh.full[i], 1 + a.never);
       mbar_init(&sh.empty[i], 1);
@@ -133,6 +158,7 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  pdl_wait();  // the kernel before may have made what is read from here on
 
   int issued = 0;
   if (warp == 0 && lane == 0) {
@@ -160,6 +186,17 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   __syncwarp();
+  // what the results are multiplied with, while the products run
+  const int tokens = min(NT, a.rows - token0);
+  const bool biased = a.bias != nullptr;
+  for (int t = threadIdx.x; t < NT; t += kThreads)
+    sh.x_scale[t] = t < tokens ? a.x_scale[token0 + t] : 0.0f;
+  {
+    const int channel = channel0 + threadIdx.x;
+    const bool inside = channel < a.n;
+    sh.w_scale[threadIdx.x] = inside ? a.w_scale[channel] : 0.0f;
+    sh.bias[threadIdx.x] = inside && biased ? a.bias[channel] : 0.0f;
+  }
   bool ok = __syncthreads_and(wait(sh, a, &sh.done, 0, 1103));
   if (!ok) {
     // nothing is in flight when shared and tensor memory go
@@ -174,53 +211,68 @@ __global__ void __launch_bounds__(kThreads)
   }
   tc_fence_after();
 
-  const int tokens = min(NT, a.rows - token0);
-  const int channel = channel0 + threadIdx.x;
-  const bool inside = channel < a.n;
-  const float sw = inside ? a.w_scale[channel] : 0.0f;
-  const float bias = inside && a.bias ? a.bias[channel] : 0.0f;
-  T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel;
-  const auto finish = [&](int sum, int t, bool good) {
-    float y = (float)sum * a.x_scale[token0 + t];
-    y = a.bias ? fmaf(y, sw, bias) : y * sw;
-    put(out + (long long)t * a.out_stride, good ? y : nanf(""));
-  };
+  T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel0;
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   if (a.split == 1) {
+    const int c = threadIdx.x;
+    const bool inside = channel0 + c < a.n;
+    const float sw = ok ? sh.w_scale[c] : nanf(""), bias = sh.bias[c];
 #pragma unroll 1
-    for (int c = 0; c < tokens; c += 8) {
-      uint32_t d[8];
-      tmem_ld8(lanes + c, d);
-      if (inside) {
+    for (int t0 = 0; t0 < tokens; t0 += 16) {
+      uint32_t d[16];
+      tmem_ld16(lanes + t0, d);
+      float y[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < tokens) finish((int)d[i], c + i, ok);
-      }
+      for (int i = 0; i < 16; ++i) y[i] = scaled((int)d[i], sh.x_scale[t0 + i], sw, bias, biased);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (inside && t0 + i < tokens) put(out + (t0 + i) * a.out_stride + c, y[i]);
     }
   } else {
     // every share leaves its sums, tokens apart, over the ring that it no longer needs;
-    // tokens are finished by the shares in turn
+    // four channels of a token are one thread's of the cluster
     int* sums = reinterpret_cast<int*>(smem);
 #pragma unroll 1
-    for (int c = 0; c < tokens; c += 8) {
-      uint32_t d[8];
-      tmem_ld8(lanes + c, d);
+    for (int t0 = 0; t0 < tokens; t0 += 16) {
+      uint32_t d[16];
+      tmem_ld16(lanes + t0, d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sums[(c + i) * kChannels + threadIdx.x] = (int)d[i];
+      for (int i = 0; i < 16; ++i) sums[(t0 + i) * kChannels + threadIdx.x] = (int)d[i];
     }
     if (threadIdx.x == 0) sh.abort_flag = !ok;
     cluster_sync_all();
-    for (int r = 0; r < a.split; ++r) ok = ok && peer_int(cluster_address(&sh.abort_flag, r)) == 0;
-    for (int t = share; t < tokens; t += a.split) {
-      const int* mine = sums + t * kChannels + threadIdx.x;
-      int v[kMaxSplit];
+    const int c = lane * 4;
+    const bool wide = reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0 &&
+                      a.out_stride % 4 == 0 && channel0 + c + 4 <= a.n;
+    const float4 sw = *reinterpret_cast<const float4*>(sh.w_scale + c);
+    const float4 bias = *reinterpret_cast<const float4*>(sh.bias + c);
+    int bad = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxSplit; ++r)
+      bad |= r < a.split ? peer_int(cluster_address(&sh.abort_flag, r)) : 0;
+#pragma unroll 2
+    for (int t = share * 4 + warp; t < tokens; t += a.split * 4) {
+      const int* mine = sums + t * kChannels + c;
+      int4 v[kMaxSplit];
 #pragma unroll
       for (int r = 0; r < kMaxSplit; ++r)
-        v[r] = r < a.split ? peer_int(cluster_address(mine, r)) : 0;
-      int sum = 0;
+        v[r] = r < a.split ? peer_int4(cluster_address(mine, r)) : make_int4(0, 0, 0, 0);
 #pragma unroll
-      for (int r = 0; r < kMaxSplit; ++r) sum += v[r];
-      if (inside) finish(sum, t, ok);
+      for (int r = 1; r < kMaxSplit; ++r)
+        v[0].x += v[r].x, v[0].y += v[r].y, v[0].z += v[r].z, v[0].w += v[r].w;
+      const float sx = bad ? nanf("") : sh.x_scale[t];
+      const float4 y = make_float4(
+          scaled(v[0].x, sx, sw.x, bias.x, biased), scaled(v[0].y, sx, sw.y, bias.y, biased),
+          scaled(v[0].z, sx, sw.z, bias.z, biased), scaled(v[0].w, sx, sw.w, bias.w, biased));
+      T* o = out + t * a.out_stride + c;
+      if (wide) {
+        put4(o, y);
+      } else {
+        const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (channel0 + c + i < a.n) put(o + i, e[i]);
+      }
     }
     cluster_sync_all();  // a CTA's shared memory lives until the others have read it
   }
@@ -236,7 +288,7 @@ __global__ void __launch_bounds__(kThreads)
 // A pair of CTAs takes 256 tokens by N channels at a time, tokens as the rows of D: each
 // CTA loads its 128 tokens and half of the channels, and the tensor cores of both read
 // both halves. Two accumulators in tensor memory: the products of a tile run while the
-// one before is scaled, turned in shared memory and stored, 128 bytes of a row at once.
+// one before is turned in shared memory, scaled and stored, 32 channels of a row at once.
 // Pairs take tiles in turn, tokens first in groups of kGroup tiles, so that the pairs at
 // work share few tiles of either matrix in L2.
 //
@@ -301,7 +353,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     token0 = (group * kGroup + r % in_group) * kPairTokens + rank * 128;
   };
 
+  pdl_launch_dependents();
   if (threadIdx.x == 0) {
+    prefetch_map(&x_map);
+    prefetch_map(&w_map);
     for (int i = 0; i < P::STAGES; ++i) {
       mbar_init(&sh.full[i], 1 + a.never);
       mbar_init(&sh.empty[i], 1);
@@ -323,6 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync_all();  // the other CTA's barriers are there
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  pdl_wait();
 
   int issued = 0;
   if (warp == 0) {
@@ -373,11 +429,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
   } else {
     const int quarter = warp & 3, thread = threadIdx.x - 64;
-    float* turn_buf = reinterpret_cast<float*>(smem + P::STAGES * P::STAGE) +
+    int* turn_buf = reinterpret_cast<int*>(smem + P::STAGES * P::STAGE) +
                       quarter * 32 * kTurnWords;
-    constexpr int COLS = 128 / (int)sizeof(T);  // channels of 128 bytes of a row
-    const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 &&
-                      a.out_stride % (16 / (int)sizeof(T)) == 0;
+    // when sums are turned, a lane has four channels of every fourth row
+    const int c4 = lane % 8 * 4, r4 = lane / 8;
+    const bool wide = reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0 &&
+                      a.out_stride % 4 == 0;
+    const bool biased = a.bias != nullptr;
     bool ok = true;
     int done = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++done) {
@@ -390,71 +448,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int c = thread; c < N; c += 128) {
         const bool inside = channel0 + c < a.n;
         sh.scale[b][c] = inside ? a.w_scale[channel0 + c] : 0.0f;
-        sh.bias[b][c] = inside && a.bias ? a.bias[channel0 + c] : 0.0f;
+        sh.bias[b][c] = inside && biased ? a.bias[channel0 + c] : 0.0f;
       }
-      const float sx = token0 + lane < a.rows ? a.x_scale[token0 + lane] : 0.0f;
+      float sx[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        sx[i] = token0 + 4 * i + r4 < a.rows ? a.x_scale[token0 + 4 * i + r4] : 0.0f;
       asm volatile("bar.sync 1, 128;" ::: "memory");
       ok = __all_sync(0xffffffffu,
                       ok && wait_pair(sh, a, &sh.sum_full[b], (uint32_t)(done >> 1) & 1u, 1114));
       tc_fence_after();
+      if (!ok) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sx[i] = nanf("");
+      }
       const uint32_t sums = tmem + b * N + ((uint32_t)(quarter * 32) << 16);
+      const int columns = min(N, (a.n - channel0 + 31) / 32 * 32);
+      T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel0 + c4;
+      const int rows = a.rows - token0;
+      uint32_t d[32];
+      tmem_ld32_start(sums, d);
 #pragma unroll 1
-      for (int c0 = 0; c0 < N; c0 += COLS) {
-        if (channel0 + c0 >= a.n) break;
-        float y[32];
+      for (int c0 = 0; c0 < columns; c0 += 32) {
+        tmem_ld32_wait(d);
 #pragma unroll
-        for (int part = 0; part < COLS / 32; ++part) {
-          uint32_t d[32];
-          if (ok) {
-            tmem_ld32_start(sums + c0 + part * 32, d);
-            tmem_ld32_wait(d);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(&sh.scale[b][c0 + part * 32 + j]);
-            const float4 z = *reinterpret_cast<const float4*>(&sh.bias[b][c0 + part * 32 + j]);
-            const float sv[4] = {s.x, s.y, s.z, s.w}, zv[4] = {z.x, z.y, z.z, z.w};
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[e] = ok ? (float)(int)d[j + e] * sx : nanf("");
-              v[e] = a.bias ? fmaf(v[e], sv[e], zv[e]) : v[e] * sv[e];
-            }
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[j + e] = v[e];
-            } else {
-              y[part * 16 + j / 2] = __uint_as_float(pack_bf16(v[0], v[1]));
-              y[part * 16 + j / 2 + 1] = __uint_as_float(pack_bf16(v[2], v[3]));
-            }
-          }
-        }
-        if (c0 + COLS >= N || channel0 + c0 + COLS >= a.n) {  // the last read of these sums
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<uint4*>(turn_buf + lane * kTurnWords + j) =
+              make_uint4(d[j], d[j + 1], d[j + 2], d[j + 3]);
+        if (c0 + 32 < columns) {
+          tmem_ld32_start(sums + c0 + 32, d);
+        } else {  // that was the last read of these sums
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(cluster_address(&sh.sum_empty[b], 0));
         }
-#pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(turn_buf + lane * kTurnWords + j) =
-              make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
         __syncwarp();
-        T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel0 + c0;
-        const int rows = min(32, a.rows - token0), cols = min(COLS, a.n - channel0 - c0);
-        if (wide && cols == COLS) {
+        const float4 s = *reinterpret_cast<const float4*>(&sh.scale[b][c0 + c4]);
+        const float4 z = *reinterpret_cast<const float4*>(&sh.bias[b][c0 + c4]);
+        int4 v[8];
 #pragma unroll
-          for (int r0 = 0; r0 < 32; r0 += 4) {
-            const int r = r0 + lane / 8;
-            const float4 v =
-                *reinterpret_cast<const float4*>(turn_buf + r * kTurnWords + lane % 8 * 4);
-            if (r < rows)
-              *reinterpret_cast<float4*>(out + r * a.out_stride + lane % 8 * (16 / sizeof(T))) = v;
+        for (int i = 0; i < 8; ++i)
+          v[i] = *reinterpret_cast<const int4*>(turn_buf + (4 * i + r4) * kTurnWords + c4);
+        float4 y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          y[i] = make_float4(
+              scaled(v[i].x, sx[i], s.x, z.x, biased), scaled(v[i].y, sx[i], s.y, z.y, biased),
+              scaled(v[i].z, sx[i], s.z, z.z, biased), scaled(v[i].w, sx[i], s.w, z.w, biased));
+        const int left = a.n - channel0 - c0 - c4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          T* o = out + (4 * i + r4) * a.out_stride + c0;
+          if (4 * i + r4 >= rows) continue;
+          if (wide && left >= 4) {
+            put4(o, y[i]);
+          } else {
+            const float e[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < left) put(o + j, e[j]);
           }
-        } else {
-          for (int r = 0; r < rows; ++r)
-            for (int c = lane; c < cols; c += 32)
-              out[r * a.out_stride + c] =
-                  reinterpret_cast<const T*>(turn_buf + r * kTurnWords)[c];
         }
         __syncwarp();
       }
@@ -561,12 +614,14 @@ void launch(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream)
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (size_t)bytes;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)a.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  cfg.numAttrs = a.split > 1 ? 2 : 1;
   MLB_CUDA(cudaLaunchKernelEx(&cfg, int8_linear_kernel<NT, T>, w_map, x_map, a));
 }
 
@@ -582,8 +637,8 @@ void launch_pair(const Operands& o, LinearArgs a, int device_id, cudaStream_t st
   const CUtensorMap x_map = tile_map(o.x, o.x_stride, a.rows, o.k, 128);
   const CUtensorMap w_map = tile_map(o.w, o.w_stride, a.n, o.k, N / 2);
   const int pairs = (int)std::min<long long>(tiles, sm_count(device_id) / 2);
-  int8_linear_pair_kernel<N, T><<<2 * pairs, kPairThreads, P::BYTES, stream>>>(x_map, w_map, a);
-  MLB_CUDA(cudaGetLastError());
+  launch_pdl(int8_linear_pair_kernel<N, T>, dim3(2 * pairs), dim3(kPairThreads), P::BYTES, stream,
+             true, x_map, w_map, a);
 }
 
 template <class T>
