@@ -40,6 +40,7 @@ constexpr int kThreads = 128;
 constexpr int kTileK = 128;      // bytes along K of a tile
 constexpr int kChannels = 128;   // channels of a CTA
 constexpr int kMaxStages = 8;
+constexpr int kHalf = 110 * 1024;  // shared memory of a CTA where two share an SM
 constexpr int kMaxSplit = 8;
 constexpr int kMaxK = 131071;
 constexpr long long kWaitCycles = 2000000000LL;  // about 1 s
@@ -58,7 +59,7 @@ struct LinearArgs {
 };
 
 struct Shared {
-  uint64_t full[kMaxStages], empty[kMaxStages], done, drain;
+  uint64_t full[kMaxStages], empty[kMaxStages], done, joined, drain;
   int abort_flag;
   uint32_t tmem;
   float x_scale[256];
@@ -81,24 +82,24 @@ __device__ __forceinline__ bool wait(Shared& sh, const LinearArgs& a, uint64_t* 
   }
   return true;
 }
+// The wait for the other shares' sums.
+__device__ __forceinline__ bool wait_joined(Shared& sh, const LinearArgs& a) {
+  if (mbar_try_wait_cluster(&sh.joined, 0)) return true;
+  const long long start = clock64();
+  while (!mbar_try_wait_cluster(&sh.joined, 0)) {
+    if (clock64() - start > a.wait_cycles) {
+      atomicExch(&g_status.code, MLB_ERR_TIMEOUT);
+      atomicExch(&g_status.where, 1104);
+      return false;
+    }
+  }
+  return true;
+}
 // The last wait for what is in flight, after which there is nothing more to be done.
 __device__ __forceinline__ void drain_wait(const LinearArgs& a, uint64_t* bar, uint32_t parity) {
   const long long start = clock64();
   while (!mbar_try_wait(bar, parity) && clock64() - start < a.wait_cycles) {
   }
-}
-
-__device__ __forceinline__ int peer_int(uint32_t address) {
-  int v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address));
-  return v;
-}
-__device__ __forceinline__ int4 peer_int4(uint32_t address) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(address));
-  return v;
 }
 
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
@@ -136,6 +137,9 @@ __global__ void __launch_bounds__(kThreads)
   // the CTA's tiles along K; a share has one at least
   const int k0 = (int)((long long)a.tiles_k * share / a.split);
   const int count = (int)((long long)a.tiles_k * (share + 1) / a.split) - k0;
+  // groups of four tokens share, share + split .. are joined here
+  const int tokens = min(NT, a.rows - token0);
+  const int owned = ((tokens + 3) / 4 - share + a.split - 1) / a.split;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -146,10 +150,14 @@ __global__ void __launch_bounds__(kThreads)
       mbar_init(&sh.empty[i], 1);
     }
     mbar_init(&sh.done, 1);
+    mbar_init(&sh.joined, 1);
     mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
     fence_mbar_init();
+    // what the shares of this CTA's tokens come to
+    if (a.split > 1) mbar_arrive_expect_tx(&sh.joined, (uint32_t)(owned * a.split) * kChannels * 16);
   }
+  if (a.split > 1) cluster_arrive();
   if (warp == 1) {
     tmem_alloc(&sh.tmem, COLS);
     tmem_relinquish();
@@ -187,7 +195,6 @@ __global__ void __launch_bounds__(kThreads)
   }
   __syncwarp();
   // what the results are multiplied with, while the products run
-  const int tokens = min(NT, a.rows - token0);
   const bool biased = a.bias != nullptr;
   for (int t = threadIdx.x; t < NT; t += kThreads)
     sh.x_scale[t] = t < tokens ? a.x_scale[token0 + t] : 0.0f;
@@ -213,10 +220,11 @@ __global__ void __launch_bounds__(kThreads)
 
   T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel0;
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  const int c = threadIdx.x;
+  const bool inside = channel0 + c < a.n;
+  const float bias = sh.bias[c];
   if (a.split == 1) {
-    const int c = threadIdx.x;
-    const bool inside = channel0 + c < a.n;
-    const float sw = ok ? sh.w_scale[c] : nanf(""), bias = sh.bias[c];
+    const float sw = ok ? sh.w_scale[c] : nanf("");
 #pragma unroll 1
     for (int t0 = 0; t0 < tokens; t0 += 16) {
       uint32_t d[16];
@@ -229,52 +237,46 @@ __global__ void __launch_bounds__(kThreads)
         if (inside && t0 + i < tokens) put(out + (t0 + i) * a.out_stride + c, y[i]);
     }
   } else {
-    // every share leaves its sums, tokens apart, over the ring that it no longer needs;
-    // four channels of a token are one thread's of the cluster
-    int* sums = reinterpret_cast<int*>(smem);
+    // every share's sums go to their tokens' owner, behind its ring, as [group][share]
+    // [channel][token]: a thread has four tokens of a channel, a warp 512 bytes
+    int4* sums = reinterpret_cast<int4*>(smem + a.stages * STAGE);
+    cluster_wait();  // every CTA's barrier is there
+    if (ok) {
 #pragma unroll 1
-    for (int t0 = 0; t0 < tokens; t0 += 16) {
-      uint32_t d[16];
-      tmem_ld16(lanes + t0, d);
+      for (int t0 = 0; t0 < tokens; t0 += 16) {
+        uint32_t d[16];
+        tmem_ld16(lanes + t0, d);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sums[(t0 + i) * kChannels + threadIdx.x] = (int)d[i];
-    }
-    if (threadIdx.x == 0) sh.abort_flag = !ok;
-    cluster_sync_all();
-    const int c = lane * 4;
-    const bool wide = reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0 &&
-                      a.out_stride % 4 == 0 && channel0 + c + 4 <= a.n;
-    const float4 sw = *reinterpret_cast<const float4*>(sh.w_scale + c);
-    const float4 bias = *reinterpret_cast<const float4*>(sh.bias + c);
-    int bad = 0;
-#pragma unroll
-    for (int r = 0; r < kMaxSplit; ++r)
-      bad |= r < a.split ? peer_int(cluster_address(&sh.abort_flag, r)) : 0;
-#pragma unroll 2
-    for (int t = share * 4 + warp; t < tokens; t += a.split * 4) {
-      const int* mine = sums + t * kChannels + c;
-      int4 v[kMaxSplit];
-#pragma unroll
-      for (int r = 0; r < kMaxSplit; ++r)
-        v[r] = r < a.split ? peer_int4(cluster_address(mine, r)) : make_int4(0, 0, 0, 0);
-#pragma unroll
-      for (int r = 1; r < kMaxSplit; ++r)
-        v[0].x += v[r].x, v[0].y += v[r].y, v[0].z += v[r].z, v[0].w += v[r].w;
-      const float sx = bad ? nanf("") : sh.x_scale[t];
-      const float4 y = make_float4(
-          scaled(v[0].x, sx, sw.x, bias.x, biased), scaled(v[0].y, sx, sw.y, bias.y, biased),
-          scaled(v[0].z, sx, sw.z, bias.z, biased), scaled(v[0].w, sx, sw.w, bias.w, biased));
-      T* o = out + t * a.out_stride + c;
-      if (wide) {
-        put4(o, y);
-      } else {
-        const float e[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (channel0 + c + i < a.n) put(o + i, e[i]);
+        for (int i = 0; i < 16; i += 4) {
+          if (t0 + i < tokens) {
+            const int group = (t0 + i) / 4, turn = group / a.split, owner = group - turn * a.split;
+            st_async4(cluster_address(sums + (turn * a.split + share) * kChannels + c, owner), d[i],
+                      d[i + 1], d[i + 2], d[i + 3], cluster_address(&sh.joined, owner));
+          }
+        }
       }
     }
-    cluster_sync_all();  // a CTA's shared memory lives until the others have read it
+    if (owned > 0) ok = __syncthreads_and(ok && wait_joined(sh, a));
+    const float sw = ok ? sh.w_scale[c] : nanf("");
+    for (int g = 0; g < owned; ++g) {
+      const int4* s = sums + g * a.split * kChannels + c;
+      int4 v[kMaxSplit];
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r) v[r] = r < a.split ? s[r * kChannels] : make_int4(0, 0, 0, 0);
+      int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        sum[0] += v[r].x, sum[1] += v[r].y, sum[2] += v[r].z, sum[3] += v[r].w;
+      const int t = (share + g * a.split) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (inside && t + i < tokens)
+          put(out + (t + i) * a.out_stride + c,
+              scaled(sum[i], sh.x_scale[t + i], sw, bias, biased));
+    }
+    // a CTA whose sums have all arrived may go; another one waits for those that might
+    // still be on their way (CTAs that have gone count as there)
+    if (!ok) cluster_sync_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -370,7 +372,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(&sh.tmem, 512);
+    tmem_alloc_pair(&sh.tmem, 2 * N);
     tmem_relinquish_pair();
   }
   tc_fence_before();
@@ -495,18 +497,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           y[i] = make_float4(
               scaled(v[i].x, sx[i], s.x, z.x, biased), scaled(v[i].y, sx[i], s.y, z.y, biased),
               scaled(v[i].z, sx[i], s.z, z.z, biased), scaled(v[i].w, sx[i], s.w, z.w, biased));
-        const int left = a.n - channel0 - c0 - c4;
+        T* o = out + r4 * a.out_stride + c0;
+        if (wide && rows >= 32 && channel0 + c0 + 32 <= a.n) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          T* o = out + (4 * i + r4) * a.out_stride + c0;
-          if (4 * i + r4 >= rows) continue;
-          if (wide && left >= 4) {
-            put4(o, y[i]);
-          } else {
+          for (int i = 0; i < 8; ++i, o += 4 * a.out_stride) put4(o, y[i]);
+        } else {
+          const int left = a.n - channel0 - c0 - c4;
+#pragma unroll
+          for (int i = 0; i < 8; ++i, o += 4 * a.out_stride) {
             const float e[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (j < left) put(o + j, e[j]);
+              if (4 * i + r4 < rows && j < left) put(o + j, e[j]);
           }
         }
         __syncwarp();
@@ -537,7 +539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync_all();  // neither CTA's memory goes while the other one's products read it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 512);
+    tmem_dealloc_pair(tmem, 2 * N);
   }
 }
 
@@ -591,20 +593,22 @@ void launch(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream)
   a.tiles_k = (o.k + kTileK - 1) / kTileK;
   a.channel_tiles = (a.n + kChannels - 1) / kChannels;
   const long long tiles = (long long)a.channel_tiles * ((a.rows + NT - 1) / NT);
-  // shares of K: double while the tiles leave SMs without their two CTAs and a share
+  // shares of K, a power of two (as NT is: groups of tokens divide evenly): double while the tiles leave SMs without their two CTAs and a share
   // keeps at least 4 tiles of K
   a.split = 1;
   while (a.split < kMaxSplit && tiles * a.split * 2 <= 2 * sm_count(device_id) &&
          a.tiles_k / (a.split * 2) >= 4)
     a.split *= 2;
   const int share = (a.tiles_k + a.split - 1) / a.split;
-  // half of an SM's shared memory, for two CTAs
-  constexpr int kMost = std::min(kMaxStages, 110 * 1024 / STAGE);
-  a.stages = std::min(kMost, share);
-  // the ring, or the sums of all tokens
-  const int bytes = std::max(a.stages * STAGE, a.split > 1 ? NT * kChannels * 4 : 0) + 1024;
-  constexpr int kMostBytes = std::max(kMost * STAGE, NT * kChannels * 4) + 1024;
-  static_assert(kMostBytes <= 227 * 1024);
+  // the ring and the sums to be joined, in half of an SM's shared memory, for two CTAs
+  // (where that leaves a ring of two at least)
+  const int joined = a.split > 1 ? std::max(NT / 4, a.split) * kChannels * 16 : 0;
+  const int room = (joined + 2 * STAGE <= kHalf ? kHalf : 2 * kHalf) - joined;
+  a.stages = std::min({kMaxStages, share, room / STAGE});
+  const int bytes = a.stages * STAGE + joined + 1024;
+  constexpr int kMostBytes = 2 * kHalf + 1024;
+  static_assert(NT * kChannels * 4 + STAGE <= 2 * kHalf);
+  static_assert(kMostBytes + sizeof(Shared) <= 227 * 1024);
   allow_smem(int8_linear_kernel<NT, T>, kMostBytes, device_id);
   if (tiles * a.split > 0x7fffffffLL) invalid("Int8Linear: too many rows");
   const CUtensorMap w_map = tile_map(o.w, o.w_stride, a.n, o.k, kChannels);

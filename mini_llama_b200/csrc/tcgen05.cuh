@@ -254,9 +254,20 @@ __device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
   return r;
 }
+// An arrival that orders no memory but what tcgen05 fences order: a release would wait
+// for every store on its way to memory.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                : "memory");
+}
+// Four words into shared memory of the cluster, counted there on a barrier of that CTA.
+__device__ __forceinline__ void st_async4(uint32_t to, uint32_t x, uint32_t y, uint32_t z,
+                                          uint32_t w, uint32_t bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.u32 [%0], {%1, %2, %3, %4}, "
+      "[%5];" ::"r"(to),
+      "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -268,6 +279,14 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "r"(smem_addr(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Every thread of every CTA of the cluster (a warp's lanes together).
 __device__ __forceinline__ void cluster_sync_all() {
