@@ -62,7 +62,7 @@ struct Shared {
   uint64_t full[kMaxStages], empty[kMaxStages], done, joined, drain;
   int abort_flag;
   uint32_t tmem;
-  float x_scale[256];
+  float x_scale[128];
   alignas(16) float w_scale[kChannels];
   alignas(16) float bias[kChannels];
 };
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads)
   extern __shared__ uint8_t dynamic[];
   __shared__ Shared sh;
   uint8_t* smem = dynamic + (-smem_addr(dynamic) & 1023u);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5;
   const int share = blockIdx.x % a.split, tile = blockIdx.x / a.split;
   const int token_tile = tile / a.channel_tiles;
   const int channel0 = (tile - token_tile * a.channel_tiles) * kChannels;
@@ -168,29 +168,43 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t tmem = sh.tmem;
   pdl_wait();  // the kernel before may have made what is read from here on
 
+  // Loads and products are a whole warp's loops of uniform values, of which one lane
+  // issues: as one lane's loops they took 600 cycles a tile of K, more than its copies.
   int issued = 0;
-  if (warp == 0 && lane == 0) {
-    for (; issued < count; ++issued) {
-      const int s = issued % a.stages, turn = issued / a.stages;
-      if (turn > 0 && !wait(sh, a, &sh.empty[s], (uint32_t)(turn - 1) & 1u, 1101)) break;
-      uint8_t* stage = smem + s * STAGE;
-      mbar_arrive_expect_tx(&sh.full[s], STAGE);
-      tma_load(stage, &w_map, (k0 + issued) * kTileK, channel0, &sh.full[s]);
-      tma_load(stage + W_BYTES, &x_map, (k0 + issued) * kTileK, token0, &sh.full[s]);
+  if (warp == 0) {
+    int s = 0, x = k0 * kTileK;
+    uint32_t phase = 1;  // the first turn waits for nothing
+    for (; issued < count; ++issued, x += kTileK) {
+      if (issued >= a.stages &&
+          !__all_sync(0xffffffffu, wait(sh, a, &sh.empty[s], phase, 1101)))
+        break;
+      if (elect_one()) {
+        uint8_t* stage = smem + s * STAGE;
+        mbar_arrive_expect_tx(&sh.full[s], STAGE);
+        tma_load(stage, &w_map, x, channel0, &sh.full[s]);
+        tma_load(stage + W_BYTES, &x_map, x, token0, &sh.full[s]);
+      }
+      __syncwarp();
+      if (++s == a.stages) s = 0, phase ^= 1u;
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     const uint32_t idesc = idesc_i8(kChannels, NT);
+    const uint64_t ring = smem_desc_sw128(smem_addr(smem));
+    int s = 0;
+    uint32_t phase = 0;
     for (int i = 0; i < count; ++i) {
-      const int s = i % a.stages, turn = i / a.stages;
-      if (!wait(sh, a, &sh.full[s], (uint32_t)turn & 1u, 1102)) break;
+      if (!__all_sync(0xffffffffu, wait(sh, a, &sh.full[s], phase, 1102))) break;
       tc_fence_after();
-      const uint64_t w = smem_desc_sw128(smem_addr(smem + s * STAGE));
-      const uint64_t x = smem_desc_sw128(smem_addr(smem + s * STAGE + W_BYTES));
+      const uint64_t w = ring + (uint32_t)(s * STAGE >> 4), x = w + (W_BYTES >> 4);
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < kTileK / 32; ++k)
-        tc_mma_i8(tmem, w + 2 * k, x + 2 * k, idesc, i > 0 || k > 0);
-      tc_commit(&sh.empty[s]);
-      if (i == count - 1) tc_commit(&sh.done);
+        for (int k = 0; k < kTileK / 32; ++k)
+          tc_mma_i8(tmem, w + 2 * k, x + 2 * k, idesc, i > 0 || k > 0);
+        tc_commit(&sh.empty[s]);
+        if (i == count - 1) tc_commit(&sh.done);
+      }
+      __syncwarp();
+      if (++s == a.stages) s = 0, phase ^= 1u;
     }
   }
   __syncwarp();
@@ -210,7 +224,7 @@ __global__ void __launch_bounds__(kThreads)
     if (threadIdx.x == 0)
       for (int j = max(0, issued - a.stages); j < issued; ++j)
         drain_wait(a, &sh.full[j % a.stages], (uint32_t)(j / a.stages) & 1u);
-    if (warp == 1 && lane == 0) {
+    if (warp == 1 && elect_one()) {
       tc_commit(&sh.drain);
       drain_wait(a, &sh.drain, 0);
     }
@@ -299,7 +313,7 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kPairThreads = 192;
 constexpr int kPairTokens = 256;
 constexpr int kGroup = 16;
-constexpr int kMaxPairStages = 6;
+constexpr int kMaxPairStages = 10;
 constexpr int kTurnWords = 36;  // a row of 32 words, its 16-byte pieces in unlike banks
 
 struct PairShared {
@@ -314,8 +328,10 @@ template <int N>
 struct PairPlan {
   static constexpr int A = 128 * kTileK, B = N / 2 * kTileK;
   static constexpr int STAGE = A + B;
-  static constexpr int STAGES = kMaxPairStages;
   static constexpr int TURN = 32 * kTurnWords * 4;  // per epilogue warp
+  // as many as there is room for: a tile of K is about 1.5 us on its way
+  static constexpr int STAGES = std::min<int>(
+      kMaxPairStages, (227 * 1024 - (int)sizeof(PairShared) - 1024 - 4 * TURN) / STAGE);
   static constexpr int BYTES = STAGES * STAGE + 4 * TURN + 1024;
 };
 
@@ -384,49 +400,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   int issued = 0;
   if (warp == 0) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int tile = pair; ok && tile < tiles; tile += pairs) {
-        int token0, channel0;
-        place(tile, token0, channel0);
-        for (int k = 0; k < a.tiles_k; ++k, ++issued) {
-          const int s = issued % P::STAGES, turn = issued / P::STAGES;
-          if (turn > 0 && !wait_pair(sh, a, &sh.empty[s], (uint32_t)(turn - 1) & 1u, 1111)) {
-            ok = false;
-            break;
-          }
-          // the first CTA's barrier counts the bytes of both
-          if (rank == 0) mbar_arrive_expect_tx(&sh.full[s], 2 * P::STAGE);
-          const uint32_t bar = cluster_address(&sh.full[s], 0);
-          uint8_t* stage = smem + s * P::STAGE;
-          tma_load_pair(stage, &x_map, k * kTileK, token0, bar);
-          tma_load_pair(stage + P::A, &w_map, k * kTileK, channel0 + rank * (N / 2), bar);
+    int s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    // the first CTA's barriers count the bytes of both
+    const uint32_t full = cluster_address(&sh.full[0], 0);
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      int token0, channel0;
+      place(tile, token0, channel0);
+      channel0 += rank * (N / 2);
+      for (int k = 0; k < a.tiles_k; ++k, ++issued) {
+        if (issued >= P::STAGES) {
+          ok = __all_sync(0xffffffffu, wait_pair(sh, a, &sh.empty[s], phase, 1111));
+          if (!ok) break;
         }
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(&sh.full[s], 2 * P::STAGE);
+          uint8_t* stage = smem + s * P::STAGE;
+          tma_load_pair(stage, &x_map, k * kTileK, token0, full + s * 8);
+          tma_load_pair(stage + P::A, &w_map, k * kTileK, channel0, full + s * 8);
+        }
+        __syncwarp();
+        if (++s == P::STAGES) s = 0, phase ^= 1u;
       }
     }
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
       const uint32_t idesc = idesc_i8(kPairTokens, N);
-      int i = 0, done = 0;
+      const uint64_t ring = smem_desc_sw128(smem_addr(smem));
+      int s = 0, done = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < tiles; tile += pairs, ++done) {
         const int b = done & 1, turn = done >> 1;
         if (turn > 0) ok = wait_pair(sh, a, &sh.sum_empty[b], (uint32_t)(turn - 1) & 1u, 1112);
-        if (!ok) break;
+        if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        for (int k = 0; k < a.tiles_k; ++k, ++i) {
-          const int s = i % P::STAGES;
-          ok = wait_pair(sh, a, &sh.full[s], (uint32_t)(i / P::STAGES) & 1u, 1113);
+        for (int k = 0; k < a.tiles_k; ++k) {
+          ok = __all_sync(0xffffffffu, wait_pair(sh, a, &sh.full[s], phase, 1113));
           if (!ok) break;
           tc_fence_after();
-          const uint64_t x = smem_desc_sw128(smem_addr(smem + s * P::STAGE));
-          const uint64_t w = smem_desc_sw128(smem_addr(smem + s * P::STAGE + P::A));
+          const uint64_t x = ring + (uint32_t)(s * P::STAGE >> 4), w = x + (P::A >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kTileK / 32; ++j)
-            tc_mma_i8_pair(tmem + b * N, x + 2 * j, w + 2 * j, idesc, k > 0 || j > 0);
-          tc_commit_pair(&sh.empty[s]);
+            for (int j = 0; j < kTileK / 32; ++j)
+              tc_mma_i8_pair(tmem + b * N, x + 2 * j, w + 2 * j, idesc, k > 0 || j > 0);
+            tc_commit_pair(&sh.empty[s]);
+          }
+          __syncwarp();
+          if (++s == P::STAGES) s = 0, phase ^= 1u;
         }
-        if (ok) tc_commit_pair(&sh.sum_full[b]);
+        if (ok && elect_one()) tc_commit_pair(&sh.sum_full[b]);
+        __syncwarp();
       }
     }
   } else {
@@ -524,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (rank == 0 && threadIdx.x == 0)
       for (int j = max(0, issued - P::STAGES); j < issued; ++j)
         drain_wait(a, &sh.full[j % P::STAGES], (uint32_t)(j / P::STAGES) & 1u);
-    if (rank == 0 && threadIdx.x == 32) {
+    if (rank == 0 && warp == 1 && elect_one()) {
       tc_commit_pair(&sh.drain);
       drain_wait(a, &sh.drain, 0);
     }
@@ -587,28 +612,40 @@ struct Operands {
   int k;
 };
 
+// How few tokens (tiles of nt) share K: in a power of two of CTAs (as nt is: groups of
+// tokens divide evenly), doubled while the tiles leave room on the SMs and a share keeps
+// at least 8 tiles of K (4096 x 4096, one token, 32 tiles: 6.0 us with 4 shares of 8, 6.8
+// with 8 of 4, 7.4 with 2 of 16). Two CTAs fit on an SM while the sums to be joined leave
+// each a ring of two.
+struct FewPlan {
+  int split, stages, bytes;
+};
+FewPlan few_plan(int nt, long long tiles, int tiles_k, int sms) {
+  const int stage = (kChannels + nt) * kTileK;
+  FewPlan p = {1, 0, 0};
+  const auto joined = [&](int split) {
+    return split > 1 ? std::max(nt / 4, split) * kChannels * 16 : 0;
+  };
+  const auto two = [&](int split) { return joined(split) + 2 * stage <= kHalf; };
+  while (p.split < kMaxSplit && tiles * p.split * 2 <= (two(p.split * 2) ? 2 : 1) * sms &&
+         tiles_k / (p.split * 2) >= 8)
+    p.split *= 2;
+  const int room = (two(p.split) ? 1 : 2) * kHalf - joined(p.split);
+  p.stages = std::min({kMaxStages, (tiles_k + p.split - 1) / p.split, room / stage});
+  p.bytes = p.stages * stage + joined(p.split) + 1024;
+  return p;
+}
+
 template <int NT, class T>
-void launch(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream) {
-  constexpr int STAGE = (kChannels + NT) * kTileK;
-  a.tiles_k = (o.k + kTileK - 1) / kTileK;
+void launch_few(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream) {
+  constexpr int kMostBytes = 2 * kHalf + 1024;
+  static_assert(NT * kChannels * 4 + (kChannels + NT) * kTileK <= 2 * kHalf);
+  static_assert(kMostBytes + sizeof(Shared) <= 227 * 1024);
   a.channel_tiles = (a.n + kChannels - 1) / kChannels;
   const long long tiles = (long long)a.channel_tiles * ((a.rows + NT - 1) / NT);
-  // shares of K, a power of two (as NT is: groups of tokens divide evenly): double while the tiles leave SMs without their two CTAs and a share
-  // keeps at least 4 tiles of K
-  a.split = 1;
-  while (a.split < kMaxSplit && tiles * a.split * 2 <= 2 * sm_count(device_id) &&
-         a.tiles_k / (a.split * 2) >= 4)
-    a.split *= 2;
-  const int share = (a.tiles_k + a.split - 1) / a.split;
-  // the ring and the sums to be joined, in half of an SM's shared memory, for two CTAs
-  // (where that leaves a ring of two at least)
-  const int joined = a.split > 1 ? std::max(NT / 4, a.split) * kChannels * 16 : 0;
-  const int room = (joined + 2 * STAGE <= kHalf ? kHalf : 2 * kHalf) - joined;
-  a.stages = std::min({kMaxStages, share, room / STAGE});
-  const int bytes = a.stages * STAGE + joined + 1024;
-  constexpr int kMostBytes = 2 * kHalf + 1024;
-  static_assert(NT * kChannels * 4 + STAGE <= 2 * kHalf);
-  static_assert(kMostBytes + sizeof(Shared) <= 227 * 1024);
+  const FewPlan p = few_plan(NT, tiles, a.tiles_k, sm_count(device_id));
+  a.split = p.split;
+  a.stages = p.stages;
   allow_smem(int8_linear_kernel<NT, T>, kMostBytes, device_id);
   if (tiles * a.split > 0x7fffffffLL) invalid("Int8Linear: too many rows");
   const CUtensorMap w_map = tile_map(o.w, o.w_stride, a.n, o.k, kChannels);
@@ -616,7 +653,7 @@ void launch(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * a.split));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)bytes;
+  cfg.dynamicSmemBytes = (size_t)p.bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -633,10 +670,9 @@ template <int N, class T>
 void launch_pair(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream) {
   using P = PairPlan<N>;
   static_assert(P::BYTES + sizeof(PairShared) <= 227 * 1024);
-  a.tiles_k = (o.k + kTileK - 1) / kTileK;
   a.channel_tiles = (a.n + N - 1) / N;
   const long long tiles = (long long)a.channel_tiles * ((a.rows + kPairTokens - 1) / kPairTokens);
-  if (tiles * a.tiles_k > 0x7fffffffLL) invalid("Int8Linear: too many rows");
+  if (tiles > 0x7fffffffLL / 2) invalid("Int8Linear: too many rows");
   allow_smem(int8_linear_pair_kernel<N, T>, P::BYTES, device_id);
   const CUtensorMap x_map = tile_map(o.x, o.x_stride, a.rows, o.k, 128);
   const CUtensorMap w_map = tile_map(o.w, o.w_stride, a.n, o.k, N / 2);
@@ -645,14 +681,40 @@ void launch_pair(const Operands& o, LinearArgs a, int device_id, cudaStream_t st
              true, x_map, w_map, a);
 }
 
+// Time of a pair kernel in us: turns of all pairs, each as long as the products of a tile
+// of N channels or the storing of the one before, and the ends. Fitted to, in us (N 64,
+// 128, 256): 256 tokens of 14336 x 4096 25.2, 26.0, 37.3; 512 of 4096 x 4096 16.4, 11.2,
+// 14.8; 1024 28.7, 17.7, 15.6; 4096 of 288 x 1536 9.9, 8.6, 9.3; of 4096 x 28672 613, 369,
+// 278.
+double pair_time(int n, const LinearArgs& a, int sms) {
+  const double k = n == 256 ? 0.28 : 0.19, store = 0.01 * n, ends = n == 256 ? 5.5 : 2.6 + 0.006 * n;
+  const long long tiles = (long long)((a.n + n - 1) / n) * ((a.rows + kPairTokens - 1) / kPairTokens);
+  const long long turns = (tiles + sms / 2 - 1) / (sms / 2);
+  return (double)turns * std::max(k * a.tiles_k, store) + ends;
+}
+// Of the other one, for tiles of 128 tokens: 96 tokens of 14336 x 4096 17.5; 65 of 4096 x
+// 4096 9.2, 128 11.7; 128 of 8192 x 10240 33.
+double few_time(const LinearArgs& a, int sms) {
+  const long long tiles = (a.n + kChannels - 1) / kChannels;
+  const FewPlan p = few_plan(128, tiles, a.tiles_k, sms);
+  const long long turns = (tiles * p.split + sms - 1) / sms;
+  return (double)turns * 0.36 * a.tiles_k / p.split + 4.0 + 0.035 * a.rows;
+}
+
 template <class T>
-void dispatch(const Operands& o, const LinearArgs& a, int device_id, cudaStream_t stream) {
-  if (a.rows > 256) return launch_pair<256, T>(o, a, device_id, stream);
-  if (a.rows <= 16) return launch<16, T>(o, a, device_id, stream);
-  if (a.rows <= 32) return launch<32, T>(o, a, device_id, stream);
-  if (a.rows <= 64) return launch<64, T>(o, a, device_id, stream);
-  if (a.rows <= 128) return launch<128, T>(o, a, device_id, stream);
-  return launch<256, T>(o, a, device_id, stream);
+void dispatch(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream) {
+  a.tiles_k = (o.k + kTileK - 1) / kTileK;
+  if (a.rows <= 16) return launch_few<16, T>(o, a, device_id, stream);
+  if (a.rows <= 32) return launch_few<32, T>(o, a, device_id, stream);
+  if (a.rows <= 64) return launch_few<64, T>(o, a, device_id, stream);
+  const int sms = sm_count(device_id);
+  const double t64 = pair_time(64, a, sms), t128 = pair_time(128, a, sms),
+               t256 = pair_time(256, a, sms);
+  if (a.rows <= 128 && few_time(a, sms) < std::min({t64, t128, t256}))
+    return launch_few<128, T>(o, a, device_id, stream);
+  if (t256 <= std::min(t64, t128)) return launch_pair<256, T>(o, a, device_id, stream);
+  if (t128 <= t64) return launch_pair<128, T>(o, a, device_id, stream);
+  return launch_pair<64, T>(o, a, device_id, stream);
 }
 
 void run(const Operands& o, LinearArgs a, int out_type, int device_id, cudaStream_t stream) {
@@ -700,6 +762,7 @@ extern "C" int mlb_int8_linear(const int8_t* x, long long x_stride, const float*
     const std::string who = "Int8Linear";
     paged_check_act("Int8Linear", out_type);
     if (rows < 0) invalid(who + ": negative row count");
+    if (rows > (1 << 30)) invalid(who + ": too many rows");
     if (in_features <= 0 || in_features > kMaxK)
       invalid(who + ": in_features must be 1 to 131071, got " + std::to_string(in_features));
     if (out_features <= 0 || out_features > (1 << 28))

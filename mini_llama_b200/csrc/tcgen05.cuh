@@ -165,6 +165,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
 }
 
+// One lane of a converged warp. What it alone issues between uniform values (barriers,
+// descriptors) stays in uniform registers, where tcgen05 instructions take them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ------------------------------------------------------- int8 operands, TMA tiles
 
 // Descriptor of a K-major operand in rows of 128 bytes with the 128-byte swizzle, as a
