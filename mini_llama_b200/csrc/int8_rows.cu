@@ -11,11 +11,12 @@
 //
 // Codes are those of 64-bit arithmetic. Computed in fp32 (v = t 127 / A), a value next
 // to a code's border could fall on either side of it, so the fp32 result is taken only
-// where it is further from the border than its error bound, and the few others (about
-// 2 in 10^5 after a norm) are computed again in 64 bits, from the inputs. That
-// needs A in 64 bits too: the threads that hold a value within the bound of the fp32
-// maximum compute theirs again. Rows whose fp32 sums or maxima leave the range where
-// those bounds hold (below 1e-30, not finite) are done in 64 bits throughout.
+// where it is further from the border than its error bound, and the few others (5 in
+// 10^5 after a norm, 4 in 10^4 of SiLU) are done again in 64 bits, from the inputs. Those
+// need A in 64 bits: the threads that hold a value within the bound of the fp32 maximum
+// compute theirs again, while the others go on, and a second barrier later the doubtful
+// codes are corrected. Rows whose fp32 sums or maxima leave the range where the bounds
+// hold (below 1e-30, not finite, gates below -87) are done in 64 bits throughout.
 //
 // A row with a NaN or an infinity among its values, or a scale past fp32's largest
 // number, gets the scale NaN: every product of it is NaN, whatever its codes.
@@ -53,12 +54,15 @@ struct RowsArgs {
 
 constexpr int kHeld = 32;  // values that a thread holds at most
 constexpr float kSmallest = 1e-30f;
-// Relative error bounds of v. After a norm: t, the maximum (rounded from 64 bits), 127
-// over it and the product of both are off by 2^-24 each, 2^-22 together. SiLU: expf and
-// the quotient are off by 2 ulp (2^-22) each, the sum and the product of t by 2^-24, and
-// what comes after t by 3 2^-24: 1.63 2^-21 together.
+constexpr float kLowestGate = -87.0f;  // e^87 is a normal number, and so is its reciprocal
+// Relative error bounds, in units of 2^-24. t: after a norm one product; SiLU: ex2 4 (2
+// ulp), the factor that corrects it, the sum and two products 1 each, the reciprocal 2: 10
+// together. v: t's, the maximum's (the same), its reciprocal times 127; the last product is
+// exact in a fused multiply-add. Kept: a little more, v's times 127 from a code's border.
 template <Kind K>
-constexpr float kBound = K == kSilu ? 0x1p-20f : 0x1p-21f;
+constexpr float kValueBound = (K == kSilu ? 12.0f : 2.0f) * 0x1p-24f;
+template <Kind K>
+constexpr float kBorder = 0.5f - 127.0f * 0x1p-24f * (K == kSilu ? 24.0f : K == kPlain ? 2.0f : 4.0f);
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -117,9 +121,15 @@ __device__ __forceinline__ float max_abs(float x, float y) {
   return r;
 }
 
-// SiLU(g) * u.
+// SiLU(g) * u. e^-g = 2^(hi + lo), -g log2(e) in two parts; 2^lo as 1 + lo ln 2.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  return __fdividef(g, 1.0f + expf(-g)) * u;
+  const float hi = g * -1.4426950408889634f;
+  // what hi's rounding and the constant's (1.92596e-8 beyond fp32) leave, times ln 2
+  const float lo = fmaf(g, -1.4426950408889634f, -hi) * 0.6931471805599453f + g * -1.33497e-8f;
+  float e = ex2(hi), r;
+  e = fmaf(e, lo, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
 }
 __device__ __noinline__ double silu_mul64(float g, float u) {
   return (double)g / (1.0 + exp(-(double)g)) * (double)u;
@@ -208,8 +218,8 @@ __device__ __noinline__ void row64(const RowsArgs& a, long long row, Shared& sh)
 // One CTA per row; thread j has elements (v blockDim + j) E + 0 .. E - 1. NV > 0: v < NV
 // covers the row and values stay in registers; NV = 0: rows of any length, computed
 // twice. ALIGNED: rows start at 16-byte boundaries.
-template <Kind K, class T, int NV, bool ALIGNED, int THREADS>
-__global__ void __launch_bounds__(THREADS) int8_rows_kernel(const RowsArgs a) {
+template <Kind K, class T, int NV, bool ALIGNED>
+__global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
   constexpr int E = 16 / (int)sizeof(T);
   constexpr bool NORM = K == kNorm || K == kNormAdd;
   __shared__ Shared sh;
@@ -219,60 +229,65 @@ __global__ void __launch_bounds__(THREADS) int8_rows_kernel(const RowsArgs a) {
   const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
   const int step = (int)blockDim.x * E;
   const int nv = NV > 0 ? NV : (a.n + step - 1) / step;
+  pdl_launch_dependents();
+  pdl_wait();
 
-  // E values of the row in fp32, their squares' sum added to ss
-  const auto values = [&](int base, float (&t)[E], float& ss, bool first) {
+  // E values of the row in fp32, their squares added to ss; low: the lowest gate
+  const auto values = [&](int base, float2 (&t)[E / 2], float2& ss, float& low, bool first) {
     const int left = a.n - base;
     if (left <= 0) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) t[i] = 0.0f;
+      for (int i = 0; i < E / 2; ++i) t[i] = make_float2(0.0f, 0.0f);
       return;
     }
-    if constexpr (K == kNormAdd) {
-      T* sum = static_cast<T*>(a.sum) + row * a.sum_stride;
-      if (!first) {
-        load_elements<ALIGNED>(sum + base, left, t);
-      } else {
-        float r[E];
-        load_elements<ALIGNED>(x + base, left, t);
-        load_elements<ALIGNED>(y + base, left, r);
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          t[i] += r[i];
-          if constexpr (sizeof(T) == 2) t[i] = to_float(__float2bfloat16_rn(t[i]));
-        }
-        store_elements<ALIGNED>(sum + base, left, t);
-      }
+    float v[E], o[E];
+    if (K == kNormAdd && !first) {
+      load_elements<ALIGNED>(static_cast<const T*>(a.sum) + row * a.sum_stride + base, left, v);
     } else {
-      load_elements<ALIGNED>(x + base, left, t);
+      load_elements<ALIGNED>(x + base, left, v);
+      if constexpr (K == kNormAdd || K == kSilu) load_elements<ALIGNED>(y + base, left, o);
     }
-    if constexpr (NORM) {
-      float w[E];
-      load_elements<true>(a.w + base, left, w);
+    if (K == kNormAdd && first) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        ss = fmaf(t[i], t[i], ss);
-        t[i] *= w[i];
+      for (int i = 0; i < E; i += 2) {
+        const float2 s = add2(make_float2(v[i], v[i + 1]), make_float2(o[i], o[i + 1]));
+        v[i] = s.x, v[i + 1] = s.y;
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t w = pack_bf16(s.x, s.y);
+          v[i] = __uint_as_float(w << 16), v[i + 1] = __uint_as_float(w & 0xffff0000u);
+        }
       }
+      store_elements<ALIGNED>(static_cast<T*>(a.sum) + row * a.sum_stride + base, left, v);
     }
-    if constexpr (K == kSilu) {
-      float u[E];
-      load_elements<ALIGNED>(y + base, left, u);
+    if constexpr (NORM) load_elements<true>(a.w + base, left, o);
 #pragma unroll
-      for (int i = 0; i < E; ++i) t[i] = silu_mul(t[i], u[i]);
+    for (int i = 0; i < E; i += 2) {
+      const float2 p = make_float2(v[i], v[i + 1]);
+      if constexpr (NORM) {
+        ss = fma2(p, p, ss);
+        t[i / 2] = mul2(p, make_float2(o[i], o[i + 1]));
+      } else if constexpr (K == kSilu) {
+        low = fminf(low, fminf(p.x, p.y));
+        t[i / 2] = make_float2(silu_mul(p.x, o[i]), silu_mul(p.y, o[i + 1]));
+      } else {
+        t[i / 2] = p;
+      }
     }
   };
 
-  float held[NV > 0 ? NV : 1][E];
-  float ss = 0.0f, top = 0.0f;
+  float2 held[NV > 0 ? NV : 1][E / 2];
+  float2 ss2 = make_float2(0.0f, 0.0f);
+  float top = 0.0f, low = 0.0f;
 #pragma unroll
   for (int v = 0; v < nv; ++v) {
-    float(&t)[E] = held[NV > 0 ? v : 0];
-    values((v * (int)blockDim.x + (int)threadIdx.x) * E, t, ss, true);
+    float2(&t)[E / 2] = held[NV > 0 ? v : 0];
+    values((v * (int)blockDim.x + (int)threadIdx.x) * E, t, ss2, low, true);
 #pragma unroll
-    for (int i = 0; i < E; ++i) top = max_abs(top, t[i]);
+    for (int i = 0; i < E / 2; ++i) top = max_abs(max_abs(top, t[i].x), t[i].y);
   }
+  if (K == kSilu && low < kLowestGate) top = nanf("");
   const float mine = top;
+  float ss = ss2.x + ss2.y;
   top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
   if (NORM) ss = warp_sum(ss);
   if (lane == 0) sh.part[warp] = make_float2(ss, top);
@@ -299,52 +314,51 @@ __global__ void __launch_bounds__(THREADS) int8_rows_kernel(const RowsArgs a) {
   }
 
   // the maximum in 64 bits: of the values that may be it
-  double top64 = (double)top;
-  if (K != kPlain) {
-    const float near = top * (1.0f - 2.0f * kBound<K>);
-    if (mine >= near) {
+  const float near = top * (1.0f - 2.0f * kValueBound<K>);
+  const auto candidate = [&](int i) {
+    const double t = fabs(value64<K, T>(a, row, i));
+    atomicMax(&sh.top, (unsigned long long)__double_as_longlong(t));
+  };
+  if (K != kPlain && mine >= near) {
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (fabsf(i & 1 ? held[v][i / 2].y : held[v][i / 2].x) >= near)
+            candidate((v * (int)blockDim.x + (int)threadIdx.x) * E + i);
+    } else {
       for (int v = 0; v < nv; ++v) {
         const int base = (v * (int)blockDim.x + (int)threadIdx.x) * E;
-        for (int i = base; i < min(base + E, a.n); ++i) {
-          const double t = fabs(value64<K, T>(a, row, i));
-          if (t >= (double)near)
-            atomicMax(&sh.top, (unsigned long long)__double_as_longlong(t));
-        }
+        for (int i = base; i < min(base + E, a.n); ++i)
+          if (fabs(value64<K, T>(a, row, i)) >= (double)near) candidate(i);
       }
     }
-    __syncthreads();
-    top64 = __longlong_as_double((long long)sh.top);
   }
+  const auto top64 = [&] {
+    return K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
+  };
+  if (NV == 0) __syncthreads();
 
-  const float inv = __fdiv_rn(127.0f, (float)top64);
+  const float inv = __fdiv_rn(127.0f, top);
+  const float2 inv2 = make_float2(inv, inv);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23
   int8_t* codes = a.codes + row * a.codes_stride;
+  uint32_t doubtful = 0;  // bit v E + i
 #pragma unroll
   for (int v = 0; v < nv; ++v) {
     const int base = (v * (int)blockDim.x + (int)threadIdx.x) * E;
-    float(&t)[E] = held[NV > 0 ? v : 0];
-    if (NV == 0) {
-      float unused = 0.0f;
-      values(base, t, unused, false);
-    }
+    float2(&t)[E / 2] = held[NV > 0 ? v : 0];
+    if (NV == 0) values(base, t, ss2, low, false);
     uint32_t c[E];
+    float2 d[E / 2];
     float worst = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float q = t[i] * inv;
-      const float r = q + 12582912.0f;  // 1.5 * 2^23: the nearest whole number in the low bits
-      const float d = q - (r - 12582912.0f);
-      c[i] = __float_as_uint(r);
-      worst = fmaxf(worst, fmaf(fabsf(q), kBound<K>, fabsf(d)));
-    }
-    if (worst > 0.5f) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const float q = t[i] * inv;
-        const float d = q - (__uint_as_float(c[i]) - 12582912.0f);
-        if (fmaf(fabsf(q), kBound<K>, fabsf(d)) > 0.5f && base + i < a.n)
-          c[i] = (uint32_t)code64(K == kPlain ? (double)t[i] : value64<K, T>(a, row, base + i),
-                                  top64);
-      }
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 r = fma2(t[i], inv2, magic);  // the nearest whole number in the low bits
+      d[i] = fma2(t[i], inv2, fma2(r, make_float2(-1.0f, -1.0f), magic));
+      c[2 * i] = __float_as_uint(r.x), c[2 * i + 1] = __float_as_uint(r.y);
+      worst = fmaxf(worst, fmaxf(fabsf(d[i].x), fabsf(d[i].y)));
     }
     uint32_t words[E / 4];
 #pragma unroll
@@ -361,9 +375,26 @@ __global__ void __launch_bounds__(THREADS) int8_rows_kernel(const RowsArgs a) {
       for (int i = 0; i < E; ++i)
         if (base + i < a.n) codes[base + i] = (int8_t)(c[i] & 0xffu);
     }
+    if (worst > kBorder<K>) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (fabsf(i & 1 ? d[i / 2].y : d[i / 2].x) > kBorder<K> && base + i < a.n) {
+          if constexpr (NV > 0)
+            doubtful |= 1u << (v * E + i);
+          else
+            codes[base + i] = (int8_t)code64(value64<K, T>(a, row, base + i), top64());
+        }
+    }
+  }
+  if (K != kPlain && NV > 0) __syncthreads();
+  while (NV > 0 && doubtful) {
+    const int j = __ffs(doubtful) - 1;
+    doubtful &= doubtful - 1;
+    const int i = (j / E * (int)blockDim.x + (int)threadIdx.x) * E + j % E;
+    codes[i] = (int8_t)code64(value64<K, T>(a, row, i), top64());
   }
   if (threadIdx.x == 0) {
-    double s = top64 / 127.0;
+    double s = top64() / 127.0;
     if (NORM) s *= 1.0 / sqrt((double)ss / a.n + (double)a.eps);
     const float scale = (float)s;
     a.scales[row] = fabsf(scale) <= 3.402823466e38f ? scale : nanf("");
@@ -372,12 +403,7 @@ __global__ void __launch_bounds__(THREADS) int8_rows_kernel(const RowsArgs a) {
 
 template <Kind K, class T, int NV, bool ALIGNED>
 void launch(const RowsArgs& a, int threads, cudaStream_t s) {
-  // 1024 threads leave 64 registers each
-  if (threads <= 512)
-    int8_rows_kernel<K, T, NV, ALIGNED, 512><<<a.rows, threads, 0, s>>>(a);
-  else
-    int8_rows_kernel<K, T, NV, ALIGNED, 1024><<<a.rows, threads, 0, s>>>(a);
-  MLB_CUDA(cudaGetLastError());
+  launch_pdl(int8_rows_kernel<K, T, NV, ALIGNED>, dim3(a.rows), dim3(threads), 0, s, true, a);
 }
 
 template <Kind K, class T>
@@ -419,41 +445,42 @@ void run_rows(const RowsArgs& a, int act_type, int device_id, void* stream) {
     dispatch<K, float>(a, aligned, device_id, s);
 }
 
-// Codes times their row's scale, 16 per thread.
+// Codes times their row's scale: a CTA takes 4096 codes of a row, a thread four times
+// four, so that a warp stores 512 bytes in a row.
+constexpr int kDequant = 4096;
+
 template <class T>
 __global__ void __launch_bounds__(256) int8_dequant_kernel(const int8_t* codes, long long stride,
-                                                           const float* scales, int rows, int n,
+                                                           const float* scales, int n, int pieces,
                                                            T* out, long long out_stride,
                                                            bool aligned) {
-  const int per_row = (n + 15) / 16;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = i / per_row;
-  if (row >= rows) return;
-  const int base = (int)(i - row * per_row) * 16;
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long row = blockIdx.x / pieces;
+  const int base = (int)(blockIdx.x - row * pieces) * kDequant + threadIdx.x * 4;
+  const int8_t* c = codes + row * stride;
+  T* o = out + row * out_stride;
   const float s = scales[row];
-  const int8_t* c = codes + row * stride + base;
-  T* o = out + row * out_stride + base;
-  float v[16];
-  if (base + 16 <= n) {
-    const uint4 u = *reinterpret_cast<const uint4*>(c);
-    const uint32_t words[4] = {u.x, u.y, u.z, u.w};
+  char4 q[4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      v[j] = (float)(int8_t)(words[j >> 2] >> (8 * (j & 3))) * s;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = base + j < n ? (float)c[j] * s : 0.0f;
-  }
-  constexpr int E = 16 / (int)sizeof(T);
-#pragma unroll
-  for (int j = 0; j < 16; j += E) {
-    float part[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) part[e] = v[j + e];
-    if (aligned)
-      store_elements<true>(o + j, n - base - j, part);
+  for (int j = 0; j < 4; ++j) {
+    const int i = base + j * 1024;
+    if (i + 4 <= n)
+      q[j] = *reinterpret_cast<const char4*>(c + i);
     else
-      store_elements<false>(o + j, n - base - j, part);
+      q[j] = make_char4(i < n ? c[i] : 0, i + 1 < n ? c[i + 1] : 0, i + 2 < n ? c[i + 2] : 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = base + j * 1024;
+    const float v[4] = {q[j].x * s, q[j].y * s, q[j].z * s, q[j].w * s};
+    if (aligned && i + 4 <= n) {
+      store_act4(o + i, make_float4(v[0], v[1], v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) store_one(o + i + e, v[e]);
+    }
   }
 }
 
@@ -617,16 +644,16 @@ extern "C" int mlb_int8_dequantize(const int8_t* codes, long long codes_stride,
     const int es = out_type == MLB_ACT_BF16 ? 2 : 4;
     const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
                          (rows == 1 || out_stride % (16 / es) == 0);
-    const long long blocks = ((long long)rows * ((n + 15) / 16) + 255) / 256;
+    const int pieces = (n + kDequant - 1) / kDequant;
+    const long long blocks = (long long)rows * pieces;
     if (blocks > 0x7fffffffLL) invalid("Int8Dequantize: too many rows");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (out_type == MLB_ACT_BF16)
-      int8_dequant_kernel<<<(unsigned)blocks, 256, 0, s>>>(
-          codes, codes_stride, scales, rows, n, static_cast<__nv_bfloat16*>(out), out_stride,
-          aligned);
+      launch_pdl(int8_dequant_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0, s, true,
+                 codes, codes_stride, scales, n, pieces, static_cast<__nv_bfloat16*>(out),
+                 out_stride, aligned);
     else
-      int8_dequant_kernel<<<(unsigned)blocks, 256, 0, s>>>(
-          codes, codes_stride, scales, rows, n, static_cast<float*>(out), out_stride, aligned);
-    MLB_CUDA(cudaGetLastError());
+      launch_pdl(int8_dequant_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, true, codes,
+                 codes_stride, scales, n, pieces, static_cast<float*>(out), out_stride, aligned);
   });
 }

@@ -97,6 +97,8 @@ __global__ void __launch_bounds__(kThreads) rope_rows_kernel(const RopeArgs a) {
   const long long row = blockIdx.x;
   const int half = a.rotary_dim / 2;
   const int units = NEOX ? half / E + (a.head_dim - a.rotary_dim) / E : a.head_dim / E;
+  pdl_launch_dependents();
+  pdl_wait();
   const double pos = (double)a.positions[row];
   for (int i = threadIdx.x; i < half; i += kThreads) {
     const double t = pos * (a.frequencies[i] * 0.15915494309189533577);  // 1 / (2 pi)
@@ -160,11 +162,9 @@ __global__ void __launch_bounds__(kThreads) rope_rows_kernel(const RopeArgs a) {
 
 template <class T, int E>
 void launch(const RopeArgs& a, int rows, bool neox, cudaStream_t s) {
-  if (neox)
-    rope_rows_kernel<T, E, true><<<rows, kThreads, 0, s>>>(a);
-  else
-    rope_rows_kernel<T, (E > 1 ? E : 2), false><<<rows, kThreads, 0, s>>>(a);
-  MLB_CUDA(cudaGetLastError());
+  const auto kernel =
+      neox ? rope_rows_kernel<T, E, true> : rope_rows_kernel<T, (E > 1 ? E : 2), false>;
+  launch_pdl(kernel, dim3(rows), dim3(kThreads), 0, s, true, a);
 }
 
 template <class T>
