@@ -55,63 +55,79 @@ struct RowsArgs {
 constexpr int kHeld = 32;  // values that a thread holds at most
 constexpr float kSmallest = 1e-30f;
 constexpr float kLowestGate = -87.0f;  // e^87 is a normal number, and so is its reciprocal
-// Relative error bounds, in units of 2^-24. t: after a norm one product; SiLU: ex2 4 (2
-// ulp), the factor that corrects it, the sum and two products 1 each, the reciprocal 2: 10
-// together. v: t's, the maximum's (the same), its reciprocal times 127; the last product is
-// exact in a fused multiply-add. Kept: a little more, v's times 127 from a code's border.
+constexpr float kUnit = 0x1p-24f;
+// Relative error bounds. t: after a norm one product (1 unit); SiLU: ex2 4 (2 ulp), the
+// factor that corrects it, the sum and two products 1 each, the reciprocal 2: 10 together.
+// A value is taken for the maximum's candidate within twice that, and a little more.
 template <Kind K>
-constexpr float kValueBound = (K == kSilu ? 12.0f : 2.0f) * 0x1p-24f;
+constexpr float kNear = 1.0f - (K == kSilu ? 24.0f : 4.0f) * kUnit;
+// v: t's, the maximum's (the same) and its reciprocal's times 127 (1); the last product is
+// exact in a fused multiply-add. A code is taken where t times that reciprocal a little
+// more than so many units up and down comes to the same.
 template <Kind K>
-constexpr float kBorder = 0.5f - 127.0f * 0x1p-24f * (K == kSilu ? 24.0f : K == kPlain ? 2.0f : 4.0f);
+constexpr float kDoubt = (K == kSilu ? 24.0f : K == kPlain ? 4.0f : 6.0f) * kUnit;
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// E consecutive elements, zeros past `left`.
-template <bool ALIGNED, class T, int E>
-__device__ __forceinline__ void load_elements(const T* p, int left, float (&v)[E]) {
-  if (ALIGNED && left >= E) {
-#pragma unroll
-    for (int i = 0; i < E; i += 16 / (int)sizeof(T)) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p + i);
-      const uint32_t words[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 4) {
-          v[i + j] = __uint_as_float(words[j]);
-        } else {
-          v[i + 2 * j] = __uint_as_float(words[j] << 16);
-          v[i + 2 * j + 1] = __uint_as_float(words[j] & 0xffff0000u);
-        }
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = i < left ? to_float(p[i]) : 0.0f;
-}
+// E elements at once: 16 bytes where rows are aligned, one element where they are not.
+template <class T, int E>
+struct Raw {
+  using type = uint4;
+  static __device__ __forceinline__ uint4 zero() { return make_uint4(0u, 0u, 0u, 0u); }
+};
+template <class T>
+struct Raw<T, 1> {
+  using type = T;
+  static __device__ __forceinline__ T zero() { return T(0.0f); }
+};
+template <class T, int E>
+using raw_t = typename Raw<T, E>::type;
 
-__device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) {
-  *p = __float2bfloat16_rn(v);
-}
-template <bool ALIGNED, class T, int E>
-__device__ __forceinline__ void store_elements(T* p, int left, const float (&v)[E]) {
-  if (ALIGNED && left >= E) {
-    uint32_t words[4];
+template <class T, int E>
+__device__ __forceinline__ void widen(const raw_t<T, E>& u, float (&v)[E]) {
+  if constexpr (E == 1) {
+    v[0] = to_float(u);
+  } else {
+    const uint32_t words[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 4)
-        words[j] = __float_as_uint(v[j]);
-      else
-        words[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+      if constexpr (sizeof(T) == 4) {
+        v[j] = __uint_as_float(words[j]);
+      } else {
+        v[2 * j] = __uint_as_float(words[j] << 16);
+        v[2 * j + 1] = __uint_as_float(words[j] & 0xffff0000u);
+      }
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(words[0], words[1], words[2], words[3]);
-    return;
   }
-#pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (i < left) store_one(p + i, v[i]);
+}
+// x + r rounded to T. Of two bf16 the fp32 sum rounds to the same bf16 as the exact one:
+// it is inexact only where one is below 2^-16 of the other, which is then the result.
+__device__ __forceinline__ float add_round(float x, float r) { return x + r; }
+__device__ __forceinline__ __nv_bfloat16 add_round(__nv_bfloat16 x, __nv_bfloat16 r) {
+  return __hadd(x, r);
+}
+__device__ __forceinline__ uint32_t add_words(uint32_t x, uint32_t r, float) {
+  return __float_as_uint(__uint_as_float(x) + __uint_as_float(r));
+}
+__device__ __forceinline__ uint32_t add_words(uint32_t x, uint32_t r, __nv_bfloat16) {
+  const __nv_bfloat162 s = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&r));
+  return *reinterpret_cast<const uint32_t*>(&s);
+}
+template <class T, int E>
+__device__ __forceinline__ raw_t<T, E> add_raw(const raw_t<T, E>& x, const raw_t<T, E>& r) {
+  if constexpr (E == 1)
+    return add_round(x, r);
+  else
+    return make_uint4(add_words(x.x, r.x, T()), add_words(x.y, r.y, T()),
+                      add_words(x.z, r.z, T()), add_words(x.w, r.w, T()));
+}
+
+// A slot on its way into shared memory.
+__device__ __forceinline__ void fetch_slot(uint4* slot, const void* p) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(slot)), "l"(p)
+               : "memory");
 }
 
 // |x| and |y|'s larger, NaN if one is.
@@ -192,16 +208,15 @@ __device__ __forceinline__ void block_sum_max64(double& sum, double& top, Shared
 }
 
 // A row in 64 bits throughout.
-template <Kind K, class T, int E>
+template <Kind K, class T>
 __device__ __noinline__ void row64(const RowsArgs& a, long long row, Shared& sh) {
-  const int step = (int)blockDim.x * E;
   double sum = 0.0, top = 0.0;
-  for (int base = threadIdx.x * E; base < a.n; base += step)
-    for (int i = base; i < min(base + E, a.n); ++i) {
-      const double t = fabs(value64<K, T>(a, row, i));
-      sum += square64<K, T>(a, row, i);
-      if (t > top || t != t) top = t != t ? __longlong_as_double(0x7ff8000000000000LL) : t;
-    }
+  __syncthreads();  // sums and inputs of every thread are there
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
+    const double t = fabs(value64<K, T>(a, row, i));
+    sum += square64<K, T>(a, row, i);
+    if (t > top || t != t) top = t != t ? __longlong_as_double(0x7ff8000000000000LL) : t;
+  }
   block_sum_max64(sum, top, sh);
   double root = 1.0;
   if (K == kNorm || K == kNormAdd) root = 1.0 / sqrt(sum / a.n + (double)a.eps);
@@ -209,93 +224,23 @@ __device__ __noinline__ void row64(const RowsArgs& a, long long row, Shared& sh)
   if (!(fabsf(scale) <= 3.402823466e38f) || !(top <= 1.7976931348623157e308)) scale = nanf("");
   int8_t* codes = a.codes + row * a.codes_stride;
   const bool none = scale != scale || top == 0.0;
-  for (int base = threadIdx.x * E; base < a.n; base += step)
-    for (int i = base; i < min(base + E, a.n); ++i)
-      codes[i] = none ? 0 : (int8_t)code64(value64<K, T>(a, row, i), top);
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x)
+    codes[i] = none ? 0 : (int8_t)code64(value64<K, T>(a, row, i), top);
   if (threadIdx.x == 0) a.scales[row] = scale;
 }
 
-// One CTA per row; thread j has elements (v blockDim + j) E + 0 .. E - 1. NV > 0: v < NV
-// covers the row and values stay in registers; NV = 0: rows of any length, computed
-// twice. ALIGNED: rows start at 16-byte boundaries.
-template <Kind K, class T, int NV, bool ALIGNED>
-__global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
-  constexpr int E = 16 / (int)sizeof(T);
-  constexpr bool NORM = K == kNorm || K == kNormAdd;
-  __shared__ Shared sh;
-  const long long row = blockIdx.x;
+// The sum of squares (of a norm) and the maximum of a row from its threads'.
+template <bool NORM>
+__device__ __forceinline__ void join_row(float& ss, float& top, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
-  const int step = (int)blockDim.x * E;
-  const int nv = NV > 0 ? NV : (a.n + step - 1) / step;
-  pdl_launch_dependents();
-  pdl_wait();
-
-  // E values of the row in fp32, their squares added to ss; low: the lowest gate
-  const auto values = [&](int base, float2 (&t)[E / 2], float2& ss, float& low, bool first) {
-    const int left = a.n - base;
-    if (left <= 0) {
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) t[i] = make_float2(0.0f, 0.0f);
-      return;
-    }
-    float v[E], o[E];
-    if (K == kNormAdd && !first) {
-      load_elements<ALIGNED>(static_cast<const T*>(a.sum) + row * a.sum_stride + base, left, v);
-    } else {
-      load_elements<ALIGNED>(x + base, left, v);
-      if constexpr (K == kNormAdd || K == kSilu) load_elements<ALIGNED>(y + base, left, o);
-    }
-    if (K == kNormAdd && first) {
-#pragma unroll
-      for (int i = 0; i < E; i += 2) {
-        const float2 s = add2(make_float2(v[i], v[i + 1]), make_float2(o[i], o[i + 1]));
-        v[i] = s.x, v[i + 1] = s.y;
-        if constexpr (sizeof(T) == 2) {
-          const uint32_t w = pack_bf16(s.x, s.y);
-          v[i] = __uint_as_float(w << 16), v[i + 1] = __uint_as_float(w & 0xffff0000u);
-        }
-      }
-      store_elements<ALIGNED>(static_cast<T*>(a.sum) + row * a.sum_stride + base, left, v);
-    }
-    if constexpr (NORM) load_elements<true>(a.w + base, left, o);
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const float2 p = make_float2(v[i], v[i + 1]);
-      if constexpr (NORM) {
-        ss = fma2(p, p, ss);
-        t[i / 2] = mul2(p, make_float2(o[i], o[i + 1]));
-      } else if constexpr (K == kSilu) {
-        low = fminf(low, fminf(p.x, p.y));
-        t[i / 2] = make_float2(silu_mul(p.x, o[i]), silu_mul(p.y, o[i + 1]));
-      } else {
-        t[i / 2] = p;
-      }
-    }
-  };
-
-  float2 held[NV > 0 ? NV : 1][E / 2];
-  float2 ss2 = make_float2(0.0f, 0.0f);
-  float top = 0.0f, low = 0.0f;
-#pragma unroll
-  for (int v = 0; v < nv; ++v) {
-    float2(&t)[E / 2] = held[NV > 0 ? v : 0];
-    values((v * (int)blockDim.x + (int)threadIdx.x) * E, t, ss2, low, true);
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) top = max_abs(max_abs(top, t[i].x), t[i].y);
-  }
-  if (K == kSilu && low < kLowestGate) top = nanf("");
-  const float mine = top;
-  float ss = ss2.x + ss2.y;
   top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
   if (NORM) ss = warp_sum(ss);
   if (lane == 0) sh.part[warp] = make_float2(ss, top);
   if (threadIdx.x == 0) sh.top = 0;
   __syncthreads();
-  ss = 0.0f;
   uint32_t bits = 0;
   if (warps <= 8) {
+    ss = 0.0f;
     for (int i = 0; i < warps; ++i) {
       const float2 p = sh.part[i];
       ss += p.x;
@@ -307,124 +252,289 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     bits = __reduce_max_sync(0xffffffffu, __float_as_uint(p.y));
   }
   top = __uint_as_float(bits);
-  // the bounds hold for neither (block-uniform; NaN fails the comparisons)
-  if (!(top >= kSmallest && top <= 3e38f) || (NORM && !(ss >= kSmallest && ss <= 3e38f))) {
-    row64<K, T, E>(a, row, sh);
-    return;
-  }
+}
+// Whether the error bounds hold (NaN fails the comparisons).
+template <bool NORM>
+__device__ __forceinline__ bool in_range(float ss, float top) {
+  return top >= kSmallest && top <= 3e38f && (!NORM || (ss >= kSmallest && ss <= 3e38f));
+}
+template <Kind K, class T>
+__device__ __forceinline__ void candidate(const RowsArgs& a, long long row, int i, Shared& sh) {
+  const double t = fabs(value64<K, T>(a, row, i));
+  atomicMax(&sh.top, (unsigned long long)__double_as_longlong(t));
+}
+template <Kind K>
+__device__ __forceinline__ void store_scale(const RowsArgs& a, long long row, double top, float ss) {
+  double s = top / 127.0;
+  if (K == kNorm || K == kNormAdd) s *= 1.0 / sqrt((double)ss / a.n + (double)a.eps);
+  const float scale = (float)s;
+  a.scales[row] = fabsf(scale) <= 3.402823466e38f ? scale : nanf("");
+}
 
-  // the maximum in 64 bits: of the values that may be it
-  const float near = top * (1.0f - 2.0f * kValueBound<K>);
-  const auto candidate = [&](int i) {
-    const double t = fabs(value64<K, T>(a, row, i));
-    atomicMax(&sh.top, (unsigned long long)__double_as_longlong(t));
+constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: a sum's low bits are the whole number
+
+// One CTA per row at a time; thread j has elements (v blockDim + j) E + 0 .. E - 1, v < NV,
+// which cover the row, and holds their values in registers. E > 1: rows start at 16-byte
+// boundaries and have whole units of E. STREAM: a CTA takes row after row and has the next
+// one on its way, every thread its own elements, in shared memory slots of its own.
+template <Kind K, class T, int E, int NV, bool STREAM>
+__global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
+  constexpr bool NORM = K == kNorm || K == kNormAdd, TWO = K == kNormAdd || K == kSilu;
+  static_assert(!STREAM || E > 1);
+  using R = raw_t<T, E>;
+  __shared__ Shared shared[2];  // of rows in turn: one is read while the next is written
+  extern __shared__ uint4 slots[];
+  const int first = (int)threadIdx.x * E, step = (int)blockDim.x * E;
+  const auto fetch = [&](long long row) {
+    if (row < a.rows) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int i = first + v * step;
+        uint4* slot = slots + v * (int)blockDim.x + threadIdx.x;
+        if (i < a.n) {
+          fetch_slot(slot, static_cast<const T*>(a.x) + row * a.x_stride + i);
+          if constexpr (TWO)
+            fetch_slot(slot + NV * (int)blockDim.x, static_cast<const T*>(a.y) + row * a.y_stride + i);
+        }
+      }
+    }
+    cp_async_commit();
   };
-  if (K != kPlain && mine >= near) {
-    if constexpr (NV > 0) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if constexpr (STREAM) fetch(blockIdx.x);
+
+  int turn = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    Shared& sh = shared[turn];
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
+    if constexpr (STREAM) cp_async_wait_all();
+    float t[NV][E], top = 0.0f, low = 0.0f;
+    float2 ss2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = first + v * step;
+      const bool there = i < a.n;
+      R u = Raw<T, E>::zero(), o = Raw<T, E>::zero();
+      if (there) {
+        if constexpr (STREAM) {
+          const uint4* slot = slots + v * (int)blockDim.x + threadIdx.x;
+          u = *slot;
+          if constexpr (TWO) o = slot[NV * (int)blockDim.x];
+        } else {
+          u = *reinterpret_cast<const R*>(x + i);
+          if constexpr (TWO) o = *reinterpret_cast<const R*>(y + i);
+        }
+      }
+      if constexpr (K == kNormAdd) {
+        u = add_raw<T, E>(u, o);
+        if (there)
+          *reinterpret_cast<R*>(static_cast<T*>(a.sum) + row * a.sum_stride + i) = u;
+      }
+      float p[E];
+      widen<T, E>(u, p);
+      if constexpr (NORM) {
+        float w[E];
+        if constexpr (E == 1) {
+          w[0] = there ? a.w[i] : 0.0f;
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; e += 4) {
+            float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (there) q = *reinterpret_cast<const float4*>(a.w + i + e);
+            w[e] = q.x, w[e + 1] = q.y, w[e + 2] = q.z, w[e + 3] = q.w;
+          }
+        }
+        if constexpr (E == 1) {
+          ss2.x = fmaf(p[0], p[0], ss2.x);
+          t[v][0] = p[0] * w[0];
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; e += 2) {
+            const float2 q = make_float2(p[e], p[e + 1]);
+            ss2 = fma2(q, q, ss2);
+            const float2 m = mul2(q, make_float2(w[e], w[e + 1]));
+            t[v][e] = m.x, t[v][e + 1] = m.y;
+          }
+        }
+      } else if constexpr (K == kSilu) {
+        float q[E];
+        widen<T, E>(o, q);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          low = fminf(low, p[e]);
+          t[v][e] = silu_mul(p[e], q[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) t[v][e] = p[e];
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = max_abs(top, t[v][e]);
+    }
+    if constexpr (STREAM) fetch(row + gridDim.x);  // the slots have been read
+    if (K == kSilu && low < kLowestGate) top = nanf("");
+    const float mine = top;
+    float ss = ss2.x + ss2.y;
+    join_row<NORM>(ss, top, sh);
+    if (!in_range<NORM>(ss, top)) {  // block-uniform
+      row64<K, T>(a, row, sh);
+      continue;
+    }
+    // the maximum in 64 bits: of the values that may be it
+    const float near = top * kNear<K>;
+    if (K != kPlain && mine >= near) {
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (fabsf(i & 1 ? held[v][i / 2].y : held[v][i / 2].x) >= near)
-            candidate((v * (int)blockDim.x + (int)threadIdx.x) * E + i);
-    } else {
-      for (int v = 0; v < nv; ++v) {
-        const int base = (v * (int)blockDim.x + (int)threadIdx.x) * E;
-        for (int i = base; i < min(base + E, a.n); ++i)
-          if (fabs(value64<K, T>(a, row, i)) >= (double)near) candidate(i);
+        for (int e = 0; e < E; ++e)
+          if (fabsf(t[v][e]) >= near) candidate<K, T>(a, row, first + v * step + e, sh);
+    }
+
+    const float inv = __fdiv_rn(127.0f, top);
+    const float up = inv * (1.0f + kDoubt<K>), down = inv * (1.0f - kDoubt<K>);
+    int8_t* codes = a.codes + row * a.codes_stride;
+    uint32_t doubtful = 0;  // bit v E + e
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = first + v * step;
+      uint32_t c[E], other[E], differ = 0;
+      if constexpr (E == 1) {
+        c[0] = __float_as_uint(fmaf(t[v][0], up, kMagic));
+        other[0] = __float_as_uint(fmaf(t[v][0], down, kMagic));
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 q = make_float2(t[v][e], t[v][e + 1]), m = make_float2(kMagic, kMagic);
+          const float2 r = fma2(q, make_float2(up, up), m);
+          const float2 s = fma2(q, make_float2(down, down), m);
+          c[e] = __float_as_uint(r.x), c[e + 1] = __float_as_uint(r.y);
+          other[e] = __float_as_uint(s.x), other[e + 1] = __float_as_uint(s.y);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) differ |= c[e] ^ other[e];
+      if (i < a.n) {
+        if constexpr (E == 1) {
+          codes[i] = (int8_t)(c[0] & 0xffu);
+        } else {
+          uint32_t words[E / 4];
+#pragma unroll
+          for (int e = 0; e < E / 4; ++e)
+            words[e] = __byte_perm(__byte_perm(c[4 * e], c[4 * e + 1], 0x0040),
+                                   __byte_perm(c[4 * e + 2], c[4 * e + 3], 0x0040), 0x5410);
+          if constexpr (E == 8)
+            *reinterpret_cast<uint2*>(codes + i) = make_uint2(words[0], words[1]);
+          else
+            *reinterpret_cast<uint32_t*>(codes + i) = words[0];
+        }
+      }
+      if (differ) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (c[e] != other[e]) doubtful |= 1u << (v * E + e);
       }
     }
-  }
-  const auto top64 = [&] {
-    return K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
-  };
-  if (NV == 0) __syncthreads();
-
-  const float inv = __fdiv_rn(127.0f, top);
-  const float2 inv2 = make_float2(inv, inv);
-  const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23
-  int8_t* codes = a.codes + row * a.codes_stride;
-  uint32_t doubtful = 0;  // bit v E + i
-#pragma unroll
-  for (int v = 0; v < nv; ++v) {
-    const int base = (v * (int)blockDim.x + (int)threadIdx.x) * E;
-    float2(&t)[E / 2] = held[NV > 0 ? v : 0];
-    if (NV == 0) values(base, t, ss2, low, false);
-    uint32_t c[E];
-    float2 d[E / 2];
-    float worst = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const float2 r = fma2(t[i], inv2, magic);  // the nearest whole number in the low bits
-      d[i] = fma2(t[i], inv2, fma2(r, make_float2(-1.0f, -1.0f), magic));
-      c[2 * i] = __float_as_uint(r.x), c[2 * i + 1] = __float_as_uint(r.y);
-      worst = fmaxf(worst, fmaxf(fabsf(d[i].x), fabsf(d[i].y)));
+    if (K != kPlain) __syncthreads();
+    const double top64 = K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
+    while (doubtful) {
+      const int j = __ffs(doubtful) - 1;
+      doubtful &= doubtful - 1;
+      const int i = first + j / E * step + j % E;
+      codes[i] = (int8_t)code64(value64<K, T>(a, row, i), top64);
     }
-    uint32_t words[E / 4];
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i)
-      words[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040),
-                             __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
-    if (base + E <= a.n) {  // rows of codes are 16-byte aligned
-      if constexpr (E == 8)
-        *reinterpret_cast<uint2*>(codes + base) = make_uint2(words[0], words[1]);
-      else
-        *reinterpret_cast<uint32_t*>(codes + base) = words[0];
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (base + i < a.n) codes[base + i] = (int8_t)(c[i] & 0xffu);
-    }
-    if (worst > kBorder<K>) {
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (fabsf(i & 1 ? d[i / 2].y : d[i / 2].x) > kBorder<K> && base + i < a.n) {
-          if constexpr (NV > 0)
-            doubtful |= 1u << (v * E + i);
-          else
-            codes[base + i] = (int8_t)code64(value64<K, T>(a, row, base + i), top64());
-        }
-    }
-  }
-  if (K != kPlain && NV > 0) __syncthreads();
-  while (NV > 0 && doubtful) {
-    const int j = __ffs(doubtful) - 1;
-    doubtful &= doubtful - 1;
-    const int i = (j / E * (int)blockDim.x + (int)threadIdx.x) * E + j % E;
-    codes[i] = (int8_t)code64(value64<K, T>(a, row, i), top64());
-  }
-  if (threadIdx.x == 0) {
-    double s = top64() / 127.0;
-    if (NORM) s *= 1.0 / sqrt((double)ss / a.n + (double)a.eps);
-    const float scale = (float)s;
-    a.scales[row] = fabsf(scale) <= 3.402823466e38f ? scale : nanf("");
+    if (threadIdx.x == 0) store_scale<K>(a, row, top64, ss);
   }
 }
 
-template <Kind K, class T, int NV, bool ALIGNED>
-void launch(const RowsArgs& a, int threads, cudaStream_t s) {
-  launch_pdl(int8_rows_kernel<K, T, NV, ALIGNED>, dim3(a.rows), dim3(threads), 0, s, true, a);
+// Rows too long for registers: the same, one element at a time, values computed twice.
+template <Kind K, class T>
+__global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) {
+  constexpr bool NORM = K == kNorm || K == kNormAdd;
+  __shared__ Shared sh;
+  const long long row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
+  T* sum = static_cast<T*>(a.sum) + row * a.sum_stride;
+  pdl_launch_dependents();
+  pdl_wait();
+  float ss = 0.0f, top = 0.0f;
+  const auto value = [&](int i, bool again) {
+    if constexpr (K == kSilu) {
+      const float g = to_float(x[i]);
+      return g < kLowestGate ? nanf("") : silu_mul(g, to_float(y[i]));
+    }
+    T h = K == kNormAdd && again ? sum[i] : x[i];
+    if constexpr (K == kNormAdd)
+      if (!again) sum[i] = h = add_round(h, y[i]);
+    const float f = to_float(h);
+    if (NORM && !again) ss = fmaf(f, f, ss);
+    return NORM ? f * a.w[i] : f;
+  };
+  for (int i = threadIdx.x; i < a.n; i += 1024) top = max_abs(top, value(i, false));
+  const float mine = top;
+  join_row<NORM>(ss, top, sh);
+  if (!in_range<NORM>(ss, top)) {
+    row64<K, T>(a, row, sh);
+    return;
+  }
+  const float near = top * kNear<K>;
+  if (K != kPlain && mine >= near)
+    for (int i = threadIdx.x; i < a.n; i += 1024)
+      if (fabsf(value(i, true)) >= near) candidate<K, T>(a, row, i, sh);
+  __syncthreads();
+  const double top64 = K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
+  const float inv = __fdiv_rn(127.0f, top);
+  const float up = inv * (1.0f + kDoubt<K>), down = inv * (1.0f - kDoubt<K>);
+  int8_t* codes = a.codes + row * a.codes_stride;
+  for (int i = threadIdx.x; i < a.n; i += 1024) {
+    const float t = value(i, true);
+    const uint32_t c = __float_as_uint(fmaf(t, up, kMagic));
+    int code = (int)(int8_t)(c & 0xffu);
+    if (c != __float_as_uint(fmaf(t, down, kMagic))) code = code64(value64<K, T>(a, row, i), top64);
+    codes[i] = (int8_t)code;
+  }
+  if (threadIdx.x == 0) store_scale<K>(a, row, top64, ss);
+}
+
+template <Kind K, class T, int E, int NV>
+void launch(const RowsArgs& a, int threads, int device_id, cudaStream_t s) {
+  if constexpr (E > 1 && NV > 1) {
+    // as many CTAs as 64 registers a thread and their slots leave room for
+    const int bytes = threads * NV * 16 * (K == kNormAdd || K == kSilu ? 2 : 1);
+    constexpr int kRoom = 220 * 1024;
+    const int per_sm = std::min(1024 / threads, kRoom / (bytes + 2 * (int)sizeof(Shared) + 1024));
+    if (per_sm > 0 && a.rows > per_sm * sm_count(device_id)) {
+      const auto kernel = int8_rows_kernel<K, T, E, NV, true>;
+      allow_smem(kernel, kRoom, device_id);
+      return launch_pdl(kernel, dim3(per_sm * sm_count(device_id)), dim3(threads), bytes, s, true, a);
+    }
+  }
+  launch_pdl(int8_rows_kernel<K, T, E, NV, false>, dim3(a.rows), dim3(threads), 0, s, true, a);
 }
 
 template <Kind K, class T>
 void dispatch(const RowsArgs& a, bool aligned, int device_id, cudaStream_t s) {
-  constexpr int E = 16 / (int)sizeof(T), MOST = kHeld / E;
-  const auto threads_for = [&](int nv) { return ((a.n + E * nv - 1) / (E * nv) + 31) / 32 * 32; };
-  if (threads_for(MOST) > 1024) {
-    if (aligned) return launch<K, T, 0, true>(a, 1024, s);
-    return launch<K, T, 0, false>(a, 1024, s);
+  constexpr int E = 16 / (int)sizeof(T);
+  const int held = (a.n + kHeld - 1) / kHeld;  // threads that hold a row
+  if (held > 1024) return launch_pdl(int8_long_rows_kernel<K, T>, dim3(a.rows), dim3(1024), 0, s, true, a);
+  // few rows: up to 512 threads for each, for the time of one; many: as few as hold it,
+  // for less work around their reductions
+  const bool few = a.rows <= 2 * sm_count(device_id);
+  const auto threads_for = [&](int per) { return ((a.n + per - 1) / per + 31) / 32 * 32; };
+  int per = aligned ? E : 8;  // elements a thread
+  while (per < kHeld && (few ? threads_for(per) > 512 : threads_for(per) > threads_for(kHeld))) per *= 2;
+  const int threads = threads_for(per);
+  if (!aligned) {
+    if (per == 8) return launch<K, T, 1, 8>(a, threads, device_id, s);
+    if (per == 16) return launch<K, T, 1, 16>(a, threads, device_id, s);
+    return launch<K, T, 1, 32>(a, threads, device_id, s);
   }
-  if (!aligned) return launch<K, T, MOST, false>(a, threads_for(MOST), s);
-  // few rows: many threads for each, for the time of one; many: fewer, for less work
-  // around their reductions
-  const int most = a.rows <= 2 * sm_count(device_id) ? 512 : 256;
-  int nv = 1;
-  while (nv < MOST && threads_for(nv) > most) nv *= 2;
-  const int threads = threads_for(nv);
-  if (nv == 1) return launch<K, T, 1, true>(a, threads, s);
-  if (nv == 2) return launch<K, T, 2, true>(a, threads, s);
-  if (nv == 4) return launch<K, T, 4, true>(a, threads, s);
-  if constexpr (MOST >= 8) return launch<K, T, 8, true>(a, threads, s);
+  if (per == E) return launch<K, T, E, 1>(a, threads, device_id, s);
+  if (per == 2 * E) return launch<K, T, E, 2>(a, threads, device_id, s);
+  if (per == 4 * E) return launch<K, T, E, 4>(a, threads, device_id, s);
+  if constexpr (8 * E <= kHeld) return launch<K, T, E, 8>(a, threads, device_id, s);
 }
 
 template <Kind K>
@@ -435,7 +545,7 @@ void run_rows(const RowsArgs& a, int act_type, int device_id, void* stream) {
   const auto on16 = [&](const void* p, long long stride) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a.rows == 1 || stride % (16 / es) == 0);
   };
-  const bool aligned = on16(a.x, a.x_stride) && (!a.y || on16(a.y, a.y_stride)) &&
+  const bool aligned = a.n % (16 / es) == 0 && on16(a.x, a.x_stride) && (!a.y || on16(a.y, a.y_stride)) &&
                        (!a.sum || on16(a.sum, a.sum_stride)) &&
                        (!a.w || reinterpret_cast<uintptr_t>(a.w) % 16 == 0);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -479,7 +589,12 @@ __global__ void __launch_bounds__(256) int8_dequant_kernel(const int8_t* codes, 
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (i + e < n) store_one(o + i + e, v[e]);
+        if (i + e < n) {
+          if constexpr (sizeof(T) == 4)
+            o[i + e] = v[e];
+          else
+            o[i + e] = __float2bfloat16_rn(v[e]);
+        }
     }
   }
 }
