@@ -555,34 +555,37 @@ void run_rows(const RowsArgs& a, int act_type, int device_id, void* stream) {
     dispatch<K, float>(a, aligned, device_id, s);
 }
 
-// Codes times their row's scale: a CTA takes 4096 codes of a row, a thread four times
-// four, so that a warp stores 512 bytes in a row.
-constexpr int kDequant = 4096;
-
+// Codes times their row's scale: `across` threads (a power of two) take 16 of each row's
+// codes, in four groups of four, so that a warp stores runs of up to 512 bytes; the
+// others of a CTA take the rows below.
 template <class T>
 __global__ void __launch_bounds__(256) int8_dequant_kernel(const int8_t* codes, long long stride,
-                                                           const float* scales, int n, int pieces,
-                                                           T* out, long long out_stride,
-                                                           bool aligned) {
+                                                           const float* scales, int rows, int n,
+                                                           int log_across, int pieces, T* out,
+                                                           long long out_stride, bool aligned) {
   pdl_launch_dependents();
-  pdl_wait();
-  const long long row = blockIdx.x / pieces;
-  const int base = (int)(blockIdx.x - row * pieces) * kDequant + threadIdx.x * 4;
+  const int across = 1 << log_across;
+  const unsigned down = blockIdx.x / (unsigned)pieces, piece = blockIdx.x - down * pieces;
+  const long long row = (long long)down * (256 >> log_across) + (threadIdx.x >> log_across);
+  const int first = ((int)threadIdx.x & (across - 1)) * 4 + (int)piece * 16 * across;
+  if (row >= rows) return;
   const int8_t* c = codes + row * stride;
   T* o = out + row * out_stride;
+  pdl_wait();
   const float s = scales[row];
   char4 q[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int i = base + j * 1024;
+    const int i = first + j * 4 * across;
+    q[j] = make_char4(0, 0, 0, 0);
     if (i + 4 <= n)
       q[j] = *reinterpret_cast<const char4*>(c + i);
-    else
-      q[j] = make_char4(i < n ? c[i] : 0, i + 1 < n ? c[i + 1] : 0, i + 2 < n ? c[i + 2] : 0, 0);
+    else if (i < n)
+      q[j] = make_char4(c[i], i + 1 < n ? c[i + 1] : 0, i + 2 < n ? c[i + 2] : 0, 0);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int i = base + j * 1024;
+    const int i = first + j * 4 * across;
     const float v[4] = {q[j].x * s, q[j].y * s, q[j].z * s, q[j].w * s};
     if (aligned && i + 4 <= n) {
       store_act4(o + i, make_float4(v[0], v[1], v[2], v[3]));
@@ -636,7 +639,7 @@ bool check_codes(const char* who, int act, int rows, int n, const int8_t* codes,
   paged_check_act(who, act);
   if (rows < 0) invalid(w + ": negative row count");
   if (n <= 0) invalid(w + ": rows must have at least one element");
-  if (n > (1 << 30)) invalid(w + ": rows have more than 2^30 elements");
+  if (n > (1 << 28)) invalid(w + ": rows have more than 2^28 elements");
   if (rows == 0) return false;
   if (!codes) invalid(w + ": null codes");
   if (!scales) invalid(w + ": null scales");
@@ -757,18 +760,23 @@ extern "C" int mlb_int8_dequantize(const int8_t* codes, long long codes_stride,
     DeviceScope scope(device_id);
     if (!any) return;
     const int es = out_type == MLB_ACT_BF16 ? 2 : 4;
-    const bool aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
-                         (rows == 1 || out_stride % (16 / es) == 0);
-    const int pieces = (n + kDequant - 1) / kDequant;
-    const long long blocks = (long long)rows * pieces;
+    // four elements at a time
+    const bool aligned = reinterpret_cast<uintptr_t>(out) % (4 * es) == 0 &&
+                         (rows == 1 || out_stride % 4 == 0);
+    int log_across = 0;
+    while (log_across < 8 && (16 << log_across) < n) ++log_across;
+    const int down = 256 >> log_across, pieces = (n + (16 << log_across) - 1) / (16 << log_across);
+    const long long blocks = ((long long)rows + down - 1) / down * pieces;
     if (blocks > 0x7fffffffLL) invalid("Int8Dequantize: too many rows");
+    const dim3 grid((unsigned)blocks);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (out_type == MLB_ACT_BF16)
-      launch_pdl(int8_dequant_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0, s, true,
-                 codes, codes_stride, scales, n, pieces, static_cast<__nv_bfloat16*>(out),
-                 out_stride, aligned);
+      launch_pdl(int8_dequant_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, codes,
+                 codes_stride, scales, rows, n, log_across, pieces,
+                 static_cast<__nv_bfloat16*>(out), out_stride, aligned);
     else
-      launch_pdl(int8_dequant_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, true, codes,
-                 codes_stride, scales, n, pieces, static_cast<float*>(out), out_stride, aligned);
+      launch_pdl(int8_dequant_kernel<float>, grid, dim3(256), 0, s, true, codes, codes_stride,
+                 scales, rows, n, log_across, pieces, static_cast<float*>(out), out_stride,
+                 aligned);
   });
 }

@@ -43,7 +43,7 @@ def test_quantize_is_refused():
     err(quantize(act=2), "unknown activation type 2")
     err(quantize(rows=-1), "negative row count")
     err(quantize(n=0), "at least one element")
-    err(quantize(n=(1 << 30) + 1), "more than 2^30")
+    err(quantize(n=(1 << 28) + 1), "more than 2^28")
     err(quantize(x=None), "null x")
     err(quantize(x=P + 2), "x is unaligned")
     err(quantize(act=1, x=P + 1), "x is unaligned")
