@@ -320,30 +320,45 @@ def CudaLogProbs(logits, tokens, top_k=0, stream=None):
 
 # ------------------------------------------- rows in 8-bit integers, their product
 
-def _act_rows(who, name, t, shape=None, index=None):
-    """Row stride of t [rows, n] (fp32 or bf16) as the kernels read it; t itself, or a
-    copy where its elements do not follow one another."""
-    if t.dim() != 2 or (shape is not None and t.shape != shape):
-        want = "[rows, n]" if shape is None else list(shape)
+# These calls of one row are bound by their time on the host: their helpers ask a tensor
+# for as little as their checks need, and hand addresses on.
+
+def _act_rows(who, name, t, index, rows=-1, n=-1):
+    """(t or a copy whose rows' elements follow one another, its address, row stride,
+    rows, n) of rows t [rows, n], of the shape given if one is."""
+    if t.dim() != 2 or (rows >= 0 and (t.shape[0] != rows or t.shape[1] != n)):
+        want = f"[{rows}, {n}]" if rows >= 0 else "[rows, n]"
         raise MlbError(-1, f"{who}: expected {name} {want}, got {list(t.shape)}")
-    if index is None:
-        if not t.is_cuda:
+    if t.get_device() != index or index < 0:
+        if index < 0:
             raise MlbError(-1, f"{who}: {name} must be on a CUDA device")
-    else:
         _on_device(who, name, t, index)
     rows, n = t.shape
+    if n == 0:
+        raise MlbError(-1, f"{who}: rows must have at least one element")
     stride, one = t.stride()
     if (one != 1 and n > 1) or (stride < n and rows > 1):
-        return t.contiguous(), n
-    return t, stride if rows > 1 else n
+        t = t.contiguous()
+        stride = n
+    return t, t.data_ptr(), stride if rows > 1 else n, rows, n
 
 
 def _new_codes(like, rows, n):
-    """Room for codes [rows, n], rows 16-byte aligned, and their scales."""
-    torch = _torch()
-    width = (n + 15) // 16 * 16
-    codes = like.new_empty(rows, width, dtype=torch.int8)
-    return codes, width, like.new_empty(rows, dtype=torch.float32)
+    """(codes [rows, n], rows 16-byte aligned, their row stride, scales)."""
+    width = (n + 15) & ~15
+    return (like.new_empty(rows, width, dtype=_torch_module.int8), width,
+            like.new_empty(rows, dtype=_torch_module.float32))
+
+
+def _float_vector(who, name, t, n, index):
+    """Address of contiguous float32 values [n]."""
+    if (t.dtype is not _torch_module.float32 or t.dim() != 1 or t.shape[0] != n
+            or not t.is_contiguous()):
+        raise MlbError(-1, f"{who}: expected contiguous float32 {name} [{n}], got {t.dtype} "
+                           f"{list(t.shape)}")
+    if t.get_device() != index:
+        _on_device(who, name, t, index)
+    return t.data_ptr()
 
 
 def CudaInt8QuantizeDeviceInput(x, stream=None):
@@ -352,15 +367,12 @@ def CudaInt8QuantizeDeviceInput(x, stream=None):
     fp32 [rows]). Of a weight [out_features, in_features]: a scale per channel."""
     who = "Int8Quantize"
     act = _act_type(who, x)
-    x, stride = _act_rows(who, "x", x)
-    rows, n = x.shape
-    if n == 0:
-        raise MlbError(-1, f"{who}: rows must have at least one element")
     index = x.get_device()
-    if stream is not None:
+    if stream is not None and index >= 0:
         return _on_stream(lambda: CudaInt8QuantizeDeviceInput(x), x.device, stream)
+    x, at, stride, rows, n = _act_rows(who, "x", x, index)
     codes, width, scales = _new_codes(x, rows, n)
-    check(lib().mlb_int8_quantize(act, x.data_ptr(), stride, rows, n, codes.data_ptr(), width,
+    check(lib().mlb_int8_quantize(act, at, stride, rows, n, codes.data_ptr(), width,
                                   scales.data_ptr(), index, _raw_stream(index)))
     return codes if width == n else codes[:, :n], scales
 
@@ -372,32 +384,22 @@ def CudaRmsNormInt8DeviceWeight(x, w, eps, residual=None, sum_out=None, stream=N
     sum_out if given: x or residual itself, or no part of them. For one row: x [n]."""
     who = "RmsNormInt8"
     act = _act_type(who, x)
+    index = x.get_device()
+    if stream is not None and index >= 0:
+        return _on_stream(lambda: CudaRmsNormInt8DeviceWeight(x, w, eps, residual, sum_out),
+                          x.device, stream)
     if x.dim() == 1:
         x = x[None]
         residual = residual[None] if residual is not None and residual.dim() == 1 else residual
         sum_out = sum_out[None] if sum_out is not None and sum_out.dim() == 1 else sum_out
-    x_in = x
-    x, stride = _act_rows(who, "x", x)
-    rows, n = x.shape
-    if n == 0:
-        raise MlbError(-1, f"{who}: rows must have at least one element")
-    index = x.get_device()
-    if w.dtype is not _torch().float32 or w.shape != (n,) or not w.is_contiguous():
-        raise MlbError(-1, f"{who}: expected contiguous float32 weights [{n}], got {w.dtype} "
-                           f"{list(w.shape)}")
-    _on_device(who, "w", w, index)
-    if residual is None and sum_out is not None:
-        raise MlbError(-1, f"{who}: sum_out without a residual")
-    if residual is not None and residual.dtype is not x.dtype:
-        raise MlbError(-1, f"{who}: x and residual differ in type")
-    if stream is not None:
-        return _on_stream(lambda: CudaRmsNormInt8DeviceWeight(x_in, w, eps, residual, sum_out),
-                          x.device, stream)
+    x, at, stride, rows, n = _act_rows(who, "x", x, index)
+    w_at = _float_vector(who, "weights", w, n, index)
     r_at = s_at = None
     r_stride = s_stride = n
     if residual is not None:
-        r, r_stride = _act_rows(who, "residual", residual, x.shape, index)
-        r_at = r.data_ptr()
+        if residual.dtype is not x.dtype:
+            raise MlbError(-1, f"{who}: x and residual differ in type")
+        residual, r_at, r_stride, _, _ = _act_rows(who, "residual", residual, index, rows, n)
         if sum_out is None:
             sum_out = x.new_empty(rows, n)
         else:
@@ -408,10 +410,12 @@ def CudaRmsNormInt8DeviceWeight(x, w, eps, residual=None, sum_out=None, stream=N
                 raise MlbError(-1, f"{who}: sum_out must be shaped like x, with elements that "
                                    "follow one another")
         s_at = sum_out.data_ptr()
+    elif sum_out is not None:
+        raise MlbError(-1, f"{who}: sum_out without a residual")
     codes, width, scales = _new_codes(x, rows, n)
-    check(lib().mlb_rmsnorm_int8(act, x.data_ptr(), stride, r_at, r_stride, w.data_ptr(), rows, n,
-                                 eps, s_at, s_stride, codes.data_ptr(), width, scales.data_ptr(),
-                                 index, _raw_stream(index)))
+    check(lib().mlb_rmsnorm_int8(act, at, stride, r_at, r_stride, w_at, rows, n, eps, s_at,
+                                 s_stride, codes.data_ptr(), width, scales.data_ptr(), index,
+                                 _raw_stream(index)))
     if width != n:
         codes = codes[:, :n]
     return (codes, scales) if residual is None else (codes, scales, sum_out)
@@ -423,50 +427,39 @@ def CudaSiluMulInt8DeviceInput(gate, up, stream=None):
     (codes, scales)."""
     who = "SiluMulInt8"
     act = _act_type(who, gate)
-    gate, g_stride = _act_rows(who, "gate", gate)
-    rows, n = gate.shape
-    if n == 0:
-        raise MlbError(-1, f"{who}: rows must have at least one element")
     index = gate.get_device()
+    if stream is not None and index >= 0:
+        return _on_stream(lambda: CudaSiluMulInt8DeviceInput(gate, up), gate.device, stream)
     if up.dtype is not gate.dtype:
         raise MlbError(-1, f"{who}: gate and up differ in type")
-    up, u_stride = _act_rows(who, "up", up, gate.shape, index)
-    if stream is not None:
-        return _on_stream(lambda: CudaSiluMulInt8DeviceInput(gate, up), gate.device, stream)
+    gate, g_at, g_stride, rows, n = _act_rows(who, "gate", gate, index)
+    up, u_at, u_stride, _, _ = _act_rows(who, "up", up, index, rows, n)
     codes, width, scales = _new_codes(gate, rows, n)
-    check(lib().mlb_silu_mul_int8(act, gate.data_ptr(), g_stride, up.data_ptr(), u_stride, rows, n,
-                                  codes.data_ptr(), width, scales.data_ptr(), index,
-                                  _raw_stream(index)))
+    check(lib().mlb_silu_mul_int8(act, g_at, g_stride, u_at, u_stride, rows, n, codes.data_ptr(),
+                                  width, scales.data_ptr(), index, _raw_stream(index)))
     return codes if width == n else codes[:, :n], scales
 
 
-def _code_rows(who, name, t, index=None):
-    """codes [rows, n] with 16-byte aligned rows (t itself, or a copy) and their stride."""
-    torch = _torch()
-    if t.dtype is not torch.int8 or t.dim() != 2 or t.shape[1] == 0:
+def _code_rows(who, name, t, index):
+    """(t or a copy with 16-byte aligned rows, its address, row stride, rows, n) of int8
+    codes [rows, n]."""
+    if t.dtype is not _torch().int8 or t.dim() != 2 or t.shape[1] == 0:
         raise MlbError(-1, f"{who}: expected int8 {name} [rows, n], got {t.dtype} {list(t.shape)}")
-    if index is None:
-        if not t.is_cuda:
+    if t.get_device() != index or index < 0:
+        if index < 0:
             raise MlbError(-1, f"{who}: {name} must be on a CUDA device")
-    else:
         _on_device(who, name, t, index)
     rows, n = t.shape
-    width = (n + 15) // 16 * 16
     stride, one = t.stride()
+    at = t.data_ptr()
     if rows <= 1:
-        stride = width
-    if (one != 1 and n > 1) or stride < n or stride % 16 or t.data_ptr() % 16:
-        padded = t.new_empty(rows, width)
+        stride = (n + 15) & ~15
+    if (one != 1 and n > 1) or stride < n or stride & 15 or at & 15:
+        stride = (n + 15) & ~15
+        padded = t.new_empty(rows, stride)
         padded[:, :n] = t
-        return padded, width
-    return t, stride
-
-
-def _scale_vector(who, name, t, n, index):
-    if t.dtype is not _torch().float32 or t.shape != (n,) or not t.is_contiguous():
-        raise MlbError(-1, f"{who}: expected contiguous float32 {name} [{n}], got {t.dtype} "
-                           f"{list(t.shape)}")
-    _on_device(who, name, t, index)
+        t, at = padded, padded.data_ptr()
+    return t, at, stride, rows, n
 
 
 def _out_type(who, dtype):
@@ -483,16 +476,15 @@ def CudaInt8DequantizeDeviceInput(codes, scales, out_dtype=None, stream=None):
     to bf16 (mlb_int8_dequantize)."""
     who = "Int8Dequantize"
     dtype, act = _out_type(who, out_dtype)
-    if stream is not None and codes.is_cuda:
+    index = codes.get_device()
+    if stream is not None and index >= 0:
         return _on_stream(lambda: CudaInt8DequantizeDeviceInput(codes, scales, out_dtype),
                           codes.device, stream)
-    c, stride = _code_rows(who, "codes", codes)
-    rows, n = codes.shape
-    index = c.get_device()
-    _scale_vector(who, "scales", scales, rows, index)
-    out = scales.new_empty(rows, n, dtype=dtype)
-    check(lib().mlb_int8_dequantize(c.data_ptr(), stride, scales.data_ptr(), rows, n, act,
-                                    out.data_ptr(), n, index, _raw_stream(index)))
+    codes, at, stride, rows, n = _code_rows(who, "codes", codes, index)
+    s_at = _float_vector(who, "scales", scales, rows, index)
+    out = scales.new_empty(rows, n) if act == 0 else scales.new_empty(rows, n, dtype=dtype)
+    check(lib().mlb_int8_dequantize(at, stride, s_at, rows, n, act, out.data_ptr(), n, index,
+                                    _raw_stream(index)))
     return out
 
 
@@ -504,40 +496,34 @@ def CudaInt8LinearDeviceInput(x, x_scale, w, w_scale, bias=None, out_dtype=None,
     given (of any row stride). Codes whose rows are not 16-byte aligned are copied at
     every call: CudaInt8QuantizeDeviceInput makes aligned ones."""
     who = "Int8Linear"
-    torch = _torch()
     if out is not None and out_dtype is None:
         out_dtype = out.dtype
     dtype, act = _out_type(who, out_dtype)
-    if stream is not None and x.is_cuda:
+    index = x.get_device()
+    if stream is not None and index >= 0:
         return _on_stream(lambda: CudaInt8LinearDeviceInput(x, x_scale, w, w_scale, bias,
                                                             out_dtype, out), x.device, stream)
     if x.dim() == 1:
         x = x[None]
-    xc, x_stride = _code_rows(who, "x", x)
-    index = xc.get_device()
-    wc, w_stride = _code_rows(who, "w", w, index)
-    rows, k = x.shape
-    n = w.shape[0]
-    if w.shape[1] != k:
-        raise MlbError(-1, f"{who}: dimension mismatch x={list(x.shape)} weight={list(w.shape)}")
-    _scale_vector(who, "x_scale", x_scale, rows, index)
-    _scale_vector(who, "w_scale", w_scale, n, index)
-    if bias is not None:
-        _scale_vector(who, "bias", bias, n, index)
+    x, x_at, x_stride, rows, k = _code_rows(who, "x", x, index)
+    w, w_at, w_stride, n, w_k = _code_rows(who, "w", w, index)
+    if w_k != k:
+        raise MlbError(-1, f"{who}: dimension mismatch x=[{rows}, {k}] weight=[{n}, {w_k}]")
+    xs_at = _float_vector(who, "x_scale", x_scale, rows, index)
+    ws_at = _float_vector(who, "w_scale", w_scale, n, index)
+    b_at = None if bias is None else _float_vector(who, "bias", bias, n, index)
     if out is None:
-        out = x_scale.new_empty(rows, n, dtype=dtype)
+        out = x_scale.new_empty(rows, n) if act == 0 else x_scale.new_empty(rows, n, dtype=dtype)
         out_stride = n
     else:
         _on_device(who, "out", out, index)
-        if (out.shape != (rows, n) or out.dtype is not dtype or (n > 1 and out.stride(1) != 1)
-                or (rows > 1 and out.stride(0) < n)):
+        if (out.dim() != 2 or out.shape[0] != rows or out.shape[1] != n or out.dtype is not dtype
+                or (n > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < n)):
             raise MlbError(-1, f"{who}: out must be {dtype} [{rows}, {n}] with elements that "
                                "follow one another")
         out_stride = out.stride(0) if rows > 1 else n
-    check(lib().mlb_int8_linear(xc.data_ptr(), x_stride, x_scale.data_ptr(), rows, k,
-                                wc.data_ptr(), w_stride, w_scale.data_ptr(), n,
-                                None if bias is None else bias.data_ptr(), act, out.data_ptr(),
-                                out_stride, index, _raw_stream(index)))
+    check(lib().mlb_int8_linear(x_at, x_stride, xs_at, rows, k, w_at, w_stride, ws_at, n, b_at, act,
+                                out.data_ptr(), out_stride, index, _raw_stream(index)))
     return out
 
 
@@ -591,7 +577,8 @@ class RopeTable:
         self.rotary_dim = rotary_dim
         self.amplitude = amplitude.value
         self.device_id = device_id
-        self.frequencies = torch.from_numpy(values).to(torch.device("cuda", device_id))
+        self.frequencies = torch.from_numpy(values[:half]).to(torch.device("cuda", device_id))
+        self.at = self.frequencies.data_ptr()
 
 
 def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NORMAL, q_out=None,
@@ -602,6 +589,11 @@ def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NO
     dimensions. Returns (q_out, k_out): new tensors, or those given (q and k themselves
     for in place, otherwise no part of either)."""
     who = "RopeRows"
+    index = table.device_id
+    if stream is not None:
+        return _on_stream(lambda: CudaRopeRowsDeviceInput(q, k, positions, table, rope_type,
+                                                          q_out, k_out),
+                          table.frequencies.device, stream)
     first = q if q is not None else k
     if first is None:
         raise MlbError(-1, f"{who}: neither q nor k")
@@ -610,46 +602,49 @@ def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NO
                            f"{list(first.shape)}")
     act = _act_type(who, first)
     rows, _, dim = first.shape
-    index = table.device_id
     _int_tensor(who, "positions", positions, (rows,), index)
-    for name, t, given in (("q", q, q_out), ("k", k, k_out)):
-        if t is None:
-            if given is not None:
-                raise MlbError(-1, f"{who}: {name}_out without {name}")
-            continue
+    q, q_at, q_stride, heads, q_out, qo_at, qo_stride = _rope_side(who, "q", q, q_out, first, rows,
+                                                                   dim, index)
+    k, k_at, k_stride, kv, k_out, ko_at, ko_stride = _rope_side(who, "k", k, k_out, first, rows,
+                                                                dim, index)
+    check(lib().mlb_rope_rows(act, q_at, q_stride, heads, k_at, k_stride, kv, dim,
+                              table.rotary_dim, positions.data_ptr(), table.at, table.amplitude,
+                              rope_type, rows, qo_at, qo_stride, ko_at, ko_stride, index,
+                              _raw_stream(index)))
+    return q_out, k_out
+
+
+def _rope_side(who, name, t, out, first, rows, dim, index):
+    """(t or a copy, its address, row stride, heads, its output, that one's address and
+    row stride) of queries or keys."""
+    if t is None:
+        if out is not None:
+            raise MlbError(-1, f"{who}: {name}_out without {name}")
+        return None, None, 0, 0, None, None, 0
+    if (t is not first and (t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim
+                            or t.dtype is not first.dtype)):
+        raise MlbError(-1, f"{who}: expected {name} [{rows}, heads, {dim}] of {first.dtype}, got "
+                           f"{t.dtype} {list(t.shape)}")
+    if t.get_device() != index:
         _on_device(who, name, t, index)
-        if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim or t.dtype is not first.dtype:
-            raise MlbError(-1, f"{who}: expected {name} [{rows}, heads, {dim}] of "
-                               f"{first.dtype}, got {t.dtype} {list(t.shape)}")
-        if given is not None:
-            _on_device(who, f"{name}_out", given, index)
-            if given.shape != t.shape or given.dtype is not t.dtype or not _whole_rows(given):
-                raise MlbError(-1, f"{who}: {name}_out must be shaped like {name}, its rows' "
-                                   "elements following one another")
-    if stream is not None:
-        return _on_stream(lambda: CudaRopeRowsDeviceInput(q, k, positions, table, rope_type,
-                                                          q_out, k_out), first.device, stream)
-    args, outs, held = [], [], []
-    for t, given in ((q, q_out), (k, k_out)):
-        if t is None:
-            args.append((None, 0, 0, None, 0))
-            outs.append(None)
-            continue
-        heads = t.shape[1]
-        if given is None:
-            given = t.new_empty(rows, heads, dim)
+    heads = t.shape[1]
+    width = heads * dim
+    if out is None:
+        out = t.new_empty(rows, heads, dim)
+        out_stride = width
+    else:
+        _on_device(who, f"{name}_out", out, index)
+        if out.shape != t.shape or out.dtype is not t.dtype or not _whole_rows(out):
+            raise MlbError(-1, f"{who}: {name}_out must be shaped like {name}, its rows' "
+                               "elements following one another")
+        out_stride = out.stride(0) if rows > 1 else width
+    if t.is_contiguous():
+        stride = width
+    else:
         if not _whole_rows(t):
             t = t.contiguous()
-            held.append(t)
-        width = heads * dim
-        args.append((t.data_ptr(), t.stride(0) if rows > 1 else width, heads, given.data_ptr(),
-                     given.stride(0) if rows > 1 else width))
-        outs.append(given)
-    (qp, qs, qh, qo, qos), (kp, ks, kh, ko, kos) = args
-    check(lib().mlb_rope_rows(act, qp, qs, qh, kp, ks, kh, dim, table.rotary_dim,
-                              positions.data_ptr(), table.frequencies.data_ptr(), table.amplitude,
-                              rope_type, rows, qo, qos, ko, kos, index, _raw_stream(index)))
-    return outs[0], outs[1]
+        stride = t.stride(0) if rows > 1 else width
+    return t, t.data_ptr(), stride, heads, out, out.data_ptr(), out_stride
 
 
 def _whole_rows(t):
