@@ -158,6 +158,9 @@ __global__ void __launch_bounds__(kThreads)
     if (a.split > 1) mbar_arrive_expect_tx(&sh.joined, (uint32_t)(owned * a.split) * kChannels * 16);
   }
   if (a.split > 1) cluster_arrive();
+  // The kernel before may have made what is read from here on; and no CTA keeps tensor
+  // memory that another one of that kernel might need while it waits for its end.
+  pdl_wait();
   if (warp == 1) {
     tmem_alloc(&sh.tmem, COLS);
     tmem_relinquish();
@@ -166,7 +169,6 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  pdl_wait();  // the kernel before may have made what is read from here on
 
   // Loads and products are a whole warp's loops of uniform values, of which one lane
   // issues: as one lane's loops they took 600 cycles a tile of K, more than its copies.
@@ -387,6 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     sh.abort_flag = 0;
     fence_mbar_init();
   }
+  pdl_wait();  // before tensor memory is taken, as above
   if (warp == 1) {
     tmem_alloc_pair(&sh.tmem, 2 * N);
     tmem_relinquish_pair();
@@ -396,7 +399,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync_all();  // the other CTA's barriers are there
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  pdl_wait();
 
   int issued = 0;
   if (warp == 0) {
