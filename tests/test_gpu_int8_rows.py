@@ -191,6 +191,28 @@ def test_strides_alignments_and_neighbours(cuda, n, pad, shift, dtype):
         check(got, ref.norm_codes(h, w, 1e-5), 45 * U)
 
 
+@pytest.mark.parametrize("rows,n", [(3, 1000), (1500, 4096), (700, 777), (2, 40000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_equal_maxima(cuda, dtype, rows, n):
+    """Clipped rows, constant rows and rows of two magnitudes among ordinary ones."""
+    t = getattr(torch, dtype)
+    g = gen(rows + n)
+    x = randn(g, rows, n)
+    x[::3] = x[::3].clamp(-1.25, 1.25)
+    x[1::5] = -0.7
+    x[2::7] = torch.where(x[2::7] > 0, 3.0, -1.5)
+    x = x.to(t)
+    w = torch.ones(n, device="cuda")
+    check(mlb.CudaInt8QuantizeDeviceInput(x), ref.to_codes(x.double()))
+    check(mlb.CudaRmsNormInt8DeviceWeight(x, w, 1e-5), ref.norm_codes(x, w, 1e-5), 45 * U)
+    w = 1 + 0.2 * randn(g, n)
+    r = torch.zeros_like(x)
+    check(mlb.CudaRmsNormInt8DeviceWeight(x, w, 1e-5, residual=r), ref.norm_codes(x, w, 1e-5), 45 * U)
+    u = torch.where(x > 0, 2.0, 1.0).to(t)
+    check(mlb.CudaSiluMulInt8DeviceInput(x, u), ref.to_codes(ref.silu_mul(x, u)))
+    check(mlb.CudaSiluMulInt8DeviceInput(u, x), ref.to_codes(ref.silu_mul(u, x)))
+
+
 def test_long_rows_in_place(cuda):
     g = gen(3)
     x, r, w = randn(g, 2, 70001), randn(g, 2, 70001), 1 + 0.1 * randn(g, 70001)
