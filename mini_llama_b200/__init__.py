@@ -346,8 +346,10 @@ def _act_rows(who, name, t, index, rows=-1, n=-1):
 def _new_codes(like, rows, n):
     """(codes [rows, n], rows 16-byte aligned, their row stride, scales)."""
     width = (n + 15) & ~15
-    return (like.new_empty(rows, width, dtype=_torch_module.int8), width,
-            like.new_empty(rows, dtype=_torch_module.float32))
+    int8 = _torch_module.int8
+    codes = (like.new_empty(rows, n, dtype=int8) if width == n
+             else like.new_empty_strided((rows, n), (width, 1), dtype=int8))
+    return codes, width, like.new_empty(rows, dtype=_torch_module.float32)
 
 
 def _float_vector(who, name, t, n, index):
@@ -374,7 +376,7 @@ def CudaInt8QuantizeDeviceInput(x, stream=None):
     codes, width, scales = _new_codes(x, rows, n)
     check(lib().mlb_int8_quantize(act, at, stride, rows, n, codes.data_ptr(), width,
                                   scales.data_ptr(), index, _raw_stream(index)))
-    return codes if width == n else codes[:, :n], scales
+    return codes, scales
 
 
 def CudaRmsNormInt8DeviceWeight(x, w, eps, residual=None, sum_out=None, stream=None):
@@ -416,8 +418,6 @@ def CudaRmsNormInt8DeviceWeight(x, w, eps, residual=None, sum_out=None, stream=N
     check(lib().mlb_rmsnorm_int8(act, at, stride, r_at, r_stride, w_at, rows, n, eps, s_at,
                                  s_stride, codes.data_ptr(), width, scales.data_ptr(), index,
                                  _raw_stream(index)))
-    if width != n:
-        codes = codes[:, :n]
     return (codes, scales) if residual is None else (codes, scales, sum_out)
 
 
@@ -437,7 +437,7 @@ def CudaSiluMulInt8DeviceInput(gate, up, stream=None):
     codes, width, scales = _new_codes(gate, rows, n)
     check(lib().mlb_silu_mul_int8(act, g_at, g_stride, u_at, u_stride, rows, n, codes.data_ptr(),
                                   width, scales.data_ptr(), index, _raw_stream(index)))
-    return codes if width == n else codes[:, :n], scales
+    return codes, scales
 
 
 def _code_rows(who, name, t, index):

@@ -11,8 +11,8 @@
 //
 // Codes are those of 64-bit arithmetic. Computed in fp32 (v = t 127 / A), a value next
 // to a code's border could fall on either side of it, so the fp32 result is taken only
-// where it is further from the border than its error bound, and the few others (5 in
-// 10^5 after a norm, 4 in 10^4 of SiLU) are done again in 64 bits, from the inputs. Those
+// where it is further from the border than its error bound, and the few others (2 in
+// 10^5 after a norm, 4 in 10^5 of SiLU) are done again in 64 bits, from the inputs. Those
 // need A in 64 bits: the threads that hold a value within the bound of the fp32 maximum
 // compute theirs again, while the others go on, and a second barrier later the doubtful
 // codes are corrected. Rows whose fp32 sums or maxima leave the range where the bounds
@@ -21,7 +21,10 @@
 // A row with a NaN or an infinity among its values, or a scale past fp32's largest
 // number, gets the scale NaN: every product of it is NaN, whatever its codes.
 //
-// Bound by HBM for many rows, by the chain load - reduction - store for few.
+// Bound by a row's chain (load, reduction, the 64-bit maximum, codes), which 32 warps per
+// SM hide in part: 4096 rows of 8192 bf16, norm with residual 51 us (4.6 TB/s), SiLU product
+// 44 (3.8), as they are 27 (3.7); fp32 103 (4.2), 66 (4.6), 35 (4.8). Codes back to values
+// are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32: 2.9, 2.4, 1.8 and 1.8 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
