@@ -127,6 +127,11 @@ __device__ __forceinline__ raw_t<T, E> add_raw(const raw_t<T, E>& x, const raw_t
                       add_words(x.z, r.z, T()), add_words(x.w, r.w, T()));
 }
 
+__device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) {
+  *p = __float2bfloat16_rn(v);
+}
+
 // A slot on its way into shared memory.
 __device__ __forceinline__ void fetch_slot(uint4* slot, const void* p) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(slot)), "l"(p)
@@ -315,20 +320,32 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     if constexpr (STREAM) cp_async_wait_all();
     float t[NV][E], top = 0.0f, low = 0.0f;
     float2 ss2 = make_float2(0.0f, 0.0f);
+    // a batch is asked for at once: the sums' stores, which may lie over the inputs, would
+    // otherwise keep each load behind the one before
+    constexpr int BATCH = E == 1 ? 8 : NV < 4 ? NV : 4;
+    R asked[2][BATCH];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = first + v * step;
       const bool there = i < a.n;
-      R u = Raw<T, E>::zero(), o = Raw<T, E>::zero();
-      if (there) {
-        if constexpr (STREAM) {
-          const uint4* slot = slots + v * (int)blockDim.x + threadIdx.x;
-          u = *slot;
-          if constexpr (TWO) o = slot[NV * (int)blockDim.x];
-        } else {
-          u = *reinterpret_cast<const R*>(x + i);
-          if constexpr (TWO) o = *reinterpret_cast<const R*>(y + i);
+      if (!STREAM && v % BATCH == 0) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int j = i + k * step;
+          asked[0][k] = asked[1][k] = Raw<T, E>::zero();
+          if (j < a.n) {
+            asked[0][k] = *reinterpret_cast<const R*>(x + j);
+            if constexpr (TWO) asked[1][k] = *reinterpret_cast<const R*>(y + j);
+          }
         }
+      }
+      R u = Raw<T, E>::zero(), o = Raw<T, E>::zero();
+      if constexpr (!STREAM) {
+        u = asked[0][v % BATCH], o = asked[1][v % BATCH];
+      } else if (there) {
+        const uint4* slot = slots + v * (int)blockDim.x + threadIdx.x;
+        u = *slot;
+        if constexpr (TWO) o = slot[NV * (int)blockDim.x];
       }
       if constexpr (K == kNormAdd) {
         u = add_raw<T, E>(u, o);
@@ -559,50 +576,69 @@ void run_rows(const RowsArgs& a, int act_type, int device_id, void* stream) {
 }
 
 // Codes times their row's scale: `across` threads (a power of two) take 16 of each row's
-// codes, in four groups of four, so that a warp stores runs of up to 512 bytes; the
-// others of a CTA take the rows below.
-template <class T>
+// codes, the others of a CTA the rows below. E codes at a time: four, so that a warp stores
+// 512 bytes in a row, or one where rows of results do not start at boundaries of four.
+template <class T, int E>
 __global__ void __launch_bounds__(256) int8_dequant_kernel(const int8_t* codes, long long stride,
                                                            const float* scales, int rows, int n,
                                                            int log_across, int pieces, T* out,
-                                                           long long out_stride, bool aligned) {
+                                                           long long out_stride) {
   pdl_launch_dependents();
   const int across = 1 << log_across;
   const unsigned down = blockIdx.x / (unsigned)pieces, piece = blockIdx.x - down * pieces;
   const long long row = (long long)down * (256 >> log_across) + (threadIdx.x >> log_across);
-  const int first = ((int)threadIdx.x & (across - 1)) * 4 + (int)piece * 16 * across;
+  const int first = ((int)threadIdx.x & (across - 1)) * E + (int)piece * 16 * across;
   if (row >= rows) return;
   const int8_t* c = codes + row * stride;
   T* o = out + row * out_stride;
   pdl_wait();
   const float s = scales[row];
-  char4 q[4];
+  if constexpr (E == 4) {
+    char4 q[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = first + j * 4 * across;
-    q[j] = make_char4(0, 0, 0, 0);
-    if (i + 4 <= n)
-      q[j] = *reinterpret_cast<const char4*>(c + i);
-    else if (i < n)
-      q[j] = make_char4(c[i], i + 1 < n ? c[i + 1] : 0, i + 2 < n ? c[i + 2] : 0, 0);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = first + j * 4 * across;
-    const float v[4] = {q[j].x * s, q[j].y * s, q[j].z * s, q[j].w * s};
-    if (aligned && i + 4 <= n) {
-      store_act4(o + i, make_float4(v[0], v[1], v[2], v[3]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < n) {
-          if constexpr (sizeof(T) == 4)
-            o[i + e] = v[e];
-          else
-            o[i + e] = __float2bfloat16_rn(v[e]);
-        }
+    for (int j = 0; j < 4; ++j) {
+      const int i = first + j * 4 * across;
+      q[j] = make_char4(0, 0, 0, 0);
+      if (i + 4 <= n)
+        q[j] = *reinterpret_cast<const char4*>(c + i);
+      else if (i < n)
+        q[j] = make_char4(c[i], i + 1 < n ? c[i + 1] : 0, i + 2 < n ? c[i + 2] : 0, 0);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = first + j * 4 * across;
+      const float v[4] = {q[j].x * s, q[j].y * s, q[j].z * s, q[j].w * s};
+      if (i + 4 <= n) {
+        store_act4(o + i, make_float4(v[0], v[1], v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e < n) store_one(o + i + e, v[e]);
+      }
+    }
+  } else {
+    int8_t q[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) q[j] = first + j * across < n ? c[first + j * across] : 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (first + j * across < n) store_one(o + first + j * across, q[j] * s);
   }
+}
+
+template <class T>
+void launch_dequant(const int8_t* codes, long long stride, const float* scales, int rows, int n,
+                    T* out, long long out_stride, cudaStream_t s) {
+  int log_across = 0;
+  while (log_across < 8 && (16 << log_across) < n) ++log_across;
+  const int down = 256 >> log_across, pieces = (n + (16 << log_across) - 1) / (16 << log_across);
+  const long long blocks = ((long long)rows + down - 1) / down * pieces;
+  if (blocks > 0x7fffffffLL) invalid("Int8Dequantize: too many rows");
+  const bool aligned = reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0 &&
+                       (rows == 1 || out_stride % 4 == 0);
+  const auto kernel = aligned ? int8_dequant_kernel<T, 4> : int8_dequant_kernel<T, 1>;
+  launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), 0, s, true, codes, stride, scales, rows, n,
+             log_across, pieces, out, out_stride);
 }
 
 // ------------------------------------------------------------ argument checks
@@ -762,24 +798,11 @@ extern "C" int mlb_int8_dequantize(const int8_t* codes, long long codes_stride,
     }
     DeviceScope scope(device_id);
     if (!any) return;
-    const int es = out_type == MLB_ACT_BF16 ? 2 : 4;
-    // four elements at a time
-    const bool aligned = reinterpret_cast<uintptr_t>(out) % (4 * es) == 0 &&
-                         (rows == 1 || out_stride % 4 == 0);
-    int log_across = 0;
-    while (log_across < 8 && (16 << log_across) < n) ++log_across;
-    const int down = 256 >> log_across, pieces = (n + (16 << log_across) - 1) / (16 << log_across);
-    const long long blocks = ((long long)rows + down - 1) / down * pieces;
-    if (blocks > 0x7fffffffLL) invalid("Int8Dequantize: too many rows");
-    const dim3 grid((unsigned)blocks);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (out_type == MLB_ACT_BF16)
-      launch_pdl(int8_dequant_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, codes,
-                 codes_stride, scales, rows, n, log_across, pieces,
-                 static_cast<__nv_bfloat16*>(out), out_stride, aligned);
+      launch_dequant(codes, codes_stride, scales, rows, n, static_cast<__nv_bfloat16*>(out),
+                     out_stride, s);
     else
-      launch_pdl(int8_dequant_kernel<float>, grid, dim3(256), 0, s, true, codes, codes_stride,
-                 scales, rows, n, log_across, pieces, static_cast<float*>(out), out_stride,
-                 aligned);
+      launch_dequant(codes, codes_stride, scales, rows, n, static_cast<float*>(out), out_stride, s);
   });
 }

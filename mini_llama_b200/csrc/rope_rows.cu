@@ -8,9 +8,11 @@
 // frequency / 2 pi, are taken in 64 bits, where the whole ones are dropped without loss;
 // sine and cosine of what is left are fp32's, so far positions cost no accuracy and no
 // 64-bit sine. They are the same for all heads: a CTA takes a row, makes them once in
-// shared memory and goes through its heads 16 bytes at a time.
+// shared memory and goes through its heads 16 bytes at a time, what is not turned first.
 //
-// Bound by HBM for many rows, by the chain position - angle - product for few.
+// Bound by the chain position - angle - barrier - product, and HBM behind it: 4096 rows of
+// 32 + 8 heads of 128 bf16 15.8 us (5.3 TB/s; 17.4 beyond L2), half of each turned 13.3
+// (18.3), fp32 28 (6.0 TB/s); one row 2.4 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -88,69 +90,17 @@ __device__ __forceinline__ void store(T* p, const float (&v)[E]) {
   }
 }
 
-// E elements at a time: 16 bytes, or the least that holds a pair (NORMAL: 2) or one
-// side of it (NEOX: 1). NEOX units are E elements of the first half with their
-// partners, then E of what is not turned.
-template <class T, int E, bool NEOX>
-__global__ void __launch_bounds__(kThreads) rope_rows_kernel(const RopeArgs a) {
-  __shared__ float2 turn[kMaxHeadDim / 2];
-  const long long row = blockIdx.x;
-  const int half = a.rotary_dim / 2;
+// body(side, head, unit) for every unit of every head, the threads in turn.
+template <class Body>
+__device__ __forceinline__ void for_units(const RopeArgs& a, int units, Body body) {
+  if (units == 0) return;
   const int threads = blockDim.x;
-  const int units = NEOX ? half / E + (a.head_dim - a.rotary_dim) / E : a.head_dim / E;
-  pdl_launch_dependents();
-  pdl_wait();
-  const double pos = (double)a.positions[row];
-  for (int i = threadIdx.x; i < half; i += threads) {
-    const double t = pos * (a.frequencies[i] * 0.15915494309189533577);  // 1 / (2 pi)
-    float s, c;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-    turn[i] = make_float2(c * a.amplitude, s * a.amplitude);
-  }
-  __syncthreads();
   const int head_step = threads / units, unit_step = threads - head_step * units;
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    const T* in = static_cast<const T*>(a.in[side]) + row * a.in_stride[side];
-    T* out = static_cast<T*>(a.out[side]) + row * a.out_stride[side];
-    const int heads = a.heads[side];
     int head = threadIdx.x / units, u = threadIdx.x - head * units;
-    while (head < heads) {
-      const T* x = in + head * a.head_dim;
-      T* y = out + head * a.head_dim;
-      if (NEOX && u * E < half) {
-        const int d = u * E;
-        float p[E], q[E];
-        load<T, E>(x + d, p);
-        load<T, E>(x + half + d, q);
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const float2 cs = turn[d + i];
-          const float lo = fmaf(p[i], cs.x, -(q[i] * cs.y));
-          q[i] = fmaf(p[i], cs.y, q[i] * cs.x);
-          p[i] = lo;
-        }
-        store<T, E>(y + d, p);
-        store<T, E>(y + half + d, q);
-      } else {
-        const int d = NEOX ? a.rotary_dim + (u - half / E) * E : u * E;
-        if (d < a.rotary_dim || a.copy[side]) {
-          float p[E];
-          load<T, E>(x + d, p);
-          if constexpr (!NEOX) {
-#pragma unroll
-            for (int i = 0; i < E; i += 2) {
-              if (d + i < a.rotary_dim) {
-                const float2 cs = turn[(d + i) / 2];
-                const float lo = fmaf(p[i], cs.x, -(p[i + 1] * cs.y));
-                p[i + 1] = fmaf(p[i], cs.y, p[i + 1] * cs.x);
-                p[i] = lo;
-              }
-            }
-          }
-          store<T, E>(y + d, p);
-        }
-      }
+    while (head < a.heads[side]) {
+      body(side, head, u);
       head += head_step;
       u += unit_step;
       if (u >= units) {
@@ -161,10 +111,76 @@ __global__ void __launch_bounds__(kThreads) rope_rows_kernel(const RopeArgs a) {
   }
 }
 
+// E elements at a time: 16 bytes, or the least that holds a pair (NORMAL: 2) or one
+// side of it (NEOX: 1). What is not turned goes first, while the angles are made; then
+// units of E elements, NEOX: of the first half, with their partners.
+template <class T, int E, bool NEOX>
+__global__ void __launch_bounds__(kThreads) rope_rows_kernel(const RopeArgs a) {
+  __shared__ float2 turn[kMaxHeadDim / 2];
+  const long long row = blockIdx.x;
+  const int half = a.rotary_dim / 2;
+  const int turned = NEOX ? half / E : (a.rotary_dim + E - 1) / E;
+  const int rest0 = NEOX ? a.rotary_dim : turned * E;  // the first dimension that is not
+  pdl_launch_dependents();
+  pdl_wait();
+  const auto in = [&](int side, int head) {
+    return static_cast<const T*>(a.in[side]) + row * a.in_stride[side] + head * a.head_dim;
+  };
+  const auto out = [&](int side, int head) {
+    return static_cast<T*>(a.out[side]) + row * a.out_stride[side] + head * a.head_dim;
+  };
+  const double pos = (double)a.positions[row];
+  for (int i = threadIdx.x; i < half; i += blockDim.x) {
+    const double t = pos * (a.frequencies[i] * 0.15915494309189533577);  // 1 / (2 pi)
+    float s, c;
+    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+    turn[i] = make_float2(c * a.amplitude, s * a.amplitude);
+  }
+  if (a.copy[0] || a.copy[1])
+    for_units(a, (a.head_dim - rest0) / E, [&](int side, int head, int u) {
+      if (!a.copy[side]) return;
+      float p[E];
+      load<T, E>(in(side, head) + rest0 + u * E, p);
+      store<T, E>(out(side, head) + rest0 + u * E, p);
+    });
+  __syncthreads();
+  for_units(a, turned, [&](int side, int head, int u) {
+    const int d = u * E;
+    const T* x = in(side, head) + d;
+    T* y = out(side, head) + d;
+    float p[E];
+    load<T, E>(x, p);
+    if constexpr (NEOX) {
+      float q[E];
+      load<T, E>(x + half, q);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float2 cs = turn[d + i];
+        const float lo = fmaf(p[i], cs.x, -(q[i] * cs.y));
+        q[i] = fmaf(p[i], cs.y, q[i] * cs.x);
+        p[i] = lo;
+      }
+      store<T, E>(y + half, q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        if (d + i < a.rotary_dim) {
+          const float2 cs = turn[(d + i) / 2];
+          const float lo = fmaf(p[i], cs.x, -(p[i + 1] * cs.y));
+          p[i + 1] = fmaf(p[i], cs.y, p[i + 1] * cs.x);
+          p[i] = lo;
+        }
+      }
+    }
+    store<T, E>(y, p);
+  });
+}
+
 // Threads of a row's CTA: many rows 128, which leaves more of them beside one another
-// while their angles are made (4096 rows of 40 heads bf16, in us, 128 / 256 / 512 threads:
-// 15.8 / 18.0 / 20.0, half of each head 18.2 / 22.4 / 26.2), few 512 (64 rows of 72 heads
-// 4.0 / 3.3 / 2.8); no more than there are units.
+// while their angles are made (4096 rows of 32 + 8 heads bf16 that L2 does not hold, in us,
+// 64 / 128 / 192 / 256 threads: 17.9 / 17.4 / 19.2 / 19.0, half of each head 19.2 / 18.3 /
+// 21.5 / 22.1), few 512 (one row fp32, 128 / 256 / 512: 4.1 / 2.8 / 2.4); no more than
+// there are units.
 template <class T, int E>
 void launch(const RopeArgs& a, int rows, bool neox, int device_id, cudaStream_t s) {
   const auto kernel =
