@@ -540,11 +540,13 @@ void dispatch(const RowsArgs& a, bool aligned, int device_id, cudaStream_t s) {
   const int held = (a.n + kHeld - 1) / kHeld;  // threads that hold a row
   if (held > 1024) return launch_pdl(int8_long_rows_kernel<K, T>, dim3(a.rows), dim3(1024), 0, s, true, a);
   // few rows: up to 512 threads for each, for the time of one; many: as few as hold it,
-  // for less work around their reductions
+  // for less work around their reductions, but twice as many for single elements (2048
+  // rows of 8191 bf16, norm with residual 78 us with 32 elements a thread, 68 with 16)
   const bool few = a.rows <= 2 * sm_count(device_id);
   const auto threads_for = [&](int per) { return ((a.n + per - 1) / per + 31) / 32 * 32; };
+  const int most = few ? 512 : std::min(1024, threads_for(aligned ? kHeld : 16));
   int per = aligned ? E : 8;  // elements a thread
-  while (per < kHeld && (few ? threads_for(per) > 512 : threads_for(per) > threads_for(kHeld))) per *= 2;
+  while (per < kHeld && threads_for(per) > most) per *= 2;
   const int threads = threads_for(per);
   if (!aligned) {
     if (per == 8) return launch<K, T, 1, 8>(a, threads, device_id, s);
