@@ -250,7 +250,8 @@ int mlb_int8_dequantize(const int8_t* codes_dev, long long codes_stride, const f
  * in_features up to 131071), bias [out_features] fp32 or null, to out [rows,
  * out_features] (out_type MLB_ACT_*, any stride and alignment, no byte of an input).
  * The sum is exact, so a row's results depend on neither the rows beside it nor the
- * run. CudaQ80LinearDeviceInput (include/mini_llama/cuda_quant.h:18) with 8-bit
+ * run; it is rounded to fp32, multiplied with x_scale, then with w_scale, and the bias
+ * added (in one step with the product). CudaQ80LinearDeviceInput (include/mini_llama/cuda_quant.h:18) with 8-bit
  * activations. */
 int mlb_int8_linear(const int8_t* x_dev, long long x_stride, const float* x_scale_dev, int rows,
                     int in_features, const int8_t* w_dev, long long w_stride,

@@ -122,6 +122,13 @@ __device__ __forceinline__ float scaled(int sum, float sx, float sw, float bias,
   return biased ? fmaf(y, sw, bias) : y * sw;
 }
 
+// After a wait that gave up: the time that what others have on its way here takes at most.
+__device__ __forceinline__ void settle() {
+  const long long start = clock64();
+  while (clock64() - start < 2000000) {  // 1 ms
+  }
+}
+
 // Grid: ((token tile * channel tiles) + channel tile) * split + share of K, the shares of
 // a tile being a cluster.
 template <int NT, class T>
@@ -295,9 +302,12 @@ __global__ void __launch_bounds__(kThreads)
           put(out + (t + i) * a.out_stride + c,
               scaled(sum[i], sh.x_scale[t + i], sw, bias, biased));
     }
-    // a CTA whose sums have all arrived may go; another one waits for those that might
-    // still be on their way (CTAs that have gone count as there)
-    if (!ok) cluster_sync_all();
+    // a CTA whose sums have all arrived may go; another one waits until no CTA sends any
+    // more (those that have gone count as there), and for what they have sent
+    if (!ok) {
+      cluster_sync_all();
+      settle();
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -552,7 +562,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __syncthreads();
   if (*(volatile int*)&sh.abort_flag) {
     // nothing is in flight when shared and tensor memory go; the second CTA's copies are
-    // counted by the first alone, so it gives them the time that a copy takes at most
+    // counted by the first alone, so it gives them time
     if (rank == 0 && threadIdx.x == 0)
       for (int j = max(0, issued - P::STAGES); j < issued; ++j)
         drain_wait(a, &sh.full[j % P::STAGES], (uint32_t)(j / P::STAGES) & 1u);
@@ -560,11 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tc_commit_pair(&sh.drain);
       drain_wait(a, &sh.drain, 0);
     }
-    if (rank == 1 && threadIdx.x == 0) {
-      const long long start = clock64();
-      while (clock64() - start < 2000000) {
-      }
-    }
+    if (rank == 1 && threadIdx.x == 0) settle();
     __syncthreads();
   }
   tc_fence_before();
