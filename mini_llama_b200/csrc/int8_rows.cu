@@ -22,9 +22,9 @@
 // number, gets the scale NaN: every product of it is NaN, whatever its codes.
 //
 // Bound by a row's chain (load, reduction, the 64-bit maximum, codes), which 32 warps per
-// SM hide in part: 4096 rows of 8192 bf16, norm with residual 51 us (4.6 TB/s), SiLU product
-// 44 (3.8), as they are 27 (3.7); fp32 103 (4.2), 66 (4.6), 35 (4.8). Codes back to values
-// are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32: 2.9, 2.4, 1.8 and 1.8 us.
+// SM hide in part: 4096 rows of 8192 bf16, norm with residual 47 us (5.0 TB/s), SiLU product
+// 44 (3.8), as they are 27 (3.7); fp32 85 (5.1), 63 (4.8), 32 (5.2). Codes back to values
+// are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32: 2.8, 2.3, 1.7 and 1.3 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -539,12 +539,16 @@ void dispatch(const RowsArgs& a, bool aligned, int device_id, cudaStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
   const int held = (a.n + kHeld - 1) / kHeld;  // threads that hold a row
   if (held > 1024) return launch_pdl(int8_long_rows_kernel<K, T>, dim3(a.rows), dim3(1024), 0, s, true, a);
-  // few rows: up to 512 threads for each, for the time of one; many: as few as hold it,
-  // for less work around their reductions, but twice as many for single elements (2048
-  // rows of 8191 bf16, norm with residual 78 us with 32 elements a thread, 68 with 16)
+  // few rows: up to 512 threads for each, for the time of one; many: 16 elements a thread,
+  // or 32 of aligned bf16 rows, for less work around their reductions, where no residual
+  // takes registers (4096 rows of 8192, 16 / 32 elements, in us: norm with residual bf16 47
+  // / 51, fp32 85 / 103; norm bf16 36 / 33; SiLU product bf16 49 / 44, fp32 63 / 66; as they
+  // are bf16 29 / 27, fp32 32 / 35; 2048 unaligned rows of 8191 bf16, norm with residual 68
+  // / 78)
   const bool few = a.rows <= 2 * sm_count(device_id);
   const auto threads_for = [&](int per) { return ((a.n + per - 1) / per + 31) / 32 * 32; };
-  const int most = few ? 512 : std::min(1024, threads_for(aligned ? kHeld : 16));
+  const bool wide = aligned && sizeof(T) == 2 && K != kNormAdd;
+  const int most = few ? 512 : std::min(1024, threads_for(wide ? kHeld : 16));
   int per = aligned ? E : 8;  // elements a thread
   while (per < kHeld && threads_for(per) > most) per *= 2;
   const int threads = threads_for(per);
