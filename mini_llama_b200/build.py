@@ -5,12 +5,15 @@
   against NCCL for tensor parallelism.
 * ``libmlb_synth.so`` — the CPU side of the seeded synthetic-weight generator
   (g++, no CUDA).
+* ``_calls.so``      — the int8 layer's calls on torch tensors (g++, torch's headers),
+  over libmlb200.so.
 
-Both land next to this file so they travel with the source tree.
+All land next to this file so they travel with the source tree.
 """
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
@@ -21,6 +24,8 @@ CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libmlb200.so")
 SYNTH_LIB = os.path.join(HERE, "libmlb_synth.so")
+
+CALLS = os.path.join(HERE, "_calls.so")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -85,9 +90,29 @@ def build_synth(force: bool = False) -> str:
     return SYNTH_LIB
 
 
+def build_calls(force: bool = False) -> str:
+    src = os.path.join(CSRC, "torch_calls.cc")
+    deps = [src, os.path.join(ROOT, "include", "mlb200.h")]
+    if not force and not _stale(CALLS, deps):
+        return CALLS
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    lib = os.path.join(torch, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", CALLS + ".tmp", src,
+           "-I", os.path.join(torch, "include"),
+           "-I", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"),
+           "-I", sysconfig.get_paths()["include"],
+           "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-L", HERE, "-l:libmlb200.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + lib]
+    subprocess.run(cmd, check=True)
+    os.replace(CALLS + ".tmp", CALLS)
+    return CALLS
+
+
 def build(force: bool = False, verbose: bool = False) -> None:
     build_synth(force)
     build_cuda(force, verbose)
+    build_calls(force)
 
 
 if __name__ == "__main__":
