@@ -22,9 +22,9 @@
 // number, gets the scale NaN: every product of it is NaN, whatever its codes.
 //
 // Bound by a row's chain (load, reduction, the 64-bit maximum, codes), which 32 warps per
-// SM hide in part: 4096 rows of 8192 bf16, norm with residual 47 us (5.0 TB/s), SiLU product
-// 44 (3.8), as they are 27 (3.7); fp32 85 (5.1), 63 (4.8), 32 (5.2). Codes back to values
-// are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32: 2.8, 2.3, 1.7 and 1.3 us.
+// SM hide in part: 4096 rows of 8192 bf16, norm with residual 47 us (5.0 TB/s), norm 29
+// (3.4), SiLU product 40 (4.2), as they are 27 (3.7); fp32 85 (5.1), 42 (4.0), 57 (5.3), 32
+// (5.2). Codes back to values are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32: 2.8, 2.3, 1.7 and 1.3 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
