@@ -30,7 +30,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
-#include <cstring>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "runtime.cuh"
@@ -58,7 +58,8 @@ struct LinearArgs {
   const float* bias;
   void* out;
   long long out_stride;
-  int rows, n, tiles_k, channel_tiles, split, stages;
+  int rows, n, tiles_k, channel_tiles, stages;
+  int split, log_split;  // CTAs that share K, a power of two
   long long wait_cycles;  // limit of a wait
   int never;              // arrivals that the first barrier waits for in vain (self-test)
 };
@@ -142,16 +143,16 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ Shared sh;
   uint8_t* smem = dynamic + (-smem_addr(dynamic) & 1023u);
   const int warp = threadIdx.x >> 5;
-  const int share = blockIdx.x % a.split, tile = blockIdx.x / a.split;
+  const int share = blockIdx.x & (a.split - 1), tile = blockIdx.x >> a.log_split;
   const int token_tile = tile / a.channel_tiles;
   const int channel0 = (tile - token_tile * a.channel_tiles) * kChannels;
   const int token0 = token_tile * NT;
   // the CTA's tiles along K; a share has one at least
-  const int k0 = (int)((long long)a.tiles_k * share / a.split);
-  const int count = (int)((long long)a.tiles_k * (share + 1) / a.split) - k0;
+  const int k0 = a.tiles_k * share >> a.log_split;
+  const int count = (a.tiles_k * (share + 1) >> a.log_split) - k0;
   // groups of four tokens share, share + split .. are joined here
   const int tokens = min(NT, a.rows - token0);
-  const int owned = ((tokens + 3) / 4 - share + a.split - 1) / a.split;
+  const int owned = ((tokens + 3) / 4 - share + a.split - 1) >> a.log_split;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -166,8 +167,9 @@ __global__ void __launch_bounds__(kThreads)
     mbar_init(&sh.drain, 1);
     sh.abort_flag = 0;
     fence_mbar_init();
-    // what the shares of this CTA's tokens come to
-    if (a.split > 1) mbar_arrive_expect_tx(&sh.joined, (uint32_t)(owned * a.split) * kChannels * 16);
+    // what the other shares of this CTA's tokens come to
+    if (a.split > 1)
+      mbar_arrive_expect_tx(&sh.joined, (uint32_t)(owned * (a.split - 1)) * kChannels * 16);
   }
   if (a.split > 1) cluster_arrive();
   // The kernel before may have made what is read from here on; and no CTA keeps tensor
@@ -222,15 +224,14 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   __syncwarp();
-  // what the results are multiplied with, while the products run
   const bool biased = a.bias != nullptr;
-  for (int t = threadIdx.x; t < NT; t += kThreads)
-    sh.x_scale[t] = t < tokens ? a.x_scale[token0 + t] : 0.0f;
-  {
-    const int channel = channel0 + threadIdx.x;
-    const bool inside = channel < a.n;
-    sh.w_scale[threadIdx.x] = inside ? a.w_scale[channel] : 0.0f;
-    sh.bias[threadIdx.x] = inside && biased ? a.bias[channel] : 0.0f;
+  if (warp >= 2) {  // what the results are multiplied with, while the products run
+    for (int i = threadIdx.x - 64; i < kChannels; i += kThreads - 64) {
+      const bool there = channel0 + i < a.n;
+      sh.w_scale[i] = there ? a.w_scale[channel0 + i] : 0.0f;
+      sh.bias[i] = there && biased ? a.bias[channel0 + i] : 0.0f;
+      if (i < NT) sh.x_scale[i] = i < tokens ? a.x_scale[token0 + i] : 0.0f;
+    }
   }
   bool ok = __syncthreads_and(wait(sh, a, &sh.done, 0, 1103));
   if (!ok) {
@@ -260,9 +261,10 @@ __global__ void __launch_bounds__(kThreads)
       float y[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) y[i] = scaled((int)d[i], sh.x_scale[t0 + i], sw, bias, biased);
+      T* o = out + t0 * a.out_stride + c;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (inside && t0 + i < tokens) put(out + (t0 + i) * a.out_stride + c, y[i]);
+      for (int i = 0; i < 16; ++i, o += a.out_stride)
+        if (inside && t0 + i < tokens) put(o, y[i]);
     }
   } else {
     // every share's sums go to their tokens' owner, behind its ring, as [group][share]
@@ -277,31 +279,50 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           if (t0 + i < tokens) {
-            const int group = (t0 + i) / 4, turn = group / a.split, owner = group - turn * a.split;
-            st_async4(cluster_address(sums + (turn * a.split + share) * kChannels + c, owner), d[i],
-                      d[i + 1], d[i + 2], d[i + 3], cluster_address(&sh.joined, owner));
+            const int group = (t0 + i) / 4, owner = group & (a.split - 1);
+            int4* to = sums + (group - owner + share) * kChannels + c;
+            if (owner == share)
+              *to = make_int4((int)d[i], (int)d[i + 1], (int)d[i + 2], (int)d[i + 3]);
+            else
+              st_async4(cluster_address(to, owner), d[i], d[i + 1], d[i + 2], d[i + 3],
+                        cluster_address(&sh.joined, owner));
           }
         }
       }
     }
     if (owned > 0) ok = __syncthreads_and(ok && wait_joined(sh, a));
     const float sw = ok ? sh.w_scale[c] : nanf("");
-    for (int g = 0; g < owned; ++g) {
-      const int4* s = sums + g * a.split * kChannels + c;
-      int4 v[kMaxSplit];
+    const auto finish = [&](auto split) {
+      constexpr int S = decltype(split)::value, AT_ONCE = S > 4 ? 1 : 2;
+#pragma unroll 1
+      for (int g0 = 0; g0 < owned; g0 += AT_ONCE) {
+        int4 v[AT_ONCE][S];
 #pragma unroll
-      for (int r = 0; r < kMaxSplit; ++r) v[r] = r < a.split ? s[r * kChannels] : make_int4(0, 0, 0, 0);
-      int sum[4] = {0, 0, 0, 0};
+        for (int g = 0; g < AT_ONCE; ++g)
 #pragma unroll
-      for (int r = 0; r < kMaxSplit; ++r)
-        sum[0] += v[r].x, sum[1] += v[r].y, sum[2] += v[r].z, sum[3] += v[r].w;
-      const int t = (share + g * a.split) * 4;
+          for (int r = 0; r < S; ++r)
+            v[g][r] = sums[(min(g0 + g, owned - 1) * S + r) * kChannels + c];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (inside && t + i < tokens)
-          put(out + (t + i) * a.out_stride + c,
-              scaled(sum[i], sh.x_scale[t + i], sw, bias, biased));
-    }
+        for (int g = 0; g < AT_ONCE; ++g) {
+          int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int r = 0; r < S; ++r)
+            sum[0] += v[g][r].x, sum[1] += v[g][r].y, sum[2] += v[g][r].z, sum[3] += v[g][r].w;
+          const int t = ((g0 + g) * S + share) * 4;
+          T* o = out + t * a.out_stride + c;
+#pragma unroll
+          for (int i = 0; i < 4; ++i, o += a.out_stride)
+            if (inside && t + i < tokens)
+              put(o, scaled(sum[i], sh.x_scale[t + i], sw, bias, biased));
+        }
+      }
+    };
+    if (a.split == 2)
+      finish(std::integral_constant<int, 2>());
+    else if (a.split == 4)
+      finish(std::integral_constant<int, 4>());
+    else
+      finish(std::integral_constant<int, 8>());
     // a CTA whose sums have all arrived may go; another one waits until no CTA sends any
     // more (those that have gone count as there), and for what they have sent
     if (!ok) {
@@ -658,6 +679,7 @@ void launch_few(const Operands& o, LinearArgs a, int device_id, cudaStream_t str
   const long long tiles = (long long)a.channel_tiles * ((a.rows + NT - 1) / NT);
   const FewPlan p = few_plan(NT, tiles, a.tiles_k, sm_count(device_id));
   a.split = p.split;
+  for (a.log_split = 0; 1 << a.log_split < a.split;) ++a.log_split;
   a.stages = p.stages;
   allow_smem(int8_linear_kernel<NT, T>, kMostBytes, device_id);
   if (tiles * a.split > 0x7fffffffLL) invalid("Int8Linear: too many rows");
