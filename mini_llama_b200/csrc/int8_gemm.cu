@@ -73,6 +73,14 @@ struct Shared {
   alignas(16) float bias[kChannels];
 };
 
+// A barrier of some warps; arriving at it without waiting.
+__device__ __forceinline__ void barrier_sync(int id, int threads) {
+  asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(int id, int threads) {
+  asm volatile("barrier.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 __device__ __forceinline__ bool wait(Shared& sh, const LinearArgs& a, uint64_t* bar,
                                      uint32_t parity, int where) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -175,14 +183,19 @@ __global__ void __launch_bounds__(kThreads)
   // The kernel before may have made what is read from here on; and no CTA keeps tensor
   // memory that another one of that kernel might need while it waits for its end.
   pdl_wait();
-  if (warp == 1) {
-    tmem_alloc(&sh.tmem, COLS);
-    tmem_relinquish();
+  // loads need no tensor memory: their warp does not wait for it
+  if (warp == 0) {
+    __syncwarp();  // the barriers are its first lane's work
+    barrier_arrive(2, kThreads);
+  } else {
+    if (warp == 1) {
+      tmem_alloc(&sh.tmem, COLS);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    barrier_sync(2, kThreads);
+    tc_fence_after();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sh.tmem;
 
   // Loads and products are a whole warp's loops of uniform values, of which one lane
   // issues: as one lane's loops they took 600 cycles a tile of K, more than its copies.
@@ -204,7 +217,7 @@ __global__ void __launch_bounds__(kThreads)
       if (++s == a.stages) s = 0, phase ^= 1u;
     }
   } else if (warp == 1) {
-    const uint32_t idesc = idesc_i8(kChannels, NT);
+    const uint32_t idesc = idesc_i8(kChannels, NT), tmem = sh.tmem;
     const uint64_t ring = smem_desc_sw128(smem_addr(smem));
     int s = 0;
     uint32_t phase = 0;
@@ -248,7 +261,7 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_after();
 
   T* out = static_cast<T*>(a.out) + (long long)token0 * a.out_stride + channel0;
-  const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  const uint32_t lanes = sh.tmem + ((uint32_t)(warp * 32) << 16);
   const int c = threadIdx.x;
   const bool inside = channel0 + c < a.n;
   const float bias = sh.bias[c];
@@ -334,7 +347,7 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, COLS);
+    tmem_dealloc(sh.tmem, COLS);
   }
 }
 
