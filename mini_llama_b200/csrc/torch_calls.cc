@@ -9,8 +9,8 @@
 // form then converts what it can and names the reason where it cannot.
 //
 // Host time of a call of one row, in us, with the Python forms' in brackets: norm with
-// residual 5.7 (12.9), product 4.3 (10.1), back to values 4.5 (7.9), rotation of queries and
-// keys 5.0 (11.8), SiLU product 4.4 (10.1), as it is 4.3 (8.9); 2.7 of it is the launch.
+// residual 5.8 (12.7), product 4.4 (9.5), back to values 4.5 (7.8), rotation of queries and
+// keys 5.1 (11.5), SiLU product 4.3 (9.8), as it is 4.4 (8.7); 2.7 of it is the launch.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -86,10 +86,12 @@ void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).str
 
 PyObject* none() { Py_RETURN_NONE; }
 
+PyObject* wrapped(const at::Tensor& t) { return THPVariable_Wrap(t); }
 template <class... T>
-PyObject* tuple(const T&... t) {
-  PyObject* items[] = {THPVariable_Wrap(t)...};
-  constexpr Py_ssize_t n = sizeof...(T);
+PyObject* wrapped(const at::Tensor& first, const at::Tensor& second, const T&... more) {
+  PyObject* items[] = {THPVariable_Wrap(first), THPVariable_Wrap(second),
+                       THPVariable_Wrap(more)...};
+  constexpr Py_ssize_t n = 2 + sizeof...(T);
   bool whole = true;
   for (PyObject* o : items) whole = whole && o;
   PyObject* r = whole ? PyTuple_New(n) : nullptr;
@@ -102,15 +104,22 @@ PyObject* tuple(const T&... t) {
   return r;
 }
 
-// Runs a call; what torch throws (no memory) is the Python form's to meet again.
-template <class F>
-PyObject* attempt(F&& f) {
+// Runs a call without the interpreter's lock, as a launch may wait for the device and the
+// device for another thread's work: f checks, allocates and launches, and returns whether
+// it did. What torch throws (no memory) is the Python form's to meet again. Returns the
+// outputs, one alone or a tuple.
+template <class F, class... T>
+PyObject* attempt(F&& f, const T&... outputs) {
+  PyThreadState* thread = PyEval_SaveThread();
+  bool done;
   try {
-    return f();
+    done = f();
   } catch (...) {
-    PyErr_Clear();
-    return none();
+    done = false;
   }
+  PyEval_RestoreThread(thread);
+  if (!done) Py_RETURN_NONE;
+  return wrapped(outputs...);
 }
 
 bool whole_number(PyObject* o, int* v) {
@@ -133,21 +142,23 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (n_args != 6 || !tensor(a[0], &x) || !tensor(a[1], &xs) || !tensor(a[2], &w) ||
       !tensor(a[3], &ws) || (a[4] != Py_None && !tensor(a[4], &b)) || !whole_number(a[5], &act))
     return none();
-  return attempt([&]() -> PyObject* {
+  at::Tensor out;
+  const auto call = [&] {
     const int device = x->get_device();
     Rows xr, wr;
     float *xp, *wp, *bp = nullptr;
     if (!codes_of(*x, device, &xr) || !codes_of(*w, device, &wr) || xr.n != wr.n ||
         !floats_of(*xs, device, xr.rows, &xp) || !floats_of(*ws, device, wr.rows, &wp) ||
         (b && !floats_of(*b, device, wr.rows, &bp)))
-      return none();
-    at::Tensor out = new_rows(*xs, xr.rows, wr.rows, act == MLB_ACT_BF16 ? at::kBFloat16 : at::kFloat);
+      return false;
+    out = new_rows(*xs, xr.rows, wr.rows, act == MLB_ACT_BF16 ? at::kBFloat16 : at::kFloat);
     if (mlb_int8_linear(static_cast<const int8_t*>(xr.p), xr.stride, xp, xr.rows, xr.n,
                         static_cast<const int8_t*>(wr.p), wr.stride, wp, wr.rows, bp, act,
                         out.data_ptr(), wr.rows, device, stream_of(device)) != MLB_OK)
-      return none();
-    return THPVariable_Wrap(out);
-  });
+      return false;
+    return true;
+  };
+  return attempt(call, out);
 }
 
 // int8_dequantize(codes, scales, MLB_ACT_*) -> values
@@ -156,58 +167,64 @@ PyObject* int8_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   int act;
   if (n_args != 3 || !tensor(a[0], &c) || !tensor(a[1], &s) || !whole_number(a[2], &act))
     return none();
-  return attempt([&]() -> PyObject* {
+  at::Tensor out;
+  const auto call = [&] {
     const int device = c->get_device();
     Rows r;
     float* sp;
-    if (!codes_of(*c, device, &r) || !floats_of(*s, device, r.rows, &sp)) return none();
-    at::Tensor out = new_rows(*s, r.rows, r.n, act == MLB_ACT_BF16 ? at::kBFloat16 : at::kFloat);
+    if (!codes_of(*c, device, &r) || !floats_of(*s, device, r.rows, &sp)) return false;
+    out = new_rows(*s, r.rows, r.n, act == MLB_ACT_BF16 ? at::kBFloat16 : at::kFloat);
     if (mlb_int8_dequantize(static_cast<const int8_t*>(r.p), r.stride, sp, r.rows, r.n, act,
                             out.data_ptr(), r.n, device, stream_of(device)) != MLB_OK)
-      return none();
-    return THPVariable_Wrap(out);
-  });
+      return false;
+    return true;
+  };
+  return attempt(call, out);
 }
 
 // int8_quantize(x) -> (codes, scales)
 PyObject* int8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const at::Tensor* x;
   if (n_args != 1 || !tensor(a[0], &x)) return none();
-  return attempt([&]() -> PyObject* {
+  at::Tensor codes, scales;
+  const auto call = [&] {
     const int device = x->get_device(), act = act_type(*x);
     Rows r;
-    if (act < 0 || !rows_of(*x, 2, &r)) return none();
+    if (act < 0 || !rows_of(*x, 2, &r)) return false;
     long long width;
-    at::Tensor codes = new_codes(*x, r.rows, r.n, &width);
-    at::Tensor scales = at::empty({r.rows}, x->options().dtype(at::kFloat));
+    codes = new_codes(*x, r.rows, r.n, &width);
+    scales = at::empty({r.rows}, x->options().dtype(at::kFloat));
     if (mlb_int8_quantize(act, r.p, r.stride, r.rows, r.n, static_cast<int8_t*>(codes.data_ptr()),
                           width, static_cast<float*>(scales.data_ptr()), device,
                           stream_of(device)) != MLB_OK)
-      return none();
-    return tuple(codes, scales);
-  });
+      return false;
+    return true;
+  };
+  return attempt(call, codes, scales);
 }
 
 // silu_mul_int8(gate, up) -> (codes, scales)
 PyObject* silu_mul_int8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const at::Tensor *g, *u;
   if (n_args != 2 || !tensor(a[0], &g) || !tensor(a[1], &u)) return none();
-  return attempt([&]() -> PyObject* {
+  at::Tensor codes, scales;
+  const auto call = [&] {
     const int device = g->get_device(), act = act_type(*g);
     Rows gr, ur;
     if (act < 0 || act_type(*u) != act || !on(*u, device) || !rows_of(*g, 2, &gr) ||
         !rows_of(*u, 2, &ur) || gr.rows != ur.rows || gr.n != ur.n)
-      return none();
+      return false;
     long long width;
-    at::Tensor codes = new_codes(*g, gr.rows, gr.n, &width);
-    at::Tensor scales = at::empty({gr.rows}, g->options().dtype(at::kFloat));
+    codes = new_codes(*g, gr.rows, gr.n, &width);
+    scales = at::empty({gr.rows}, g->options().dtype(at::kFloat));
     if (mlb_silu_mul_int8(act, gr.p, gr.stride, ur.p, ur.stride, gr.rows, gr.n,
                           static_cast<int8_t*>(codes.data_ptr()), width,
                           static_cast<float*>(scales.data_ptr()), device,
                           stream_of(device)) != MLB_OK)
-      return none();
-    return tuple(codes, scales);
-  });
+      return false;
+    return true;
+  };
+  return attempt(call, codes, scales);
 }
 
 // rmsnorm_int8(x, w, eps, residual or None) -> (codes, scales) or (codes, scales, sum)
@@ -217,26 +234,28 @@ PyObject* rmsnorm_int8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (n_args != 4 || !tensor(a[0], &x) || !tensor(a[1], &w) || !real_number(a[2], &eps) ||
       (a[3] != Py_None && !tensor(a[3], &res)))
     return none();
-  return attempt([&]() -> PyObject* {
+  at::Tensor codes, scales, sum;
+  const auto call = [&] {
     const int device = x->get_device(), act = act_type(*x);
     Rows xr, rr;
     float* wp;
-    if (act < 0 || !rows_of(*x, 2, &xr) || !floats_of(*w, device, xr.n, &wp)) return none();
+    if (act < 0 || !rows_of(*x, 2, &xr) || !floats_of(*w, device, xr.n, &wp)) return false;
     if (res && (act_type(*res) != act || !on(*res, device) || !rows_of(*res, 2, &rr) ||
                 rr.rows != xr.rows || rr.n != xr.n))
-      return none();
+      return false;
     long long width;
-    at::Tensor codes = new_codes(*x, xr.rows, xr.n, &width);
-    at::Tensor scales = at::empty({xr.rows}, x->options().dtype(at::kFloat)), sum;
+    codes = new_codes(*x, xr.rows, xr.n, &width);
+    scales = at::empty({xr.rows}, x->options().dtype(at::kFloat));
     if (res) sum = new_rows(*x, xr.rows, xr.n, x->scalar_type());
     if (mlb_rmsnorm_int8(act, xr.p, xr.stride, rr.p, rr.stride, wp, xr.rows, xr.n, (float)eps,
                          res ? sum.data_ptr() : nullptr, xr.n,
                          static_cast<int8_t*>(codes.data_ptr()), width,
                          static_cast<float*>(scales.data_ptr()), device,
                          stream_of(device)) != MLB_OK)
-      return none();
-    return res ? tuple(codes, scales, sum) : tuple(codes, scales);
-  });
+      return false;
+    return true;
+  };
+  return res ? attempt(call, codes, scales, sum) : attempt(call, codes, scales);
 }
 
 // rope_rows(q, k, positions, frequencies, amplitude, rope_type) -> (q_out, k_out)
@@ -247,24 +266,27 @@ PyObject* rope_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (n_args != 6 || !tensor(a[0], &q) || !tensor(a[1], &k) || !tensor(a[2], &pos) ||
       !tensor(a[3], &f) || !real_number(a[4], &amplitude) || !whole_number(a[5], &type))
     return none();
-  return attempt([&]() -> PyObject* {
+  at::Tensor q_out, k_out;
+  const auto call = [&] {
     const int device = f->get_device(), act = act_type(*q);
     Rows qr, kr;
     if (act < 0 || act_type(*k) != act || !on(*q, device) || !on(*k, device) ||
         !on(*pos, device) || !rows_of(*q, 3, &qr) || !rows_of(*k, 3, &kr) || qr.rows != kr.rows ||
         q->sizes()[2] != k->sizes()[2] || pos->scalar_type() != at::kInt || pos->dim() != 1 ||
         pos->sizes()[0] != qr.rows || !pos->is_contiguous())
-      return none();
-    at::Tensor q_out = at::empty(q->sizes(), q->options()), k_out = at::empty(k->sizes(), k->options());
+      return false;
+    q_out = at::empty(q->sizes(), q->options());
+    k_out = at::empty(k->sizes(), k->options());
     if (mlb_rope_rows(act, qr.p, qr.stride, (int)q->sizes()[1], kr.p, kr.stride,
                       (int)k->sizes()[1], (int)q->sizes()[2], 2 * (int)f->sizes()[0],
                       static_cast<const int*>(pos->data_ptr()),
                       static_cast<const double*>(f->data_ptr()), (float)amplitude, type, qr.rows,
                       q_out.data_ptr(), qr.n, k_out.data_ptr(), kr.n, device,
                       stream_of(device)) != MLB_OK)
-      return none();
-    return tuple(q_out, k_out);
-  });
+      return false;
+    return true;
+  };
+  return attempt(call, q_out, k_out);
 }
 
 #define CALL(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}

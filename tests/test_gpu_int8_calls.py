@@ -1,5 +1,8 @@
 """The int8 layer's calls have two forms: one for plain arguments, without the interpreter,
 and one in Python for the rest. Both give the same bits; each takes what it should."""
+import threading
+import time
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +141,34 @@ def test_memory_that_is_not_there(cuda):
         mlb.CudaInt8LinearDeviceInput(x, s, x, s)
     y = mlb.CudaInt8LinearDeviceInput(x[:4], s[:4], x[:4], s[:4])
     assert y.shape == (4, 4) and not y.any()
+
+
+def test_another_thread_goes_on_while_a_call_waits_for_the_queue():
+    """More launches than the device's queue takes, behind a wait of a second and a half:
+    a call that waits for room there holds no interpreter lock."""
+    x = torch.randn(1, 256, device="cuda")
+    mlb.CudaInt8QuantizeDeviceInput(x)
+    torch.cuda.synchronize()
+    going, worst = True, 0.0
+
+    def tick():
+        nonlocal worst
+        last = time.perf_counter()
+        while going:
+            time.sleep(0.001)
+            now = time.perf_counter()
+            worst, last = max(worst, now - last), now
+
+    other = threading.Thread(target=tick)
+    other.start()
+    try:
+        torch.cuda._sleep(3_000_000_000)
+        for _ in range(4000):
+            codes, scales = mlb.CudaInt8QuantizeDeviceInput(x)
+        torch.cuda.synchronize()
+    finally:
+        going = False
+        other.join()
+    assert worst < 0.5, worst
+    want, want_scales = mlb.CudaInt8QuantizeDeviceInput(x)
+    assert torch.equal(codes, want) and torch.equal(scales, want_scales)
