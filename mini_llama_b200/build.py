@@ -90,12 +90,21 @@ def build_synth(force: bool = False) -> str:
     return SYNTH_LIB
 
 
+def _torch_dir():
+    """Where torch with CUDA is installed, or None."""
+    spec = importlib.util.find_spec("torch")
+    at = os.path.dirname(spec.origin) if spec and spec.origin else ""
+    return at if os.path.exists(os.path.join(at, "lib", "libc10_cuda.so")) else None
+
+
 def build_calls(force: bool = False) -> str:
     src = os.path.join(CSRC, "torch_calls.cc")
     deps = [src, os.path.join(ROOT, "include", "mlb200.h")]
     if not force and not _stale(CALLS, deps):
         return CALLS
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    torch = _torch_dir()
+    if torch is None:
+        raise RuntimeError("calls on torch tensors need torch with CUDA")
     lib = os.path.join(torch, "lib")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", CALLS + ".tmp", src,
            "-I", os.path.join(torch, "include"),
@@ -112,7 +121,8 @@ def build_calls(force: bool = False) -> str:
 def build(force: bool = False, verbose: bool = False) -> None:
     build_synth(force)
     build_cuda(force, verbose)
-    build_calls(force)
+    if _torch_dir():
+        build_calls(force)
 
 
 if __name__ == "__main__":

@@ -273,3 +273,21 @@ def test_python_forms_refuse_before_the_device():
         mlb.CudaInt8LinearDeviceInput(x, x[0], q, x[0])
     with pytest.raises(mlb.MlbError, match="rotary_dim must be even"):
         mlb.RopeTable(63)
+
+
+@pytest.mark.parametrize("there", [True, False])
+def test_a_build_without_torch_leaves_out_its_calls(monkeypatch, there):
+    from mini_llama_b200 import build
+
+    made = []
+    for name in ("build_synth", "build_cuda", "build_calls"):
+        monkeypatch.setattr(build, name, lambda *a, name=name: made.append(name))
+    monkeypatch.setattr(build.importlib.util, "find_spec",
+                        build.importlib.util.find_spec if there else lambda name: None)
+    build.build()
+    assert made == ["build_synth", "build_cuda"] + ["build_calls"] * there
+    if not there:
+        monkeypatch.undo()
+        monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: None)
+        with pytest.raises(RuntimeError, match="need torch"):
+            build.build_calls(force=True)
