@@ -15,8 +15,8 @@
 // channels. Where the tiles alone leave SMs idle, a cluster of CTAs shares K; each pushes
 // its sums to the CTA that owns their tokens and goes: no workspace, one launch. Bound by
 // HBM (the weights are read once) behind the start of the stream: one row of 4096 x 4096
-// 4.8 us, of 4096 x 28672 21.6 (5.4 TB/s), 32 of 8192 x 10240 15.3, or 19 with weights that
-// L2 does not hold (4.4 TB/s).
+// 4.6 us, 5.0 with weights that L2 does not hold, of 4096 x 28672 21.2 (5.5 TB/s), 32 of 8192
+// x 10240 14.4 and 18.7 (4.5 TB/s).
 //
 // Many tokens (int8_linear_pair_kernel): pairs of CTAs, 256 tokens by up to 256 channels.
 // Bound by the tensor cores: 4096 x 4096 x 28672 279 to 293 us (3290 to 3450 TOPS, twice the
@@ -59,6 +59,7 @@ struct LinearArgs {
   void* out;
   long long out_stride;
   int rows, n, tiles_k, channel_tiles, stages;
+  int ahead;             // tiles of weights that a CTA asks for before its turn
   int split, log_split;  // CTAs that share K, a power of two
   long long wait_cycles;  // limit of a wait
   int never;              // arrivals that the first barrier waits for in vain (self-test)
@@ -180,6 +181,11 @@ __global__ void __launch_bounds__(kThreads)
       mbar_arrive_expect_tx(&sh.joined, (uint32_t)(owned * (a.split - 1)) * kChannels * 16);
   }
   if (a.split > 1) cluster_arrive();
+  // weights on their way to L2 while the kernel before still runs: what that one may write
+  // there is read all the same, as L2 is where every SM's stores come together
+  if (warp == 3)
+    for (int i = 0; i < min(count, a.ahead); ++i)
+      if (elect_one()) tma_prefetch(&w_map, (k0 + i) * kTileK, channel0);
   // The kernel before may have made what is read from here on; and no CTA keeps tensor
   // memory that another one of that kernel might need while it waits for its end.
   pdl_wait();
@@ -694,6 +700,12 @@ void launch_few(const Operands& o, LinearArgs a, int device_id, cudaStream_t str
   a.split = p.split;
   for (a.log_split = 0; 1 << a.log_split < a.split;) ++a.log_split;
   a.stages = p.stages;
+  // Four tiles of short shares, whose time is mostly their start (weights beyond L2, in us,
+  // with / without: one row of 4096 x 4096, 8 tiles a share, 4.97 / 5.84, of 14336 x 4096, 14
+  // tiles, 11.9 / 12.7); eight keep the kernel before waiting (norm and product of 32 x 4096
+  // x 4096 8.7 with four, 9.4 with eight, 9.2 without). None of long ones: 32 of 8192 x
+  // 10240, 32 tiles, 19.5 / 18.7, one of 4096 x 28672 22.0 / 21.8.
+  a.ahead = (a.tiles_k + p.split - 1) / p.split <= 16 ? 4 : 0;
   allow_smem(int8_linear_kernel<NT, T>, kMostBytes, device_id);
   if (tiles * a.split > 0x7fffffffLL) invalid("Int8Linear: too many rows");
   const CUtensorMap w_map = tile_map(o.w, o.w_stride, a.n, o.k, kChannels);

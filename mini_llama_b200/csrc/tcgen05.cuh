@@ -214,6 +214,13 @@ __device__ __forceinline__ void tma_load(void* dst, const void* map, int x, int 
       : "memory");
 }
 
+// One tile of a tensor map into L2.
+__device__ __forceinline__ void tma_prefetch(const void* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x),
+               "r"(y)
+               : "memory");
+}
+
 // ------------------------------------------------- pairs of CTAs (cta_group::2)
 // Two CTAs of a cluster work on one D of 256 rows, 128 in the tensor memory of each;
 // the first issues the products. Each holds its rows of A and half of B's rows.

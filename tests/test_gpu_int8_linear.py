@@ -12,6 +12,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 import mini_llama_b200 as mlb  # noqa: E402
+from mini_llama_b200 import _lib  # noqa: E402
 from tests import int8_ref as ref  # noqa: E402
 
 U = 2.0 ** -24
@@ -152,3 +153,41 @@ def test_streams_and_graphs(cuda):
     graph.replay()
     torch.cuda.synchronize()
     check(out, *other)
+
+
+@pytest.mark.parametrize("n,k", [(4096, 1024), (513, 300), (4096, 4096)])
+def test_weights_that_the_kernel_before_writes(n, k):
+    """Weights are asked for while the kernel before runs: one that makes them, over and
+    over in the same place, is waited for all the same, in a graph too."""
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    many = torch.randn(6, n, k, device="cuda", generator=g)
+    x, xs = mlb.CudaInt8QuantizeDeviceInput(torch.randn(3, k, device="cuda", generator=g))
+    width = (k + 15) // 16 * 16
+    place, scales = torch.empty(n, width, dtype=torch.int8, device="cuda"), None
+    w = place[:, :k]
+    want = []
+    for v in many:
+        codes, scales = mlb.CudaInt8QuantizeDeviceInput(v)
+        want.append(mlb.CudaInt8LinearDeviceInput(x, xs, codes.clone(), scales.clone()))
+    scales = torch.empty(n, device="cuda")
+    lib = _lib.lib()
+
+    def chain():
+        out = []
+        for v in many:
+            assert lib.mlb_int8_quantize(0, v.data_ptr(), k, n, k, w.data_ptr(), width,
+                                         scales.data_ptr(), 0,
+                                         torch.cuda.current_stream().cuda_stream) == 0
+            out.append(mlb.CudaInt8LinearDeviceInput(x, xs, w, scales))
+        return out
+
+    for made, right in zip(chain(), want):
+        assert torch.equal(made, right)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain()
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    for made, right in zip(out, want):
+        assert torch.equal(made, right)
