@@ -33,12 +33,14 @@
 #include "common.cuh"
 #include "paged.cuh"
 #include "rows.cuh"
+#include "tcgen05.cuh"
 
 namespace mlb {
 
 namespace {
 
 enum Kind { kPlain, kNorm, kNormAdd, kSilu };
+enum Form { kAlone, kStream, kShared };  // how CTAs and rows meet, as at the kernel
 
 struct RowsArgs {
   const void* x;  // kSilu: gate
@@ -53,9 +55,11 @@ struct RowsArgs {
   float* scales;
   int rows, n;
   float eps;
+  int log_share;  // 2^log_share CTAs, a cluster, share a row
 };
 
 constexpr int kHeld = 32;  // values that a thread holds at most
+constexpr int kMostLogShare = 3;
 constexpr float kSmallest = 1e-30f;
 constexpr float kLowestGate = -87.0f;  // e^87 is a normal number, and so is its reciprocal
 constexpr float kUnit = 0x1p-24f;
@@ -197,6 +201,7 @@ struct Shared {
   float2 part[32];  // per warp: sum of squares, maximum
   double part64[32];
   unsigned long long top;  // bits of the 64-bit maximum
+  float2 share[1 << kMostLogShare];  // per CTA of the row's: sum of squares, maximum
 };
 
 // Block-wide sum and maximum of one double per thread each (top: NaN above all).
@@ -261,6 +266,35 @@ __device__ __forceinline__ void join_row(float& ss, float& top, Shared& sh) {
   }
   top = __uint_as_float(bits);
 }
+// The same of a row that CTAs share, from theirs.
+__device__ __forceinline__ void join_shares(float& ss, float& top, int rank, int log_share,
+                                            Shared& sh) {
+  cluster_wait();  // every CTA is there
+  if (threadIdx.x < 1u << log_share)
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+                     cluster_address(&sh.share[rank], threadIdx.x)),
+                 "f"(ss), "f"(top)
+                 : "memory");
+  cluster_sync_all();
+  ss = 0.0f;
+  uint32_t bits = 0;
+  for (int i = 0; i < 1 << log_share; ++i) {
+    const float2 p = sh.share[i];
+    ss += p.x;
+    bits = max(bits, __float_as_uint(p.y));
+  }
+  top = __uint_as_float(bits);
+}
+__device__ __forceinline__ double join_tops(double top, int rank, int log_share, Shared& sh) {
+  if (threadIdx.x < 1u << log_share)
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(
+                     cluster_address(&sh.part64[rank], threadIdx.x)),
+                 "d"(top)
+                 : "memory");
+  cluster_sync_all();
+  for (int i = 0; i < 1 << log_share; ++i) top = fmax(top, sh.part64[i]);
+  return top;
+}
 // Whether the error bounds hold (NaN fails the comparisons).
 template <bool NORM>
 __device__ __forceinline__ bool in_range(float ss, float top) {
@@ -283,16 +317,23 @@ constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: a sum's low bits are the w
 
 // One CTA per row at a time; thread j has elements (v blockDim + j) E + 0 .. E - 1, v < NV,
 // which cover the row, and holds their values in registers. E > 1: rows start at 16-byte
-// boundaries and have whole units of E. STREAM: a CTA takes row after row and has the next
+// boundaries and have whole units of E. kStream: a CTA takes row after row and has the next
 // one on its way, every thread its own elements, in shared memory slots of its own.
-template <Kind K, class T, int E, int NV, bool STREAM>
+// kShared: a cluster takes a row; blockDim above is that of all its CTAs, and what their
+// barriers join the cluster's join once more. (As a choice at run time it spilled: one row
+// of 29568 fp32, norm with residual 10.8 us instead of 8.3.)
+template <Kind K, class T, int E, int NV, Form F>
 __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
   constexpr bool NORM = K == kNorm || K == kNormAdd, TWO = K == kNormAdd || K == kSilu;
+  constexpr bool STREAM = F == kStream, SHARED = F == kShared;
   static_assert(!STREAM || E > 1);
   using R = raw_t<T, E>;
   __shared__ Shared shared[2];  // of rows in turn: one is read while the next is written
   extern __shared__ uint4 slots[];
-  const int first = (int)threadIdx.x * E, step = (int)blockDim.x * E;
+  const int log_share = SHARED ? a.log_share : 0, rank = blockIdx.x & ((1 << log_share) - 1);
+  const int first = (rank * (int)blockDim.x + (int)threadIdx.x) * E;
+  const int step = ((int)blockDim.x << log_share) * E;
+  if constexpr (SHARED) cluster_arrive();
   const auto fetch = [&](long long row) {
     if (row < a.rows) {
 #pragma unroll
@@ -313,7 +354,8 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
   if constexpr (STREAM) fetch(blockIdx.x);
 
   int turn = 0;
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+  for (long long row = blockIdx.x >> log_share; row < a.rows;
+       row += gridDim.x >> log_share, turn ^= 1) {
     Shared& sh = shared[turn];
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
@@ -402,9 +444,10 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     const float mine = top;
     float ss = ss2.x + ss2.y;
     join_row<NORM>(ss, top, sh);
-    if (!in_range<NORM>(ss, top)) {  // block-uniform
+    if constexpr (SHARED) join_shares(ss, top, rank, log_share, sh);
+    if (!in_range<NORM>(ss, top)) {  // the same for all threads of the row
       if constexpr (STREAM && !EARLY) fetch(row + gridDim.x);
-      row64<K, T>(a, row, sh);
+      if (rank == 0) row64<K, T>(a, row, sh);
       continue;
     }
     // the maximum in 64 bits: of the values that may be it
@@ -489,18 +532,19 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
       }
     }
     if (K != kPlain) __syncthreads();
-    const double top64 = K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
+    double top64 = K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
+    if constexpr (K != kPlain && SHARED) top64 = join_tops(top64, rank, log_share, sh);
     while (doubtful) {
       const int j = __ffs(doubtful) - 1;
       doubtful &= doubtful - 1;
       const int i = first + j / E * step + j % E;
       codes[i] = (int8_t)code64(value64<K, T>(a, row, i), top64);
     }
-    if (threadIdx.x == 0) store_scale<K>(a, row, top64, ss);
+    if (rank == 0 && threadIdx.x == 0) store_scale<K>(a, row, top64, ss);
   }
 }
 
-// Rows too long for registers: the same, one element at a time, values computed twice.
+// Rows too long for eight CTAs' registers: the same, one element at a time, values computed twice.
 template <Kind K, class T>
 __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) {
   constexpr bool NORM = K == kNorm || K == kNormAdd;
@@ -557,20 +601,57 @@ void launch(const RowsArgs& a, int threads, int device_id, cudaStream_t s) {
     const int bytes = threads * NV * 16 * (K == kNormAdd || K == kSilu ? 2 : 1);
     constexpr int kRoom = 220 * 1024;
     const int per_sm = std::min(1024 / threads, kRoom / (bytes + 2 * (int)sizeof(Shared) + 1024));
-    if (per_sm > 0 && a.rows > per_sm * sm_count(device_id)) {
-      const auto kernel = int8_rows_kernel<K, T, E, NV, true>;
+    if (a.log_share == 0 && per_sm > 0 && a.rows > per_sm * sm_count(device_id)) {
+      const auto kernel = int8_rows_kernel<K, T, E, NV, kStream>;
       allow_smem(kernel, kRoom, device_id);
       return launch_pdl(kernel, dim3(per_sm * sm_count(device_id)), dim3(threads), bytes, s, true, a);
     }
   }
-  launch_pdl(int8_rows_kernel<K, T, E, NV, false>, dim3(a.rows), dim3(threads), 0, s, true, a);
+  if (a.log_share == 0)
+    return launch_pdl(int8_rows_kernel<K, T, E, NV, kAlone>, dim3(a.rows), dim3(threads), 0, s, true, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.rows << a.log_share);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1u << a.log_share;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  MLB_CUDA(cudaLaunchKernelEx(&cfg, int8_rows_kernel<K, T, E, NV, kShared>, a));
 }
 
 template <Kind K, class T>
-void dispatch(const RowsArgs& a, bool aligned, int device_id, cudaStream_t s) {
+void dispatch(RowsArgs a, bool aligned, int device_id, cudaStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
-  const int held = (a.n + kHeld - 1) / kHeld;  // threads that hold a row
-  if (held > 1024) return launch_pdl(int8_long_rows_kernel<K, T>, dim3(a.rows), dim3(1024), 0, s, true, a);
+  // CTAs that share a row: as many as its values take registers of, rather than passing
+  // over it twice (norm with residual, norm, SiLU product, as it is, 300 rows of 65536, in
+  // us: fp32 168, 90, 185, 54 with one CTA's two passes, 87, 51, 64, 37 shared, bf16 143, 79,
+  // 129, 30 and 57, 39, 48, 30)
+  const auto held = [&](int log_share) {  // threads that hold a row, of each CTA
+    return ((a.n + (kHeld << log_share) - 1) / (kHeld << log_share));
+  };
+  a.log_share = 0;
+  while (a.log_share < kMostLogShare && held(a.log_share) > 1024) ++a.log_share;
+  if (held(a.log_share) > 1024 || (a.log_share > 0 && a.rows >= 1 << (31 - kMostLogShare)))
+    return launch_pdl(int8_long_rows_kernel<K, T>, dim3(a.rows), dim3(1024), 0, s, true, a);
+  // Few rows of more than 32 KB: as many as SMs and 2048 elements each allow, if they are
+  // four or more of 8192 or less (SiLU product and as it is, alone / shared, in us: one row
+  // of 29568 fp32 6.3, 3.9 / 3.8, 2.4, bf16 5.7, 3.3 / 3.9, 2.5; 16 rows 6.8, 4.1 / 5.0, 3.3
+  // and 6.1, 3.7 / 4.9, 3.4; one of 14336 fp32 4.1, 2.7 / 3.8, 2.5; in two, 64 of 14336 fp32
+  // 4.7, 3.2 / 5.4, 3.5). Not norms, whose sums of squares would be split otherwise than
+  // beside many rows.
+  if ((K == kPlain || K == kSilu) && (long long)a.n * (int)sizeof(T) > 32768) {
+    int log_share = a.log_share;
+    while (log_share < kMostLogShare &&
+           (long long)a.rows << (log_share + 1) <= sm_count(device_id) &&
+           a.n >> (log_share + 1) >= 2048)
+      ++log_share;
+    if (log_share >= 2 && a.n >> log_share <= 8192) a.log_share = log_share;
+  }
   // few rows: up to 512 threads for each, for the time of one; many: 16 elements a thread,
   // or 32 of aligned bf16 rows, for less work around their reductions, where no residual
   // takes registers (4096 rows of 8192, 16 / 32 elements, in us: norm with residual bf16 47
@@ -578,7 +659,10 @@ void dispatch(const RowsArgs& a, bool aligned, int device_id, cudaStream_t s) {
   // are bf16 29 / 27, fp32 32 / 35; 2048 unaligned rows of 8191 bf16, norm with residual 68
   // / 78)
   const bool few = a.rows <= 2 * sm_count(device_id);
-  const auto threads_for = [&](int per) { return ((a.n + per - 1) / per + 31) / 32 * 32; };
+  const auto threads_for = [&](int per) {
+    per <<= a.log_share;
+    return ((a.n + per - 1) / per + 31) / 32 * 32;
+  };
   const bool wide = aligned && sizeof(T) == 2 && K != kNormAdd;
   const int most = few ? 512 : std::min(1024, threads_for(wide ? kHeld : 16));
   int per = aligned ? E : 8;  // elements a thread
