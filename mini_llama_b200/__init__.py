@@ -597,7 +597,9 @@ class RopeTable:
     contexts by ROPE_SCALING_LINEAR (factor), ROPE_SCALING_LLAMA3 (factor, original_len,
     low_freq_factor, high_freq_factor) or ROPE_SCALING_YARN (factor, original_len,
     beta_fast, beta_slow; sine and cosine times `amplitude`). `factors` [rotary_dim / 2]
-    divides each pair's frequency instead (what a checkpoint's table of factors holds)."""
+    divides each pair's frequency instead (what a checkpoint's table of factors holds).
+    `frequencies` (float64 [rotary_dim / 2]) is what the calls read: others may take its
+    place."""
 
     def __init__(self, rotary_dim, theta=10000.0, scaling=ROPE_SCALING_NONE, factor=1.0,
                  original_len=0, low_freq_factor=1.0, high_freq_factor=4.0, beta_fast=32.0,
@@ -619,7 +621,6 @@ class RopeTable:
         self.amplitude = amplitude.value
         self.device_id = device_id
         self.frequencies = torch.from_numpy(values[:half]).to(torch.device("cuda", device_id))
-        self.at = self.frequencies.data_ptr()
 
 
 def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NORMAL, q_out=None,
@@ -649,12 +650,17 @@ def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NO
     act = _act_type(who, first)
     rows, _, dim = first.shape
     _int_tensor(who, "positions", positions, (rows,), index)
+    f = table.frequencies
+    if f.dtype is not _torch().float64 or f.dim() != 1 or not f.is_contiguous():
+        raise MlbError(-1, f"{who}: expected contiguous float64 frequencies [rotary_dim / 2], got "
+                           f"{f.dtype} {list(f.shape)}")
+    _on_device(who, "frequencies", f, index)
     q, q_at, q_stride, heads, q_out, qo_at, qo_stride = _rope_side(who, "q", q, q_out, first, rows,
                                                                    dim, index)
     k, k_at, k_stride, kv, k_out, ko_at, ko_stride = _rope_side(who, "k", k, k_out, first, rows,
                                                                 dim, index)
     check(lib().mlb_rope_rows(act, q_at, q_stride, heads, k_at, k_stride, kv, dim,
-                              table.rotary_dim, positions.data_ptr(), table.at, table.amplitude,
+                              2 * f.shape[0], positions.data_ptr(), f.data_ptr(), table.amplitude,
                               rope_type, rows, qo_at, qo_stride, ko_at, ko_stride, index,
                               _raw_stream(index)))
     return q_out, k_out

@@ -270,6 +270,9 @@ PyObject* rope_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const auto call = [&] {
     const int device = f->get_device(), act = act_type(*q);
     Rows qr, kr;
+    if (f->scalar_type() != at::kDouble || f->dim() != 1 || f->sizes()[0] > kMostInt / 2 ||
+        !f->is_contiguous())
+      return false;
     if (act < 0 || act_type(*k) != act || !on(*q, device) || !on(*k, device) ||
         !on(*pos, device) || !rows_of(*q, 3, &qr) || !rows_of(*k, 3, &kr) || qr.rows != kr.rows ||
         q->sizes()[2] != k->sizes()[2] || pos->scalar_type() != at::kInt || pos->dim() != 1 ||

@@ -137,3 +137,25 @@ def test_no_rows_and_non_finite_values(cuda):
     out, _ = mlb.CudaRopeRowsDeviceInput(x, None, torch.tensor([3, 3], dtype=torch.int32, device="cuda"), tab)
     bad = torch.isnan(out)
     assert bad[0, 0, 4:6].all() and int(bad.sum()) == 2
+
+
+def test_replaced_frequencies(cuda):
+    """What stands in a table's place of frequencies is read in every form, or refused."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(3, 2, 64, device="cuda", generator=g)
+    k = torch.randn(3, 1, 64, device="cuda", generator=g)
+    pos = torch.tensor([5, 900, 131071], dtype=torch.int32, device="cuda")
+    tab = mlb.RopeTable(64)
+    f = ref.frequencies(32, 500000.0)[0]
+    tab.frequencies = f.cuda()
+    q_out, k_out = mlb.CudaRopeRowsDeviceInput(q, k, pos, tab)
+    check(q_out, q, pos, f, 1.0, False)
+    check(k_out, k, pos, f, 1.0, False)
+    alone, _ = mlb.CudaRopeRowsDeviceInput(q, None, pos, tab)
+    assert torch.equal(alone, q_out)
+    for bad in (f.float().cuda(), f.cuda()[None], f.cuda()[::2], f):
+        tab.frequencies = bad
+        with pytest.raises(mlb.MlbError, match="frequencies"):
+            mlb.CudaRopeRowsDeviceInput(q, k, pos, tab)
+        with pytest.raises(mlb.MlbError, match="frequencies"):
+            mlb.CudaRopeRowsDeviceInput(q, None, pos, tab)
