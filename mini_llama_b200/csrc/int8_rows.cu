@@ -150,7 +150,11 @@ __device__ __forceinline__ float max_abs(float x, float y) {
   return r;
 }
 
-// SiLU(g) * u. e^-g = 2^(hi + lo), -g log2(e) in two parts; 2^lo as 1 + lo ln 2.
+// SiLU(g) * u. e^-g = 2^(hi + lo), -g log2(e) in two parts; 2^lo as 1 + lo ln 2. The
+// reciprocal goes to u first: g may be any number, u a large one, and g times the reciprocal
+// below the normal numbers, where it loses its bits. The reciprocal times u does so only
+// where u is that small: then it is u itself (a reciprocal of 1, to half a step of u), or,
+// as g is between -87 and 17, the result is below 1e-36, 0 beside any maximum in range.
 __device__ __forceinline__ float silu_mul(float g, float u) {
   const float hi = g * -1.4426950408889634f;
   // what hi's rounding and the constant's (1.92596e-8 beyond fp32) leave, times ln 2
@@ -158,7 +162,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   float e = ex2(hi), r;
   e = fmaf(e, lo, e);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
+  return g * (r * u);
 }
 __device__ __noinline__ double silu_mul64(float g, float u) {
   return (double)g / (1.0 + exp(-(double)g)) * (double)u;
