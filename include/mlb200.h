@@ -213,7 +213,9 @@ int mlb_logprobs(int logits_type, const void* logits_dev, long long row_stride, 
 /* ------------------------------------------- rows in 8-bit integers, their product
  * A row of values t is held as int8 codes in [-127, 127] with one fp32 scale:
  *   A = max |t|,  code = rint(127 t / A) (ties to even),  scale = A / 127
- * computed as if in 64 bits; A = 0 gives codes and scale 0. A row with a NaN or an
+ * computed as if in 64 bits, a norm's sum of squares too (its order goes by the number
+ * of rows: a scale next to the middle of two fp32 numbers, by 64-bit rounding, may come
+ * out as either); A = 0 gives codes and scale 0. A row with a NaN or an
  * infinity among its values, or a scale past fp32's largest number, gets the scale
  * NaN: every product of it is NaN, whatever its codes. Rows of codes are 16-byte
  * aligned, a row stride (in codes, a multiple of 16) apart; rows of activations

@@ -7,7 +7,10 @@
 // for a row of values t. RMSNorm's root is a factor of the whole row, so it cancels in
 // the codes: they are those of t = h w, h the (rounded) sum, and the root enters the
 // scale alone. One pass over the row in registers therefore yields both the sum of
-// squares and the maximum, and one reduction joins them.
+// squares and the maximum. The sum is 64-bit throughout, so that scales keep their accuracy
+// in the longest rows, and do not go by how a row is divided among threads, which goes by
+// the number of rows (of fp32 sums every fourth scale did; of these one in 2^23 or fewer, whose
+// exact value lies within 64-bit rounding of the middle of two fp32 numbers).
 //
 // Codes are those of 64-bit arithmetic. Computed in fp32 (v = t 127 / A), a value next
 // to a code's border could fall on either side of it, so the fp32 result is taken only
@@ -15,8 +18,8 @@
 // 10^5 after a norm, 4 in 10^5 of SiLU) are done again in 64 bits, from the inputs. Those
 // need A in 64 bits: the threads that hold a value within the bound of the fp32 maximum
 // compute theirs again, while the others go on, and a second barrier later the doubtful
-// codes are corrected. Rows whose fp32 sums or maxima leave the range where the bounds
-// hold (below 1e-30, not finite, gates below -87) are done in 64 bits throughout.
+// codes are corrected. Rows whose fp32 maximum leaves the range where the bounds hold
+// (below 1e-30, not finite, gates below -87) are done in 64 bits throughout.
 //
 // A row with a NaN or an infinity among its values, or a scale past fp32's largest
 // number, gets the scale NaN: every product of it is NaN, whatever its codes.
@@ -203,10 +206,11 @@ __device__ __forceinline__ int code64(double t, double top) {
 }
 
 struct Shared {
-  float2 part[32];  // per warp: sum of squares, maximum
-  double part64[32];
+  float part[32];    // per warp: maximum
+  double part64[32];  // per warp: sum of squares
   unsigned long long top;  // bits of the 64-bit maximum
-  float2 share[1 << kMostLogShare];  // per CTA of the row's: sum of squares, maximum
+  float share[1 << kMostLogShare];  // per CTA of the row's: maximum
+  double2 share64[1 << kMostLogShare];  // per CTA: maximum and sum of squares in 64 bits
 };
 
 // Block-wide sum and maximum of one double per thread each (top: NaN above all).
@@ -247,73 +251,73 @@ __device__ __noinline__ void row64(const RowsArgs& a, long long row, Shared& sh)
   if (threadIdx.x == 0) a.scales[row] = scale;
 }
 
-// The sum of squares (of a norm) and the maximum of a row from its threads'.
-template <bool NORM>
-__device__ __forceinline__ void join_row(float& ss, float& top, Shared& sh) {
+// The maximum of a row from its threads'.
+__device__ __forceinline__ float join_row(float top, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-  if (NORM) ss = warp_sum(ss);
-  if (lane == 0) sh.part[warp] = make_float2(ss, top);
+  if (lane == 0) sh.part[warp] = top;
   if (threadIdx.x == 0) sh.top = 0;
   __syncthreads();
   uint32_t bits = 0;
   if (warps <= 8) {
-    ss = 0.0f;
-    for (int i = 0; i < warps; ++i) {
-      const float2 p = sh.part[i];
-      ss += p.x;
-      bits = max(bits, __float_as_uint(p.y));
-    }
+    for (int i = 0; i < warps; ++i) bits = max(bits, __float_as_uint(sh.part[i]));
   } else {
-    const float2 p = lane < warps ? sh.part[lane] : make_float2(0.0f, 0.0f);
-    if (NORM) ss = warp_sum(p.x);
-    bits = __reduce_max_sync(0xffffffffu, __float_as_uint(p.y));
+    bits = __reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(sh.part[lane]) : 0u);
   }
-  top = __uint_as_float(bits);
+  return __uint_as_float(bits);
 }
 // The same of a row that CTAs share, from theirs.
-__device__ __forceinline__ void join_shares(float& ss, float& top, int rank, int log_share,
-                                            Shared& sh) {
+__device__ __forceinline__ float join_shares(float top, int rank, int log_share, Shared& sh) {
   cluster_wait();  // every CTA is there
   if (threadIdx.x < 1u << log_share)
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(
                      cluster_address(&sh.share[rank], threadIdx.x)),
-                 "f"(ss), "f"(top)
+                 "f"(top)
                  : "memory");
   cluster_sync_all();
-  ss = 0.0f;
   uint32_t bits = 0;
-  for (int i = 0; i < 1 << log_share; ++i) {
-    const float2 p = sh.share[i];
-    ss += p.x;
-    bits = max(bits, __float_as_uint(p.y));
-  }
-  top = __uint_as_float(bits);
+  for (int i = 0; i < 1 << log_share; ++i) bits = max(bits, __float_as_uint(sh.share[i]));
+  return __uint_as_float(bits);
 }
-__device__ __forceinline__ double join_tops(double top, int rank, int log_share, Shared& sh) {
+// The sum of squares: each warp's before a barrier, all warps' behind it, which the one
+// thread that stores the scale adds up.
+__device__ __forceinline__ void put_squares(double ss, Shared& sh) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if ((threadIdx.x & 31) == 0) sh.part64[threadIdx.x >> 5] = ss;
+}
+__device__ __forceinline__ double all_squares(const Shared& sh) {
+  const int warps = blockDim.x >> 5;
+  double ss = 0.0;
+  for (int i = 0; i < warps; ++i) ss += sh.part64[i];
+  return ss;
+}
+// Maximum and sum of squares in 64 bits of a row that CTAs share.
+__device__ __forceinline__ void join_shares64(double& top, double& ss, int rank, int log_share,
+                                              Shared& sh) {
   if (threadIdx.x < 1u << log_share)
-    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(
-                     cluster_address(&sh.part64[rank], threadIdx.x)),
-                 "d"(top)
+    asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(
+                     cluster_address(&sh.share64[rank], threadIdx.x)),
+                 "d"(top), "d"(ss)
                  : "memory");
   cluster_sync_all();
-  for (int i = 0; i < 1 << log_share; ++i) top = fmax(top, sh.part64[i]);
-  return top;
+  ss = 0.0;
+  for (int i = 0; i < 1 << log_share; ++i) {
+    top = fmax(top, sh.share64[i].x);
+    ss += sh.share64[i].y;
+  }
 }
 // Whether the error bounds hold (NaN fails the comparisons).
-template <bool NORM>
-__device__ __forceinline__ bool in_range(float ss, float top) {
-  return top >= kSmallest && top <= 3e38f && (!NORM || (ss >= kSmallest && ss <= 3e38f));
-}
+__device__ __forceinline__ bool in_range(float top) { return top >= kSmallest && top <= 3e38f; }
 template <Kind K, class T>
 __device__ __forceinline__ void candidate(const RowsArgs& a, long long row, int i, Shared& sh) {
   const double t = fabs(value64<K, T>(a, row, i));
   atomicMax(&sh.top, (unsigned long long)__double_as_longlong(t));
 }
 template <Kind K>
-__device__ __forceinline__ void store_scale(const RowsArgs& a, long long row, double top, float ss) {
+__device__ __forceinline__ void store_scale(const RowsArgs& a, long long row, double top, double ss) {
   double s = top / 127.0;
-  if (K == kNorm || K == kNormAdd) s *= 1.0 / sqrt((double)ss / a.n + (double)a.eps);
+  if (K == kNorm || K == kNormAdd) s *= 1.0 / sqrt(ss / a.n + (double)a.eps);
   const float scale = (float)s;
   a.scales[row] = fabsf(scale) <= 3.402823466e38f ? scale : nanf("");
 }
@@ -366,10 +370,11 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
     if constexpr (STREAM) cp_async_wait_all();
     float t[NV][E], top = 0.0f, low = 0.0f;
-    float2 ss2 = make_float2(0.0f, 0.0f);
+    double ss = 0.0;
     // a batch is asked for at once: the sums' stores, which may lie over the inputs, would
-    // otherwise keep each load behind the one before
-    constexpr int BATCH = E == 1 ? 8 : NV < 4 ? NV : 4;
+    // otherwise keep each load behind the one before (2048 rows of 8191, norm with residual, 8 /
+    // 16 elements: fp32 79 / 65 us, bf16 85 / 65; 32 spilled)
+    constexpr int BATCH = E == 1 ? (NV <= 16 ? NV : 8) : NV < 4 ? NV : 4;
     R asked[2][BATCH];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -414,13 +419,14 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
           }
         }
         if constexpr (E == 1) {
-          ss2.x = fmaf(p[0], p[0], ss2.x);
+          ss = fma((double)p[0], (double)p[0], ss);
           t[v][0] = p[0] * w[0];
         } else {
 #pragma unroll
           for (int e = 0; e < E; e += 2) {
             const float2 q = make_float2(p[e], p[e + 1]);
-            ss2 = fma2(q, q, ss2);
+            ss = fma((double)q.x, (double)q.x, ss);
+            ss = fma((double)q.y, (double)q.y, ss);
             const float2 m = mul2(q, make_float2(w[e], w[e + 1]));
             t[v][e] = m.x, t[v][e + 1] = m.y;
           }
@@ -447,10 +453,14 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     if constexpr (EARLY) fetch(row + gridDim.x);
     if (K == kSilu && low < kLowestGate) top = nanf("");
     const float mine = top;
-    float ss = ss2.x + ss2.y;
-    join_row<NORM>(ss, top, sh);
-    if constexpr (SHARED) join_shares(ss, top, rank, log_share, sh);
-    if (!in_range<NORM>(ss, top)) {  // the same for all threads of the row
+    // the warps' sums of squares, before the first barrier or behind it (norm of 4096 rows of
+    // 14336 fp32 76 / 81 us, bf16 54.4 / 53; of 16384 rows of 1000 fp32 26.0 / 28.3; of 64 of
+    // 29568 fp32 6.0 / 5.7)
+    constexpr bool FIRST = sizeof(T) == 4 && (STREAM || K == kNormAdd);
+    if constexpr (NORM && FIRST) put_squares(ss, sh);
+    top = join_row(top, sh);
+    if constexpr (SHARED) top = join_shares(top, rank, log_share, sh);
+    if (!in_range(top)) {  // the same for all threads of the row
       if constexpr (STREAM && !EARLY) fetch(row + gridDim.x);
       if (rank == 0) row64<K, T>(a, row, sh);
       continue;
@@ -491,6 +501,7 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
       }
     }
     if constexpr (STREAM && !EARLY) fetch(row + gridDim.x);
+    if constexpr (NORM && !FIRST) put_squares(ss, sh);
 
     const float inv = __fdiv_rn(127.0f, top);
     const float up = inv * (1.0f + kDoubt<K>), down = inv * (1.0f - kDoubt<K>);
@@ -538,14 +549,20 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     }
     if (K != kPlain) __syncthreads();
     double top64 = K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
-    if constexpr (K != kPlain && SHARED) top64 = join_tops(top64, rank, log_share, sh);
+    if constexpr (K != kPlain && SHARED) {
+      ss = NORM && threadIdx.x < 1u << log_share ? all_squares(sh) : 0.0;
+      join_shares64(top64, ss, rank, log_share, sh);
+    }
     while (doubtful) {
       const int j = __ffs(doubtful) - 1;
       doubtful &= doubtful - 1;
       const int i = first + j / E * step + j % E;
       codes[i] = (int8_t)code64(value64<K, T>(a, row, i), top64);
     }
-    if (rank == 0 && threadIdx.x == 0) store_scale<K>(a, row, top64, ss);
+    if (rank == 0 && threadIdx.x == 0) {
+      if constexpr (NORM && !SHARED) ss = all_squares(sh);
+      store_scale<K>(a, row, top64, ss);
+    }
   }
 }
 
@@ -561,7 +578,8 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) 
   T* sum = static_cast<T*>(a.sum) + row * a.sum_stride;
   pdl_launch_dependents();
   pdl_wait();
-  float ss = 0.0f, top = 0.0f;
+  float top = 0.0f;
+  double ss = 0.0;
   const auto value = [&](int i, bool again) {
     if constexpr (K == kSilu) {
       const float g = to_float(x[i]);
@@ -571,16 +589,17 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) 
     if constexpr (K == kNormAdd)
       if (!again) sum[i] = h = add_round(h, y[i]);
     const float f = to_float(h);
-    if (NORM && !again) ss = fmaf(f, f, ss);
+    if (NORM && !again) ss = fma((double)f, (double)f, ss);
     return NORM ? f * a.w[i] : f;
   };
   for (int i = threadIdx.x; i < a.n; i += 1024) top = max_abs(top, value(i, false));
   const float mine = top;
-  join_row<NORM>(ss, top, sh);
-  if (!in_range<NORM>(ss, top)) {
+  top = join_row(top, sh);
+  if (!in_range(top)) {
     row64<K, T>(a, row, sh);
     return;
   }
+  if constexpr (NORM) put_squares(ss, sh);
   const float near = top * kNear<K>;
   if (K != kPlain && mine >= near)
     for (int i = threadIdx.x; i < a.n; i += 1024)
@@ -597,7 +616,7 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) 
     if (c != __float_as_uint(fmaf(t, down, kMagic))) code = code64(value64<K, T>(a, row, i), top64);
     codes[i] = (int8_t)code;
   }
-  if (threadIdx.x == 0) store_scale<K>(a, row, top64, ss);
+  if (threadIdx.x == 0) store_scale<K>(a, row, top64, NORM ? all_squares(sh) : 0.0);
 }
 
 template <Kind K, class T, int E, int NV>
@@ -648,8 +667,7 @@ void dispatch(RowsArgs a, bool aligned, int device_id, cudaStream_t s) {
   // four or more of 8192 or less (SiLU product and as it is, alone / shared, in us: one row
   // of 29568 fp32 6.3, 3.9 / 3.8, 2.4, bf16 5.7, 3.3 / 3.9, 2.5; 16 rows 6.8, 4.1 / 5.0, 3.3
   // and 6.1, 3.7 / 4.9, 3.4; one of 14336 fp32 4.1, 2.7 / 3.8, 2.5; in two, 64 of 14336 fp32
-  // 4.7, 3.2 / 5.4, 3.5). Not norms, whose sums of squares would be split otherwise than
-  // beside many rows.
+  // 4.7, 3.2 / 5.4, 3.5). Norms were not measured in this form.
   if ((K == kPlain || K == kSilu) && (long long)a.n * (int)sizeof(T) > 32768) {
     int log_share = a.log_share;
     while (log_share < kMostLogShare &&
