@@ -12,7 +12,11 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.machinery
+import importlib.util
 import os
+import subprocess
+import warnings
 
 import numpy as np
 
@@ -331,16 +335,29 @@ def CudaLogProbs(logits, tokens, top_k=0, stream=None):
 _fast = None
 
 
+class _PythonForms:
+    """Leaves every call to the forms below."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def _load_calls():
     global _fast
     if _fast is None:
         _torch()  # its libraries, and the one that the calls are linked to
         lib()
-        if not os.path.exists(_build.CALLS):
-            _build.build_calls()
-        from . import _calls
-
-        _fast = _calls
+        try:
+            path = _build.build_calls()  # as it is, if it is there
+            loader = importlib.machinery.ExtensionFileLoader(f"{__name__}._calls", path)
+            calls = importlib.util.module_from_spec(
+                importlib.util.spec_from_loader(loader.name, loader))
+            loader.exec_module(calls)
+            _fast = calls
+        except (OSError, ImportError, RuntimeError, subprocess.SubprocessError) as e:
+            warnings.warn(f"int8 calls take their Python forms, about twice the host time: {e}",
+                          RuntimeWarning, stacklevel=3)
+            _fast = _PythonForms()
     return _fast
 
 

@@ -5,16 +5,18 @@
   against NCCL for tensor parallelism.
 * ``libmlb_synth.so`` — the CPU side of the seeded synthetic-weight generator
   (g++, no CUDA).
-* ``_calls.so``      — the int8 layer's calls on torch tensors (g++, torch's headers),
-  over libmlb200.so.
+* ``_calls-*.so``    — the int8 layer's calls on torch tensors (g++, torch's headers),
+  over libmlb200.so; named after its sources and the torch and Python it is for.
 
 All land next to this file so they travel with the source tree.
 """
 from __future__ import annotations
 
 import glob
+import hashlib
 import importlib.util
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -24,8 +26,6 @@ CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libmlb200.so")
 SYNTH_LIB = os.path.join(HERE, "libmlb_synth.so")
-
-CALLS = os.path.join(HERE, "_calls.so")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -97,31 +97,61 @@ def _torch_dir():
     return at if os.path.exists(os.path.join(at, "lib", "libc10_cuda.so")) else None
 
 
-def build_calls(force: bool = False) -> str:
-    src = os.path.join(CSRC, "torch_calls.cc")
-    deps = [src, os.path.join(ROOT, "include", "mlb200.h")]
-    if not force and not _stale(CALLS, deps):
-        return CALLS
+def _torch_version(torch: str) -> str:
+    """Of the torch in a directory, without importing it."""
+    with open(os.path.join(torch, "version.py")) as f:
+        found = re.search(r"__version__ = ['\"]([^'\"]+)", f.read())
+    return found.group(1) if found else "unknown"
+
+
+def calls_path() -> str:
+    """Where the calls on torch tensors belong: built from other sources, or for another
+    torch or Python, they have another name."""
     torch = _torch_dir()
     if torch is None:
         raise RuntimeError("calls on torch tensors need torch with CUDA")
+    h = hashlib.sha1()
+    for path in (os.path.join(CSRC, "torch_calls.cc"), os.path.join(ROOT, "include", "mlb200.h")):
+        with open(path, "rb") as f:
+            h.update(f.read())
+    h.update(f"{_torch_version(torch)} {sysconfig.get_config_var('SOABI')}".encode())
+    return os.path.join(HERE, f"_calls-{h.hexdigest()[:12]}.so")
+
+
+def _calls_headers(torch: str) -> bool:
+    return all(os.path.exists(os.path.join(*at)) for at in (
+        (torch, "include", "ATen", "ATen.h"), (sysconfig.get_paths()["include"], "Python.h")))
+
+
+def build_calls(force: bool = False) -> str:
+    path = calls_path()
+    if not force and os.path.exists(path):
+        return path
+    torch = _torch_dir()
     lib = os.path.join(torch, "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", CALLS + ".tmp", src,
+    made = f"{path}.{os.getpid()}.tmp"  # processes that build at once stay apart
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", made,
+           os.path.join(CSRC, "torch_calls.cc"),
            "-I", os.path.join(torch, "include"),
            "-I", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
            "-I", os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"),
            "-I", sysconfig.get_paths()["include"],
            "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
            "-L", HERE, "-l:libmlb200.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + lib]
-    subprocess.run(cmd, check=True)
-    os.replace(CALLS + ".tmp", CALLS)
-    return CALLS
+    try:
+        subprocess.run(cmd, check=True)
+        os.replace(made, path)
+    finally:
+        if os.path.exists(made):
+            os.remove(made)
+    return path
 
 
 def build(force: bool = False, verbose: bool = False) -> None:
     build_synth(force)
     build_cuda(force, verbose)
-    if _torch_dir():
+    torch = _torch_dir()
+    if torch and _calls_headers(torch):  # without them the Python forms do the calls' work
         build_calls(force)
 
 
