@@ -361,6 +361,13 @@ def _load_calls():
     return _fast
 
 
+def _int32(who, name, v):
+    """v, which the C ABI takes as an int: ctypes would drop the bits above."""
+    if not -0x80000000 <= v <= 0x7fffffff:
+        raise MlbError(-1, f"{who}: {name} {v} is out of range")
+    return v
+
+
 def _act_rows(who, name, t, index, rows=-1, n=-1):
     """(t or a copy whose rows' elements follow one another, its address, row stride,
     rows, n) of rows t [rows, n], of the shape given if one is."""
@@ -374,6 +381,8 @@ def _act_rows(who, name, t, index, rows=-1, n=-1):
     rows, n = t.shape
     if n == 0:
         raise MlbError(-1, f"{who}: rows must have at least one element")
+    if n > 0x7fffffff or rows > 0x7fffffff:
+        raise MlbError(-1, f"{who}: {name} {list(t.shape)} is out of range")
     stride, one = t.stride()
     if (one != 1 and n > 1) or (stride < n and rows > 1):
         t = t.contiguous()
@@ -500,6 +509,8 @@ def _code_rows(who, name, t, index):
             raise MlbError(-1, f"{who}: {name} must be on a CUDA device")
         _on_device(who, name, t, index)
     rows, n = t.shape
+    if n > 0x7fffffff or rows > 0x7fffffff:
+        raise MlbError(-1, f"{who}: {name} {list(t.shape)} is out of range")
     stride, one = t.stride()
     at = t.data_ptr()
     if rows <= 1:
@@ -591,7 +602,8 @@ def int8_linear_status(device_id=0):
     (mlb_int8_linear_status); results that it left undone are NaN. Waits for the
     device."""
     code, where = ctypes.c_int(0), ctypes.c_int(0)
-    check(lib().mlb_int8_linear_status(device_id, ctypes.byref(code), ctypes.byref(where)))
+    check(lib().mlb_int8_linear_status(_int32("Int8Linear", "device", device_id),
+                                       ctypes.byref(code), ctypes.byref(where)))
     return code.value, where.value
 
 
@@ -600,7 +612,8 @@ def int8_linear_wait_selftest(rows=8, limit_ms: float = 1.0, device_id: int = 0)
     (status code, site, rows that became NaN): (MLB_ERR_TIMEOUT, 1101 .., rows) when its
     waits gave up after limit_ms (mlb_int8_linear_wait_selftest)."""
     code, where, nan = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
-    check(lib().mlb_int8_linear_wait_selftest(device_id, rows, float(limit_ms),
+    check(lib().mlb_int8_linear_wait_selftest(_int32("Int8Linear", "device", device_id),
+                                              _int32("Int8Linear", "rows", rows), float(limit_ms),
                                               ctypes.byref(code), ctypes.byref(where),
                                               ctypes.byref(nan)))
     return code.value, where.value, nan.value
@@ -622,7 +635,8 @@ class RopeTable:
                  original_len=0, low_freq_factor=1.0, high_freq_factor=4.0, beta_fast=32.0,
                  beta_slow=1.0, factors=None, device_id=0):
         torch = _torch()
-        half = max(0, rotary_dim // 2)
+        half = max(0, _int32("RopeTable", "rotary_dim", rotary_dim) // 2)
+        _int32("RopeTable", "scaling", scaling)
         values = np.zeros(max(half, 1), np.float64)
         amplitude = ctypes.c_double(1.0)
         check(lib().mlb_rope_frequencies(
@@ -667,11 +681,15 @@ def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NO
     act = _act_type(who, first)
     rows, _, dim = first.shape
     _int_tensor(who, "positions", positions, (rows,), index)
+    _int32(who, "rope type", rope_type)
     f = table.frequencies
     if f.dtype is not _torch().float64 or f.dim() != 1 or not f.is_contiguous():
         raise MlbError(-1, f"{who}: expected contiguous float64 frequencies [rotary_dim / 2], got "
                            f"{f.dtype} {list(f.shape)}")
     _on_device(who, "frequencies", f, index)
+    if max(rows, dim, 2 * f.shape[0]) > 0x7fffffff:
+        raise MlbError(-1, f"{who}: rows {list(first.shape)} or frequencies {list(f.shape)} are "
+                           "out of range")
     q, q_at, q_stride, heads, q_out, qo_at, qo_stride = _rope_side(who, "q", q, q_out, first, rows,
                                                                    dim, index)
     k, k_at, k_stride, kv, k_out, ko_at, ko_stride = _rope_side(who, "k", k, k_out, first, rows,
@@ -696,7 +714,7 @@ def _rope_side(who, name, t, out, first, rows, dim, index):
                            f"{t.dtype} {list(t.shape)}")
     if t.get_device() != index:
         _on_device(who, name, t, index)
-    heads = t.shape[1]
+    heads = _int32(who, f"heads of {name}", t.shape[1])
     width = heads * dim
     if out is None:
         out = t.new_empty(rows, heads, dim)

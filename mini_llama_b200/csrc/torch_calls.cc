@@ -123,8 +123,9 @@ PyObject* attempt(F&& f, const T&... outputs) {
 }
 
 bool whole_number(PyObject* o, int* v) {
-  *v = (int)PyLong_AsLong(o);
-  if (!PyErr_Occurred()) return true;
+  const long long wide = PyLong_AsLongLong(o);
+  *v = (int)wide;
+  if (!PyErr_Occurred()) return *v == wide;
   PyErr_Clear();
   return false;
 }
