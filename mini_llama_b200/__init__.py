@@ -368,6 +368,13 @@ def _int32(who, name, v):
     return v
 
 
+def _as_written(who, name, t):
+    """Refuses a negated view (of a conjugate's imaginary part, say): its memory holds the
+    values' negatives."""
+    if t.is_neg():
+        raise MlbError(-1, f"{who}: {name} is a negated view")
+
+
 def _act_rows(who, name, t, index, rows=-1, n=-1):
     """(t or a copy whose rows' elements follow one another, its address, row stride,
     rows, n) of rows t [rows, n], of the shape given if one is."""
@@ -383,6 +390,7 @@ def _act_rows(who, name, t, index, rows=-1, n=-1):
         raise MlbError(-1, f"{who}: rows must have at least one element")
     if n > 0x7fffffff or rows > 0x7fffffff:
         raise MlbError(-1, f"{who}: {name} {list(t.shape)} is out of range")
+    t = t.resolve_neg()
     stride, one = t.stride()
     if (one != 1 and n > 1) or (stride < n and rows > 1):
         t = t.contiguous()
@@ -407,6 +415,7 @@ def _float_vector(who, name, t, n, index):
                            f"{list(t.shape)}")
     if t.get_device() != index:
         _on_device(who, name, t, index)
+    _as_written(who, name, t)
     return t.data_ptr()
 
 
@@ -461,6 +470,7 @@ def CudaRmsNormInt8DeviceWeight(x, w, eps, residual=None, sum_out=None, stream=N
             sum_out = x.new_empty(rows, n)
         else:
             _on_device(who, "sum_out", sum_out, index)
+            _as_written(who, "sum_out", sum_out)
             s_stride = sum_out.stride(0) if sum_out.dim() == 2 and rows > 1 else n
             if (sum_out.shape != x.shape or sum_out.dtype is not x.dtype
                     or (sum_out.stride(1) != 1 and n > 1) or s_stride < n):
@@ -511,6 +521,7 @@ def _code_rows(who, name, t, index):
     rows, n = t.shape
     if n > 0x7fffffff or rows > 0x7fffffff:
         raise MlbError(-1, f"{who}: {name} {list(t.shape)} is out of range")
+    t = t.resolve_neg()
     stride, one = t.stride()
     at = t.data_ptr()
     if rows <= 1:
@@ -586,6 +597,7 @@ def CudaInt8LinearDeviceInput(x, x_scale, w, w_scale, bias=None, out_dtype=None,
         out_stride = n
     else:
         _on_device(who, "out", out, index)
+        _as_written(who, "out", out)
         if (out.dim() != 2 or out.shape[0] != rows or out.shape[1] != n or out.dtype is not dtype
                 or (n > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < n)):
             raise MlbError(-1, f"{who}: out must be {dtype} [{rows}, {n}] with elements that "
@@ -687,6 +699,7 @@ def CudaRopeRowsDeviceInput(q, k, positions, table: RopeTable, rope_type=ROPE_NO
         raise MlbError(-1, f"{who}: expected contiguous float64 frequencies [rotary_dim / 2], got "
                            f"{f.dtype} {list(f.shape)}")
     _on_device(who, "frequencies", f, index)
+    _as_written(who, "frequencies", f)
     if max(rows, dim, 2 * f.shape[0]) > 0x7fffffff:
         raise MlbError(-1, f"{who}: rows {list(first.shape)} or frequencies {list(f.shape)} are "
                            "out of range")
@@ -721,10 +734,12 @@ def _rope_side(who, name, t, out, first, rows, dim, index):
         out_stride = width
     else:
         _on_device(who, f"{name}_out", out, index)
+        _as_written(who, f"{name}_out", out)
         if out.shape != t.shape or out.dtype is not t.dtype or not _whole_rows(out):
             raise MlbError(-1, f"{who}: {name}_out must be shaped like {name}, its rows' "
                                "elements following one another")
         out_stride = out.stride(0) if rows > 1 else width
+    t = t.resolve_neg()
     if t.is_contiguous():
         stride = width
     else:

@@ -32,7 +32,8 @@ struct Rows {  // [rows, n], or [rows, heads, dim] with n = heads * dim
 bool tensor(PyObject* o, const at::Tensor** t) {
   if (!THPVariable_CheckExact(o)) return false;
   *t = &THPVariable_Unpack(o);
-  return (*t)->is_cuda() && (*t)->layout() == at::kStrided;
+  // a negated view's memory holds the values' negatives
+  return (*t)->is_cuda() && (*t)->layout() == at::kStrided && !(*t)->is_neg();
 }
 
 bool on(const at::Tensor& t, int device) { return t.get_device() == device; }
