@@ -207,7 +207,7 @@ __device__ __forceinline__ int code64(double t, double top) {
 
 struct Shared {
   float part[32];    // per warp: maximum
-  double part64[32];  // per warp: sum of squares
+  double part64[32];
   unsigned long long top;  // bits of the 64-bit maximum
   float share[1 << kMostLogShare];  // per CTA of the row's: maximum
   double2 share64[1 << kMostLogShare];  // per CTA: maximum and sum of squares in 64 bits
@@ -279,25 +279,32 @@ __device__ __forceinline__ float join_shares(float top, int rank, int log_share,
   for (int i = 0; i < 1 << log_share; ++i) bits = max(bits, __float_as_uint(sh.share[i]));
   return __uint_as_float(bits);
 }
-// The sum of squares: each warp's before a barrier, all warps' behind it, which the one
-// thread that stores the scale adds up.
-__device__ __forceinline__ void put_squares(double ss, Shared& sh) {
+// The sum of squares from its threads', which lie in shared memory behind a barrier: one
+// warp's work while the others make codes. (Every warp's lanes' by shuffles: 4096 rows of 8192
+// as fast, one of 4096 fp32 2.5 us instead of 2.3, 5768 of 12664 bf16 with residual 123
+// instead of 111.)
+__device__ __forceinline__ double all_squares(const double* squares) {
+  const int lane = threadIdx.x & 31;
+  const int pairs = blockDim.x / 2;
+  const double2* p = reinterpret_cast<const double2*>(squares);
+  double2 a = make_double2(0.0, 0.0), b = a;
+  for (int i = lane; i < pairs; i += 64) {
+    const double2 q = p[i];
+    const double2 r = i + 32 < pairs ? p[i + 32] : make_double2(0.0, 0.0);
+    a.x += q.x, a.y += q.y, b.x += r.x, b.y += r.y;
+  }
+  double ss = (a.x + a.y) + (b.x + b.y);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if ((threadIdx.x & 31) == 0) sh.part64[threadIdx.x >> 5] = ss;
-}
-__device__ __forceinline__ double all_squares(const Shared& sh) {
-  const int warps = blockDim.x >> 5;
-  double ss = 0.0;
-  for (int i = 0; i < warps; ++i) ss += sh.part64[i];
   return ss;
 }
 // Maximum and sum of squares in 64 bits of a row that CTAs share.
-__device__ __forceinline__ void join_shares64(double& top, double& ss, int rank, int log_share,
-                                              Shared& sh) {
-  if (threadIdx.x < 1u << log_share)
+__device__ __forceinline__ void join_shares64(double& top, double& ss, bool keeper, int rank,
+                                              int log_share, Shared& sh) {
+  const unsigned lane = threadIdx.x & 31;
+  if (keeper && lane < 1u << log_share)
     asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(
-                     cluster_address(&sh.share64[rank], threadIdx.x)),
+                     cluster_address(&sh.share64[rank], lane)),
                  "d"(top), "d"(ss)
                  : "memory");
   cluster_sync_all();
@@ -339,6 +346,9 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
   using R = raw_t<T, E>;
   __shared__ Shared shared[2];  // of rows in turn: one is read while the next is written
   extern __shared__ uint4 slots[];
+  // of a norm: its threads' sums of squares, and the warp that keeps the row's
+  double* squares = reinterpret_cast<double*>(slots + (STREAM ? NV * (TWO ? 2 : 1) : 0) * (int)blockDim.x);
+  const bool keeper = threadIdx.x >> 5 == (NORM ? (blockDim.x >> 5) - 1 : 0);
   const int log_share = SHARED ? a.log_share : 0, rank = blockIdx.x & ((1 << log_share) - 1);
   const int first = (rank * (int)blockDim.x + (int)threadIdx.x) * E;
   const int step = ((int)blockDim.x << log_share) * E;
@@ -453,11 +463,7 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     if constexpr (EARLY) fetch(row + gridDim.x);
     if (K == kSilu && low < kLowestGate) top = nanf("");
     const float mine = top;
-    // the warps' sums of squares, before the first barrier or behind it (norm of 4096 rows of
-    // 14336 fp32 76 / 81 us, bf16 54.4 / 53; of 16384 rows of 1000 fp32 26.0 / 28.3; of 64 of
-    // 29568 fp32 6.0 / 5.7)
-    constexpr bool FIRST = sizeof(T) == 4 && (STREAM || K == kNormAdd);
-    if constexpr (NORM && FIRST) put_squares(ss, sh);
+    if constexpr (NORM) squares[threadIdx.x] = ss;
     top = join_row(top, sh);
     if constexpr (SHARED) top = join_shares(top, rank, log_share, sh);
     if (!in_range(top)) {  // the same for all threads of the row
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
       }
     }
     if constexpr (STREAM && !EARLY) fetch(row + gridDim.x);
-    if constexpr (NORM && !FIRST) put_squares(ss, sh);
+    if (NORM && keeper) ss = all_squares(squares);
 
     const float inv = __fdiv_rn(127.0f, top);
     const float up = inv * (1.0f + kDoubt<K>), down = inv * (1.0f - kDoubt<K>);
@@ -550,8 +556,7 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     if (K != kPlain) __syncthreads();
     double top64 = K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
     if constexpr (K != kPlain && SHARED) {
-      ss = NORM && threadIdx.x < 1u << log_share ? all_squares(sh) : 0.0;
-      join_shares64(top64, ss, rank, log_share, sh);
+      join_shares64(top64, ss, keeper, rank, log_share, sh);
     }
     while (doubtful) {
       const int j = __ffs(doubtful) - 1;
@@ -559,19 +564,19 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
       const int i = first + j / E * step + j % E;
       codes[i] = (int8_t)code64(value64<K, T>(a, row, i), top64);
     }
-    if (rank == 0 && threadIdx.x == 0) {
-      if constexpr (NORM && !SHARED) ss = all_squares(sh);
-      store_scale<K>(a, row, top64, ss);
-    }
+    if (rank == 0 && keeper && (threadIdx.x & 31) == 0) store_scale<K>(a, row, top64, ss);
   }
 }
 
 // Rows too long for eight CTAs' registers: the same, one element at a time, values computed
-// twice.
+// twice. With a residual two CTAs fit on an SM, at 32 registers (300 rows of 300000 fp32 784
+// us, one at the 39 that it takes otherwise 1181).
 template <Kind K, class T>
-__global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) {
+__global__ void __launch_bounds__(1024, K == kNormAdd ? 2 : 1) int8_long_rows_kernel(const RowsArgs a) {
   constexpr bool NORM = K == kNorm || K == kNormAdd;
   __shared__ Shared sh;
+  extern __shared__ uint4 slots[];
+  double* squares = reinterpret_cast<double*>(slots);
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
@@ -594,12 +599,12 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) 
   };
   for (int i = threadIdx.x; i < a.n; i += 1024) top = max_abs(top, value(i, false));
   const float mine = top;
+  if constexpr (NORM) squares[threadIdx.x] = ss;
   top = join_row(top, sh);
   if (!in_range(top)) {
     row64<K, T>(a, row, sh);
     return;
   }
-  if constexpr (NORM) put_squares(ss, sh);
   const float near = top * kNear<K>;
   if (K != kPlain && mine >= near)
     for (int i = threadIdx.x; i < a.n; i += 1024)
@@ -616,14 +621,21 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(const RowsArgs a) 
     if (c != __float_as_uint(fmaf(t, down, kMagic))) code = code64(value64<K, T>(a, row, i), top64);
     codes[i] = (int8_t)code;
   }
-  if (threadIdx.x == 0) store_scale<K>(a, row, top64, NORM ? all_squares(sh) : 0.0);
+  __syncwarp();
+  if (threadIdx.x < 32) {
+    if constexpr (NORM) ss = all_squares(squares);
+    if (threadIdx.x == 0) store_scale<K>(a, row, top64, ss);
+  }
 }
+
+constexpr int kSquareBytes = sizeof(double);  // of a norm's thread
 
 template <Kind K, class T, int E, int NV>
 void launch(const RowsArgs& a, int threads, int device_id, cudaStream_t s) {
+  const int squares = K == kNorm || K == kNormAdd ? threads * kSquareBytes : 0;
   if constexpr (E > 1 && NV > 1) {
     // as many CTAs as 64 registers a thread and their slots leave room for
-    const int bytes = threads * NV * 16 * (K == kNormAdd || K == kSilu ? 2 : 1);
+    const int bytes = threads * NV * 16 * (K == kNormAdd || K == kSilu ? 2 : 1) + squares;
     constexpr int kRoom = 220 * 1024;
     const int per_sm = std::min(1024 / threads, kRoom / (bytes + 2 * (int)sizeof(Shared) + 1024));
     if (a.log_share == 0 && per_sm > 0 && a.rows > per_sm * sm_count(device_id)) {
@@ -633,10 +645,12 @@ void launch(const RowsArgs& a, int threads, int device_id, cudaStream_t s) {
     }
   }
   if (a.log_share == 0)
-    return launch_pdl(int8_rows_kernel<K, T, E, NV, kAlone>, dim3(a.rows), dim3(threads), 0, s, true, a);
+    return launch_pdl(int8_rows_kernel<K, T, E, NV, kAlone>, dim3(a.rows), dim3(threads), squares, s,
+                      true, a);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows << a.log_share);
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = (size_t)squares;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -662,7 +676,8 @@ void dispatch(RowsArgs a, bool aligned, int device_id, cudaStream_t s) {
   a.log_share = 0;
   while (a.log_share < kMostLogShare && held(a.log_share) > 1024) ++a.log_share;
   if (held(a.log_share) > 1024 || (a.log_share > 0 && a.rows >= 1 << (31 - kMostLogShare)))
-    return launch_pdl(int8_long_rows_kernel<K, T>, dim3(a.rows), dim3(1024), 0, s, true, a);
+    return launch_pdl(int8_long_rows_kernel<K, T>, dim3(a.rows), dim3(1024),
+                      K == kNorm || K == kNormAdd ? 1024 * kSquareBytes : 0, s, true, a);
   // Few rows of more than 32 KB: as many as SMs and 2048 elements each allow, if they are
   // four or more of 8192 or less (SiLU product and as it is, alone / shared, in us: one row
   // of 29568 fp32 6.3, 3.9 / 3.8, 2.4, bf16 5.7, 3.3 / 3.9, 2.5; 16 rows 6.8, 4.1 / 5.0, 3.3
