@@ -20,6 +20,7 @@ import re
 import subprocess
 import sys
 import sysconfig
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -129,7 +130,8 @@ def build_calls(force: bool = False) -> str:
         return path
     torch = _torch_dir()
     lib = os.path.join(torch, "lib")
-    made = f"{path}.{os.getpid()}.tmp"  # processes that build at once stay apart
+    # processes and threads that build at once stay apart
+    made = f"{path}.{os.getpid()}.{threading.get_ident()}.tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", made,
            os.path.join(CSRC, "torch_calls.cc"),
            "-I", os.path.join(torch, "include"),
