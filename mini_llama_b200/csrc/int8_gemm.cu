@@ -22,10 +22,18 @@
 // Bound by the tensor cores: 4096 x 4096 x 28672 279 to 293 us (3290 to 3450 TOPS, twice the
 // measured bf16 rate; in a long run the power cap, 2800), 512 of 4096 x 4096 11.2.
 //
-// Every wait is bounded: on a timeout the waiting thread records MLB_ERR_TIMEOUT in the
-// device's status word (mlb_int8_linear_status) and raises the CTA's abort flag, copies
-// and products in flight are waited for (bounded), the results of the cluster's tile
-// become NaN, tensor memory is released and the CTA exits.
+// Every wait for a copy, a product or another CTA's sums is bounded: on a timeout the
+// waiting thread records MLB_ERR_TIMEOUT in the device's status word
+// (mlb_int8_linear_status) and raises the CTA's abort flag, copies and products in flight
+// are waited for (bounded), the results of the cluster's tile become NaN, tensor memory is
+// released and the CTA exits. Three waits have no limit of their own, as what they wait for
+// ends without this CTA. The kernel before on the stream (pdl_wait). The cluster's other CTAs
+// at its barriers, which they reach behind bounded waits or the third kind. Tensor memory:
+// whoever holds some on this SM releases it without waiting for another CTA to get any. A CTA
+// alone (one share of K, or another kernel of this library) waits for no CTA; those of a
+// cluster that shares K take 128 of the 512 columns at most and shared memory for no more
+// than two on an SM; a pair's CTA leaves no shared memory for any that takes tensor memory
+// (asserted below).
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -667,8 +675,8 @@ struct Operands {
 
 // How few tokens (tiles of nt) share K: in a power of two of CTAs (as nt is: groups of
 // tokens divide evenly), doubled while the tiles leave room on the SMs and a share keeps
-// at least 8 tiles of K (4096 x 4096, one token, 32 tiles: 6.0 us with 4 shares of 8, 6.8
-// with 8 of 4, 7.4 with 2 of 16). Two CTAs fit on an SM while the sums to be joined leave
+// at least 8 tiles of K (4096 x 4096, 32 tiles, in us with 4 shares of 8, 8 of 4 and 2 of
+// 16: one token 4.9, 6.5, 6.7, 32 tokens 5.4, 7.0, 7.7). Two CTAs fit on an SM while the sums to be joined leave
 // each a ring of two.
 struct FewPlan {
   int split, stages, bytes;
@@ -701,10 +709,11 @@ void launch_few(const Operands& o, LinearArgs a, int device_id, cudaStream_t str
   for (a.log_split = 0; 1 << a.log_split < a.split;) ++a.log_split;
   a.stages = p.stages;
   // Four tiles of short shares, whose time is mostly their start (weights beyond L2, in us,
-  // with / without: one row of 4096 x 4096, 8 tiles a share, 4.97 / 5.84, of 14336 x 4096, 14
-  // tiles, 11.9 / 12.7); eight keep the kernel before waiting (norm and product of 32 x 4096
-  // x 4096 8.7 with four, 9.4 with eight, 9.2 without). None of long ones: 32 of 8192 x
-  // 10240, 32 tiles, 19.5 / 18.7, one of 4096 x 28672 22.0 / 21.8.
+  // with / without: one row of 4096 x 4096, 8 tiles a share, 5.7 / 6.3, behind a norm and with
+  // it 8.1 / 8.8, of 14336 x 4096, 14 tiles, 12.3 / 13.2 and 18.5 / 19.3, 32 of 4096 x 4096
+  // 6.3 / 6.9 and 9.5 / 10.1); eight kept the norm before waiting. None of long ones: 32 of
+  // 8192 x 10240, 32 tiles, 19.8 / 19.0 and 25.0 / 24.4, one of 4096 x 28672 21.9 / 21.6 and
+  // 25.1 / 25.1.
   a.ahead = (a.tiles_k + p.split - 1) / p.split <= 16 ? 4 : 0;
   allow_smem(int8_linear_kernel<NT, T>, kMostBytes, device_id);
   if (tiles * a.split > 0x7fffffffLL) invalid("Int8Linear: too many rows");
@@ -730,6 +739,10 @@ template <int N, class T>
 void launch_pair(const Operands& o, LinearArgs a, int device_id, cudaStream_t stream) {
   using P = PairPlan<N>;
   static_assert(P::BYTES + sizeof(PairShared) <= 227 * 1024);
+  // of an SM's 228 KB (1 KB for each CTA is the system's) nothing is left for the smallest CTA
+  // that takes tensor memory, one of few tokens with a ring of one: none waits for this one's
+  constexpr size_t kSmallest = (kChannels + 16) * kTileK + 1024 + sizeof(Shared);
+  static_assert(P::BYTES + sizeof(PairShared) + 1024 + kSmallest + 1024 > 228 * 1024);
   a.channel_tiles = (a.n + N - 1) / N;
   const long long tiles = (long long)a.channel_tiles * ((a.rows + kPairTokens - 1) / kPairTokens);
   if (tiles > 0x7fffffffLL / 2) invalid("Int8Linear: too many rows");
@@ -742,10 +755,12 @@ void launch_pair(const Operands& o, LinearArgs a, int device_id, cudaStream_t st
 }
 
 // Time of a pair kernel in us: turns of all pairs, each as long as the products of a tile
-// of N channels or the storing of the one before, and the ends. Fitted to, in us (N 64,
-// 128, 256): 256 tokens of 14336 x 4096 25.2, 26.0, 37.3; 512 of 4096 x 4096 16.4, 11.2,
-// 14.8; 1024 28.7, 17.7, 15.6; 4096 of 288 x 1536 9.9, 8.6, 9.3; of 4096 x 28672 613, 369,
-// 278.
+// of N channels or the storing of the one before, and the ends. It is for the choice of N
+// alone. Measured, in us (N 64, 128, 256): 256 tokens of 4096 x 14336 29.2, 18.9, 17.2; 512 of
+// 4096 x 4096 17.1, 11.7, 15.9; 1024 29.4, 18.1, 15.7; 4096 of 4096 x 28672 618, 383, 294,
+// where it chooses the fastest. It underrates stores where K is short, and does not there:
+// 4096 of 288 x 1536 10.6 (chosen), 9.3, 10.2; of 512 x 2048 13.0 (chosen), 11.6, 10.5; of 1024
+// x 4096 30.7, 21.1 (chosen), 20.1; 777 of 288 x 1536 6.1 (chosen), 6.0, 8.4.
 double pair_time(int n, const LinearArgs& a, int sms) {
   const double k = n == 256 ? 0.28 : 0.19, store = 0.01 * n, ends = n == 256 ? 5.5 : 2.6 + 0.006 * n;
   const long long tiles = (long long)((a.n + n - 1) / n) * ((a.rows + kPairTokens - 1) / kPairTokens);
