@@ -25,10 +25,10 @@
 // number, gets the scale NaN: every product of it is NaN, whatever its codes.
 //
 // Bound by a row's chain (load, reduction, the 64-bit maximum, codes), which 32 warps per
-// SM hide in part: 4096 rows of 8192 bf16, norm with residual 47 us (5.0 TB/s), norm 29
-// (3.4), SiLU product 40 (4.2), as they are 27 (3.7); fp32 85 (5.1), 42 (4.0), 57 (5.3), 32
-// (5.2). Codes back to values are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32:
-// norm with residual 3.0 us, norm 2.5, SiLU product 2.5, as it is 1.8, back 1.3.
+// SM hide in part: 4096 rows of 8192 bf16, norm with residual 45.5 us (5.2 TB/s), norm 31
+// (3.2), SiLU product 40 (4.2), as they are 25.5 (4.0); fp32 81 (5.4), 40.3 (4.2), 52 (5.8),
+// 29.5 (5.7). Codes back to values are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32:
+// norm with residual 2.8 us, norm 2.3, SiLU product 2.5, as it is 1.8, back 1.3.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -336,8 +336,8 @@ constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: a sum's low bits are the w
 // boundaries and have whole units of E. kStream: a CTA takes row after row and has the next
 // one on its way, every thread its own elements, in shared memory slots of its own.
 // kShared: a cluster takes a row; blockDim above is that of all its CTAs, and what their
-// barriers join the cluster's join once more. (As a choice at run time it spilled: one row
-// of 29568 fp32, norm with residual 10.8 us instead of 8.3.)
+// barriers join the cluster's join once more. (As a choice at run time it spilled, for a
+// quarter more time of one row of 29568 fp32, norm with residual.)
 template <Kind K, class T, int E, int NV, Form F>
 __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
   constexpr bool NORM = K == kNorm || K == kNormAdd, TWO = K == kNormAdd || K == kSilu;
@@ -668,8 +668,8 @@ void dispatch(RowsArgs a, bool aligned, int device_id, cudaStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
   // CTAs that share a row: as many as its values take registers of, rather than passing
   // over it twice (norm with residual, norm, SiLU product, as it is, 300 rows of 65536, in
-  // us: fp32 168, 90, 185, 54 with one CTA's two passes, 87, 51, 64, 37 shared, bf16 143, 79,
-  // 129, 30 and 57, 39, 48, 30)
+  // us: fp32 178, 90, 186, 53 with one CTA's two passes, 79, 50, 65, 37.5 shared, bf16 142, 81,
+  // 129, 28 and 57, 39, 50, 30)
   const auto held = [&](int log_share) {  // threads that hold a row, of each CTA
     return ((a.n + (kHeld << log_share) - 1) / (kHeld << log_share));
   };
@@ -680,9 +680,10 @@ void dispatch(RowsArgs a, bool aligned, int device_id, cudaStream_t s) {
                       K == kNorm || K == kNormAdd ? 1024 * kSquareBytes : 0, s, true, a);
   // Few rows of more than 32 KB: as many as SMs and 2048 elements each allow, if they are
   // four or more of 8192 or less (SiLU product and as it is, alone / shared, in us: one row
-  // of 29568 fp32 6.3, 3.9 / 3.8, 2.4, bf16 5.7, 3.3 / 3.9, 2.5; 16 rows 6.8, 4.1 / 5.0, 3.3
-  // and 6.1, 3.7 / 4.9, 3.4; one of 14336 fp32 4.1, 2.7 / 3.8, 2.5; in two, 64 of 14336 fp32
-  // 4.7, 3.2 / 5.4, 3.5). Norms were not measured in this form.
+  // of 29568 fp32 6.5, 3.8 / 3.8, 2.4, bf16 5.7, 3.2 / 3.7, 2.7; 16 rows 6.9, 3.9 / 4.9, 3.4
+  // and 6.1, 3.7 / 4.9, 3.5; one of 14336 fp32 4.4, 2.6 / 3.8, 2.4; in two, 64 of 14336 fp32
+  // 4.7, 3.2 / 5.4, 3.5). Norms, which would gain as much (one row of 29568 fp32 with
+  // residual 8.7 / 4.2, 16 rows 8.8 / 5.4), are not shared yet.
   if ((K == kPlain || K == kSilu) && (long long)a.n * (int)sizeof(T) > 32768) {
     int log_share = a.log_share;
     while (log_share < kMostLogShare &&
@@ -693,10 +694,10 @@ void dispatch(RowsArgs a, bool aligned, int device_id, cudaStream_t s) {
   }
   // few rows: up to 512 threads for each, for the time of one; many: 16 elements a thread,
   // or 32 of aligned bf16 rows, for less work around their reductions, where no residual
-  // takes registers (4096 rows of 8192, 16 / 32 elements, in us: norm with residual bf16 47
-  // / 51, fp32 85 / 103; norm bf16 36 / 33; SiLU product bf16 49 / 44, fp32 63 / 66; as they
-  // are bf16 29 / 27, fp32 32 / 35; 2048 unaligned rows of 8191 bf16, norm with residual 68
-  // / 78)
+  // takes registers (4096 rows of 8192, 16 / 32 elements, in us: norm with residual bf16 45.5
+  // / 50, fp32 81 / 100; norm bf16 32.5 / 31, fp32 40 / 44.5; SiLU product bf16 41.5 / 40, fp32
+  // 52 / 54; as they are bf16 27.6 / 25.5, fp32 29.5 / 32; 2048 unaligned rows of 8191 bf16,
+  // norm with residual 64 / 82, SiLU product 46 / 55, but norm 54 / 48.5)
   const bool few = a.rows <= 2 * sm_count(device_id);
   const auto threads_for = [&](int per) {
     per <<= a.log_share;
