@@ -355,9 +355,9 @@ def _load_calls():
             loader.exec_module(calls)
             _fast = calls
         except (OSError, ImportError, RuntimeError, subprocess.SubprocessError) as e:
+            _fast = _PythonForms()  # before the warning, which may be made an error
             warnings.warn(f"int8 calls take their Python forms, about twice the host time: {e}",
                           RuntimeWarning, stacklevel=3)
-            _fast = _PythonForms()
     return _fast
 
 

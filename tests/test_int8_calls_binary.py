@@ -54,6 +54,17 @@ def test_the_python_forms_are_reached(monkeypatch, tmp_path, how):
     assert os.listdir(tmp_path) in ([], ["_calls-broken.so"])
 
 
+def test_a_warning_made_an_error_ends_one_call_alone(monkeypatch, tmp_path):
+    unloadable(monkeypatch, tmp_path, "no compiler")
+    x = torch.zeros(2, 32)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with pytest.raises(RuntimeWarning):
+            mlb.CudaInt8QuantizeDeviceInput(x)
+        with pytest.raises(mlb.MlbError, match="must be on a CUDA device"):
+            mlb.CudaInt8QuantizeDeviceInput(x)
+
+
 def test_a_file_for_another_torch_or_source_is_not_taken(monkeypatch, tmp_path):
     here = build.calls_path()
     assert here == build.calls_path()
