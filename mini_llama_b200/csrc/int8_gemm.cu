@@ -676,8 +676,8 @@ struct Operands {
 // How few tokens (tiles of nt) share K: in a power of two of CTAs (as nt is: groups of
 // tokens divide evenly), doubled while the tiles leave room on the SMs and a share keeps
 // at least 8 tiles of K (4096 x 4096, 32 tiles, in us with 4 shares of 8, 8 of 4 and 2 of
-// 16: one token 4.9, 6.5, 6.7, 32 tokens 5.4, 7.0, 7.7). Two CTAs fit on an SM while the sums to be joined leave
-// each a ring of two.
+// 16: one token 4.9, 6.5, 6.7, 32 tokens 5.4, 7.0, 7.7). Two CTAs fit on an SM while the sums
+// to be joined leave each a ring of two.
 struct FewPlan {
   int split, stages, bytes;
 };

@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
   __shared__ Shared shared[2];  // of rows in turn: one is read while the next is written
   extern __shared__ uint4 slots[];
   // of a norm: its threads' sums of squares, and the warp that keeps the row's
-  double* squares = reinterpret_cast<double*>(slots + (STREAM ? NV * (TWO ? 2 : 1) : 0) * (int)blockDim.x);
+  constexpr int SLOTS = STREAM ? NV * (TWO ? 2 : 1) : 0;  // of a thread
+  double* squares = reinterpret_cast<double*>(slots + SLOTS * (int)blockDim.x);
   const bool keeper = threadIdx.x >> 5 == (NORM ? (blockDim.x >> 5) - 1 : 0);
   const int log_share = SHARED ? a.log_share : 0, rank = blockIdx.x & ((1 << log_share) - 1);
   const int first = (rank * (int)blockDim.x + (int)threadIdx.x) * E;
@@ -555,9 +556,7 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
     }
     if (K != kPlain) __syncthreads();
     double top64 = K == kPlain ? (double)top : __longlong_as_double((long long)sh.top);
-    if constexpr (K != kPlain && SHARED) {
-      join_shares64(top64, ss, keeper, rank, log_share, sh);
-    }
+    if constexpr (K != kPlain && SHARED) join_shares64(top64, ss, keeper, rank, log_share, sh);
     while (doubtful) {
       const int j = __ffs(doubtful) - 1;
       doubtful &= doubtful - 1;
@@ -572,7 +571,8 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(const RowsArgs a) {
 // twice. With a residual two CTAs fit on an SM, at 32 registers (300 rows of 300000 fp32 784
 // us, one at the 39 that it takes otherwise 1181).
 template <Kind K, class T>
-__global__ void __launch_bounds__(1024, K == kNormAdd ? 2 : 1) int8_long_rows_kernel(const RowsArgs a) {
+__global__ void __launch_bounds__(1024, K == kNormAdd ? 2 : 1)
+    int8_long_rows_kernel(const RowsArgs a) {
   constexpr bool NORM = K == kNorm || K == kNormAdd;
   __shared__ Shared sh;
   extern __shared__ uint4 slots[];
