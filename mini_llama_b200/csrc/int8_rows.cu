@@ -25,9 +25,9 @@
 // number, gets the scale NaN: every product of it is NaN, whatever its codes.
 //
 // Bound by a row's chain (load, reduction, the 64-bit maximum, codes), which 32 warps per
-// SM hide in part: 4096 rows of 8192 bf16, norm with residual 45.5 us (5.2 TB/s), norm 31
-// (3.2), SiLU product 40 (4.2), as they are 25.5 (4.0); fp32 81 (5.4), 40.3 (4.2), 52 (5.8),
-// 29.5 (5.7). Codes back to values are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32:
+// SM hide in part: 4096 rows of 8192 bf16, norm with residual 44 us (5.4 TB/s), norm 30.6
+// (3.3), SiLU product 40 (4.2), as they are 25 (4.0); fp32 79 (5.5), 40.3 (4.2), 52 (5.8),
+// 29.6 (5.7). Codes back to values are bound by HBM (26.5 us, 6.3 TB/s). One row of 4096 fp32:
 // norm with residual 2.8 us, norm 2.3, SiLU product 2.5, as it is 1.8, back 1.3.
 #include <cuda_bf16.h>
 
@@ -704,9 +704,9 @@ void dispatch(RowsArgs a, bool aligned, int device_id, cudaStream_t s) {
   }
   // few rows: up to 512 threads for each, for the time of one; many: 16 elements a thread,
   // or 32 of aligned bf16 rows, for less work around their reductions, where no residual
-  // takes registers (4096 rows of 8192, 16 / 32 elements, in us: norm with residual bf16 45.5
-  // / 50, fp32 81 / 100; norm bf16 32.5 / 31, fp32 40 / 44.5; SiLU product bf16 41.5 / 40, fp32
-  // 52 / 54; as they are bf16 27.6 / 25.5, fp32 29.5 / 32; 2048 unaligned rows of 8191 bf16,
+  // takes registers (4096 rows of 8192, 16 / 32 elements, in us: norm with residual bf16 44
+  // / 50, fp32 79 / 98; norm bf16 32.6 / 30.6, fp32 40 / 44; SiLU product bf16 41.6 / 39.6,
+  // fp32 52 / 54; as they are bf16 27.6 / 25, fp32 29.6 / 32; 2048 unaligned rows of 8191 bf16,
   // norm with residual 64 / 82, SiLU product 46 / 55, but norm 54 / 48.5)
   const bool few = a.rows <= 2 * sm_count(device_id);
   const auto threads_for = [&](int per) {
